@@ -22,7 +22,8 @@ extern "C" {
 typedef struct FLCtx FLCtx;
 
 /* formats (src/fused_layer.h:11): experts in FL_IQ2; routed down also FL_Q2K / FL_Q3K and the shared expert also
- * K-quants (the reference's real shards), read in place in ggml's block layout */
+ * K-quants (the reference's real shards), read in place in ggml's block layout; FL_Q4K in fl_kq_matvec_dev and the
+ * device-resident block (fl_set_layer_formats) */
 enum { FL_Q4K = 0, FL_Q6K = 1, FL_Q80 = 2, FL_Q5K = 3, FL_IQ2 = 4, FL_Q2K = 5, FL_Q3K = 6 };
 /* IQ2_XXS byte layouts of expert matrices: ggml's row-major blocks, or the tiled resident layout of fl_pack_iq2xxs */
 enum { FL_LAYOUT_GGML = 0, FL_LAYOUT_TILED = 1 };
@@ -125,7 +126,7 @@ typedef struct FLMoeLayer {
     int E, H;                  /* hidden (7168) and expert intermediate (2048) sizes; E, H multiples of 1024 */
 } FLMoeLayer;
 /* formats of fl_moe_layer's routed down and shared gate / up / down (default FL_IQ2 x 4; FLMoeLayer carries none):
- * FL_IQ2 matrices in the tiled layout, K-quants (the real shards' Q2_K / Q3_K down, Q5_K / Q5_K / Q6_K shared) read in
+ * FL_IQ2 matrices in the tiled layout, K-quants (the real shards' Q2_K / Q3_K down, Q5_K / Q5_K / Q6_K shared; Q4_K) read in
  * place in ggml's layout, 4-byte aligned. With any K-quant the block runs its per-pass kernels for every n. */
 int fl_set_layer_formats(FLCtx *, int down_fmt, int sh_gate_fmt, int sh_up_fmt, int sh_down_fmt);
 /* y[n][E] = MoE(x[n][E]) on the context's stream (x, y device pointers; asynchronous). n <= 65536.
@@ -155,14 +156,40 @@ int fl_moe_layer_noalloc(FLCtx *, const FLMoeLayer * L, const float * x, int n, 
 /* router only: sel/w [n][topk] (device), logits/probs [n][n_exp] may be NULL */
 int fl_route_dev(FLCtx *, const float * gate_inp, const float * probs_b, const float * x, int n, int n_exp, int E,
                  float * logits, float * probs, int * sel, float * w);
+/* The balance loss of n routed rows and their per-expert counts (no counterpart in the reference, which does not train):
+ * logits [n][n_exp] and sel [n][topk] as fl_route_dev gives them. Rows belong to nseq sequences, sequence s being rows
+ * seq[s] .. seq[s + 1] - 1 (nseq + 1 ascending device offsets; NULL: one sequence, all n rows); rows before seq[0] and from
+ * seq[nseq] on belong to none and are not read. With p = sigmoid(z) / (the row's sum of sigmoid(z)), per sequence of T rows
+ *   counts[s][e] = picks of expert e (entries of sel outside 0 .. n_exp - 1 count for none),   f_e = n_exp counts / (topk T)
+ *   loss[s] = alpha * sum_e f_e * (mean of p_e over the rows)
+ * (0 for a sequence of no rows; a row of -inf adds nothing). n_exp <= 256, topk <= 8, n * topk <= 2^24, nseq <= 65534. Sums
+ * are in a fixed order: equal calls give equal bits. Offsets are clamped to 0 .. n; ones that are not ascending give
+ * unspecified values. */
+int fl_balance_loss_dev(FLCtx *, const float * logits, const int * sel, const int * seq, int n, int nseq, int n_exp, int topk, float alpha,
+                        int * counts, float * loss);
+/* its gradient: dlogits [n][n_exp] = (accumulate: +=) sum_s gloss[s] * d loss[s] / d logits, with counts as fl_balance_loss_dev
+ * left them (constants of the derivative) and gloss [nseq] (NULL: ones). Rows of no sequence get 0 (accumulate: stay). */
+int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, const int * seq, const float * gloss, int n, int nseq, int n_exp,
+                             int topk, float alpha, int accumulate, float * dlogits);
+/* The router's backward pass, for fl_route_dev's w under the context's routing rule (topk, scale): from dw [n][topk], the
+ * gradient of the routing weights, and dz [n][n_exp], a gradient of the logits themselves such as fl_balance_loss_grad_dev's
+ * (either may be NULL),
+ *   dlogits [n][n_exp] = dz + the part through w (may be dz's own buffer),
+ *   dW [n_exp][E] = (accumulate: +=) dlogits^T x,   dx [n][E] = dlogits W
+ * (each of the three may be NULL: not computed). logits and sel are fl_route_dev's; the bias has no gradient; entries of sel
+ * outside 0 .. n_exp - 1 are skipped. n <= 65536, E a multiple of 1024 up to 65536. Deterministic, no atomics. */
+int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
+                      int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
 /* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device) */
 int fl_dispatch_dev(FLCtx *, const int * sel, int n, int topk, int n_exp, int * counts, int * offsets, int * perm, int * inv, int * act, int * nact);
 /* Q8_K of nrows x K floats (device): q [nrows][K] int8, d [nrows][K/256] */
 int fl_quant_q8k_dev(FLCtx *, const float * x, int nrows, int K, int8_t * q, float * d);
-/* y [n][R] = W . x_t for a K-quant matrix W (fmt FL_Q2K, FL_Q3K, FL_Q5K or FL_Q6K; R rows of K/256 ggml blocks, in
- * place, start and size multiples of 4 bytes) and n Q8_K rows q [n][K], d [n][K/256] (device; K % 256 == 0, K <= 8192).
+/* y [n][R] = W . x_t for a K-quant matrix W (fmt FL_Q2K, FL_Q3K, FL_Q4K, FL_Q5K or FL_Q6K; R rows of K/256 ggml blocks, in
+ * place, start and size multiples of 4 bytes) and n Q8_K rows q [n][K], d [n][K/256] (device; K % 256 == 0, K <= 8192; for
+ * FL_Q4K, the format of attention, dense layers and heads, K <= 65536).
  * The per-format mat-vec behind fl_moe / fl_ffn_begin (the reference's tc_matvec<F>, src/fused_layer.cu:102-158,
- * 203-254): integer sub-block sums exact, fp32 over the blocks in order (Q2_K bit-identical to ggml's scalar dot). */
+ * 203-254): integer sub-block sums exact, fp32 over the blocks in order (Q2_K bit-identical to ggml's scalar dot).
+ * FL_Q4K: y = fma(d8, fma(-dmin, summ, d * isum), y) per block, whatever n and R: a row's output has the same bits in any batch. */
 int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y);
 /* IQ2_XXS ggml layout <-> tiled layout for nmat matrices of R x K at byte strides (device, may not alias) */
 int fl_pack_iq2xxs(FLCtx *, const void * src_ggml, size_t src_stride, void * dst_tiled, size_t dst_stride, int R, int K, int nmat);
@@ -221,7 +248,8 @@ int fl_gguf_read(const FLGguf *, const FLGgufTensor *, uint64_t off, uint64_t by
  * fl_moe_layer_normed (K-quant ones stay as stored: call fl_set_layer_formats with fmt_down / fmt_sh_*);
  * FL_LAYOUT_GGML keeps every matrix as stored, for fl_moe / fl_wide_moe (the layer as the arena, ids = expert ids,
  * down_fmt = fmt_down) and fl_ffn_begin (FLW from L, fl_set_shared_formats with fmt_sh_*). Routed gate/up must be
- * IQ2_XXS, down IQ2_XXS, Q2_K or Q3_K, the shared expert IQ2_XXS or K-quants (FL_ESCOPE otherwise). */
+ * IQ2_XXS, down IQ2_XXS, Q2_K or Q3_K, the shared expert IQ2_XXS or K-quants, Q4_K (down too) with FL_LAYOUT_TILED only
+ * (FL_ESCOPE otherwise). */
 typedef struct FLGgufLayer {
     FLMoeLayer L;
     const float * ffn_norm;                 /* [E] F32, device; NULL when the layer has no ffn_norm */

@@ -18,8 +18,8 @@ QK_K = 256
 IQ2_BYTES = 66
 
 FL_IQ2 = 4
-FL_Q6K, FL_Q5K, FL_Q2K, FL_Q3K = 1, 3, 5, 6
-KQ_BYTES = {FL_Q2K: 84, FL_Q3K: 110, FL_Q5K: 176, FL_Q6K: 210}
+FL_Q4K, FL_Q6K, FL_Q5K, FL_Q2K, FL_Q3K = 0, 1, 3, 5, 6
+KQ_BYTES = {FL_Q2K: 84, FL_Q3K: 110, FL_Q4K: 144, FL_Q5K: 176, FL_Q6K: 210}
 FL_LAYOUT_GGML, FL_LAYOUT_TILED = 0, 1
 FL_OK, FL_EINVAL, FL_ENOMEM, FL_EHIP, FL_ERANGE, FL_ESCOPE = 0, -1, -2, -3, -4, -5
 
@@ -127,7 +127,7 @@ ABI_SYMBOLS = [
     "fl_wide_outs", "fl_wide_skip", "fl_spec", "fl_sketch", "fl_fetch", "fl_moe", "fl_skip", "fl_h2d", "fl_h2d_bytes", "fl_wait_event",
     "fl_gpu_ms", "fl_ffn_begin", "fl_set_experts", "fl_set_routing", "fl_set_keep", "fl_set_share_experts", "fl_set_shared_formats", "fl_set_layer_formats", "fl_kq_matvec_dev",
     "fl_gguf_open", "fl_gguf_close", "fl_gguf_n_tensors", "fl_gguf_tensor_name", "fl_gguf_tensor", "fl_gguf_tensor_at",
-    "fl_gguf_get_int", "fl_gguf_get_float", "fl_gguf_get_str", "fl_gguf_read", "fl_gguf_load_moe_layer", "fl_gguf_free_layer", "fl_moe_layer", "fl_moe_layer_normed", "fl_moe_layer_noalloc", "fl_route_dev", "fl_dispatch_dev", "fl_quant_q8k_dev",
+    "fl_gguf_get_int", "fl_gguf_get_float", "fl_gguf_get_str", "fl_gguf_read", "fl_gguf_load_moe_layer", "fl_gguf_free_layer", "fl_moe_layer", "fl_moe_layer_normed", "fl_moe_layer_noalloc", "fl_route_dev", "fl_balance_loss_dev", "fl_balance_loss_grad_dev", "fl_route_grad_dev", "fl_dispatch_dev", "fl_quant_q8k_dev",
     "fl_pack_iq2xxs", "fl_unpack_iq2xxs", "fl_register_tiled", "fl_unregister_tiled", "fl_rmsnorm_dev", "fl_synth_iq2xxs", "fl_synth_normal", "fl_probe_exp",
     "fl_debug", "fl_set_debug", "fl_set_fused", "fl_set_decode1", "fl_set_prefill_mfma", "fl_stream", "fl_set_stream", "fl_d2h", "fl_set_profile", "fl_stage_ms", "fl_sync", "fl_last_error", "fl_free",
 ]
@@ -182,6 +182,9 @@ def lib():
             "fl_moe_layer_normed": (I, [P_, ctypes.POINTER(FLMoeLayer), P_, F, P_, I, I, P_]),
             "fl_moe_layer_noalloc": (I, [P_, ctypes.POINTER(FLMoeLayer), P_, I, P_]),
             "fl_route_dev": (I, [P_, P_, P_, P_, I, I, I, P_, P_, P_, P_]),
+            "fl_balance_loss_dev": (I, [P_, P_, P_, P_, I, I, I, I, F, P_, P_]),
+            "fl_balance_loss_grad_dev": (I, [P_, P_, P_, P_, P_, I, I, I, I, F, I, P_]),
+            "fl_route_grad_dev": (I, [P_, P_, P_, P_, P_, P_, P_, I, I, I, P_, P_, I, P_]),
             "fl_dispatch_dev": (I, [P_, P_, I, I, I, P_, P_, P_, P_, P_, P_]),
             "fl_quant_q8k_dev": (I, [P_, P_, I, I, P_, P_]),
             "fl_pack_iq2xxs": (I, [P_, P_, S, P_, S, I, I, I]),
@@ -287,6 +290,12 @@ class Context:
 
     def set_routing(self, n_group=8, topk_group=4, topk=8, scale=2.5):
         self.check(lib().fl_set_routing(self.ctx, n_group, topk_group, topk, scale))
+        self._topk = topk
+
+    @property
+    def routing_topk(self):
+        """Picks per row of the context's routing rule (the library's default 8 until set_routing is called)."""
+        return getattr(self, "_topk", 8)
 
     def set_keep(self, keep=0, renorm=2.5):
         """fl_moe_layer keeps each row's `keep` heaviest experts, rescaled to sum to renorm (0 = all topk, default)."""
@@ -385,6 +394,61 @@ class Context:
         w = t.empty((n, topk), dtype=t.float32, device=x.device)
         self.check(lib().fl_route_dev(self.ctx, _ptr(W), _ptr(bias), _ptr(x), n, ne, E, _ptr(logits), _ptr(probs), _ptr(sel), _ptr(w)))
         return logits, probs, sel, w
+
+    def balance_loss(self, logits, sel, alpha, seq=None):
+        """(counts [nseq][n_exp] int32, loss [nseq]) of routed rows (route()'s logits and sel). seq: int32 device offsets of
+        the sequences' rows, ascending (None: one sequence); rows of no sequence are not read."""
+        t = self.torch
+        n, ne = logits.shape
+        topk = sel.shape[1]
+        nseq = 1 if seq is None else seq.numel() - 1
+        self._need("balance_loss", (logits, t.float32, (n, ne)), (sel, t.int32, (n, topk)), (seq, t.int32, (nseq + 1,)))
+        counts = t.empty((nseq, ne), dtype=t.int32, device=logits.device)
+        loss = t.empty(nseq, dtype=t.float32, device=logits.device)
+        self.check(lib().fl_balance_loss_dev(self.ctx, _ptr(logits), _ptr(sel), _ptr(seq), n, nseq, ne, topk, alpha, _ptr(counts), _ptr(loss)))
+        return counts, loss
+
+    def balance_loss_grad(self, logits, counts, topk, alpha, seq=None, gloss=None, dlogits=None):
+        """The gradient of sum_s gloss[s] * loss[s] (gloss None: ones) to the logits, [n][n_exp]; counts: balance_loss's. A
+        dlogits tensor is added to in place; rows of no sequence get (or add) 0."""
+        t = self.torch
+        n, ne = logits.shape
+        nseq = 1 if seq is None else seq.numel() - 1
+        self._need("balance_loss_grad", (logits, t.float32, (n, ne)), (counts, t.int32, (nseq, ne)), (seq, t.int32, (nseq + 1,)),
+                   (gloss, t.float32, (nseq,)), (dlogits, t.float32, (n, ne)))
+        add = dlogits is not None
+        if not add:
+            dlogits = t.empty_like(logits)
+        self.check(lib().fl_balance_loss_grad_dev(self.ctx, _ptr(logits), _ptr(counts), _ptr(seq), _ptr(gloss), n, nseq, ne, topk, alpha,
+                                                  1 if add else 0, _ptr(dlogits)))
+        return dlogits
+
+    def route_grad(self, W, x, logits, sel, dw=None, dz=None, dW=None, need_dW=True, need_dx=True):
+        """The router's backward pass, for route()'s weights under the context's rule: (dlogits, dW, dx) from dw [n][topk] (the
+        weights' gradient) and dz [n][n_exp] (a gradient of the logits themselves). A dW tensor is added to in place."""
+        t = self.torch
+        n, E = x.shape
+        ne = W.shape[0]
+        topk = sel.shape[1]
+        self._need("route_grad", (W, t.float32, (ne, E)), (x, t.float32, (n, E)), (logits, t.float32, (n, ne)), (sel, t.int32, (n, topk)),
+                   (dw, t.float32, (n, topk)), (dz, t.float32, (n, ne)), (dW, t.float32, (ne, E)))
+        if topk != self.routing_topk:
+            raise LokiError("route_grad: sel has %d picks a row, the context's rule %d" % (topk, self.routing_topk))
+        add = dW is not None
+        dl = t.empty_like(logits)
+        if dW is None and need_dW:
+            dW = t.empty_like(W)
+        dx = t.empty_like(x) if need_dx else None
+        self.check(lib().fl_route_grad_dev(self.ctx, _ptr(W), _ptr(x), _ptr(logits), _ptr(sel), _ptr(dw), _ptr(dz), n, ne, E, _ptr(dl), _ptr(dW),
+                                           1 if add else 0, _ptr(dx)))
+        return dl, dW, dx
+
+    def _need(self, who, *args):
+        """Each (tensor, dtype, shape): contiguous on the GPU as the library reads it (None passes)."""
+        for t, dtype, shape in args:
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda):
+                raise LokiError("%s: a contiguous %s tensor of shape %s on the GPU is needed, not %s %s on %s" %
+                                (who, dtype, shape, t.dtype, tuple(t.shape), t.device))
 
     def dispatch(self, sel, n_exp=N_EXPERT):
         t = self.torch

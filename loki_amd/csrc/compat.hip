@@ -1034,7 +1034,7 @@ extern "C" int fl_set_shared_formats(FLCtx * c, int gate_fmt, int up_fmt, int do
     if (!c) { return FL_EINVAL; }
     const int f[3] = { gate_fmt, up_fmt, down_fmt };
     for (int i = 0; i < 3; ++i) {
-        if (f[i] != FL_IQ2 && kq_block_bytes(f[i]) == 0) { return fail(c, FL_EINVAL, "format %d is not IQ2_XXS or a K-quant (Q2_K, Q3_K, Q5_K, Q6_K)", f[i]); }
+        if (f[i] != FL_IQ2 && (f[i] == FL_Q4K || kq_block_bytes(f[i]) == 0)) { return fail(c, FL_EINVAL, "format %d is not IQ2_XXS or a K-quant (Q2_K, Q3_K, Q5_K, Q6_K)", f[i]); }
     }
     if ((gate_fmt == FL_IQ2) != (up_fmt == FL_IQ2)) { return fail(c, FL_EINVAL, "gate and up must both be IQ2_XXS or both K-quants"); }
     Compat * s = cs(c);

@@ -26,6 +26,28 @@ template <class T> struct DBuf {
     void release() { if (p) { (void) hipFree(p); } p = nullptr; cap = 0; }
 };
 
+// a workspace that a captured graph may hold on to: growing it keeps the older allocations until the context ends, and
+// sizes go up in powers of two, so all of them together are at most twice the largest
+struct KeptBuf {
+    void * p = nullptr; size_t cap = 0; std::vector<void *> old;
+    hipError_t ensure(size_t bytes) {
+        if (p && bytes <= cap) { return hipSuccess; }
+        size_t want = 1 << 16;
+        while (want < bytes) { want *= 2; }
+        void * q = nullptr;
+        const hipError_t e = hipMalloc(&q, want);
+        if (e != hipSuccess) { return e; }
+        if (p) { old.push_back(p); }
+        p = q; cap = want;
+        return hipSuccess;
+    }
+    void release() {
+        for (void * q : old) { (void) hipFree(q); }
+        if (p) { (void) hipFree(p); }
+        old.clear(); p = nullptr; cap = 0;
+    }
+};
+
 [[noreturn]] inline void fatal(const char * what, hipError_t e, const char * file, int line) {
     std::fprintf(stderr, "[fused] HIP error %s (%s) at %s:%d\n", hipGetErrorString(e), what, file, line);
     std::exit(7);
@@ -73,6 +95,7 @@ struct FLCtx {
     DBuf<unsigned> rcnt;                       // the one-launch routing's self-resetting counter (launch_router_fused)
     DBuf<double> rpart;                        // the matrix-core router's parts [router_parts][n][n_exp]
     DBuf<int> dscr;                            // the multi-workgroup dispatch's per-round counts and bases
+    KeptBuf bal, rg;                           // fl_balance_loss_dev's partial sums, fl_route_grad_dev's operands
     size_t h2d_zc = 0, h2d_ce = 0; int h2d_said = 0;   // fl_h2d bytes by kernel (mapped pinned) / by copy engine
     // fl_ffn_begin's event pairs (recorded, not yet folded into ms_ffn by fl_gpu_ms) and the reusable ones
     std::vector<std::pair<hipEvent_t, hipEvent_t>> ffn_ev_pending, ffn_ev_free; double ms_ffn = 0.0;

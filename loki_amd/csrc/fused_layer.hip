@@ -10,6 +10,7 @@
 #include "fl_ctx.h"
 
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -130,6 +131,7 @@ extern "C" void fl_free(FLCtx * c) {
     c->tab.release(); c->derr.release(); c->dlogit.release(); c->dth.release(); c->dto.release(); c->dxq.release();
     c->ptab.release(); c->pcols.release(); c->pcolsk.release(); c->pncols.release(); c->xh.release(); c->hh.release();
     c->ksg.release(); c->ksu.release(); c->rcnt.release(); c->rpart.release(); c->dscr.release();
+    c->bal.release(); c->rg.release();
     for (auto & v : c->ev_free) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto & v : c->ev_pending) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto * l : { &c->ffn_ev_pending, &c->ffn_ev_free, &c->moe_ev_pending, &c->moe_ev_free }) { for (auto & e : *l) { (void) hipEventDestroy(e.first); (void) hipEventDestroy(e.second); } }
@@ -279,8 +281,9 @@ extern "C" int fl_quant_q8k_dev(FLCtx * c, const float * x, int nrows, int K, in
 extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y) {
     if (!c) { return FL_EINVAL; }
     const int bs = kq_block_bytes(fmt);
-    if (bs == 0) { return fail(c, FL_EINVAL, "format %d is not a K-quant (FL_Q2K, FL_Q3K, FL_Q5K, FL_Q6K)", fmt); }
-    if (R <= 0 || K <= 0 || K % 256 || K > 8192 || n < 0) { return fail(c, FL_EINVAL, "R %d, K %d (a multiple of 256, at most 8192), n %d", R, K, n); }
+    if (bs == 0) { return fail(c, FL_EINVAL, "format %d is not a K-quant (FL_Q2K, FL_Q3K, FL_Q4K, FL_Q5K, FL_Q6K)", fmt); }
+    const int kmax = fmt == FL_Q4K ? 65536 : 8192;
+    if (R <= 0 || K <= 0 || K % 256 || K > kmax || n < 0) { return fail(c, FL_EINVAL, "R %d, K %d (a multiple of 256, at most %d), n %d", R, K, kmax, n); }
     if (n == 0) { return FL_OK; }
     if (!w || !q || !d || !y) { return fail(c, FL_EINVAL, "null pointer"); }
     const size_t mb = (size_t) R * (size_t) (K / 256) * (size_t) bs;
@@ -292,6 +295,85 @@ extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K
     a.w = (const uint8_t *) w; a.estride = mb; a.aq = q; a.ad = d; a.K = K; a.R = R;
     a.act = nullptr; a.nact = nullptr; a.offsets = nullptr; a.n = n; a.out = y; a.ldo = R;
     TRY(c, launch_kq_matvec(a, fmt, n, 1, c->st));
+    return FL_OK;
+}
+
+// ---------------------------------------------------------------- the router's training side
+// the context's device has to be the current one (its stream and workspaces live there)
+static int need_device(FLCtx * c) {
+    int dev = -1;
+    TRY(c, hipGetDevice(&dev));
+    return dev == c->dev ? FL_OK : fail(c, FL_EINVAL, "the current device is %d, the context's %d", dev, c->dev);
+}
+static int balance_args(FLCtx * c, BalanceArgs & b) {
+    if (b.n < 0 || b.topk < 1 || b.topk > MAXK || (int64_t) b.n * b.topk > (1 << 24)) { return fail(c, FL_ERANGE, "n %d, topk %d (1..%d, n * topk at most 2^24)", b.n, b.topk, MAXK); }
+    if (b.n_exp < 1 || b.n_exp > NEXP_MAX) { return fail(c, FL_EINVAL, "n_exp %d outside 1..%d", b.n_exp, NEXP_MAX); }
+    if (b.nseq < 1 || b.nseq > 65534 || (!b.seq && b.nseq != 1)) { return fail(c, FL_EINVAL, "nseq %d outside 1..65534, or not 1 without offsets", b.nseq); }
+    if (!std::isfinite(b.alpha)) { return fail(c, FL_EINVAL, "alpha %g is not finite", (double) b.alpha); }
+    if (b.n > 0 && !b.logits) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (!b.counts) { return fail(c, FL_EINVAL, "null pointer"); }
+    if ((b.n > 0 && !covers(b.logits, (size_t) b.n * b.n_exp * 4)) || !covers(b.counts, (size_t) b.nseq * b.n_exp * 4) ||
+        (b.seq && !covers(b.seq, (size_t) (b.nseq + 1) * 4))) {
+        return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, n_exp %d, nseq %d)", b.n, b.n_exp, b.nseq);
+    }
+    b.chunks = balance_chunks(b.n, b.nseq);
+    return need_device(c);
+}
+extern "C" int fl_balance_loss_dev(FLCtx * c, const float * logits, const int * sel, const int * seq, int n, int nseq, int n_exp, int topk,
+                                   float alpha, int * counts, float * loss) {
+    if (!c) { return FL_EINVAL; }
+    BalanceArgs b{};
+    b.logits = logits; b.sel = sel; b.seq = seq; b.n = n; b.nseq = nseq; b.n_exp = n_exp; b.topk = topk; b.alpha = alpha; b.counts = counts; b.loss = loss;
+    if (int rc = balance_args(c, b)) { return rc; }
+    if (!loss || (n > 0 && !sel)) { return fail(c, FL_EINVAL, "null pointer"); }
+    if ((n > 0 && !covers(sel, (size_t) n * topk * 4)) || !covers(loss, (size_t) nseq * 4)) { return fail(c, FL_EINVAL, "sel's or loss's allocation is smaller than its shape"); }
+    if (b.chunks > 1) {   // (at most 256 workgroups then: the workspace never grows)
+        if (c->bal.ensure((size_t) 256 * NEXP_MAX * 8) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
+        b.part = (float *) c->bal.p; b.pcnt = (int *) c->bal.p + 256 * NEXP_MAX;
+    }
+    TRY(c, launch_balance(b, c->st));
+    return FL_OK;
+}
+extern "C" int fl_balance_loss_grad_dev(FLCtx * c, const float * logits, const int * counts, const int * seq, const float * gloss, int n, int nseq,
+                                        int n_exp, int topk, float alpha, int accumulate, float * dlogits) {
+    if (!c) { return FL_EINVAL; }
+    BalanceArgs b{};
+    b.logits = logits; b.seq = seq; b.n = n; b.nseq = nseq; b.n_exp = n_exp; b.topk = topk; b.alpha = alpha; b.counts = const_cast<int *>(counts);
+    b.gloss = gloss; b.accumulate = accumulate ? 1 : 0; b.dlogits = dlogits;
+    if (int rc = balance_args(c, b)) { return rc; }
+    if (n == 0) { return FL_OK; }
+    if (!dlogits) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (!covers(dlogits, (size_t) n * n_exp * 4) || (gloss && !covers(gloss, (size_t) nseq * 4))) { return fail(c, FL_EINVAL, "dlogits' or gloss's allocation is smaller than its shape"); }
+    TRY(c, launch_balance_grad(b, c->st));
+    return FL_OK;
+}
+extern "C" int fl_route_grad_dev(FLCtx * c, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz,
+                                 int n, int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx) {
+    if (!c) { return FL_EINVAL; }
+    if (n < 0 || n > 65536) { return fail(c, FL_ERANGE, "n = %d outside 0..65536", n); }
+    if (n_exp < 1 || n_exp > NEXP_MAX) { return fail(c, FL_EINVAL, "n_exp %d outside 1..%d", n_exp, NEXP_MAX); }
+    if (E <= 0 || E % 1024 || E > 65536) { return fail(c, FL_EINVAL, "E = %d must be a positive multiple of 1024, at most 65536", E); }
+    if (n == 0 && !dW) { return FL_OK; }
+    if (!dlogits && !dW && !dx) { return fail(c, FL_EINVAL, "nothing to compute: dlogits, dW and dx are all null"); }
+    if (n > 0 && !dw && !dz) { return fail(c, FL_EINVAL, "no gradient to start from: dw and dz are both null"); }
+    if (n > 0 && ((dw && (!logits || !sel)) || (dW && !x) || (dx && !W))) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (dx && (dx == x || dx == W || dx == dW)) { return fail(c, FL_EINVAL, "dx must not be x, W or dW"); }
+    if (dW && (dW == W || dW == x)) { return fail(c, FL_EINVAL, "dW must not be W or x"); }
+    const size_t nz = (size_t) n * n_exp * 4, nx = (size_t) n * E * 4, nw = (size_t) n_exp * E * 4, nk = (size_t) n * c->topk * 4;
+    if (n > 0 && ((dw && (!covers(logits, nz) || !covers(sel, nk) || !covers(dw, nk))) || (dz && !covers(dz, nz)) || (dlogits && !covers(dlogits, nz)) ||
+                  (dW && !covers(x, nx)) || (dx && (!covers(W, nw) || !covers(dx, nx))))) {
+        return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, n_exp %d, E %d, topk %d)", n, n_exp, E, c->topk);
+    }
+    if (dW && !covers(dW, nw)) { return fail(c, FL_EINVAL, "dW's allocation is smaller than its shape (n_exp %d, E %d)", n_exp, E); }
+    if (int rc = need_device(c)) { return rc; }
+    RouteGradArgs a{};
+    a.W = W; a.x = x; a.logits = logits; a.sel = sel; a.dw = dw; a.dz_in = dz; a.n = n; a.n_exp = n_exp; a.E = E; a.topk = c->topk; a.scale = c->scale;
+    a.dz = dlogits; a.dW = dW; a.accumulate = accumulate ? 1 : 0; a.dx = dx;
+    if (!a.dz) {
+        if (c->rg.ensure(nz) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
+        a.dz = (float *) c->rg.p;
+    }
+    TRY(c, launch_route_grad(a, c->st));
     return FL_OK;
 }
 
@@ -718,6 +800,9 @@ static int moe_layer(FLCtx * c, const FLMoeLayer * L, const float * x, int n, fl
         if (lf[0] == FL_IQ2) {   // routed (+ the shared expert when it is IQ2_XXS)
             d.part = sh_iq ? PF_ALL : PF_ROUTED;
             TRY(c, launch_prefill_gemm(d, c->ncu, st));
+        } else if (lf[0] == FL_Q4K) {
+            TRY(c, routed_down_kq(c, L, P, E, H, ne));
+            if (sh_iq) { d.part = PF_SHARED; TRY(c, launch_prefill_gemm(d, c->ncu, st)); }
         } else {
             PrefillArgs k = d;
             k.estride = fmt_mat_bytes(lf[0], E, H); k.cols = kt.cols; k.ncols = kt.ncols; k.col0 = nsh;
@@ -809,7 +894,7 @@ extern "C" int fl_set_layer_formats(FLCtx * c, int down_fmt, int sh_gate_fmt, in
     if (!c) { return FL_EINVAL; }
     const int f[4] = { down_fmt, sh_gate_fmt, sh_up_fmt, sh_down_fmt };
     for (int i = 0; i < 4; ++i) {
-        if (f[i] != FL_IQ2 && kq_block_bytes(f[i]) == 0) { return fail(c, FL_EINVAL, "format %d is not IQ2_XXS or a K-quant (Q2_K, Q3_K, Q5_K, Q6_K)", f[i]); }
+        if (f[i] != FL_IQ2 && kq_block_bytes(f[i]) == 0) { return fail(c, FL_EINVAL, "format %d is not IQ2_XXS or a K-quant (Q2_K .. Q6_K)", f[i]); }
     }
     if ((sh_gate_fmt == FL_IQ2) != (sh_up_fmt == FL_IQ2)) { return fail(c, FL_EINVAL, "shared gate and up must both be IQ2_XXS or both K-quants"); }
     for (int i = 0; i < 4; ++i) { c->lf[i] = f[i]; }

@@ -323,9 +323,12 @@ extern "C" int fl_gguf_load_moe_layer(FLCtx * c, const FLGguf * g, int layer, in
     int fm[6];
     for (int k = 0; k < 3; ++k) { fm[k] = te[k].fl_format; fm[3 + k] = ts[k].fl_format; }
     if (fm[0] != FL_IQ2 || fm[1] != FL_IQ2) { return fail(c, FL_ESCOPE, "%s: routed gate/up must be IQ2_XXS (types %d, %d)", p.c_str(), te[0].type, te[1].type); }
-    if (fm[2] != FL_IQ2 && fm[2] != FL_Q2K && fm[2] != FL_Q3K) { return fail(c, FL_ESCOPE, "%s: routed down type %d (IQ2_XXS, Q2_K or Q3_K)", p.c_str(), te[2].type); }
+    const bool q4 = layout == FL_LAYOUT_TILED;   // Q4_K: fl_moe_layer reads it, the reference-named entry points do not
+    if (fm[2] != FL_IQ2 && fm[2] != FL_Q2K && fm[2] != FL_Q3K && !(q4 && fm[2] == FL_Q4K)) {
+        return fail(c, FL_ESCOPE, "%s: routed down type %d (IQ2_XXS, Q2_K, Q3_K or, in the tiled layout, Q4_K)", p.c_str(), te[2].type);
+    }
     for (int k = 3; k < 6; ++k) {
-        if (fm[k] != FL_IQ2 && kq_block_bytes(fm[k]) == 0) { return fail(c, FL_ESCOPE, "%s: shared-expert type %d (IQ2_XXS or Q2_K / Q3_K / Q5_K / Q6_K)", p.c_str(), ts[k - 3].type); }
+        if (fm[k] != FL_IQ2 && (kq_block_bytes(fm[k]) == 0 || (!q4 && fm[k] == FL_Q4K))) { return fail(c, FL_ESCOPE, "%s: shared-expert type %d (IQ2_XXS, Q2_K / Q3_K / Q5_K / Q6_K or, in the tiled layout, Q4_K)", p.c_str(), ts[k - 3].type); }
     }
     if ((fm[3] == FL_IQ2) != (fm[4] == FL_IQ2)) { return fail(c, FL_ESCOPE, "%s: shared gate and up must both be IQ2_XXS or both K-quants", p.c_str()); }
     // one allocation: router (F32), bias, norm, 3 routed tensors, 3 shared matrices; 256-byte aligned parts

@@ -156,10 +156,11 @@ template <int F> hipError_t go_f(const KqArgs & a, int tt, unsigned gy, hipStrea
 }  // namespace
 
 int kq_block_bytes(int fmt) {
-    switch (fmt) { case KF_Q2K: return 84; case KF_Q3K: return 110; case KF_Q5K: return 176; case KF_Q6K: return 210; default: return 0; }
+    switch (fmt) { case KF_Q4K: return 144; case KF_Q2K: return 84; case KF_Q3K: return 110; case KF_Q5K: return 176; case KF_Q6K: return 210; default: return 0; }
 }
 
 hipError_t launch_kq_matvec(const KqArgs & args, int fmt, int max_slots, int grid_experts, hipStream_t st) {
+    if (fmt == KF_Q4K) { return launch_q4k(args, max_slots, grid_experts, st); }
     KqArgs a = args;
     if (a.K <= 0 || a.K % QK || a.K > QK * NB_MAX || a.R <= 0 || max_slots <= 0 || grid_experts <= 0 || kq_block_bytes(fmt) == 0) { return hipErrorInvalidValue; }
     const int tt = max_slots <= 1 ? 1 : max_slots <= 2 ? 2 : max_slots <= 4 ? 4 : 8;

@@ -1,5 +1,5 @@
-// kquant_device.h -- per-lane pieces of the K-quant x Q8_K block dot (Q2_K, Q3_K, Q5_K, Q6_K in ggml's block layout,
-// read in place), shared by the K-quant mat-vec (kquant.hip) and the one-token decode block (moe_decode1.hip).
+// kquant_device.h -- per-lane pieces of the K-quant x Q8_K block dot (Q2_K .. Q6_K in ggml's block layout,
+// read in place), shared by the K-quant mat-vecs (kquant.hip, q4k.hip) and the one-token decode block (moe_decode1.hip).
 //
 // A block's 256 weights are split over 8 lane slices q = 0..7; each slice's integer partials (isum, and summ for the
 // formats with mins) are exact, and the 8 slices' sums (red8, or a lane's own loop) give ggml's integer block sums
@@ -9,8 +9,8 @@
 
 namespace lk {
 
-enum { KF_Q6K = 1, KF_Q5K = 3, KF_Q2K = 5, KF_Q3K = 6 };
-template <int F> constexpr int kbytes() { return F == KF_Q2K ? 84 : F == KF_Q3K ? 110 : F == KF_Q5K ? 176 : 210; }
+enum { KF_Q4K = 0, KF_Q6K = 1, KF_Q5K = 3, KF_Q2K = 5, KF_Q3K = 6 };
+template <int F> constexpr int kbytes() { return F == KF_Q4K ? 144 : F == KF_Q2K ? 84 : F == KF_Q3K ? 110 : F == KF_Q5K ? 176 : 210; }
 
 constexpr int KQ_WAVES = 4;     // waves per workgroup
 
@@ -38,10 +38,11 @@ __device__ __forceinline__ uint32_t byte_of3(uint32_t w0, uint32_t w1, uint32_t 
 // jq = q % 4 the 8 columns l = 8 jq .. 8 jq + 7, taken in all four 32-weight rows s of the half: piece s = weights
 // 128 n + 32 s + l (one sub-block, 2 words). Q5_K (32-weight sub-blocks, 64-weight quant groups jj): jj = q / 2,
 // columns l = 16 (q % 2) .. + 15 of both halves h of the group: piece h = weights 64 jj + 32 h + l (sub-block 2 jj + h,
-// 4 words). So each lane reads only the bytes of its own columns, 16 contiguous bytes per field.
+// 4 words). Q4_K is cut as Q5_K. So each lane reads only the bytes of its own columns, 16 contiguous bytes per field.
 template <int F> struct Raw;
 template <> struct Raw<KF_Q2K> { uint32_t q[2], sc[2], dd; };
 template <> struct Raw<KF_Q3K> { uint32_t q[3], h[3], s[4], dd; uint32_t shq, shh, shs; };
+template <> struct Raw<KF_Q4K> { uint32_t q[4], s[3], dd; };
 template <> struct Raw<KF_Q5K> { uint32_t q[4], h[4], s[3], dd; };
 template <> struct Raw<KF_Q6K> { uint32_t qa[3], qb[3], h[3], sc[3], dd; uint32_t sha, shb, shh, shs; };
 
@@ -74,6 +75,10 @@ template <int F> __device__ __forceinline__ void load_raw(const Src & b, int q, 
     } else if constexpr (F == KF_Q3K) {   // hmask[32] qs[64] scales[12] d
         r.shq = ld_aligned<2>(b, 32 + 32 * n + 8 * jq, r.q); r.shh = ld_aligned<2>(b, 8 * jq, r.h);
         r.shs = ld_aligned<3>(b, 96, r.s); r.dd = ld_u16(b, 108);
+    } else if constexpr (F == KF_Q4K) {   // d dmin scales[12] qs[128]
+        const u32x4 q4 = ld128(b, 16 + 16 * (uint32_t) q), hd = ld128(b, 0);
+        r.q[0] = q4.x; r.q[1] = q4.y; r.q[2] = q4.z; r.q[3] = q4.w;
+        r.dd = hd.x; r.s[0] = hd.y; r.s[1] = hd.z; r.s[2] = hd.w;
     } else if constexpr (F == KF_Q5K) {   // d dmin scales[12] qh[32] qs[128]
         const uint32_t jj = (uint32_t) q >> 1, hf = (uint32_t) q & 1u;
         const u32x4 q4 = ld128(b, 48 + 32 * jj + 16 * hf), h4 = ld128(b, 16 + 16 * hf), hd = ld128(b, 0);   // qs, qh, d dmin scales
@@ -88,7 +93,7 @@ template <int F> __device__ __forceinline__ void load_raw(const Src & b, int q, 
 }
 
 // decoded slice: u = unsigned quants (4 per word, an offset quant with its offset still added); piece p's scale sc[p]
-// and min mn[p] (pieces: 4 of 2 words for the 16-weight formats, 2 of 4 words for Q5_K)
+// and min mn[p] (pieces: 4 of 2 words for the 16-weight formats, 2 of 4 words for Q4_K and Q5_K)
 struct Chunk {
     uint32_t u[8];
     int sc[4], mn[4];
@@ -130,13 +135,16 @@ template <int F> __device__ __forceinline__ void decode(const Raw<F> & r, int q,
         k.sc[2] = __builtin_amdgcn_sbfe((int) p23, 0u, 6u); k.sc[3] = __builtin_amdgcn_sbfe((int) p23, 16u, 6u);
         k.mn[0] = k.mn[1] = k.mn[2] = k.mn[3] = 0;
         k.d = h2f((uint16_t) r.dd); k.dmin = 0.f;
-    } else if constexpr (F == KF_Q5K) {   // weight 64 jj + 32 h + l: nibble h of qs[32 jj + l], bit 2 jj + h of qh[l]
+    } else if constexpr (F == KF_Q4K || F == KF_Q5K) {   // weight 64 jj + 32 h + l: nibble h of qs[32 jj + l], Q5_K's bit 2 jj + h of qh[l]
         const int jj = q >> 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int j = 2 * jj + h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { k.u[4 * h + i] = ((r.q[i] >> (4 * h)) & 0x0F0F0F0Fu) | (rotr(r.h[i], (uint32_t) j - 4u) & 0x10101010u); }
+            for (int i = 0; i < 4; ++i) {
+                k.u[4 * h + i] = (r.q[i] >> (4 * h)) & 0x0F0F0F0Fu;
+                if constexpr (F == KF_Q5K) { k.u[4 * h + i] |= rotr(r.h[i], (uint32_t) j - 4u) & 0x10101010u; }
+            }
             int sv, mv;
             if (j < 4) { sv = (int) (byte_of3(r.s[0], r.s[1], r.s[2], j) & 63u); mv = (int) (byte_of3(r.s[0], r.s[1], r.s[2], j + 4) & 63u); }
             else {
@@ -168,7 +176,7 @@ template <int F> __device__ __forceinline__ void decode(const Raw<F> & r, int q,
 
 // the lane's activation words (same weight order as u), per piece the start value of its dot accumulator (the
 // quants' offset folded in: Q3_K -4 * bsum, Q6_K -32 * bsum, else 0) and the sum of its Q8_K integers (bsum: the
-// min term of Q2_K / Q5_K)
+// min term of Q2_K / Q4_K / Q5_K)
 struct XChunk { uint32_t x[8]; int c0[4], bx[4]; float d8; };
 
 // 8- and 16-byte activation reads from global memory or LDS
@@ -188,7 +196,7 @@ template <int F> __device__ __forceinline__ void x_starts(XChunk & x) {
 // xb: the block's 256 Q8_K integers in element order (global memory or LDS)
 template <int F, class P> __device__ __forceinline__ void load_x(P xb, int q, XChunk & x) {
     const uint32_t ones = 0x01010101u;
-    if constexpr (F == KF_Q5K) {
+    if constexpr (F == KF_Q4K || F == KF_Q5K) {
         const int jj = q >> 1, hf = q & 1;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -216,7 +224,7 @@ template <int F, class P> __device__ __forceinline__ void load_x(P xb, int q, XC
 // 24 signed bits (scales and mins <= 8 bits, piece dots |.| < 2^17), so the products use the full-rate 24-bit multiply.
 template <int F> __device__ __forceinline__ void chunk_dot(const Chunk & k, const XChunk & x, int & isum, int & summ) {
     isum = 0; summ = 0;
-    if constexpr (F == KF_Q5K) {
+    if constexpr (F == KF_Q4K || F == KF_Q5K) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             int dp = 0;

@@ -246,11 +246,34 @@ struct KqArgs {
     const uint8_t * w2; float * out2;    // act == null: a second matrix of the same shape and format on the same rows
                                          // (workgroup row y = 1), e.g. the shared expert's up beside its gate
 };
-// block bytes of a K-quant format code (FL_Q2K 84, FL_Q3K 110, FL_Q5K 176, FL_Q6K 210; 0 = not a K-quant)
+// block bytes of a K-quant format code (FL_Q2K 84, FL_Q3K 110, FL_Q4K 144, FL_Q5K 176, FL_Q6K 210; 0 = not a K-quant)
 int kq_block_bytes(int fmt);
 // max_slots sizes the token groups (a bound or the expected slots of one expert; more run as extra groups);
 // grid_experts >= *nact
 hipError_t launch_kq_matvec(const KqArgs & a, int fmt, int max_slots, int grid_experts, hipStream_t st);
+// the Q4_K products behind it (q4k.hip): any n, K <= 65536
+hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStream_t st);
+
+// ---------------------------------------------------------------- the router's training side (balance.hip, route_grad.hip)
+// Rows of sequence s: seq[s] .. seq[s + 1] - 1 (device offsets, clamped to 0 .. n; null: one sequence of all n rows).
+struct BalanceArgs {
+    const float * logits; const int * sel; const int * seq;
+    int n, nseq, n_exp, topk; float alpha;
+    int chunks;                          // workgroups per sequence (balance_chunks)
+    float * part; int * pcnt;            // chunks > 1: [nseq][chunks][n_exp] partial sums of p and counts
+    int * counts; float * loss;          // [nseq][n_exp], [nseq]
+    const float * gloss; int accumulate; float * dlogits;   // the gradient: of each sequence's loss (null: ones), += or =
+};
+int balance_chunks(int n, int nseq);
+hipError_t launch_balance(const BalanceArgs & a, hipStream_t st);
+hipError_t launch_balance_grad(const BalanceArgs & a, hipStream_t st);
+struct RouteGradArgs {
+    const float * W, * x, * logits; const int * sel; const float * dw; const float * dz_in;   // (dw, dz_in may be null)
+    int n, n_exp, E, topk; float scale;
+    float * dz;                          // [n][n_exp], may be dz_in
+    float * dW; int accumulate; float * dx;   // [n_exp][E] (= or +=), [n][E]; may be null
+};
+hipError_t launch_route_grad(const RouteGradArgs & a, hipStream_t st);
 // h = silu(g) * u, element-wise under the exp contract
 hipError_t launch_swiglu(const float * g, const float * u, int64_t n, float * h, hipStream_t st);
 // the same h for nrows rows of K (K % 256 == 0) and its Q8_K (q [nrows][K], d [nrows][K/256]) in one pass

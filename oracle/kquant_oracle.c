@@ -9,18 +9,21 @@
  *   Q2_K: sumf += dall * isum - dmin * summs per block;
  *   Q3_K, Q6_K: sums[l] += d * aux32[l] per block (l = 0..7), then sumf = sums[0] + .. + sums[7] in order;
  *   Q5_K: as Q3_K / Q6_K, with sumf -= dmin * sumi per block before the final sums[l] are added.
- * Block layouts (bytes): Q2_K 84 = scales[16] qs[64] d dmin; Q3_K 110 = hmask[32] qs[64] scales[12] d;
+ *   Q4_K (the reference's attention and dense-layer format): the library's own chain, term = fma(-dmin, summ, d * isum),
+ *         sumf = fma(d8, term, sumf) per block, which ggml's 8 partial sums differ from by fp32 rounding only.
+ * Block layouts (bytes): Q4_K 144 = d dmin scales[12] qs[128]; Q2_K 84 = scales[16] qs[64] d dmin; Q3_K 110 = hmask[32] qs[64] scales[12] d;
  * Q5_K 176 = d dmin scales[12] qh[32] qs[128]; Q6_K 210 = ql[128] qh[64] scales[16] d.
  *
  * Build: gcc -O3 -fopenmp -ffp-contract=off (see Makefile).
  */
 #include "moe_oracle.h"
+#include <math.h>
 #include <string.h>
 
 #define QK_K 256
 
 int or_kq_block_bytes(int fmt) {
-    switch (fmt) { case OR_Q2K: return 84; case OR_Q3K: return 110; case OR_Q5K: return 176; case OR_Q6K: return 210; default: return 0; }
+    switch (fmt) { case OR_Q4K: return 144; case OR_Q2K: return 84; case OR_Q3K: return 110; case OR_Q5K: return 176; case OR_Q6K: return 210; default: return 0; }
 }
 static float h16(const uint8_t * p) { return or_fp16_to_fp32((uint16_t) (p[0] | (p[1] << 8))); }
 
@@ -69,6 +72,13 @@ static void kq_unpack(int fmt, const uint8_t * b, int8_t * q, int * sc, int * mn
                 m = (uint8_t) (m << 1);
             }
         }
+    } else if (fmt == OR_Q4K) {
+        const uint8_t * scales = b + 4, * ql = b + 16;
+        *d = h16(b); *dmin = h16(b + 2);
+        for (int j = 0; j < 8; ++j) { uint8_t s, m; scale_min_k4(j, scales, &s, &m); sc[j] = s; mn[j] = m; }
+        for (int j = 0; j < 4; ++j) {
+            for (int l = 0; l < 32; ++l) { q[64 * j + l] = (int8_t) (ql[32 * j + l] & 0xF); q[64 * j + 32 + l] = (int8_t) (ql[32 * j + l] >> 4); }
+        }
     } else if (fmt == OR_Q5K) {
         const uint8_t * scales = b + 4, * qh = b + 16, * ql = b + 48;
         *d = h16(b); *dmin = h16(b + 2);
@@ -103,7 +113,7 @@ void or_dequantize_row_kq(int fmt, const uint8_t * blocks, float * y, int64_t k)
         kq_unpack(fmt, blocks + i * bs, q, sc, mn, &d, &dmin);
         for (int e = 0; e < QK_K; ++e) {
             float v;
-            if (fmt == OR_Q5K) { const int j = e / 32; v = (d * (float) sc[j]) * (float) q[e] - dmin * (float) mn[j]; }
+            if (fmt == OR_Q4K || fmt == OR_Q5K) { const int j = e / 32; v = (d * (float) sc[j]) * (float) q[e] - dmin * (float) mn[j]; }
             else if (fmt == OR_Q2K) { const int j = e / 16; v = (d * (float) sc[j]) * (float) q[e] - dmin * (float) mn[j]; }
             else { const int j = e / 16; v = (d * (float) sc[j]) * (float) q[e]; }
             y[i * QK_K + e] = v;
@@ -119,7 +129,15 @@ float or_vec_dot_kq_q8_K(int fmt, int64_t k, const uint8_t * w, const int8_t * q
         int8_t a[QK_K]; int sc[16], mn[16]; float d, dmin;
         kq_unpack(fmt, w + i * bs, a, sc, mn, &d, &dmin);
         const int8_t * x = q8 + i * QK_K; const int16_t * bsm = bsums + i * 16;
-        if (fmt == OR_Q2K) {
+        if (fmt == OR_Q4K) {
+            int isum = 0, summ = 0;
+            for (int j = 0; j < 8; ++j) {
+                int dot = 0;
+                for (int l = 0; l < 32; ++l) { dot += x[32 * j + l] * a[32 * j + l]; }
+                isum += sc[j] * dot; summ += mn[j] * (bsm[2 * j] + bsm[2 * j + 1]);
+            }
+            sumf = fmaf(d8[i], fmaf(-dmin, (float) summ, d * (float) isum), sumf);
+        } else if (fmt == OR_Q2K) {
             int summs = 0, isum = 0;
             for (int j = 0; j < 16; ++j) { summs += bsm[j] * mn[j]; }
             for (int j = 0; j < 16; ++j) { int isuml = 0; for (int l = 0; l < 16; ++l) { isuml += x[16 * j + l] * a[16 * j + l]; } isum += sc[j] * isuml; }
@@ -141,7 +159,7 @@ float or_vec_dot_kq_q8_K(int fmt, int64_t k, const uint8_t * w, const int8_t * q
             }
         }
     }
-    if (fmt != OR_Q2K) { for (int l = 0; l < 8; ++l) { sumf += sums[l]; } }
+    if (fmt != OR_Q2K && fmt != OR_Q4K) { for (int l = 0; l < 8; ++l) { sumf += sums[l]; } }
     return sumf;
 }
 

@@ -69,7 +69,7 @@ int or_moe_experts(const float * x, int64_t n, int64_t E, int64_t H, int topk, c
 void or_rmsnorm(const float * x, const float * w, float * y, int64_t n, int64_t d, float eps);
 
 /* K-quant formats of the reference's real shards (kquant_oracle.c) */
-enum { OR_Q2K = 5, OR_Q3K = 6, OR_Q5K = 3, OR_Q6K = 1, OR_IQ2 = 4 };   /* the FL_* codes of include/loki_moe.h */
+enum { OR_Q4K = 0, OR_Q2K = 5, OR_Q3K = 6, OR_Q5K = 3, OR_Q6K = 1, OR_IQ2 = 4 };   /* the FL_* codes of include/loki_moe.h */
 int or_kq_block_bytes(int fmt);
 void or_dequantize_row_kq(int fmt, const uint8_t * blocks, float * y, int64_t k);
 float or_vec_dot_kq_q8_K(int fmt, int64_t k, const uint8_t * w, const int8_t * q8, const float * d8, const int16_t * bsums);

@@ -110,7 +110,7 @@ def quantize_q8k(x):
 
 
 # K-quant formats (kquant_oracle.c): the FL_* codes of include/loki_moe.h
-Q2K, Q3K, Q5K, Q6K = 5, 6, 3, 1
+Q4K, Q2K, Q3K, Q5K, Q6K = 0, 5, 6, 3, 1
 
 
 def kq_block_bytes(fmt):
