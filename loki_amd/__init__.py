@@ -237,7 +237,7 @@ def exported_symbols():
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()   # (the declared argument types take an address as it is)
 
 
 def iq2_matrix_bytes(rows, cols):

@@ -131,7 +131,7 @@ extern "C" void fl_free(FLCtx * c) {
     c->tab.release(); c->derr.release(); c->dlogit.release(); c->dth.release(); c->dto.release(); c->dxq.release();
     c->ptab.release(); c->pcols.release(); c->pcolsk.release(); c->pncols.release(); c->xh.release(); c->hh.release();
     c->ksg.release(); c->ksu.release(); c->rcnt.release(); c->rpart.release(); c->dscr.release();
-    c->bal.release(); c->rg.release();
+    c->bal.release(); c->rg.release(); c->q4.release();
     for (auto & v : c->ev_free) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto & v : c->ev_pending) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto * l : { &c->ffn_ev_pending, &c->ffn_ev_free, &c->moe_ev_pending, &c->moe_ev_free }) { for (auto & e : *l) { (void) hipEventDestroy(e.first); (void) hipEventDestroy(e.second); } }
@@ -278,6 +278,14 @@ extern "C" int fl_quant_q8k_dev(FLCtx * c, const float * x, int nrows, int K, in
     return FL_OK;
 }
 
+// Q4_K products of many rows take a scratch (their rows' sub-block sums)
+static int q4_scratch(FLCtx * c, KqArgs & k, int fmt) {
+    const size_t bytes = fmt == FL_Q4K ? q4k_scratch_bytes(k.n, k.w2 ? 2 * k.R : k.R, k.K) : 0;
+    if (bytes == 0) { return FL_OK; }
+    if (c->q4.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
+    k.xs = c->q4.p;
+    return FL_OK;
+}
 extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y) {
     if (!c) { return FL_EINVAL; }
     const int bs = kq_block_bytes(fmt);
@@ -294,6 +302,7 @@ extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K
     KqArgs a{};
     a.w = (const uint8_t *) w; a.estride = mb; a.aq = q; a.ad = d; a.K = K; a.R = R;
     a.act = nullptr; a.nact = nullptr; a.offsets = nullptr; a.n = n; a.out = y; a.ldo = R;
+    if (int rc = q4_scratch(c, a, fmt)) { return rc; }
     TRY(c, launch_kq_matvec(a, fmt, n, 1, c->st));
     return FL_OK;
 }

@@ -1,6 +1,7 @@
 // launch_rules.h -- which kernel a call's sizes get: plain functions of the sizes, without HIP, so that a CPU test can hold
 // them against each other (tests/test_launch_rules.py).
 #pragma once
+#include <stdint.h>
 
 namespace lk {
 
@@ -43,5 +44,18 @@ constexpr int split_shared_tok(int n, int P) { return P > 0 ? SPLIT_TOK : n <= 8
 // the K-quant shared expert's columns: enough (column, 128 rows) items of its gate and up for the 256 CUs (at 201 tokens
 // 64-slot columns are 128 items in two launches, 32-slot ones 224 in one)
 constexpr int kq_shared_tok(int n) { return n <= 128 ? 16 : n <= 256 ? 32 : KQ_TOK; }
+
+// ---------------------------------------------------------------- Q4_K products (q4k.hip)
+// Every kernel gives the same bits; which one is faster goes by tokens, rows and blocks a row. The mat-vecs take one row at a time (n = 1,
+// or 2 through a matrix with rows enough), the K-split ones 16 or 32 rows and up to 32 tokens a workgroup, the tiled ones rows x tokens.
+enum { Q4_VEC1, Q4_VEC2, Q4_KS_1_1, Q4_KS_2_1, Q4_KS_2_2, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_256_128 };
+constexpr int q4k_kernel(int n, int R, int K, bool tiles) {
+    if (n <= 1 && (K <= 8192 || R >= 32768)) { return Q4_VEC1; }
+    if (n == 2 && R >= 32768) { return Q4_VEC2; }
+    if (n <= 16) { return R >= 6144 ? Q4_KS_2_1 : Q4_KS_1_1; }
+    if (n <= 32 || !tiles) { return Q4_KS_2_2; }
+    auto enough = [&](int rows, int toks) { return (int64_t) ((R + rows - 1) / rows) * ((n + toks - 1) / toks) >= 384; };
+    return enough(256, 128) ? Q4_MM_256_128 : enough(128, 64) ? Q4_MM_128_64 : enough(64, 64) && n > 32 ? Q4_MM_64_64 : Q4_MM_64_32;
+}
 
 }  // namespace lk

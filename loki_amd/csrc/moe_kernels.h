@@ -245,6 +245,7 @@ struct KqArgs {
     int rw;                              // rows per workgroup tile (set by launch_kq_matvec)
     const uint8_t * w2; float * out2;    // act == null: a second matrix of the same shape and format on the same rows
                                          // (workgroup row y = 1), e.g. the shared expert's up beside its gate
+    void * xs;                           // Q4_K: scratch of q4k_scratch_bytes (null: the kernels without one)
 };
 // block bytes of a K-quant format code (FL_Q2K 84, FL_Q3K 110, FL_Q4K 144, FL_Q5K 176, FL_Q6K 210; 0 = not a K-quant)
 int kq_block_bytes(int fmt);
@@ -252,6 +253,7 @@ int kq_block_bytes(int fmt);
 // grid_experts >= *nact
 hipError_t launch_kq_matvec(const KqArgs & a, int fmt, int max_slots, int grid_experts, hipStream_t st);
 // the Q4_K products behind it (q4k.hip): any n, K <= 65536
+size_t q4k_scratch_bytes(int n, int R, int K);   // R: rows of all matrices of the call
 hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStream_t st);
 
 // ---------------------------------------------------------------- the router's training side (balance.hip, route_grad.hip)
