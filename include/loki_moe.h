@@ -177,7 +177,9 @@ int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, 
  *   dlogits [n][n_exp] = dz + the part through w (may be dz's own buffer),
  *   dW [n_exp][E] = (accumulate: +=) dlogits^T x,   dx [n][E] = dlogits W
  * (each of the three may be NULL: not computed). logits and sel are fl_route_dev's; the bias has no gradient; entries of sel
- * outside 0 .. n_exp - 1 are skipped. n <= 65536, E a multiple of 1024 up to 65536. Deterministic, no atomics. */
+ * outside 0 .. n_exp - 1 are skipped. n <= 65536, E a multiple of 1024 up to 65536, dW and dx 16-byte aligned. Deterministic, no
+ * atomics. The products are exact to about 2^-22 of each term (route_grad.hip); the operands' split copies are the context's, n *
+ * n_exp * 8 + n_exp * E * 4 bytes and dW's partial sums, kept until fl_free. */
 int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
 /* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device) */

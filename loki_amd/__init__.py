@@ -446,7 +446,7 @@ class Context:
     def _need(self, who, *args):
         """Each (tensor, dtype, shape): contiguous on the GPU as the library reads it (None passes)."""
         for t, dtype, shape in args:
-            if t is not None and (t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or not t.is_cuda):
+            if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda):
                 raise LokiError("%s: a contiguous %s tensor of shape %s on the GPU is needed, not %s %s on %s" %
                                 (who, dtype, shape, t.dtype, tuple(t.shape), t.device))
 

@@ -9,13 +9,16 @@
 #include "moe_kernels.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lk {
 
 namespace {
 
-constexpr int BL_W = 16, BL_T = BL_W * 64;   // waves / threads per workgroup: a wave takes a row at a time
-constexpr int BL_ROWS = 128;                 // rows per workgroup that a sequence is cut into, at least
+#pragma clang fp contract(fast)   // (no bit contract here: fewer and larger steps)
+
+constexpr int BL_B = 4;                      // rows a wave takes at a time: their loads and reductions overlap
+constexpr int BL_JOIN = 1024;                // threads of the joining workgroups
 constexpr float BL_TINY = 1e-10f;            // a row's sigmoid sum below which 1 + exp(-z) is exp(-z) to fp32 in every column
 
 template <int CTRL> __device__ __forceinline__ float dppf(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v))); }
@@ -34,33 +37,67 @@ __device__ __forceinline__ void bl_rows(const BalanceArgs & g, int s, int c, int
     int lo = 0, hi = g.n;
     if (g.seq) { lo = min(max(g.seq[s], 0), g.n); hi = min(max(g.seq[s + 1], lo), g.n); }
     T = hi - lo;
-    a = lo + (int) ((int64_t) T * c / g.chunks); b = lo + (int) ((int64_t) T * (c + 1) / g.chunks);
+    const int per = (int) (((uint32_t) T + (uint32_t) g.chunks - 1) / (uint32_t) g.chunks);   // (T <= 2^24)
+    a = min(lo + per * c, hi); b = min(a + per, hi);
 }
 
-// a row's sigmoids: lane l holds the columns e = l + 64 j. q: the sigmoids (or their scaled stand-ins), om: 1 - sigmoid;
-// returns 1 / sum q (0 where the row is all -inf)
-template <int J> __device__ __forceinline__ float bl_sigmoids(const float (&z)[J], float (&q)[J], float (&om)[J]) {
-    float sum = 0.f;
+// exp(x) for x <= 0: 2^h with h = x log2 e rounded, times what the rounding left out (v_exp_f32 and two products: 3 half steps
+// of fp32; below 2^-126 the result is 0)
+__device__ __forceinline__ float bl_exp(float x) {
+    const float h = x * 0x1.715476p+0f, l = __builtin_fmaf(x, 0x1.715476p+0f, -h) + x * 0x1.4ae0cp-26f;
+    const float p = __builtin_amdgcn_exp2f(h);
+    return x < -126.f ? 0.f : __builtin_fmaf(p, l * 0x1.62e43p-1f, p);
+}
+
+// B rows' columns: lane l holds the columns e = l + 64 j of row t0 + i (rows from `end` on: the last row again, for the caller to
+// leave out; columns past n_exp: -inf). The last columns' mask is opaque to the compiler, which would otherwise put each load
+// behind a branch and wait for it there.
+template <int J, int B> __device__ __forceinline__ void bl_load(const BalanceArgs & g, int t0, int end, float (&z)[B][J]) {
+    const int lane = lane_id();
+    uint32_t off = lane + 64 * (J - 1) < g.n_exp ? 0u : ~0u;
+    __asm__ volatile("" : "+v"(off));
+    const uint32_t last = (uint32_t) min(lane + 64 * (J - 1), g.n_exp - 1);
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const float t = expf(-fabsf(z[j])), r = 1.f / (1.f + t);
-        q[j] = z[j] >= 0.f ? r : t * r;
-        om[j] = z[j] >= 0.f ? t * r : r;
-        sum += q[j];
+    for (int i = 0; i < B; ++i) {
+        const float * row = g.logits + (size_t) min(t0 + i, end - 1) * g.n_exp;
+#pragma unroll
+        for (int j = 0; j < J - 1; ++j) { z[i][j] = row[lane + 64 * j]; }
+        z[i][J - 1] = row[last];
     }
-    sum = wave_sum(sum);
-    if (sum < BL_TINY) {
-        float m = z[0];
 #pragma unroll
-        for (int j = 1; j < J; ++j) { m = fmaxf(m, z[j]); }
-        m = wave_maxf(m);
-        if (m == -INFINITY) { return 0.f; }
-        sum = 0.f;
+    for (int i = 0; i < B; ++i) { z[i][J - 1] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, z[i][J - 1]) & ~off) | (0xff800000u & off)); }
+}
+// their sigmoids q (or the scaled stand-ins), om = 1 - sigmoid, and inv = 1 / sum q (0 where the row is all -inf)
+template <int J, int B> __device__ __forceinline__ void bl_sigmoids(const float (&z)[B][J], float (&q)[B][J], float (&om)[B][J], float (&inv)[B]) {
+    float sum[B];
 #pragma unroll
-        for (int j = 0; j < J; ++j) { q[j] = expf(z[j] - m); sum += q[j]; }
-        sum = wave_sum(sum);
+    for (int i = 0; i < B; ++i) {
+        sum[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const float t = bl_exp(-fabsf(z[i][j])), r = __builtin_amdgcn_rcpf(1.f + t), tr = t * r;
+            q[i][j] = z[i][j] >= 0.f ? r : tr;
+            om[i][j] = z[i][j] >= 0.f ? tr : r;
+            sum[i] += q[i][j];
+        }
     }
-    return 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < B; ++i) { sum[i] = wave_sum(sum[i]); }
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+        inv[i] = __builtin_amdgcn_rcpf(sum[i]);
+        if (sum[i] < BL_TINY) {
+            float m = z[i][0];
+#pragma unroll
+            for (int j = 1; j < J; ++j) { m = fmaxf(m, z[i][j]); }
+            m = wave_maxf(m);
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) { q[i][j] = m == -INFINITY ? 0.f : bl_exp(z[i][j] - m); s += q[i][j]; }
+            s = wave_sum(s);
+            inv[i] = m == -INFINITY ? 0.f : __builtin_amdgcn_rcpf(s);
+        }
+    }
 }
 
 // f_e from a count (exact below 2^24)
@@ -79,13 +116,14 @@ __device__ __forceinline__ void bl_finish(const BalanceArgs & g, int s, int T, f
     __syncthreads();
     if (threadIdx.x == 0) {
         float tot = 0.f;
-        for (int w = 0; w < NEXP_MAX / 64; ++w) { tot += scr[w]; }
+        for (int w = 0; w < NEXP_MAX / 64; ++w) { tot += scr[w]; }   // (the waves that hold experts)
         g.loss[s] = g.alpha * tot;
     }
 }
 
-template <int J>
-__global__ void __launch_bounds__(BL_T) k_balance(BalanceArgs g) {
+template <int J, int BL_W>
+__global__ void __launch_bounds__(64 * BL_W) k_balance(BalanceArgs g) {
+    constexpr int BL_T = 64 * BL_W;
     __shared__ float s_p[BL_W][64 * J];
     __shared__ int s_c[NEXP_MAX];
     __shared__ float s_f[BL_W];
@@ -101,13 +139,17 @@ __global__ void __launch_bounds__(BL_T) k_balance(BalanceArgs g) {
     float acc[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) { acc[j] = 0.f; }
-    for (int t = a + w; t < b; t += BL_W) {
-        float z[J], q[J], om[J];
+    for (int t = a + __builtin_amdgcn_readfirstlane(w) * BL_B; t < b; t += BL_W * BL_B) {
+        float z[BL_B][J], q[BL_B][J], om[BL_B][J], inv[BL_B];
+        bl_load<J, BL_B>(g, t, b, z);
+        bl_sigmoids<J, BL_B>(z, q, om, inv);
 #pragma unroll
-        for (int j = 0; j < J; ++j) { const int e = lane + 64 * j; z[j] = e < ne ? g.logits[(size_t) t * ne + e] : -INFINITY; }
-        const float inv = bl_sigmoids<J>(z, q, om);
+        for (int i = 0; i < BL_B; ++i) {
+            if (t + i < b) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) { acc[j] += q[j] * inv; }
+                for (int j = 0; j < J; ++j) { acc[j] += q[i][j] * inv[i]; }
+            }
+        }
     }
 #pragma unroll
     for (int j = 0; j < J; ++j) { s_p[w][lane + 64 * j] = acc[j]; }
@@ -126,10 +168,10 @@ __global__ void __launch_bounds__(BL_T) k_balance(BalanceArgs g) {
 }
 
 // chunks > 1: a sequence's sums over its chunks, four slices of them side by side and then in order, and its loss
-__global__ void __launch_bounds__(BL_T) k_balance_join(BalanceArgs g) {
+__global__ void __launch_bounds__(BL_JOIN) k_balance_join(BalanceArgs g) {
     __shared__ float s_p[4][NEXP_MAX];
     __shared__ int s_c[4][NEXP_MAX];
-    __shared__ float s_f[BL_W];
+    __shared__ float s_f[BL_JOIN / 64];
     const int s = blockIdx.x, e = threadIdx.x & 255, k = threadIdx.x >> 8;
     int a, b, T;
     bl_rows(g, s, 0, a, b, T);
@@ -148,8 +190,9 @@ __global__ void __launch_bounds__(BL_T) k_balance_join(BalanceArgs g) {
     bl_finish(g, s, T, k == 0 ? psum : 0.f, cnt, s_f);
 }
 
-template <int J>
-__global__ void __launch_bounds__(BL_T) k_balance_grad(BalanceArgs g) {
+template <int J, int BL_W>
+__global__ void __launch_bounds__(64 * BL_W) k_balance_grad(BalanceArgs g) {
+    constexpr int BL_T = 64 * BL_W;
     const int s = blockIdx.y, lane = lane_id(), w = threadIdx.x >> 6, ne = g.n_exp;
     if (s == g.nseq) {   // rows of no sequence: their gradient is 0
         const int64_t lo = min(max(g.seq[0], 0), g.n), hi = min(max(g.seq[g.nseq], 0), g.n);
@@ -166,22 +209,29 @@ __global__ void __launch_bounds__(BL_T) k_balance_grad(BalanceArgs g) {
     float f[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) { const int e = lane + 64 * j; f[j] = e < ne ? bl_f(g.counts[(size_t) s * ne + e], g, T) : 0.f; }
-    for (int t = a + w; t < b; t += BL_W) {
-        float z[J], q[J], om[J];
+    for (int t = a + __builtin_amdgcn_readfirstlane(w) * BL_B; t < b; t += BL_W * BL_B) {
+        float z[BL_B][J], q[BL_B][J], om[BL_B][J], inv[BL_B], d[BL_B];
+        bl_load<J, BL_B>(g, t, b, z);
+        bl_sigmoids<J, BL_B>(z, q, om, inv);
 #pragma unroll
-        for (int j = 0; j < J; ++j) { const int e = lane + 64 * j; z[j] = e < ne ? g.logits[(size_t) t * ne + e] : -INFINITY; }
-        const float inv = bl_sigmoids<J>(z, q, om);
-        float d = 0.f;
+        for (int i = 0; i < BL_B; ++i) {
+            d[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < J; ++j) { d += f[j] * q[j]; }
-        d = wave_sum(d) * inv;
+            for (int j = 0; j < J; ++j) { d[i] += f[j] * q[i][j]; }
+        }
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const int e = lane + 64 * j;
-            if (e < ne) {
-                float * o = g.dlogits + (size_t) t * ne + e;
-                const float v = (k * (q[j] * inv)) * (om[j] * (f[j] - d));
-                *o = g.accumulate ? *o + v : v;
+        for (int i = 0; i < BL_B; ++i) { d[i] = wave_sum(d[i]) * inv[i]; }
+#pragma unroll
+        for (int i = 0; i < BL_B; ++i) {
+            if (t + i < b) {
+                float * o = g.dlogits + (size_t) (t + i) * ne + lane;
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    if (j < J - 1 || lane + 64 * j < ne) {
+                        const float v = (k * (q[i][j] * inv[i])) * (om[i][j] * (f[j] - d[i]));
+                        o[64 * j] = g.accumulate ? o[64 * j] + v : v;
+                    }
+                }
             }
         }
     }
@@ -189,35 +239,52 @@ __global__ void __launch_bounds__(BL_T) k_balance_grad(BalanceArgs g) {
 
 }  // namespace
 
-int balance_chunks(int n, int nseq) {
-    return std::max(1, std::min((int) (((int64_t) n + (int64_t) nseq * BL_ROWS - 1) / ((int64_t) nseq * BL_ROWS)), 256 / nseq));
+// Waves of a workgroup (a batch of BL_B rows each at a time) and workgroups a sequence, for the sums and for the gradient, which has
+// nothing to join. One sequence of 4100 rows: 4 waves 23.2 us (257 partial sums to join), 16 waves 10.8; 128 rows in one workgroup of
+// 16 waves 7.0, cut in 8 of 4 waves 10.2. The gradient of 4100 rows: 4 waves 5.5, 16 waves 6.4; of 16384 11.4 and 8.8.
+static int balance_waves(int n, bool grad) { return grad && n <= 8192 ? 4 : 16; }
+static int chunks_of(int n, int nseq, bool grad) {
+    const int w = balance_waves(n, grad), rows = w * BL_B, most = w == 4 ? BALANCE_PARTS : BALANCE_PARTS / 2;
+    if (!grad && n <= 128 * nseq) { return 1; }
+    return std::max(1, std::min({ (int) (((int64_t) n + (int64_t) nseq * rows - 1) / ((int64_t) nseq * rows)), most / nseq, 256 }));
+}
+int balance_chunks(int n, int nseq) { return chunks_of(n, nseq, false); }
+
+template <class F> static hipError_t by_shape(const BalanceArgs & a, bool grad, F && go) {
+    const int j = (a.n_exp + 63) / 64;
+    if (balance_waves(a.n, grad) == 4) {
+        switch (j) {
+        case 1: go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}); break;
+        case 2: go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}, std::integral_constant<int, 4>{}); break;
+        default: go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}); break;
+        }
+    } else {
+        switch (j) {
+        case 1: go(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}); break;
+        case 2: go(std::integral_constant<int, 2>{}, std::integral_constant<int, 16>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}, std::integral_constant<int, 16>{}); break;
+        default: go(std::integral_constant<int, 4>{}, std::integral_constant<int, 16>{}); break;
+        }
+    }
+    return hipGetLastError();
 }
 
 hipError_t launch_balance(const BalanceArgs & a, hipStream_t st) {
     if (a.n < 0 || a.nseq < 1 || a.nseq > 65535 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.topk < 1 || a.chunks < 1 || (!a.seq && a.nseq != 1)) { return hipErrorInvalidValue; }
-    const dim3 grid(a.chunks, a.nseq);
-    switch ((a.n_exp + 63) / 64) {
-    case 1: k_balance<1><<<grid, BL_T, 0, st>>>(a); break;
-    case 2: k_balance<2><<<grid, BL_T, 0, st>>>(a); break;
-    case 3: k_balance<3><<<grid, BL_T, 0, st>>>(a); break;
-    default: k_balance<4><<<grid, BL_T, 0, st>>>(a); break;
-    }
-    if (const hipError_t e = hipGetLastError()) { return e; }
-    if (a.chunks > 1) { k_balance_join<<<a.nseq, BL_T, 0, st>>>(a); }
+    const hipError_t e = by_shape(a, false, [&](auto j, auto w) { k_balance<decltype(j)::value, decltype(w)::value><<<dim3(a.chunks, a.nseq), 64 * decltype(w)::value, 0, st>>>(a); });
+    if (e != hipSuccess || a.chunks == 1) { return e; }
+    k_balance_join<<<a.nseq, BL_JOIN, 0, st>>>(a);
     return hipGetLastError();
 }
 
-hipError_t launch_balance_grad(const BalanceArgs & a, hipStream_t st) {
+hipError_t launch_balance_grad(const BalanceArgs & args, hipStream_t st) {
+    BalanceArgs a = args;
+    a.chunks = chunks_of(a.n, std::max(1, a.nseq), true);
     if (a.n < 0 || a.nseq < 1 || a.nseq >= 65535 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.topk < 1 || a.chunks < 1 || (!a.seq && a.nseq != 1)) { return hipErrorInvalidValue; }
     if (a.n == 0) { return hipSuccess; }
     const dim3 grid(a.chunks, a.nseq + (a.seq && !a.accumulate ? 1 : 0));
-    switch ((a.n_exp + 63) / 64) {
-    case 1: k_balance_grad<1><<<grid, BL_T, 0, st>>>(a); break;
-    case 2: k_balance_grad<2><<<grid, BL_T, 0, st>>>(a); break;
-    case 3: k_balance_grad<3><<<grid, BL_T, 0, st>>>(a); break;
-    default: k_balance_grad<4><<<grid, BL_T, 0, st>>>(a); break;
-    }
-    return hipGetLastError();
+    return by_shape(a, true, [&](auto j, auto w) { k_balance_grad<decltype(j)::value, decltype(w)::value><<<grid, 64 * decltype(w)::value, 0, st>>>(a); });
 }
 
 }  // namespace lk

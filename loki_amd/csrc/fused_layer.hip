@@ -280,7 +280,7 @@ extern "C" int fl_quant_q8k_dev(FLCtx * c, const float * x, int nrows, int K, in
 
 // Q4_K products of many rows take a scratch (their rows' sub-block sums)
 static int q4_scratch(FLCtx * c, KqArgs & k, int fmt) {
-    const size_t bytes = fmt == FL_Q4K ? q4k_scratch_bytes(k.n, k.w2 ? 2 * k.R : k.R, k.K) : 0;
+    const size_t bytes = fmt == FL_Q4K ? q4k_scratch_bytes(k.n, (int64_t) k.R * (k.w2 ? 2 : 1), k.K) : 0;
     if (bytes == 0) { return FL_OK; }
     if (c->q4.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
     k.xs = c->q4.p;
@@ -336,9 +336,9 @@ extern "C" int fl_balance_loss_dev(FLCtx * c, const float * logits, const int * 
     if (int rc = balance_args(c, b)) { return rc; }
     if (!loss || (n > 0 && !sel)) { return fail(c, FL_EINVAL, "null pointer"); }
     if ((n > 0 && !covers(sel, (size_t) n * topk * 4)) || !covers(loss, (size_t) nseq * 4)) { return fail(c, FL_EINVAL, "sel's or loss's allocation is smaller than its shape"); }
-    if (b.chunks > 1) {   // (at most 256 workgroups then: the workspace never grows)
-        if (c->bal.ensure((size_t) 256 * NEXP_MAX * 8) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
-        b.part = (float *) c->bal.p; b.pcnt = (int *) c->bal.p + 256 * NEXP_MAX;
+    if (b.chunks > 1) {   // (the workspace has one size)
+        if (c->bal.ensure((size_t) BALANCE_PARTS * NEXP_MAX * 8) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
+        b.part = (float *) c->bal.p; b.pcnt = (int *) c->bal.p + BALANCE_PARTS * NEXP_MAX;
     }
     TRY(c, launch_balance(b, c->st));
     return FL_OK;
@@ -368,6 +368,7 @@ extern "C" int fl_route_grad_dev(FLCtx * c, const float * W, const float * x, co
     if (n > 0 && ((dw && (!logits || !sel)) || (dW && !x) || (dx && !W))) { return fail(c, FL_EINVAL, "null pointer"); }
     if (dx && (dx == x || dx == W || dx == dW)) { return fail(c, FL_EINVAL, "dx must not be x, W or dW"); }
     if (dW && (dW == W || dW == x)) { return fail(c, FL_EINVAL, "dW must not be W or x"); }
+    if ((reinterpret_cast<uintptr_t>(dW) | reinterpret_cast<uintptr_t>(dx)) & 15u) { return fail(c, FL_EINVAL, "dW and dx must be 16-byte aligned"); }
     const size_t nz = (size_t) n * n_exp * 4, nx = (size_t) n * E * 4, nw = (size_t) n_exp * E * 4, nk = (size_t) n * c->topk * 4;
     if (n > 0 && ((dw && (!covers(logits, nz) || !covers(sel, nk) || !covers(dw, nk))) || (dz && !covers(dz, nz)) || (dlogits && !covers(dlogits, nz)) ||
                   (dW && !covers(x, nx)) || (dx && (!covers(W, nw) || !covers(dx, nx))))) {
@@ -378,11 +379,13 @@ extern "C" int fl_route_grad_dev(FLCtx * c, const float * W, const float * x, co
     RouteGradArgs a{};
     a.W = W; a.x = x; a.logits = logits; a.sel = sel; a.dw = dw; a.dz_in = dz; a.n = n; a.n_exp = n_exp; a.E = E; a.topk = c->topk; a.scale = c->scale;
     a.dz = dlogits; a.dW = dW; a.accumulate = accumulate ? 1 : 0; a.dx = dx;
-    if (!a.dz) {
-        if (c->rg.ensure(nz) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
-        a.dz = (float *) c->rg.p;
+    if (n == 0) {   // no rows: dW is 0, or stays
+        if (!accumulate) { k_zero16<<<512, 256, 0, c->st>>>(reinterpret_cast<uint4 *>(dW), nw / 16); TRY(c, hipGetLastError()); }
+        return FL_OK;
     }
-    TRY(c, launch_route_grad(a, c->st));
+    const size_t bytes = route_grad_scratch(n, n_exp, E, dW != nullptr, dx != nullptr);
+    if (c->rg.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
+    TRY(c, launch_route_grad(a, c->rg.p, c->st));
     return FL_OK;
 }
 

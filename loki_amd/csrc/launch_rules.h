@@ -46,16 +46,35 @@ constexpr int split_shared_tok(int n, int P) { return P > 0 ? SPLIT_TOK : n <= 8
 constexpr int kq_shared_tok(int n) { return n <= 128 ? 16 : n <= 256 ? 32 : KQ_TOK; }
 
 // ---------------------------------------------------------------- Q4_K products (q4k.hip)
-// Every kernel gives the same bits; which one is faster goes by tokens, rows and blocks a row. The mat-vecs take one row at a time (n = 1,
-// or 2 through a matrix with rows enough), the K-split ones 16 or 32 rows and up to 32 tokens a workgroup, the tiled ones rows x tokens.
-enum { Q4_VEC1, Q4_VEC2, Q4_KS_1_1, Q4_KS_2_1, Q4_KS_2_2, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_256_128 };
-constexpr int q4k_kernel(int n, int R, int K, bool tiles) {
-    if (n <= 1 && (K <= 8192 || R >= 32768)) { return Q4_VEC1; }
-    if (n == 2 && R >= 32768) { return Q4_VEC2; }
-    if (n <= 16) { return R >= 6144 ? Q4_KS_2_1 : Q4_KS_1_1; }
-    if (n <= 32 || !tiles) { return Q4_KS_2_2; }
-    auto enough = [&](int rows, int toks) { return (int64_t) ((R + rows - 1) / rows) * ((n + toks - 1) / toks) >= 384; };
-    return enough(256, 128) ? Q4_MM_256_128 : enough(128, 64) ? Q4_MM_128_64 : enough(64, 64) && n > 32 ? Q4_MM_64_64 : Q4_MM_64_32;
+// Every kernel gives the same bits; a call gets the one that should take least time. All but the mat-vec cut the output into workgroups
+// of rows x tokens, G of them, and with nb blocks a row a launch takes about
+//   max(s0 + s1 nb, ceil(G / 256) (p0 + p1 nb)) us:
+// what one workgroup needs from start to end, or the rounds of workgroups a CU goes through at its steady rate. The constants are
+// fitted to 223 sizes (512 .. 65536 rows, 4 .. 64 blocks, 4 .. 2000 tokens, weights from memory): 6 to 14 % rms a kernel, and
+// the pick is within 1.5 % of the best kernel on average. Examples, us: 40 tokens through 16384 -> 7168 39 (K split, 48
+// tokens a workgroup) against 46 (64 x 32 tiles), 59 (32 tokens, split); 128 through 7168 -> 16384 46 (128 x 64) against 51 (64 x 64)
+// and 75 (128 x 128); 2048 through it 485 (128 x 128) against 658 and 722.
+struct Q4Kernel { int rows, toks; float s0, s1, p0, p1; };
+enum { Q4_KS_16_16, Q4_KS_32_32, Q4_KS_32_48, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_128_128, Q4_KERNELS, Q4_VEC = Q4_KERNELS };
+constexpr Q4Kernel Q4_KERNEL[Q4_KERNELS] = {
+    { 16, 16, 3.8f, 0.13f, 1.1f, 0.14f }, { 32, 32, 4.1f, 0.37f, 2.9f, 0.39f }, { 32, 48, 4.7f, 0.48f, 3.5f, 0.50f }, { 64, 32, 5.8f, 0.62f, 1.5f, 0.58f },
+    { 64, 64, 5.1f, 0.90f, 1.9f, 0.77f }, { 128, 64, 5.5f, 1.28f, 4.2f, 1.32f }, { 128, 128, 6.5f, 2.33f, 4.0f, 2.15f } };
+constexpr float q4k_us(const Q4Kernel & k, int n, int64_t R, int K) {
+    const int64_t g = (R + k.rows - 1) / k.rows * ((n + k.toks - 1) / k.toks), q = (g + 255) / 256;
+    const float nb = (float) (K / 256), one = k.s0 + k.s1 * nb, all = (float) q * (k.p0 + k.p1 * nb);
+    return one > all ? one : all;
 }
+// R: rows of all matrices of the call; tiles: the tiled kernels may be taken (their scratch is there). One token: the mat-vec for very
+// many rows (65536 of 7168: 51 us against 67) and for few (512 of 16384: 7.2 against 10.4), the K-split kernel between (7168 of 16384: 17.7
+// against 19.4).
+constexpr int q4k_kernel(int n, int64_t R, int K, bool tiles) {
+    if (n <= 1 && (R > 24576 || R <= 1024)) { return Q4_VEC; }
+    int best = Q4_KS_16_16;
+    for (int k = 1; k < (tiles && n > 16 ? (int) Q4_KERNELS : (int) Q4_MM_64_32); ++k) {   // (the tiled ones' times are of more than 16 tokens)
+        if (q4k_us(Q4_KERNEL[k], n, R, K) < q4k_us(Q4_KERNEL[best], n, R, K)) { best = k; }
+    }
+    return best;
+}
+constexpr bool q4k_tiled(int kernel) { return kernel >= Q4_MM_64_32 && kernel < Q4_KERNELS; }
 
 }  // namespace lk

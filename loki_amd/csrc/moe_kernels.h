@@ -253,7 +253,7 @@ int kq_block_bytes(int fmt);
 // grid_experts >= *nact
 hipError_t launch_kq_matvec(const KqArgs & a, int fmt, int max_slots, int grid_experts, hipStream_t st);
 // the Q4_K products behind it (q4k.hip): any n, K <= 65536
-size_t q4k_scratch_bytes(int n, int R, int K);   // R: rows of all matrices of the call
+size_t q4k_scratch_bytes(int n, int64_t R, int K);   // R: rows of all matrices of the call
 hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStream_t st);
 
 // ---------------------------------------------------------------- the router's training side (balance.hip, route_grad.hip)
@@ -266,16 +266,18 @@ struct BalanceArgs {
     int * counts; float * loss;          // [nseq][n_exp], [nseq]
     const float * gloss; int accumulate; float * dlogits;   // the gradient: of each sequence's loss (null: ones), += or =
 };
+constexpr int BALANCE_PARTS = 1024;   // nseq * chunks at most, where chunks > 1
 int balance_chunks(int n, int nseq);
 hipError_t launch_balance(const BalanceArgs & a, hipStream_t st);
 hipError_t launch_balance_grad(const BalanceArgs & a, hipStream_t st);
 struct RouteGradArgs {
     const float * W, * x, * logits; const int * sel; const float * dw; const float * dz_in;   // (dw, dz_in may be null)
     int n, n_exp, E, topk; float scale;
-    float * dz;                          // [n][n_exp], may be dz_in
+    float * dz;                          // [n][n_exp], may be dz_in or null
     float * dW; int accumulate; float * dx;   // [n_exp][E] (= or +=), [n][E]; may be null
 };
-hipError_t launch_route_grad(const RouteGradArgs & a, hipStream_t st);
+size_t route_grad_scratch(int n, int n_exp, int E, bool dW, bool dx);
+hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_t st);   // (n == 0: nothing is done)
 // h = silu(g) * u, element-wise under the exp contract
 hipError_t launch_swiglu(const float * g, const float * u, int64_t n, float * h, hipStream_t st);
 // the same h for nrows rows of K (K % 256 == 0) and its Q8_K (q [nrows][K], d [nrows][K/256]) in one pass

@@ -26,15 +26,14 @@ constexpr int V_NB = 256;               // blocks per row at most (K <= 65536)
 constexpr int v_wk(int nb) { return nb > 24 ? 4 : nb > 16 ? 3 : nb > 8 ? 2 : 1; }
 constexpr int v_wr(int nb) { return nb > 16 ? 1 : nb > 8 ? 2 : 4; }
 
-// Mat-vecs: a workgroup takes one expert, a tile of rows and that expert's slots in token groups of up to TT, whose Q8_K
-// columns it holds in registers. Lane = (block of 8, 32-weight slice of the block), so a wave reads 1152 consecutive bytes
-// of a row per pass; the next row's bytes are in flight while one is computed. Each block's term goes to LDS, one lane
-// per (row, token) then runs the chain.
-template <int TT>
+// Mat-vec: a workgroup takes one expert and a tile of rows, that expert's slots one after the other, whose Q8_K columns it holds in
+// registers. Lane = (block of 8, 32-weight slice of the block), so a wave reads 1152 consecutive bytes of a row per pass; the
+// next row's bytes are in flight while one is computed. Each block's term goes to LDS, one lane per row then runs the chain.
+// Bound by memory where the rows are many: one token through 131072 rows of 7168 94 us, 5.6 TB/s.
 __global__ void __launch_bounds__(256) k_q4k_vec(KqArgs a) {
 #pragma clang fp contract(off)
     constexpr int BS = 144;
-    extern __shared__ float s_lds[];   // terms [rw][TT][nbp], then block scales [TT][nbp]
+    extern __shared__ float s_lds[];   // terms [rw][nbp], then block scales [nbp]
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int e, s_beg, s_end;
     if (a.act) {
@@ -45,7 +44,7 @@ __global__ void __launch_bounds__(256) k_q4k_vec(KqArgs a) {
     const int tr0 = (int) blockIdx.x * a.rw;
     if (tr0 >= a.R || s_beg >= s_end) { return; }
     const int nrow = min(a.rw, a.R - tr0), nb = a.K / QK, nbp = nb | 1, npass = (nb + 7) / 8;
-    float * s_d = s_lds + a.rw * TT * nbp;
+    float * s_d = s_lds + a.rw * nbp;
     const int wk = v_wk(nb), wr = v_wr(nb), kw = wv % wk, rg = wv / wk, c = lane & 7;
     const uint32_t rowb = (uint32_t) (nb * BS);
     // the tile's rows: reads past them give 0 (a lane past the row's last block reads the next row's bytes, unused)
@@ -58,36 +57,21 @@ __global__ void __launch_bounds__(256) k_q4k_vec(KqArgs a) {
         const uint32_t lo = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) p);
         src.rs = __builtin_amdgcn_make_buffer_rsrc((void *) (((uint64_t) hi << 32) | lo), (short) 0, (int) ((uint32_t) nrow * rowb), 0x00020000);
     }
-    for (int sg = s_beg; sg < s_end; sg += TT) {
-        const int nt = min(TT, s_end - sg);
+    for (int t = s_beg; t < s_end; ++t) {
         for (int p = kw; p < npass; p += wk) {
             const int b = 8 * p + (lane >> 3);
             const bool active = b < nb;
-            XChunk xc[TT];
-#pragma unroll
-            for (int t = 0; t < TT; ++t) {
-                XChunk & x = xc[t];
-                if (active && t < nt) {
-                    load_x<KF_Q4K>(a.aq + (size_t) (sg + t) * a.K + 256 * b, c, x);
-                    if (c == 0 && rg == 0) { s_d[t * nbp + b] = a.ad[(size_t) (sg + t) * nb + b]; }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { x.x[i] = 0u; }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { x.c0[i] = 0; x.bx[i] = 0; }
-                }
+            XChunk x{};
+            if (active) {
+                load_x<KF_Q4K>(a.aq + (size_t) t * a.K + 256 * b, c, x);
+                if (c == 0 && rg == 0) { s_d[b] = a.ad[(size_t) t * nb + b]; }
             }
             auto row = [&](const Raw<KF_Q4K> & raw, int ri) {
                 Chunk ck; decode<KF_Q4K>(raw, c, ck);
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    if (t < nt) {
-                        int is, sm;
-                        chunk_dot<KF_Q4K>(ck, xc[t], is, sm);
-                        is = red8(is); sm = red8(sm);
-                        if (c == 0 && active) { s_lds[(ri * TT + t) * nbp + b] = __builtin_fmaf(-ck.dmin, (float) sm, ck.d * (float) is); }
-                    }
-                }
+                int is, sm;
+                chunk_dot<KF_Q4K>(ck, x, is, sm);
+                is = red8(is); sm = red8(sm);
+                if (c == 0 && active) { s_lds[ri * nbp + b] = __builtin_fmaf(-ck.dmin, (float) sm, ck.d * (float) is); }
             };
             const uint32_t step = (uint32_t) wr * rowb;
             Src sp = src; sp.vb = (uint32_t) (b * BS); sp.so = (uint32_t) rg * rowb;
@@ -105,22 +89,20 @@ __global__ void __launch_bounds__(256) k_q4k_vec(KqArgs a) {
             }
         }
         __syncthreads();
-        for (int p = threadIdx.x; p < nrow * nt; p += blockDim.x) {   // blocks in order, one lane per (row, token)
-            const int ri = p / nt, t = p % nt;
-            const float * tp = s_lds + (ri * TT + t) * nbp, * dp = s_d + t * nbp;
+        for (int ri = threadIdx.x; ri < nrow; ri += blockDim.x) {   // blocks in order, one lane per row
             float acc = 0.f;
-            for (int j = 0; j < nb; ++j) { acc = __builtin_fmaf(dp[j], tp[j], acc); }
-            Out[(size_t) (sg + t) * a.ldo + tr0 + ri] = acc;
+            for (int j = 0; j < nb; ++j) { acc = __builtin_fmaf(s_d[j], s_lds[ri * nbp + j], acc); }
+            Out[(size_t) t * a.ldo + tr0 + ri] = acc;
         }
         __syncthreads();
     }
 }
 
-template <int TT> hipError_t vec(KqArgs a, unsigned gy, hipStream_t st) {
+hipError_t vec(KqArgs a, unsigned gy, hipStream_t st) {
     const int nb = a.K / QK, nbp = nb | 1;
-    a.rw = std::max(1, std::min(a.rw, V_LDS / (int) (TT * nbp * sizeof(float)) - 1));
+    a.rw = (int) std::max<int64_t>(1, std::min<int64_t>({ V_ROWS, (int64_t) a.R * gy / 1024, V_LDS / (int) (nbp * sizeof(float)) - 1 }));   // ~1024 workgroups
     const dim3 grid((unsigned) ((a.R + a.rw - 1) / a.rw), gy);
-    k_q4k_vec<TT><<<grid, 64 * v_wk(nb) * v_wr(nb), (size_t) (a.rw + 1) * TT * nbp * sizeof(float), st>>>(a);
+    k_q4k_vec<<<grid, 64 * v_wk(nb) * v_wr(nb), (size_t) (a.rw + 1) * nbp * sizeof(float), st>>>(a);
     return hipGetLastError();
 }
 
@@ -152,6 +134,16 @@ template <int BYTES> __device__ __forceinline__ void q4_lds(__amdgpu_buffer_rsrc
 #else
     (void) r; (void) dst; (void) voff; (void) soff;
 #endif
+}
+// A barrier for what the waves wrote to LDS themselves: __syncthreads would also wait for the copies into LDS that are under way for
+// later rounds (VM: loads that may stay out)
+template <int VM> __device__ __forceinline__ void q4_barrier() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070 | (VM & 15) | ((VM >> 4) << 14));   // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    __asm__ volatile("" ::: "memory");
 }
 __device__ __forceinline__ uint32_t pk_mul(uint32_t a, uint32_t b) { return __builtin_bit_cast(uint32_t, (qu2) (__builtin_bit_cast(qu2, a) * __builtin_bit_cast(qu2, b))); }
 
@@ -204,17 +196,28 @@ __device__ __forceinline__ void q4_mins(const u32x4 & hd, uint32_t (&mm)[2]) {
     mm[0] = hd.z & 0x3F3F3F3Fu; mm[1] = ((hd.w >> 4) & 0x0F0F0F0Fu) | ((hd.z >> 2) & 0x30303030u);
 }
 
-// Few tokens: a workgroup's 8 waves share its rows and tokens and split K, wave w taking blocks w, w + 8, ...; operands come
-// straight from memory into registers, the wave's next block while it multiplies one. Each round of 8 blocks leaves their terms
-// in LDS (double-buffered, one barrier a round), and the workgroup's lanes run the chains over them, an output or two a lane.
-// summ comes from a third product with the step's min in every byte (here the matrix cores have time to spare).
-constexpr int KS_W = 8;
+// Few tokens: a workgroup's 8 waves share its rows and tokens and split K, wave w taking blocks w, w + 8, ... of the rows. A round's 8
+// blocks of a row are 1152 consecutive bytes: they are copied into LDS in whole (a wave's lanes fetching 16 rows' pieces of 64
+// bytes themselves make twice the cache accesses, which then bound the kernel: 73 us instead of 5x for one token through 65536
+// rows of 7168), a round ahead. Activations come into registers straight from the caches, also a round ahead. Each round leaves the
+// blocks' terms in LDS, and the workgroup's lanes run the chains over them, an output or two a lane. summ comes from a third
+// product with the step's min in every byte (here the matrix cores have time to spare).
+constexpr int KS_W = 8, KS_PITCH = 9 * KS_W + 1;   // 16-byte chunks from row to row in LDS: 16 rows start in 16 different quads of banks
+// copy i of a wave (past the last one: an earlier one of its own again, the same bytes, so that every wave has as many out)
+template <int ALLC> __device__ __forceinline__ int q4_copy(int wave, int i) { const int k = wave + KS_W * i; return k < ALLC ? k : wave; }
+template <int RT, int NT> struct KsLds {
+    static constexpr int ALLC = (16 * RT * KS_PITCH + 63) / 64, COPIES = (ALLC + KS_W - 1) / KS_W, WB = ALLC * 1024;   // copies of a round, a wave's, bytes
+    static constexpr int TOK = 16 * NT, TT = 80 * 4 * NT;   // a wave's terms of a row tile: token t, row r at 80 (t / 4) + 16 (t % 4) + r
+    static constexpr int T0 = 2 * WB, D0 = T0 + KS_W * RT * TT * 4, ALL = D0 + KS_W * TOK * 4;
+};
 template <int RT, int NT>
 __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
 #pragma clang fp contract(off)
-    constexpr int BS = 144, TOK = 16 * NT, TT = 80 * 4 * NT;   // a wave's terms of a row tile: token t, row r at 80 (t / 4) + 16 (t % 4) + r
-    __shared__ float s_t[2][KS_W][RT][TT];
-    __shared__ float s_d[2][KS_W][TOK];
+    using L = KsLds<RT, NT>;
+    constexpr int BS = 144, TOK = L::TOK, TT = L::TT;
+    extern __shared__ __attribute__((aligned(16))) uint8_t q4_dyn[];
+    LK_LOCAL uint8_t * lds = (LK_LOCAL uint8_t *) q4_dyn;
+    LK_LOCAL float * s_t = (LK_LOCAL float *) (lds + L::T0), * s_d = (LK_LOCAL float *) (lds + L::D0);   // [wave][row tile][TT], [wave][TOK]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, g = lane >> 4;
     int e, s_beg, s_end;
     if (a.act) {
@@ -225,49 +228,63 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
     const int row0 = (int) blockIdx.x * 16 * RT, nrow = min(16 * RT, a.R - row0), nb = a.K / QK;
     const uint32_t rowb = (uint32_t) (nb * BS);
     float * Out = second ? a.out2 : a.out;
-    // rows past the matrix's end and tokens past the group's read 0
+    // rows past the matrix's end and tokens past the group's read 0, as does a lane offset of OUT: a descriptor spans less than
+    // 2^31 bytes, and the scalar offset beside it stays inside the span
+    constexpr uint32_t OUT = 0x80000000u;
     const __amdgpu_buffer_rsrc_t rw = q4_rsrc((second ? a.w2 : a.w) + (size_t) e * a.estride + (size_t) row0 * rowb, (uint32_t) nrow * rowb);
-    uint32_t vw[RT], vx[NT];
+    uint32_t vw[L::COPIES], vx[NT];
+    int cw[L::COPIES];   // the chunk of its row that the lane copies
 #pragma unroll
-    for (int i = 0; i < RT; ++i) { vw[i] = (uint32_t) (16 * i + r) * rowb; }
+    for (int i = 0; i < L::COPIES; ++i) {
+        const int p = 64 * q4_copy<L::ALLC>(wave, i) + lane, row = p / KS_PITCH;
+        cw[i] = p % KS_PITCH; vw[i] = (uint32_t) row * rowb + (uint32_t) (cw[i] * 16);
+    }
 #pragma unroll
     for (int t = 0; t < NT; ++t) { vx[t] = (uint32_t) (16 * t + r) * (uint32_t) a.K + (uint32_t) (64 * (g >> 1) + 16 * (g & 1)); }
     const uint32_t sel0 = 0x0c000c00u | (uint32_t) (2 * (g >> 1)) * 0x00010001u, selm = (uint32_t) (2 * (g >> 1)) * 0x01010101u;
+    const uint32_t lw = (uint32_t) (size_t) lds + (uint32_t) (r * KS_PITCH * 16 + wave * BS);
     for (int sg = s_beg; sg < s_end; sg += TOK) {
         const int nt = min(TOK, s_end - sg);
         const __amdgpu_buffer_rsrc_t rx = q4_rsrc(a.aq + (size_t) sg * a.K, (uint32_t) nt * (uint32_t) a.K);
         const __amdgpu_buffer_rsrc_t rd = q4_rsrc(a.ad + (size_t) sg * nb, (uint32_t) nt * (uint32_t) nb * 4);
-        struct Ops { u32x4 w[RT][3]; qi4 x[NT][4]; uint32_t d; };
-        auto load = [&](int b, Ops & o) {   // (past the last block: the last one, unread)
-            const uint32_t sw = (uint32_t) (min(b, nb - 1) * BS), sx = (uint32_t) (min(b, nb - 1) * QK);
+        auto copy = [&](int j, int s) {   // blocks j .. j + 7 of every row (past the row's end: nothing is fetched)
+            const int nc = 9 * min(KS_W, nb - j);   // (none or fewer: every lane stays out)
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                o.w[i][0] = __builtin_amdgcn_raw_buffer_load_b128(rw, vw[i], sw, 0);
-                o.w[i][1] = __builtin_amdgcn_raw_buffer_load_b128(rw, vw[i] + 16u * g + 16u, sw, 0);
-                o.w[i][2] = __builtin_amdgcn_raw_buffer_load_b128(rw, vw[i] + 16u * g + 80u, sw, 0);
+            for (int i = 0; i < L::COPIES; ++i) {
+                q4_lds<16>(rw, lds + s * L::WB + q4_copy<L::ALLC>(wave, i) * 1024, cw[i] < nc ? vw[i] : OUT, (uint32_t) (min(j, nb - 1) * BS));
             }
+        };
+        struct Act { qi4 x[NT][4]; uint32_t d; };
+        auto load_x = [&](int b, Act & o) {   // (past the last block: nothing is fetched)
+            const uint32_t out = b < nb ? 0u : OUT;
+            b = min(b, nb - 1);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {   // step (p, h) = (k / 2, k % 2): 128 p + 32 h further
-                    o.x[t][k] = __builtin_bit_cast(qi4, __builtin_amdgcn_raw_buffer_load_b128(rx, vx[t] + (uint32_t) (128 * (k >> 1) + 32 * (k & 1)), sx, 0));
+                    o.x[t][k] = __builtin_bit_cast(qi4, __builtin_amdgcn_raw_buffer_load_b128(rx, (vx[t] | out) + (uint32_t) (128 * (k >> 1) + 32 * (k & 1)), (uint32_t) (b * QK), 0));
                 }
             }
-            o.d = __builtin_amdgcn_raw_buffer_load_b32(rd, (uint32_t) ((lane < TOK ? lane : 0) * nb * 4), (uint32_t) (min(b, nb - 1) * 4), 0);
+            o.d = __builtin_amdgcn_raw_buffer_load_b32(rd, (uint32_t) ((lane < TOK ? lane : 0) * nb * 4) | out, (uint32_t) (b * 4), 0);
         };
         float acc[(RT * TOK * 16 + 64 * KS_W - 1) / (64 * KS_W)];
         constexpr int NO = sizeof(acc) / sizeof(acc[0]);
 #pragma unroll
         for (int i = 0; i < NO; ++i) { acc[i] = 0.f; }
-        auto round = [&](const Ops & o, int j0, int s) {
+        auto round = [&](const Act & v, int j0, int s) {
             if (j0 + wave < nb) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
+                    const uint32_t at = lw + (uint32_t) (s * L::WB + 16 * i * KS_PITCH * 16);
+                    u32x4 w[3];
+                    w[0] = *(const LK_LOCAL u32x4 *) (size_t) at;
+                    w[1] = *(const LK_LOCAL u32x4 *) (size_t) (at + 16u + 16u * g);
+                    w[2] = *(const LK_LOCAL u32x4 *) (size_t) (at + 80u + 16u * g);
                     qi4 wl[4], wh[4];
                     uint32_t mm[2];
-                    q4_digits(o.w[i], sel0, wl, wh);
-                    q4_mins(o.w[i][0], mm);
-                    const float dd = h2f((uint16_t) (o.w[i][0].x & 0xFFFFu)), dm = -h2f((uint16_t) (o.w[i][0].x >> 16));
+                    q4_digits(w, sel0, wl, wh);
+                    q4_mins(w[0], mm);
+                    const float dd = h2f((uint16_t) (w[0].x & 0xFFFFu)), dm = -h2f((uint16_t) (w[0].x >> 16));
                     qi4 mv[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
@@ -279,26 +296,26 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
                         qi4 hs = { 0, 0, 0, 0 }, ls = hs, ms = hs;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
-                            hs = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[t][k], wh[k], hs, 0, 0, 0);
-                            ls = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[t][k], wl[k], ls, 0, 0, 0);
-                            ms = __builtin_amdgcn_mfma_i32_16x16x64_i8(o.x[t][k], mv[k], ms, 0, 0, 0);
+                            hs = __builtin_amdgcn_mfma_i32_16x16x64_i8(v.x[t][k], wh[k], hs, 0, 0, 0);
+                            ls = __builtin_amdgcn_mfma_i32_16x16x64_i8(v.x[t][k], wl[k], ls, 0, 0, 0);
+                            ms = __builtin_amdgcn_mfma_i32_16x16x64_i8(v.x[t][k], mv[k], ms, 0, 0, 0);
                         }
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {   // token 16 t + 4 g + k
                             const float fi = (float) (int) (((uint32_t) hs[k] << 3) + (uint32_t) ls[k]);
-                            s_t[s][wave][i][80 * (4 * t + g) + 16 * k + r] = __builtin_fmaf(dm, (float) ms[k], dd * fi);
+                            s_t[(wave * RT + i) * TT + 80 * (4 * t + g) + 16 * k + r] = __builtin_fmaf(dm, (float) ms[k], dd * fi);
                         }
                     }
                 }
-                if (lane < TOK) { s_d[s][wave][lane] = __builtin_bit_cast(float, o.d); }
+                if (lane < TOK) { s_d[wave * TOK + lane] = __builtin_bit_cast(float, v.d); }
             }
-            __syncthreads();
+            q4_barrier<63>();
             const int m = min(KS_W, nb - j0);
 #pragma unroll
             for (int i = 0; i < NO; ++i) {
                 const int p = threadIdx.x + 64 * KS_W * i, q = p >> 4, t = q % TOK, ri = q / TOK;   // row p % 16 of row tile ri, token t
                 if (p < RT * TOK * 16) {
-                    const float * tp = &s_t[s][0][ri][80 * (t >> 2) + 16 * (t & 3) + (p & 15)], * dp = &s_d[s][0][t];
+                    const LK_LOCAL float * tp = s_t + ri * TT + 80 * (t >> 2) + 16 * (t & 3) + (p & 15), * dp = s_d + t;
                     if (m == KS_W) {
 #pragma unroll
                         for (int w = 0; w < KS_W; ++w) { acc[i] = __builtin_fmaf(dp[w * TOK], tp[w * RT * TT], acc[i]); }
@@ -308,28 +325,34 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
                 }
             }
         };
-        Ops o0, o1;
-        load(wave, o0);
+        Act x[2];
+        constexpr int XL = 4 * NT + 1;   // the next round's activations may still be out when a round starts
+        copy(0, 0);
+        load_x(wave, x[0]);
         for (int j0 = 0;;) {
-            load(j0 + KS_W + wave, o1);
-            __builtin_amdgcn_sched_barrier(0);
-            round(o0, j0, 0);
-            if ((j0 += KS_W) >= nb) { break; }
-            load(j0 + KS_W + wave, o0);
-            __builtin_amdgcn_sched_barrier(0);
-            round(o1, j0, 1);
-            if ((j0 += KS_W) >= nb) { break; }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                q4_barrier<XL>();   // the round's copies have landed, this wave's and so everyone's; the last round's buffer and the terms are free
+                copy(j0 + KS_W, i ^ 1);
+                load_x(j0 + KS_W + wave, x[i ^ 1]);
+                __builtin_amdgcn_sched_barrier(0);
+                round(x[i], j0, i);
+                if ((j0 += KS_W) >= nb) { goto done; }
+            }
         }
+done:
 #pragma unroll
         for (int i = 0; i < NO; ++i) {
             const int p = threadIdx.x + 64 * KS_W * i, q = p >> 4, t = q % TOK, row = 16 * (q / TOK) + (p & 15);
             if (p < RT * TOK * 16 && t < nt && row < nrow) { Out[(size_t) (sg + t) * a.ldo + row0 + row] = acc[i]; }
         }
-        __syncthreads();   // the terms' buffers are free for the next group
+        __syncthreads();   // the buffers are free for the next group
     }
 }
 template <int RT, int NT> hipError_t ks(const KqArgs & a, unsigned gy, hipStream_t st) {
-    k_q4k_ks<RT, NT><<<dim3((unsigned) ((a.R + 16 * RT - 1) / (16 * RT)), gy, a.act ? 1u : (unsigned) ((a.n + 16 * NT - 1) / (16 * NT))), 64 * KS_W, 0, st>>>(a);
+    static const hipError_t set = hipFuncSetAttribute((const void *) k_q4k_ks<RT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, KsLds<RT, NT>::ALL);
+    if (set != hipSuccess) { return set; }
+    k_q4k_ks<RT, NT><<<dim3((unsigned) ((a.R + 16 * RT - 1) / (16 * RT)), gy, a.act ? 1u : (unsigned) ((a.n + 16 * NT - 1) / (16 * NT))), 64 * KS_W, KsLds<RT, NT>::ALL, st>>>(a);
     return hipGetLastError();
 }
 
@@ -349,9 +372,10 @@ __global__ void __launch_bounds__(64 * W, 2) k_q4k_mm(Q4Args a) {
     const bool second = blockIdx.y == 1;
     const int nb = a.K / QK, row0 = (rt0 * W + wave) * RT * 16, t0 = tt0 * TOK, nt = min(TOK, a.n - t0);
     const uint32_t rowb = (uint32_t) (nb * BS);
-    // a wave's rows (past the matrix's end: none, its loads give 0 and nothing is stored)
-    const int nrow = max(0, min(RT * 16, a.R - row0));
-    const __amdgpu_buffer_rsrc_t rw = q4_rsrc((second ? a.w2 : a.w) + (size_t) (nrow > 0 ? row0 : 0) * rowb, (uint32_t) nrow * rowb);
+    // a wave's rows; one wholly past the matrix's end reads the first rows and stores nothing. Rows past the end read 0: scalar offsets stay
+    // inside the descriptor's span, lane offsets pass it
+    const int nrow = max(0, min(RT * 16, a.R - row0)), rrow = nrow > 0 ? row0 : 0;
+    const __amdgpu_buffer_rsrc_t rw = q4_rsrc((second ? a.w2 : a.w) + (size_t) rrow * rowb, (uint32_t) min(RT * 16, a.R - rrow) * rowb);
     const __amdgpu_buffer_rsrc_t rx = q4_rsrc(a.aq + (size_t) t0 * a.K, (uint32_t) nt * (uint32_t) a.K);
     const __amdgpu_buffer_rsrc_t rs = q4_rsrc(a.xs + (size_t) t0 * nb * 16, (uint32_t) nt * (uint32_t) nb * 32);
     const __amdgpu_buffer_rsrc_t rd = q4_rsrc(a.ad + (size_t) t0 * nb, (uint32_t) nt * (uint32_t) nb * 4);
@@ -478,6 +502,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_q4k_mm(Q4Args a) {
             copy(j + D - 1, (s + D - 1) % D);
             __builtin_amdgcn_sched_barrier(0);
             block(raw[s % (D - 1)], s % D, j + D - 1);
+            __builtin_amdgcn_sched_barrier(0);   // (register moves of the next block's weights stay here: inside the block they would wait for them)
             if (++j == nb) { goto done; }   // (a jump, not a guard around each block: the compiler then knows which loads are out)
         }
     }
@@ -499,12 +524,12 @@ done:
     }
 }
 
-template <int RT, int NT, int W, int D> hipError_t mm(const KqArgs & k, void * xs, hipStream_t st) {
+template <int RT, int NT, int W, int D> hipError_t mm(const KqArgs & k, hipStream_t st) {
     constexpr int LDS = D * 16 * NT * (256 + 32 + 4);
     static const hipError_t set = hipFuncSetAttribute((const void *) k_q4k_mm<RT, NT, W, D>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (set != hipSuccess) { return set; }
     Q4Args a{};
-    a.w = k.w; a.w2 = k.w2; a.aq = k.aq; a.ad = k.ad; a.xs = (const _Float16 *) xs; a.K = k.K; a.R = k.R; a.n = k.n;
+    a.w = k.w; a.w2 = k.w2; a.aq = k.aq; a.ad = k.ad; a.xs = (const _Float16 *) k.xs; a.K = k.K; a.R = k.R; a.n = k.n;
     a.out = k.out; a.out2 = k.out2; a.ldo = k.ldo;
     a.rt = (k.R + 16 * RT * W - 1) / (16 * RT * W); a.tt = (k.n + 16 * NT - 1) / (16 * NT);
     k_q4k_mm<RT, NT, W, D><<<dim3((unsigned) (a.rt * a.tt), k.w2 ? 2 : 1), 64 * W, LDS, st>>>(a);
@@ -513,29 +538,27 @@ template <int RT, int NT, int W, int D> hipError_t mm(const KqArgs & k, void * x
 
 }  // namespace
 
-size_t q4k_scratch_bytes(int n, int R, int K) { return q4k_kernel(n, R, K, true) >= Q4_MM_64_32 ? (size_t) n * (K / QK) * 32 : 0; }
+size_t q4k_scratch_bytes(int n, int64_t R, int K) { return q4k_tiled(q4k_kernel(n, R, K, true)) ? (size_t) n * (K / QK) * 32 : 0; }
 
-hipError_t launch_q4k(const KqArgs & args, int max_slots, int grid_experts, hipStream_t st) {
-    KqArgs a = args;
+hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStream_t st) {
     if (a.K <= 0 || a.K % QK || a.K > QK * V_NB || a.R <= 0 || max_slots <= 0 || grid_experts <= 0) { return hipErrorInvalidValue; }
     const unsigned gy = a.act ? (unsigned) grid_experts : (a.w2 ? 2u : 1u);
-    switch (q4k_kernel(max_slots, a.R * (int) (a.act ? 1 : gy), a.K, !a.act && a.xs)) {
-    case Q4_VEC1: case Q4_VEC2:
-        a.rw = (int) std::max<int64_t>(1, std::min<int64_t>(V_ROWS, (int64_t) a.R * gy / 1024));
-        return max_slots <= 1 ? vec<1>(a, gy, st) : vec<2>(a, gy, st);
-    case Q4_KS_1_1: return ks<1, 1>(a, gy, st);
-    case Q4_KS_2_1: return ks<2, 1>(a, gy, st);
-    case Q4_KS_2_2: return ks<2, 2>(a, gy, st);
-    default: break;
+    // (an expert's slots are known on the device alone: their expected number goes for the tokens)
+    const int kernel = q4k_kernel(max_slots, (int64_t) a.R * gy, a.K, !a.act && a.xs);
+    if (q4k_tiled(kernel)) {
+        const int64_t nsub = (int64_t) a.n * (a.K / 32);
+        k_q4k_sums<<<(unsigned) ((nsub + 255) / 256), 256, 0, st>>>(a.aq, nsub, (_Float16 *) a.xs);
+        if (const hipError_t e = hipGetLastError()) { return e; }
     }
-    const int64_t nsub = (int64_t) a.n * (a.K / 32);
-    k_q4k_sums<<<(unsigned) ((nsub + 255) / 256), 256, 0, st>>>(a.aq, nsub, (_Float16 *) a.xs);
-    if (const hipError_t e = hipGetLastError()) { return e; }
-    switch (q4k_kernel(max_slots, a.R * (int) gy, a.K, true)) {
-    case Q4_MM_64_32: return mm<1, 2, 4, 5>(a, a.xs, st);
-    case Q4_MM_64_64: return mm<1, 4, 4, 3>(a, a.xs, st);
-    case Q4_MM_128_64: return mm<2, 4, 4, 2>(a, a.xs, st);
-    default: return mm<2, 8, 8, 2>(a, a.xs, st);
+    switch (kernel) {
+    case Q4_VEC: return vec(a, gy, st);
+    case Q4_KS_16_16: return ks<1, 1>(a, gy, st);
+    case Q4_KS_32_32: return ks<2, 2>(a, gy, st);
+    case Q4_KS_32_48: return ks<2, 3>(a, gy, st);
+    case Q4_MM_64_32: return mm<1, 2, 4, 5>(a, st);
+    case Q4_MM_64_64: return mm<1, 4, 4, 3>(a, st);
+    case Q4_MM_128_64: return mm<1, 4, 8, 3>(a, st);
+    default: return mm<2, 8, 4, 2>(a, st);
     }
 }
 

@@ -5,92 +5,452 @@
 //   S > 2^-14:  ds_k = scale / S (dw_k - sum_j dw_j s_j / S),  else  ds_k = scale / 2^-14 dw_k
 //   dz = dz_in + sum over the picks of ds_k s_k (1 - s_k),   dW = dz^T x,   dx = dz W
 // The bias only takes part in the selection and has no gradient.
+//
+// The two products run on the fp16 matrix cores at fp32's precision: an operand v is taken as v 2^k = hi + lo, two fp16 of 11 bits
+// each, and a product is hi hi + hi lo + lo hi in fp32 sums; what is left out, lo lo, and lo's own rounding are below 2^-22 of the
+// product. Three fp16 products cost a third of what the fp32 matrix cores take. k puts the largest finite |v| at 2^14 .. 2^15, so
+// that values down to 2^-18 of it keep both halves whole and smaller ones an absolute error of 2^-39 of it:
+//   dz   one k per row t, which both products can take: dx's row t is scaled back by 2^-k_t, and in dW's sum over t the factor
+//        goes to x (x 2^(K0 - k_t), K0 the smallest k of the rows summed, so no factor exceeds 1)
+//   W    one k per 64 columns, found by the kernel that splits it
+//   x    one k per column, running: a slab's maximum that passes the present range lowers k, and the accumulators of that column
+//        follow (as the running maximum of an online softmax)
+// Non-finite values take no part in the maxima; they make the outputs that they enter non-finite.
 #include "moe_device.h"
 #include "moe_kernels.h"
+
+#include <algorithm>
 
 namespace lk {
 
 namespace {
 
 constexpr float RG_CLAMP = 0x1p-14f;   // select_token_p's
+constexpr int RG_NONE = 1000;          // k of a row without gradient: its factor is 0
 typedef float gf4 __attribute__((ext_vector_type(4)));
+typedef _Float16 gh8 __attribute__((ext_vector_type(8)));
+typedef short gs8 __attribute__((ext_vector_type(8)));
 
-// one wave per row: lane k < topk holds pick k; the columns e = lane + 64 j of the row
-__global__ void __launch_bounds__(256) k_route_dz(RouteGradArgs g) {
-    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = lane_id();
-    if (t >= g.n) { return; }
-    const int ne = g.n_exp;
-    int e = -1; float gz = 0.f;
-    if (g.dw) {
-        float s = 0.f, om = 0.f, dw = 0.f;
-        if (lane < g.topk) {
-            e = g.sel[(size_t) t * g.topk + lane];
-            if ((unsigned) e < (unsigned) ne) {
-                const float z = g.logits[(size_t) t * ne + e], u = expf(-fabsf(z)), r = 1.f / (1.f + u);
-                s = z >= 0.f ? r : u * r; om = z >= 0.f ? u * r : r;
-                dw = g.dw[(size_t) t * g.topk + lane];
-            } else { e = -1; }
-        }
-        float S = 0.f, D = 0.f;
-        for (int k = 0; k < g.topk; ++k) {   // in pick order, as the forward pass adds
-            const float sk = __builtin_bit_cast(float, rdlane(__builtin_bit_cast(uint32_t, s), k));
-            S += sk; D += __builtin_bit_cast(float, rdlane(__builtin_bit_cast(uint32_t, dw), k)) * sk;
-        }
-        const float ds = S > RG_CLAMP ? g.scale / S * (dw - D / S) : g.scale / RG_CLAMP * dw;
-        gz = ds * (s * om);
-    }
+// the k that puts m > 0 at 2^14 .. 2^15 (m finite; subnormals as the smallest normal number)
+__device__ __forceinline__ int rg_k(float m) { return min(126, 141 - max(1, (int) (__builtin_bit_cast(uint32_t, m) >> 23))); }
+__device__ __forceinline__ float rg_pow2(int k) { return __builtin_bit_cast(float, (uint32_t) (min(max(k, -126), 127) + 127) << 23); }
+__device__ __forceinline__ float rg_mag(float v) { const float a = fabsf(v); return a < INFINITY ? a : 0.f; }
+__device__ __forceinline__ void rg_split(float v, _Float16 & hi, _Float16 & lo) { hi = (_Float16) v; lo = (_Float16) (v - (float) hi); }
+template <int CTRL> __device__ __forceinline__ float rg_dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v))); }
+__device__ __forceinline__ float rg_lane(float v, int l) { return __builtin_bit_cast(float, rdlane(__builtin_bit_cast(uint32_t, v), l)); }
+__device__ __forceinline__ float rg_wave_max(float v) {
+    v = fmaxf(v, rg_dpp<DPP_XOR1>(v)); v = fmaxf(v, rg_dpp<DPP_XOR2>(v)); v = fmaxf(v, rg_dpp<DPP_HALF_MIRROR>(v)); v = fmaxf(v, rg_dpp<DPP_MIRROR>(v));
+    return fmaxf(fmaxf(rg_lane(v, 0), rg_lane(v, 16)), fmaxf(rg_lane(v, 32), rg_lane(v, 48)));
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rg_rsrc(const void * p, uint32_t bytes) {
+    const uint64_t v = (uint64_t) p;
+    const uint32_t hi = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (v >> 32)), lo = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) v);
+    return __builtin_amdgcn_make_buffer_rsrc((void *) (((uint64_t) hi << 32) | lo), (short) 0, __builtin_amdgcn_readfirstlane((int) bytes), 0x00020000);
+}
+// 16 bytes per lane from a buffer straight into LDS, lane L at dst + 16 L; the builtin exists for the device pass only
+__device__ __forceinline__ void rg_lds16(__amdgpu_buffer_rsrc_t r, LK_LOCAL uint8_t * dst, uint32_t voff, uint32_t soff) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LK_LOCAL void *) dst, 16, voff, soff, 0, 0);
+#else
+    (void) r; (void) dst; (void) voff; (void) soff;
+#endif
+}
+
+// The operands in memory, halves of 16 bytes = 8 consecutive K values:
+//   zs [t][hi, lo][kp]          dz of row t, K = experts (kp: n_exp up to a multiple of 32, zeros)
+//   zt [t / 8][hi, lo][ea][8]   dz of 8 rows, K = rows (ea: n_exp up to 64, 128 or 256, zeros; rows up to a multiple of 32, zeros)
+//   kt [t]                      the rows' k
+//   wt [hi, lo][kp / 8][E][8]   W, K = experts; kw [E / 64] its k
+struct Ops { _Float16 * zs, * zt, * wt; short * kt; int * kw; int kp, ea, np; };
+
+// The first nw workgroups split 64 columns of W each (all experts in registers between the maximum and the split). The others take 8
+// rows, two a wave: lane k < topk holds pick k, then the columns e = lane + 64 j of the row.
+__global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int nw) {
+    __shared__ _Float16 s_h[2][8][NEXP_MAX];
+    __shared__ float s_m[4];
+    const int lane = lane_id(), wv = threadIdx.x >> 6, ne = g.n_exp;
+    if ((int) blockIdx.x < nw) {
+        constexpr int NB = NEXP_MAX / 32;   // experts 8 (wv + 4 i) .. + 7 a wave
+        const int c = (int) blockIdx.x * 64 + lane;
+        float v[NB][8], m = 0.f;
 #pragma unroll
-    for (int j = 0; j < NEXP_MAX / 64; ++j) {
-        const int c = lane + 64 * j;
-        float v = g.dz_in && c < ne ? g.dz_in[(size_t) t * ne + c] : 0.f;
-        if (g.dw) {
-            for (int k = 0; k < g.topk; ++k) {
-                const int ek = (int) rdlane((uint32_t) e, k);
-                const float gk = __builtin_bit_cast(float, rdlane(__builtin_bit_cast(uint32_t, gz), k));
-                v += ek == c ? gk : 0.f;
+        for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { const int e = 8 * (wv + 4 * i) + u; v[i][u] = e < ne ? g.W[(size_t) e * g.E + c] : 0.f; }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { m = fmaxf(m, rg_mag(v[i][u])); }
+        }
+        m = rg_wave_max(m);
+        if (lane == 0) { s_m[wv] = m; }
+        __syncthreads();
+        const int k = rg_k(fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3])));
+        const float sc = rg_pow2(k);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int b = wv + 4 * i;
+            if (b < o.kp / 8) {
+                gh8 hi, lo;
+#pragma unroll
+                for (int u = 0; u < 8; ++u) { _Float16 h, l; rg_split(v[i][u] * sc, h, l); hi[u] = h; lo[u] = l; }
+                *reinterpret_cast<gh8 *>(o.wt + ((size_t) b * g.E + c) * 8) = hi;
+                *reinterpret_cast<gh8 *>(o.wt + ((size_t) (o.kp / 8 + b) * g.E + c) * 8) = lo;
             }
         }
-        if (c < ne) { g.dz[(size_t) t * ne + c] = v; }
+        if (threadIdx.x == 0) { o.kw[blockIdx.x] = k; }
+        return;
+    }
+    const int tb = (int) blockIdx.x - nw, t0 = tb * 8;
+    constexpr int J = NEXP_MAX / 64;
+    float v[2][J], s[2], om[2], dw[2];
+    int e[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int t = t0 + wv + 4 * h;
+        const bool in = t < g.n, pick = in && g.dw && lane < g.topk;
+#pragma unroll
+        for (int j = 0; j < J; ++j) { const int c = lane + 64 * j; v[h][j] = in && g.dz_in && c < ne ? g.dz_in[(size_t) t * ne + c] : 0.f; }
+        e[h] = pick ? g.sel[(size_t) t * g.topk + lane] : -1;
+        dw[h] = pick ? g.dw[(size_t) t * g.topk + lane] : 0.f;
+        if ((unsigned) e[h] >= (unsigned) ne) { e[h] = -1; dw[h] = 0.f; }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float z = e[h] >= 0 ? g.logits[(size_t) (t0 + wv + 4 * h) * ne + e[h]] : -INFINITY;
+        const float u = expf(-fabsf(z)), r = 1.f / (1.f + u);
+        s[h] = z >= 0.f ? r : u * r; om[h] = z >= 0.f ? u * r : r;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int t = t0 + wv + 4 * h;
+        float S = 0.f, D = 0.f;
+#pragma unroll
+        for (int k = 0; k < MAXK; ++k) { const float sk = rg_lane(s[h], k); S += sk; D += rg_lane(dw[h], k) * sk; }   // in pick order, as the forward pass adds; none: 0
+        const float ds = S > RG_CLAMP ? g.scale / S * (dw[h] - D / S) : g.scale / RG_CLAMP * dw[h], gz = ds * (s[h] * om[h]);
+#pragma unroll
+        for (int k = 0; k < MAXK; ++k) {
+            const int ek = (int) rdlane((uint32_t) e[h], k);
+            const float gk = rg_lane(gz, k);
+#pragma unroll
+            for (int j = 0; j < J; ++j) { v[h][j] += ek == lane + 64 * j ? gk : 0.f; }
+        }
+        float m = 0.f;
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < J; ++j) { m = fmaxf(m, rg_mag(v[h][j])); odd = odd || !(fabsf(v[h][j]) < INFINITY); }
+        m = rg_wave_max(m);
+        const bool none = m == 0.f && __ballot(odd) == 0;
+        const int k = none ? RG_NONE : rg_k(m);
+        const float sc = none ? 1.f : rg_pow2(k);
+        if (lane == 0) { o.kt[t] = (short) k; }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int c = lane + 64 * j;
+            if (t < g.n && c < ne && g.dz) { g.dz[(size_t) t * ne + c] = v[h][j]; }
+            _Float16 a, l;
+            rg_split(v[h][j] * sc, a, l);
+            s_h[0][wv + 4 * h][c] = a; s_h[1][wv + 4 * h][c] = l;
+        }
+    }
+    __syncthreads();
+    for (int p = threadIdx.x; p < 2 * o.ea; p += 256) {   // 8 rows of an expert
+        const int q = p / o.ea, c = p % o.ea;
+        gh8 h;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { h[i] = s_h[q][i][c]; }
+        *reinterpret_cast<gh8 *>(o.zt + (((size_t) tb * 2 + q) * o.ea + c) * 8) = h;
+    }
+    const int nc = o.kp / 8;
+    for (int p = threadIdx.x; p < 16 * nc; p += 256) {    // 8 experts of a row
+        const int i = p / (2 * nc), c = p % (2 * nc);
+        if (t0 + i < g.n) { *reinterpret_cast<gh8 *>(o.zs + (size_t) (t0 + i) * 2 * o.kp + c * 8) = *reinterpret_cast<const gh8 *>(&s_h[c / nc][i][8 * (c % nc)]); }
     }
 }
 
-// C [M][N] = (or +=) sum_k A(m, k) B[k][N], A(m, k) = a[m sm + k sk]: a wave takes 16 rows x 64 columns on the fp32 matrix
-// cores (v_mfma_f32_16x16x4_f32: lane (r, g) holds row / column r at k = g), operands straight from memory
-__global__ void __launch_bounds__(64) k_route_mm(const float * __restrict__ a, int64_t sm, int64_t sk, const float * __restrict__ b, int M, int N, int K,
-                                                 float * __restrict__ c, int accumulate) {
-    const int lane = lane_id(), r = lane & 15, g = lane >> 4, m0 = blockIdx.y * 16, n0 = blockIdx.x * 64;
-    gf4 acc[4] = {};
-    const float * ap = a + (int64_t) min(m0 + r, M - 1) * sm;
-    for (int k = 0; k < K; k += 4) {
-        const bool in = k + g < K;
-        const float av = in ? ap[(int64_t) (k + g) * sk] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float bv = in ? b[(int64_t) (k + g) * N + n0 + 16 * i + r] : 0.f;
-            acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(av, bv, acc[i], 0, 0, 0);
-        }
+constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128;
+
+// dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 16 RT rows at a
+// time, whose dz comes straight from memory, the next 32 experts' in flight; no barrier after the first. The product runs with the
+// columns as rows of the matrix core's tile, so a lane stores 4 consecutive columns.
+template <int RT>
+__device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int part, int parts) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
+    const int j0 = ct * RG_COLS, nb = o.kp / 8, ns = o.kp / 32;
+    const __amdgpu_buffer_rsrc_t rw = rg_rsrc(o.wt, (uint32_t) ((size_t) 2 * nb * g.E * 16));
+    for (int i = wave; i < 2 * nb * 2; i += RG_W) {   // half and 8 experts i / 2, columns 64 (i % 2) ..
+        rg_lds16(rw, lds + i * 1024, (uint32_t) (lane * 16), (uint32_t) ((size_t) (i >> 1) * g.E * 16 + (size_t) (j0 + 64 * (i & 1)) * 16));
     }
+    const int kw[2] = { o.kw[j0 / 64], o.kw[j0 / 64 + 1] };
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    __syncthreads();
+    const uint32_t lo_off = (uint32_t) nb * 2048, lb = (uint32_t) (size_t) lds + (uint32_t) (q * 2048 + r * 16);
+    const int tiles = (g.n + 16 * RT - 1) / (16 * RT);
+    for (int tt = part * RG_W + wave; tt < tiles; tt += parts * RG_W) {
+        const int t0 = tt * 16 * RT, nt = min(16 * RT, g.n - t0);
+        // rows past the batch's end read 0
+        const __amdgpu_buffer_rsrc_t rz = rg_rsrc(o.zs + (size_t) t0 * 2 * o.kp, (uint32_t) nt * (uint32_t) o.kp * 4);
+        uint32_t vz[RT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < RT; ++i) { vz[i] = (uint32_t) (16 * i + r) * (uint32_t) (o.kp * 4) + 16u * q; }
+        gh8 z[2][RT][2];
+        auto load = [&](int s, gh8 (&d)[RT][2]) {
+            const uint32_t so = (uint32_t) (min(s, ns - 1) * 64);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int m = m0 + 4 * g + q;
-            if (m < M) {
-                float * o = c + (int64_t) m * N + n0 + 16 * i + r;
-                *o = accumulate ? *o + acc[i][q] : acc[i][q];
+            for (int i = 0; i < RT; ++i) {
+                d[i][0] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i], so, 0));
+                d[i][1] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i] + (uint32_t) (o.kp * 2), so, 0));
+            }
+        };
+        gf4 acc[8][RT];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+#pragma unroll
+            for (int i = 0; i < RT; ++i) { acc[c][i] = (gf4) { 0.f, 0.f, 0.f, 0.f }; }
+        }
+        auto step = [&](int s, const gh8 (&d)[RT][2]) {
+            const uint32_t a = lb + (uint32_t) s * 8192;   // 4 x 8 experts
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const gh8 wh = *(const LK_LOCAL gh8 *) (size_t) (a + c * 256), wl = *(const LK_LOCAL gh8 *) (size_t) (a + lo_off + c * 256);
+#pragma unroll
+                for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, d[i][0], acc[c][i], 0, 0, 0); }
+#pragma unroll
+                for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, d[i][1], acc[c][i], 0, 0, 0); }
+#pragma unroll
+                for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, d[i][0], acc[c][i], 0, 0, 0); }
+            }
+        };
+        load(0, z[0]);
+        for (int s = 0;;) {
+            load(s + 1, z[1]);
+            step(s, z[0]);
+            if (++s == ns) { break; }
+            load(s + 1, z[0]);
+            step(s, z[1]);
+            if (++s == ns) { break; }
+        }
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+            const int t = t0 + 16 * i + r;
+            if (t < g.n) {
+                const int kt = (int) o.kt[t];
+                float * row = g.dx + (size_t) t * g.E + j0 + 4 * q;
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const int k = kt == RG_NONE ? 0 : -kt - kw[c >> 2];
+                    gf4 v;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) { v[u] = ldexpf(acc[c][i][u], k); }
+                    *reinterpret_cast<gf4 *>(row + 16 * c) = v;
+                }
             }
         }
     }
+}
+
+// dW: a workgroup takes 128 columns of x, all experts (64 WR) and a run of 32-row steps. dz of a step is copied into LDS as it is
+// stored; x is read once, each wave 16 columns x 32 rows of it into registers (8 consecutive rows a lane), scaled, split and
+// written to LDS as 16-byte halves. Both are double-buffered: a step's barrier, the next step's copies and conversion, its products.
+// Waves: WR along the experts (64 each), 8 / WR along the columns (16 WR each).
+template <int WR>
+__device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int run, int splits, float * part) {
+    constexpr int EA = 64 * WR, AB = 4 * 2 * EA * 16, BB = 4 * 2 * RG_COLS * 16, BUF = AB + BB + RG_COLS * 4, JW = WR;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
+    const int j0 = ct * RG_COLS, we = wave % WR, wj = wave / WR;
+    const int steps = o.np / 32, s0 = (int) ((int64_t) steps * run / splits), s1 = (int) ((int64_t) steps * (run + 1) / splits);
+    // K0: the smallest k of the run's rows
+    int K0 = RG_NONE;
+    for (int t = 32 * s0 + (int) threadIdx.x; t < 32 * s1; t += RG_T) { K0 = min(K0, (int) o.kt[t]); }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) { K0 = min(K0, __shfl_xor(K0, d)); }
+    if (lane == 0) { *(LK_LOCAL int *) (lds + 4 * wave) = K0; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < RG_W; ++i) { K0 = min(K0, *(const LK_LOCAL int *) (lds + 4 * i)); }
+    __syncthreads();
+
+    struct Slab { float x[8]; gs8 k; };
+    auto load_x = [&](int s, Slab & d) {   // rows 32 s + 8 q .. + 7, column j0 + 16 wave + r; rows past the batch's end read 0
+        const int t = 32 * min(s, s1 - 1), nt = min(32, g.n - t);
+        const __amdgpu_buffer_rsrc_t rx = rg_rsrc(g.x + (size_t) t * g.E, (uint32_t) nt * (uint32_t) g.E * 4);
+        const uint32_t v = ((uint32_t) (8 * q) * (uint32_t) g.E + (uint32_t) (j0 + 16 * wave + r)) * 4;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { d.x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rx, v + (uint32_t) i * (uint32_t) g.E * 4, 0, 0)); }
+        d.k = *reinterpret_cast<const gs8 *>(o.kt + t + 8 * q);
+    };
+    auto copy_z = [&](int s, int b) {   // 4 x 8 rows' halves, as they are stored
+        const int st = min(s, s1 - 1);
+        const __amdgpu_buffer_rsrc_t rz = rg_rsrc(o.zt + (size_t) st * 4 * 2 * EA * 8, (uint32_t) AB);
+#pragma unroll
+        for (int i = 0; i < AB / 1024 / RG_W; ++i) { rg_lds16(rz, lds + b * BUF + (wave + i * RG_W) * 1024, (uint32_t) (lane * 16), (uint32_t) ((wave + i * RG_W) * 1024)); }
+    };
+    int kc = 200;   // the wave's columns' k (column r, the same in the four lane groups)
+    auto convert = [&](const Slab & sl, int b) {
+        float y[8], m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { y[i] = ldexpf(sl.x[i], K0 - (int) sl.k[i]); m = fmaxf(m, fabsf(y[i])); }
+        if (__ballot(!(m < INFINITY))) {
+            m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { m = fmaxf(m, rg_mag(y[i])); }
+        }
+        m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+        if (m > 0.f) { kc = min(kc, rg_k(m)); }
+        const float sc = rg_pow2(kc);
+        gh8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { _Float16 h, l; rg_split(y[i] * sc, h, l); hi[i] = h; lo[i] = l; }
+        LK_LOCAL uint8_t * d = lds + b * BUF + AB + (q * 2 * RG_COLS + 16 * wave + r) * 16;
+        *(LK_LOCAL gh8 *) d = hi; *(LK_LOCAL gh8 *) (d + RG_COLS * 16) = lo;
+        if (q == 0) { *(LK_LOCAL int *) (lds + b * BUF + AB + BB + (16 * wave + r) * 4) = kc; }
+    };
+    gf4 acc[4][JW];
+    int cur[JW];
+#pragma unroll
+    for (int c = 0; c < JW; ++c) {
+        cur[c] = 200;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { acc[i][c] = (gf4) { 0.f, 0.f, 0.f, 0.f }; }
+    }
+    Slab sl[3];   // three steps of x ahead: a step is about 0.6 us, memory answers in 1 to 2
+    constexpr int LX = 9;   // loads of a slab
+    auto step = [&](int s, Slab & next) {   // next: step s + 1's slab
+            const int b = (s - s0) & 1;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0x0f70 | LX);   // all but the last slab's loads: this wave's copies of step s have landed
+            __syncthreads();                           // and everyone's, with x's halves; the other buffer is free
+            if (s + 1 < s1) { copy_z(s + 1, b ^ 1); convert(next, b ^ 1); }
+            load_x(s + 4, next);
+            __builtin_amdgcn_sched_barrier(0);
+            const uint32_t lb = (uint32_t) (size_t) lds + (uint32_t) (b * BUF);
+#pragma unroll
+            for (int c = 0; c < JW; ++c) {   // columns whose k went down: what is summed so far follows
+                const int k = *(const LK_LOCAL int *) (size_t) (lb + AB + BB + (uint32_t) ((16 * JW * wj + 16 * c + r) * 4));
+                if (__ballot(k != cur[c])) {
+                    const float f = rg_pow2(k - cur[c]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { acc[i][c] = acc[i][c] * f; }
+                    cur[c] = k;
+                }
+            }
+            gh8 xh[JW], xl[JW];
+#pragma unroll
+            for (int c = 0; c < JW; ++c) {
+                const uint32_t a = lb + AB + (uint32_t) ((q * 2 * RG_COLS + 16 * JW * wj + 16 * c + r) * 16);
+                xh[c] = *(const LK_LOCAL gh8 *) (size_t) a; xl[c] = *(const LK_LOCAL gh8 *) (size_t) (a + RG_COLS * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t a = lb + (uint32_t) ((q * 2 * EA + 64 * we + 16 * i + r) * 16);
+                const gh8 zh = *(const LK_LOCAL gh8 *) (size_t) a, zl = *(const LK_LOCAL gh8 *) (size_t) (a + EA * 16);
+#pragma unroll
+                for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, xh[c], acc[i][c], 0, 0, 0); }
+#pragma unroll
+                for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, xl[c], acc[i][c], 0, 0, 0); }
+#pragma unroll
+                for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zl, xh[c], acc[i][c], 0, 0, 0); }
+            }
+    };
+    load_x(s0, sl[0]);
+    copy_z(s0, 0);
+    convert(sl[0], 0);
+    load_x(s0 + 1, sl[0]); load_x(s0 + 2, sl[1]); load_x(s0 + 3, sl[2]);
+    for (int s = s0;;) {   // (past the run's end: its last rows again, unread)
+        step(s, sl[0]);
+        if (++s == s1) { break; }
+        step(s, sl[1]);
+        if (++s == s1) { break; }
+        step(s, sl[2]);
+        if (++s == s1) { break; }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // no copy into LDS outlives the workgroup
+    float * out = splits > 1 ? part + (size_t) run * g.n_exp * g.E : g.dW;
+#pragma unroll
+    for (int c = 0; c < JW; ++c) {
+        const int k = cur[c] == 200 || K0 == RG_NONE ? 0 : -cur[c] - K0;   // (200: nothing but zeros in the column)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int e = 64 * we + 16 * i + 4 * q + u;
+                if (e < g.n_exp) {
+                    float * d = out + (size_t) e * g.E + j0 + 16 * JW * wj + 16 * c + r;
+                    const float v = ldexpf(acc[i][c][u], k);
+                    *d = splits == 1 && g.accumulate ? *d + v : v;
+                }
+            }
+        }
+    }
+}
+// both products in one launch: the first E / 128 x splits workgroups dW, the others dx (E / 128 x parts)
+template <int RT, int WR>
+__global__ void __launch_bounds__(RG_T, 2) k_route_mm(RouteGradArgs g, Ops o, int splits, int parts, float * part) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t rg_dyn[];
+    const int ct = g.E / RG_COLS, b = (int) blockIdx.x, dw = g.dW ? ct * splits : 0;
+    if (b < dw) { route_dw<WR>(g, o, (LK_LOCAL uint8_t *) rg_dyn, b % ct, b / ct, splits, part); }
+    else { route_dx<RT>(g, o, (LK_LOCAL uint8_t *) rg_dyn, (b - dw) % ct, (b - dw) / ct, parts); }
+}
+// the runs' sums, in order
+__global__ void __launch_bounds__(256) k_route_join(const float * __restrict__ part, int splits, int64_t n4, int accumulate, float * __restrict__ dW) {
+    const int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) { return; }
+    gf4 v = reinterpret_cast<const gf4 *>(part)[i];
+    for (int s = 1; s < splits; ++s) { v = v + reinterpret_cast<const gf4 *>(part)[(int64_t) s * n4 + i]; }
+    gf4 * d = reinterpret_cast<gf4 *>(dW) + i;
+    *d = accumulate ? *d + v : v;
+}
+
+int rg_splits(int n, int E) { return std::max(1, std::min((n + 127) / 128, 256 / (E / RG_COLS))); }
+constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+struct Sizes { int kp, ea, np; size_t zs, zt, kt, wt, kw, part, all; };
+Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
+    Sizes z{};
+    z.kp = (ne + 31) / 32 * 32; z.ea = ne <= 64 ? 64 : ne <= 128 ? 128 : 256; z.np = (n + 31) / 32 * 32;
+    z.zs = up256((size_t) n * 2 * z.kp * 2); z.zt = up256((size_t) z.np * 2 * z.ea * 2); z.kt = up256((size_t) z.np * 2);
+    z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = up256((size_t) (E / 64) * 4);
+    const int sp = rg_splits(n, E);
+    z.part = dW && sp > 1 ? (size_t) sp * ne * E * 4 : 0;
+    z.all = z.zs + z.zt + z.kt + z.wt + z.kw + z.part;
+    return z;
+}
+template <class F> hipError_t allow_lds(F * f, int bytes) { return hipFuncSetAttribute((const void *) f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
+template <int RT, int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
+    constexpr int DW = 2 * (4 * 2 * 64 * WR * 16 + 4 * 2 * RG_COLS * 16 + RG_COLS * 4), DX = 2 * 64 * WR * RG_COLS * 2;
+    static const hipError_t set = allow_lds(&k_route_mm<RT, WR>, std::max(DW, DX));
+    if (set != hipSuccess) { return set; }
+    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RT - 1) / (16 * RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, 256 / ct));
+    k_route_mm<RT, WR><<<(unsigned) (ct * ((a.dW ? sp : 0) + (a.dx ? parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, sp, parts, part);
+    return hipGetLastError();
+}
+template <int RT> hipError_t go_wr(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
+    return o.ea == 64 ? go<RT, 1>(a, o, sp, part, st) : o.ea == 128 ? go<RT, 2>(a, o, sp, part, st) : go<RT, 4>(a, o, sp, part, st);
 }
 
 }  // namespace
 
-hipError_t launch_route_grad(const RouteGradArgs & a, hipStream_t st) {
-    if (a.n < 0 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.E <= 0 || a.E % 64 || a.topk < 1 || a.topk > MAXK || !a.dz) { return hipErrorInvalidValue; }
-    if (a.n > 0) { k_route_dz<<<(a.n + 3) / 4, 256, 0, st>>>(a); }
-    if (a.dW) { k_route_mm<<<dim3(a.E / 64, (a.n_exp + 15) / 16), 64, 0, st>>>(a.dz, 1, a.n_exp, a.x, a.n_exp, a.E, a.n, a.dW, a.accumulate); }
-    if (a.dx && a.n > 0) { k_route_mm<<<dim3(a.E / 64, (a.n + 15) / 16), 64, 0, st>>>(a.dz, a.n_exp, 1, a.W, a.n, a.E, a.n_exp, a.dx, 0); }
-    return hipGetLastError();
+size_t route_grad_scratch(int n, int n_exp, int E, bool dW, bool dx) { return n > 0 ? rg_sizes(n, n_exp, E, dW, dx).all : 0; }
+
+hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_t st) {
+    if (a.n < 0 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.E <= 0 || a.E % 1024 || a.topk < 1 || a.topk > MAXK || (a.n > 0 && !scratch)) { return hipErrorInvalidValue; }
+    if (a.n == 0) { return hipSuccess; }
+    const Sizes z = rg_sizes(a.n, a.n_exp, a.E, a.dW != nullptr, a.dx != nullptr);
+    Ops o{};
+    uint8_t * p = (uint8_t *) scratch;
+    o.kp = z.kp; o.ea = z.ea; o.np = z.np;
+    o.zs = (_Float16 *) p; p += z.zs; o.zt = (_Float16 *) p; p += z.zt; o.kt = (short *) p; p += z.kt; o.wt = (_Float16 *) p; p += z.wt; o.kw = (int *) p; p += z.kw;
+    float * part = (float *) p;
+    const int nw = a.dx ? a.E / 64 : 0, sp = rg_splits(a.n, a.E);
+    k_route_prep<<<nw + z.np / 8, 256, 0, st>>>(a, o, nw);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && (a.dW || a.dx)) { e = a.n <= 2048 ? go_wr<2>(a, o, sp, part, st) : go_wr<4>(a, o, sp, part, st); }
+    if (e == hipSuccess && a.dW && sp > 1) {
+        const int64_t n4 = (int64_t) a.n_exp * a.E / 4;
+        k_route_join<<<(unsigned) ((n4 + 255) / 256), 256, 0, st>>>(part, sp, n4, a.accumulate, a.dW);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 }  // namespace lk

@@ -2,12 +2,12 @@
 (_train_ref.py).
 
 Tolerances, with u = 2^-24 (half an fp32 step):
-  loss    every term is positive, so relative errors add up along the longest chain. p: exp and its argument's sign (2 u), 1 + t, a
-          division and a product (3 u), the row's sum (4 + 8 adds, and its terms' 5 u), the reciprocal and a product (2 u): 24 u.
-          The mean: rows of a wave one after another, 16 waves, chunks / 4 + 3, the division. f and alpha: 6 u; the experts' sum: 12.
-          n rows: (24 + n + 16 + 68 + 1 + 6 + 12 + 2) u is an upper bound.
-  dlogits a product of p (24 u), 1 - s (5 u), k (4 u) and f - D: f 3 u, D = sum f p 24 + 3 + 12 u, relative to f + D:
-          90 u of |k| p (1 - s) (f + D).
+  loss    every term is positive, so relative errors add up along the longest chain. p: exp (3 u), 1 + t, a reciprocal of 2 u and a
+          product (7 u in all), the row's sum (4 + 7 adds, and its terms' 7 u), its reciprocal and a product (3 u): 28 u. The mean:
+          rows of a wave one after another (at most n / 16 + 4), 16 waves, chunks / 4 + 3 <= 67, the division. f and alpha: 6 u; the
+          experts' sum: 12. (130 + n) u is an upper bound from n = 5 on, and below there is one chunk: 28 + n + 16 + 21 u.
+  dlogits a product of p (28 u), 1 - s (7 u), k (4 u) and f - D: f 3 u, D = sum f p 28 + 3 + 12 u, relative to f + D, and three
+          roundings: within 90 u of |k| p (1 - s) (f + D).
   dz      s and 1 - s 5 u each, S and D over at most 8 picks: 60 u of scale / S (|dw| + sum |dw| s / S) s (1 - s), and one rounding
           for dz_in.
   dW, dx  against the 64-bit product of the kernel's own dlogits: per product 3 * 2^-22 (operands in two 11-bit halves, the product

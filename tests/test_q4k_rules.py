@@ -1,0 +1,63 @@
+"""CPU: which Q4_K kernel a product gets (loki_amd/csrc/launch_rules.h), compiled as it is and checked over the sizes that the entry
+point takes."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "loki_amd", "csrc", "launch_rules.h")
+NS = [1, 2, 3, 8, 16, 17, 32, 33, 48, 49, 64, 100, 128, 129, 500, 2048, 65536]
+RS = [1, 15, 16, 17, 64, 512, 1024, 1025, 2048, 7168, 24576, 24577, 131072, 1 << 22]
+KS = [256, 512, 2048, 7168, 16384, 65536]
+
+
+@pytest.fixture(scope="module")
+def rules(tmp_path_factory):
+    d = tmp_path_factory.mktemp("q4")
+    src, so = d / "rules.cpp", d / "rules.so"
+    src.write_text('#include "%s"\nusing namespace lk;\n' % HEADER +
+                   'extern "C" int pick(int n, int64_t R, int K, int tiles) { return q4k_kernel(n, R, K, tiles); }\n'
+                   'extern "C" int tiled(int k) { return q4k_tiled(k); }\n'
+                   'extern "C" int count() { return Q4_KERNELS; }\n'
+                   'extern "C" int toks(int k) { return Q4_KERNEL[k].toks; }\n'
+                   'extern "C" float us(int k, int n, int64_t R, int K) { return q4k_us(Q4_KERNEL[k], n, R, K); }\n')
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
+    lib = ctypes.CDLL(str(so))
+    lib.pick.argtypes = [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int]
+    lib.us.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int]
+    lib.us.restype = ctypes.c_float
+    return lib
+
+
+def test_every_size_gets_a_kernel_that_may_be_taken(rules):
+    vec = rules.count()
+    seen = set()
+    for n in NS:
+        for R in RS:
+            for K in KS:
+                for tiles in (0, 1):
+                    k = rules.pick(n, R, K, tiles)
+                    assert 0 <= k <= vec
+                    assert k != vec or n == 1
+                    assert tiles or not rules.tiled(k)
+                    seen.add(k)
+                    if k < vec:   # the least estimate of those allowed
+                        assert all(rules.us(k, n, R, K) <= rules.us(j, n, R, K) for j in range(vec) if (tiles and n > 16) or not rules.tiled(j))
+    assert seen == set(range(vec + 1)), "a kernel that no size reaches"
+
+
+def test_estimates_grow_with_the_work(rules):
+    for k in range(rules.count()):
+        for R in RS:
+            for K in KS:
+                t = [rules.us(k, n, R, K) for n in NS]
+                assert t == sorted(t)
+        assert all(rules.us(k, n, 7168, K1) < rules.us(k, n, 7168, K2) for n in NS for K1, K2 in zip(KS, KS[1:]))
+
+
+def test_few_tokens_do_not_take_many_token_tiles(rules):
+    for R in RS:
+        for K in KS:
+            assert rules.pick(1, R, K, 1) in (0, rules.count())
+            assert not rules.tiled(rules.pick(16, R, K, 1))
