@@ -4,10 +4,26 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <stddef.h>
+#include <atomic>
 #include "moe_common.h"
 #include "launch_rules.h"
 
 namespace lk {
+
+// a kernel's limit of dynamic LDS, set on each device before its first launch there
+struct LdsLimit {
+    std::atomic<uint64_t> set{0};   // a bit a device
+    hipError_t operator()(const void * kernel, int bytes) {
+        int dev = 0;
+        hipError_t e = hipGetDevice(&dev);
+        if (e != hipSuccess) { return e; }
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (set.load(std::memory_order_acquire) & bit) { return hipSuccess; }
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == hipSuccess) { set.fetch_or(bit, std::memory_order_release); }
+        return e;
+    }
+};
 
 // Q8_K of nrows rows of K floats (K % 256 == 0): q [nrows][K], d [nrows][K/256]
 hipError_t launch_quant_q8k(const float * x, int64_t nrows, int K, int8_t * q, float * d, hipStream_t st);

@@ -15,7 +15,7 @@
 //   W    one k per 64 columns, found by the kernel that splits it
 //   x    one k per column, running: a slab's maximum that passes the present range lowers k, and the accumulators of that column
 //        follow (as the running maximum of an online softmax)
-// Non-finite values take no part in the maxima; they make the outputs that they enter non-finite.
+// Non-finite values take no part in the maxima of dz and W; they make the outputs that they enter non-finite.
 #include "moe_device.h"
 #include "moe_kernels.h"
 
@@ -169,13 +169,14 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
     }
 }
 
-constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128;
+constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128, RG_RT = 2;
 
-// dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 16 RT rows at a
-// time, whose dz comes straight from memory, the next 32 experts' in flight; no barrier after the first. The product runs with the
-// columns as rows of the matrix core's tile, so a lane stores 4 consecutive columns.
-template <int RT>
+// dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 32 rows at a time,
+// whose dz comes straight from memory, the next 32 experts' in flight; no barrier after the first. The product runs with the columns
+// as rows of the matrix core's tile, so a lane stores 4 consecutive columns. 64 rows a wave read LDS half as often and are 1 to 2 %
+// faster from 12000 rows on, but leave waves idle before: 1001 rows of 7168, 256 experts, both products 62 us instead of 51.
 __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int part, int parts) {
+    constexpr int RT = RG_RT;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
     const int j0 = ct * RG_COLS, nb = o.kp / 8, ns = o.kp / 32;
     const __amdgpu_buffer_rsrc_t rw = rg_rsrc(o.wt, (uint32_t) ((size_t) 2 * nb * g.E * 16));
@@ -291,20 +292,15 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
         float y[8], m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { y[i] = ldexpf(sl.x[i], K0 - (int) sl.k[i]); m = fmaxf(m, fabsf(y[i])); }
-        if (__ballot(!(m < INFINITY))) {
-            m = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { m = fmaxf(m, rg_mag(y[i])); }
-        }
         m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
-        if (m > 0.f) { kc = min(kc, rg_k(m)); }
+        kc = min(kc, m > 0.f ? rg_k(m) : kc);   // (a column with an infinity is non-finite in every expert, whatever its k)
         const float sc = rg_pow2(kc);
         gh8 hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { _Float16 h, l; rg_split(y[i] * sc, h, l); hi[i] = h; lo[i] = l; }
         LK_LOCAL uint8_t * d = lds + b * BUF + AB + (q * 2 * RG_COLS + 16 * wave + r) * 16;
         *(LK_LOCAL gh8 *) d = hi; *(LK_LOCAL gh8 *) (d + RG_COLS * 16) = lo;
-        if (q == 0) { *(LK_LOCAL int *) (lds + b * BUF + AB + BB + (16 * wave + r) * 4) = kc; }
+        *(LK_LOCAL int *) (lds + b * BUF + AB + BB + (16 * wave + r) * 4) = kc;   // (the same from the four lane groups)
     };
     gf4 acc[4][JW];
     int cur[JW];
@@ -321,8 +317,7 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(0x0f70 | LX);   // all but the last slab's loads: this wave's copies of step s have landed
             __syncthreads();                           // and everyone's, with x's halves; the other buffer is free
-            if (s + 1 < s1) { copy_z(s + 1, b ^ 1); convert(next, b ^ 1); }
-            load_x(s + 4, next);
+            copy_z(s + 1, b ^ 1);
             __builtin_amdgcn_sched_barrier(0);
             const uint32_t lb = (uint32_t) (size_t) lds + (uint32_t) (b * BUF);
 #pragma unroll
@@ -352,6 +347,11 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
 #pragma unroll
                 for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zl, xh[c], acc[i][c], 0, 0, 0); }
             }
+            convert(next, b ^ 1);
+            load_x(s + 4, next);
+#pragma unroll
+            for (int i = 0; i < 12 * JW; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x002, 2, 0); }
+            __builtin_amdgcn_sched_barrier(0);
     };
     load_x(s0, sl[0]);
     copy_z(s0, 0);
@@ -385,12 +385,12 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
     }
 }
 // both products in one launch: the first E / 128 x splits workgroups dW, the others dx (E / 128 x parts)
-template <int RT, int WR>
+template <int WR>
 __global__ void __launch_bounds__(RG_T, 2) k_route_mm(RouteGradArgs g, Ops o, int splits, int parts, float * part) {
     extern __shared__ __attribute__((aligned(16))) uint8_t rg_dyn[];
     const int ct = g.E / RG_COLS, b = (int) blockIdx.x, dw = g.dW ? ct * splits : 0;
     if (b < dw) { route_dw<WR>(g, o, (LK_LOCAL uint8_t *) rg_dyn, b % ct, b / ct, splits, part); }
-    else { route_dx<RT>(g, o, (LK_LOCAL uint8_t *) rg_dyn, (b - dw) % ct, (b - dw) / ct, parts); }
+    else { route_dx(g, o, (LK_LOCAL uint8_t *) rg_dyn, (b - dw) % ct, (b - dw) / ct, parts); }
 }
 // the runs' sums, in order
 __global__ void __launch_bounds__(256) k_route_join(const float * __restrict__ part, int splits, int64_t n4, int accumulate, float * __restrict__ dW) {
@@ -415,17 +415,13 @@ Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
     z.all = z.zs + z.zt + z.kt + z.wt + z.kw + z.part;
     return z;
 }
-template <class F> hipError_t allow_lds(F * f, int bytes) { return hipFuncSetAttribute((const void *) f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); }
-template <int RT, int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
+template <int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
     constexpr int DW = 2 * (4 * 2 * 64 * WR * 16 + 4 * 2 * RG_COLS * 16 + RG_COLS * 4), DX = 2 * 64 * WR * RG_COLS * 2;
-    static const hipError_t set = allow_lds(&k_route_mm<RT, WR>, std::max(DW, DX));
-    if (set != hipSuccess) { return set; }
-    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RT - 1) / (16 * RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, 256 / ct));
-    k_route_mm<RT, WR><<<(unsigned) (ct * ((a.dW ? sp : 0) + (a.dx ? parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, sp, parts, part);
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_route_mm<WR>, std::max(DW, DX))) { return e; }
+    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RG_RT - 1) / (16 * RG_RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, 256 / ct));
+    k_route_mm<WR><<<(unsigned) (ct * ((a.dW ? sp : 0) + (a.dx ? parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, sp, parts, part);
     return hipGetLastError();
-}
-template <int RT> hipError_t go_wr(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
-    return o.ea == 64 ? go<RT, 1>(a, o, sp, part, st) : o.ea == 128 ? go<RT, 2>(a, o, sp, part, st) : go<RT, 4>(a, o, sp, part, st);
 }
 
 }  // namespace
@@ -444,7 +440,7 @@ hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_
     const int nw = a.dx ? a.E / 64 : 0, sp = rg_splits(a.n, a.E);
     k_route_prep<<<nw + z.np / 8, 256, 0, st>>>(a, o, nw);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && (a.dW || a.dx)) { e = a.n <= 2048 ? go_wr<2>(a, o, sp, part, st) : go_wr<4>(a, o, sp, part, st); }
+    if (e == hipSuccess && (a.dW || a.dx)) { e = o.ea == 64 ? go<1>(a, o, sp, part, st) : o.ea == 128 ? go<2>(a, o, sp, part, st) : go<4>(a, o, sp, part, st); }
     if (e == hipSuccess && a.dW && sp > 1) {
         const int64_t n4 = (int64_t) a.n_exp * a.E / 4;
         k_route_join<<<(unsigned) ((n4 + 255) / 256), 256, 0, st>>>(part, sp, n4, a.accumulate, a.dW);
