@@ -278,6 +278,12 @@ extern "C" int fl_quant_q8k_dev(FLCtx * c, const float * x, int nrows, int K, in
     return FL_OK;
 }
 
+// the context's device has to be the current one (its stream and workspaces live there)
+static int need_device(FLCtx * c) {
+    int dev = -1;
+    TRY(c, hipGetDevice(&dev));
+    return dev == c->dev ? FL_OK : fail(c, FL_EINVAL, "the current device is %d, the context's %d", dev, c->dev);
+}
 // Q4_K products of many rows take a scratch (their rows' sub-block sums)
 static int q4_scratch(FLCtx * c, KqArgs & k, int fmt) {
     const size_t bytes = fmt == FL_Q4K ? q4k_scratch_bytes(k.n, (int64_t) k.R * (k.w2 ? 2 : 1), k.K) : 0;
@@ -292,12 +298,19 @@ extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K
     if (bs == 0) { return fail(c, FL_EINVAL, "format %d is not a K-quant (FL_Q2K, FL_Q3K, FL_Q4K, FL_Q5K, FL_Q6K)", fmt); }
     const int kmax = fmt == FL_Q4K ? 65536 : 8192;
     if (R <= 0 || K <= 0 || K % 256 || K > kmax || n < 0) { return fail(c, FL_EINVAL, "R %d, K %d (a multiple of 256, at most %d), n %d", R, K, kmax, n); }
+    if (fmt == FL_Q4K && (R > 1 << 26 || n > 1 << 19)) { return fail(c, FL_EINVAL, "R %d, n %d: at most 2^26 rows and 2^19 tokens", R, n); }
     if (n == 0) { return FL_OK; }
     if (!w || !q || !d || !y) { return fail(c, FL_EINVAL, "null pointer"); }
     const size_t mb = (size_t) R * (size_t) (K / 256) * (size_t) bs;
     if (mb % 4 || (reinterpret_cast<uintptr_t>(w) & 3u)) { return fail(c, FL_EINVAL, "the matrix must start and end on 4-byte boundaries (%zu bytes)", mb); }
     if (!covers(w, mb) || !covers(q, (size_t) n * K) || !covers(d, (size_t) n * (K / 256) * 4) || !covers(y, (size_t) n * R * 4)) {
         return fail(c, FL_EINVAL, "an allocation is smaller than its shape");
+    }
+    if (fmt == FL_Q4K) {
+        if ((reinterpret_cast<uintptr_t>(q) & 15u) || ((reinterpret_cast<uintptr_t>(d) | reinterpret_cast<uintptr_t>(y)) & 3u)) {
+            return fail(c, FL_EINVAL, "q must be 16-byte aligned, d and y 4-byte");
+        }
+        if (int rc = need_device(c)) { return rc; }
     }
     KqArgs a{};
     a.w = (const uint8_t *) w; a.estride = mb; a.aq = q; a.ad = d; a.K = K; a.R = R;
@@ -308,12 +321,6 @@ extern "C" int fl_kq_matvec_dev(FLCtx * c, int fmt, const void * w, int R, int K
 }
 
 // ---------------------------------------------------------------- the router's training side
-// the context's device has to be the current one (its stream and workspaces live there)
-static int need_device(FLCtx * c) {
-    int dev = -1;
-    TRY(c, hipGetDevice(&dev));
-    return dev == c->dev ? FL_OK : fail(c, FL_EINVAL, "the current device is %d, the context's %d", dev, c->dev);
-}
 static int balance_args(FLCtx * c, BalanceArgs & b) {
     if (b.n < 0 || b.topk < 1 || b.topk > MAXK || (int64_t) b.n * b.topk > (1 << 24)) { return fail(c, FL_ERANGE, "n %d, topk %d (1..%d, n * topk at most 2^24)", b.n, b.topk, MAXK); }
     if (b.n_exp < 1 || b.n_exp > NEXP_MAX) { return fail(c, FL_EINVAL, "n_exp %d outside 1..%d", b.n_exp, NEXP_MAX); }
@@ -525,9 +532,12 @@ static hipError_t launch_decode(FLCtx * c, const DecodeArgs & d, hipStream_t st)
 // the block on x, or on RMSNorm(x) * nw when prenorm (nw may be null: ones); resid (may be null) is added to the output
 // bytes of one R x K matrix in format f (IQ2_XXS or a K-quant)
 static size_t fmt_mat_bytes(int f, int R, int K) { return (size_t) R * (K / 256) * (size_t) (f == FL_IQ2 ? IQ2B : kq_block_bytes(f)); }
+// the Q4_K tiles' scratch, where it is as large as a product of R rows takes (moe_layer sees to it for its own)
+static void * kq_xs(FLCtx * c, int fmt, int n, int64_t R, int K) { return fmt == FL_Q4K && q4k_scratch_bytes(n, R, K) <= c->q4.cap ? c->q4.p : nullptr; }
 // K-quant mat-vec of one matrix (ggml layout, in place) on n Q8_K rows -> out [n][R]
 static hipError_t kq_one(FLCtx * c, int fmt, const void * w, const int8_t * q, const float * d, int n, int K, int R, float * out, hipStream_t st) {
     KqArgs k{};
+    k.xs = kq_xs(c, fmt, n, R, K);
     k.w = (const uint8_t *) w; k.estride = fmt_mat_bytes(fmt, R, K); k.aq = q; k.ad = d; k.K = K; k.R = R;
     k.n = n; k.out = out; k.ldo = R;
     return launch_kq_matvec(k, fmt, n, 1, st);
@@ -563,6 +573,7 @@ static int shared_gateup_sep(FLCtx * c, const FLMoeLayer * L, int n, int P, int 
         KqArgs k{};
         k.w = (const uint8_t *) L->sh_gate; k.w2 = (const uint8_t *) L->sh_up; k.estride = fmt_mat_bytes(lf[1], H, E);
         k.aq = c->xq.p; k.ad = c->xd.p; k.K = E; k.R = H; k.n = n; k.out = c->ksg.p; k.out2 = c->ksu.p; k.ldo = H;
+        k.xs = kq_xs(c, lf[1], n, 2 * (int64_t) H, E);
         TRY(c, launch_kq_matvec(k, lf[1], n, 1, st));
     } else {
         TRY(c, kq_one(c, lf[1], L->sh_gate, c->xq.p, c->xd.p, n, E, H, c->ksg.p, st));
@@ -698,6 +709,11 @@ static int moe_layer(FLCtx * c, const FLMoeLayer * L, const float * x, int n, fl
     if (!fused) { ALLOC(c, c->h, rows * H); ALLOC(c, c->hq, rows * H); ALLOC(c, c->hd, rows * (H / 256)); ALLOC(c, c->o, rows * E); }
     if (c->dbg_gu) { ALLOC(c, c->g, rows * H); ALLOC(c, c->u, rows * H); }
     if (int rc = ensure_expert_scratch(c, rows, E, H)) { return rc; }
+    {   // the shared expert's Q4_K matrices on tiles
+        const size_t gu = q4k_scratch_bytes(n, lf[1] == lf[2] ? 2 * (int64_t) H : H, E), dn = q4k_scratch_bytes(n, E, H);
+        const size_t q4 = std::max(lf[1] == FL_Q4K || lf[2] == FL_Q4K ? gu : 0, lf[3] == FL_Q4K ? dn : 0);
+        if (q4 > 0 && c->q4.ensure(q4) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", q4); }
+    }
     c->last_n = n; c->last_P = P; c->last_fused = fused ? 1 : 0; c->last_kernel = 0;
     hipStream_t st = c->st;
     std::vector<hipEvent_t> * ev = prof_begin(c);

@@ -197,9 +197,9 @@ __device__ __forceinline__ void q4_mins(const u32x4 & hd, uint32_t (&mm)[2]) {
 }
 
 // Few tokens: a workgroup's 8 waves share its rows and tokens and split K, wave w taking blocks w, w + 8, ... of the rows. A round's 8
-// blocks of a row are 1152 consecutive bytes: they are copied into LDS in whole (a wave's lanes fetching 16 rows' pieces of 64
-// bytes themselves make twice the cache accesses, which then bound the kernel: 73 us instead of 5x for one token through 65536
-// rows of 7168), a round ahead. Activations come into registers straight from the caches, also a round ahead. Each round leaves the
+// blocks of a row are 1152 consecutive bytes: they are copied into LDS in whole, a round ahead (a wave's lanes fetching 16 rows'
+// pieces of 64 bytes themselves make twice the cache accesses, 37 a load instead of 19, and those bound the kernel: 32 tokens through
+// 7168 rows of 16384 36.6 us instead of 31.8, 16 tokens through 65536 rows of 7168 95 instead of 86). Activations come into registers straight from the caches, also a round ahead. Each round leaves the
 // blocks' terms in LDS, and the workgroup's lanes run the chains over them, an output or two a lane. summ comes from a third
 // product with the step's min in every byte (here the matrix cores have time to spare).
 constexpr int KS_W = 8, KS_PITCH = 9 * KS_W + 1;   // 16-byte chunks from row to row in LDS: 16 rows start in 16 different quads of banks
@@ -346,12 +346,13 @@ done:
             const int p = threadIdx.x + 64 * KS_W * i, q = p >> 4, t = q % TOK, row = 16 * (q / TOK) + (p & 15);
             if (p < RT * TOK * 16 && t < nt && row < nrow) { Out[(size_t) (sg + t) * a.ldo + row0 + row] = acc[i]; }
         }
-        __syncthreads();   // the buffers are free for the next group
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // no copy into LDS is out (the last rounds' fetch nothing, but write)
+        __syncthreads();                      // the buffers are free for the next group, or the next workgroup
     }
 }
 template <int RT, int NT> hipError_t ks(const KqArgs & a, unsigned gy, hipStream_t st) {
-    static const hipError_t set = hipFuncSetAttribute((const void *) k_q4k_ks<RT, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, KsLds<RT, NT>::ALL);
-    if (set != hipSuccess) { return set; }
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_q4k_ks<RT, NT>, KsLds<RT, NT>::ALL)) { return e; }
     k_q4k_ks<RT, NT><<<dim3((unsigned) ((a.R + 16 * RT - 1) / (16 * RT)), gy, a.act ? 1u : (unsigned) ((a.n + 16 * NT - 1) / (16 * NT))), 64 * KS_W, KsLds<RT, NT>::ALL, st>>>(a);
     return hipGetLastError();
 }
@@ -526,8 +527,8 @@ done:
 
 template <int RT, int NT, int W, int D> hipError_t mm(const KqArgs & k, hipStream_t st) {
     constexpr int LDS = D * 16 * NT * (256 + 32 + 4);
-    static const hipError_t set = hipFuncSetAttribute((const void *) k_q4k_mm<RT, NT, W, D>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (set != hipSuccess) { return set; }
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_q4k_mm<RT, NT, W, D>, LDS)) { return e; }
     Q4Args a{};
     a.w = k.w; a.w2 = k.w2; a.aq = k.aq; a.ad = k.ad; a.xs = (const _Float16 *) k.xs; a.K = k.K; a.R = k.R; a.n = k.n;
     a.out = k.out; a.out2 = k.out2; a.ldo = k.ldo;

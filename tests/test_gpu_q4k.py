@@ -8,6 +8,7 @@ import pytest
 
 from oracle import oracle as orc
 from tests._q4k import matrix, q8k_rows
+from tests.test_q4k_rules import SIZES
 
 pytestmark = pytest.mark.gpu
 
@@ -106,6 +107,30 @@ def test_unaligned_start_and_untouched_surroundings(ctx, n):
     assert same(o[16:16 + n * R].reshape(n, R), orc.matvec_kq(orc.Q4K, w, R, K, q, d, bs))
 
 
+@pytest.mark.parametrize("name", SIZES)
+def test_every_kernel(ctx, name):
+    """ragged sizes that the launch rule gives each of the kernels for many tokens (test_q4k_rules.py holds it to that), the matrix 4
+    bytes off a 16-byte boundary; the largest block sums in three rows and two tokens"""
+    import torch
+    for R, K, n in SIZES[name][1]:
+        w = matrix(R + 7, R, K).reshape(R, K // 256, 144).copy()
+        for r in (0, 17, R - 1):
+            w[r, :, 4:] = 0xFF
+        w = w.reshape(-1)
+        q, d, _ = q8k_rows(n, K, seed=R + n)
+        q[0], q[n - 1] = 127, -127
+        bs = q.reshape(n, K // 16, 16).sum(axis=2).astype(np.int16)
+        buf = torch.zeros(len(w) + 64, dtype=torch.uint8, device="cuda")
+        buf[4:4 + len(w)] = torch.from_numpy(w).cuda()
+        out = torch.full((n * R + 32,), -7.0, device="cuda")
+        print("q4_K %s R %d K %d n %d" % (name, R, K, n), flush=True)
+        ctx.kq_matvec(orc.Q4K, buf[4:4 + len(w)], R, K, torch.from_numpy(q).cuda(), torch.from_numpy(d).cuda(), out[16:16 + n * R])
+        ctx.sync()
+        o = out.cpu().numpy()
+        assert np.all(o[:16] == -7.0) and np.all(o[16 + n * R:] == -7.0)
+        assert same(o[16:16 + n * R].reshape(n, R), orc.matvec_kq(orc.Q4K, w, R, K, q, d, bs)), (R, K, n)
+
+
 def test_refusals(ctx):
     import torch
     from loki_amd import FL_EINVAL, FL_OK, FL_Q4K, lib
@@ -120,11 +145,68 @@ def test_refusals(ctx):
     big = 1 << 26
     assert call(big, 256, 1) == FL_EINVAL and b"smaller" in L.fl_last_error(ctx.ctx)
     assert L.fl_kq_matvec_dev(ctx.ctx, FL_Q4K, None, 2, 256, P(q), P(d), 1, P(y)) == FL_EINVAL
+    assert call((1 << 26) + 1, 256, 1) == FL_EINVAL and call(2, 256, (1 << 19) + 1) == FL_EINVAL and b"2^19" in L.fl_last_error(ctx.ctx)
+    assert L.fl_kq_matvec_dev(ctx.ctx, FL_Q4K, P(w), 2, 256, P(q, 4), P(d), 1, P(y)) == FL_EINVAL and b"aligned" in L.fl_last_error(ctx.ctx)
+    assert call(2, 256, 1, yp=P(y, 2)) == FL_EINVAL
     assert call(2, 256, 0) == FL_OK and call(2, 256, 2) == FL_OK
     ctx.sync()
 
 
 # ---------------------------------------------------------------- as a format of the block
+def random_matrix(fmt, R, K, seed):
+    """device bytes of a matrix of the format, its scales small"""
+    import torch
+    from tests.test_gpu_kquant import KQ_BLOCK
+    bs, od, om = {**KQ_BLOCK, orc.Q4K: (144, 0, 2)}[fmt]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    b = torch.randint(0, 256, (R * (K // 256), bs), dtype=torch.uint8, device="cuda", generator=g)
+    for off in (od, om):
+        if off is not None:
+            v = torch.randint(0x0C00, 0x1C00, (b.shape[0],), dtype=torch.int32, device="cuda", generator=g).to(torch.int16)
+            b[:, off:off + 2] = v.view(torch.uint8).view(-1, 2)
+    return b.view(-1)
+
+
+def test_layer_of_many_rows(ctx):
+    """fl_moe_layer's shared Q4_K matrices on the tiled kernels (rows enough for them): the shared expert's part, formed by the
+    products and Q8_K quantisation of their own, is what the block leaves in o's last rows, bit for bit; on the GEMM path and the
+    per-pass one (second stream)"""
+    import torch
+    from loki_amd import FL_Q4K, MoeLayerWeights, lib
+    from tests._helpers import make_x
+    ne, n = 16, 300
+    base = MoeLayerWeights.synthetic(ctx, 9190, n_exp=ne)
+    sg, su, sd = (random_matrix(FL_Q4K, r, k, 9191 + i) for i, (r, k) in enumerate(((H, E), (H, E), (E, H))))
+    layer = MoeLayerWeights(base.gate_inp, base.probs_b, base.gate, base.up, base.down, sg, su, sd, n_exp=ne)
+    x = make_x(ctx, n, seed=9192)
+    xq, xd = ctx.quant_q8k(x)
+    gate, up = (ctx.kq_matvec(FL_Q4K, m, H, E, xq, xd) for m in (sg, su))
+    ctx.sync()
+    gate, up = gate.cpu().numpy(), up.cpu().numpy()
+    ctx.set_routing(8, 4, 8, 2.5)
+    ctx.set_layer_formats(4, orc.Q4K, orc.Q4K, orc.Q4K)
+    try:
+        ys = []
+        for mfma in (1, 0):
+            lib().fl_set_prefill_mfma(ctx.ctx, mfma)
+            ys.append(ctx.moe_layer(layer, x))
+            ctx.sync()
+            h = ctx.d2h(ctx.debug().h, (n * KE + n, H), np.float32)[n * KE:]
+            hq, hd = ctx.quant_q8k(torch.from_numpy(h).cuda())
+            down = ctx.kq_matvec(FL_Q4K, sd, E, H, hq, hd)
+            ctx.sync()
+            o = ctx.d2h(ctx.debug().o, (n * KE + n, E), np.float32)[n * KE:]
+            assert same(o, down.cpu().numpy())
+            if mfma:
+                first = h
+            assert same(h, first)
+            assert same(h[[0, 7, n - 1]], np.stack([orc.silu(gate[t]) * up[t] for t in (0, 7, n - 1)]))
+    finally:
+        lib().fl_set_prefill_mfma(ctx.ctx, 1)
+        ctx.set_layer_formats()
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("fm", [(orc.Q4K, orc.Q4K, orc.Q4K, orc.Q4K), (orc.Q4K, orc.Q5K, orc.Q5K, orc.Q6K), (orc.Q2K, orc.Q4K, orc.Q5K, orc.Q4K),
                                 (orc.Q4K, 4, 4, 4)], ids=["all", "down", "shared", "down_iq2_shared"])
 def test_layer_formats(ctx, fm):

@@ -21,6 +21,7 @@ def rules(tmp_path_factory):
                    'extern "C" int tiled(int k) { return q4k_tiled(k); }\n'
                    'extern "C" int count() { return Q4_KERNELS; }\n'
                    'extern "C" int toks(int k) { return Q4_KERNEL[k].toks; }\n'
+                   'extern "C" int rows(int k) { return Q4_KERNEL[k].rows; }\n'
                    'extern "C" float us(int k, int n, int64_t R, int K) { return q4k_us(Q4_KERNEL[k], n, R, K); }\n')
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", str(src), "-o", str(so)], check=True)
     lib = ctypes.CDLL(str(so))
@@ -61,3 +62,35 @@ def test_few_tokens_do_not_take_many_token_tiles(rules):
         for K in KS:
             assert rules.pick(1, R, K, 1) in (0, rules.count())
             assert not rules.tiled(rules.pick(16, R, K, 1))
+
+
+# rows, columns, tokens of the device tests that go through each kernel (test_gpu_q4k.py), ragged in rows and tokens: 1 to 13 blocks a row
+SIZES = {"ks_32_32": (1, [(1001, 1024, 200), (7001, 512, 17)]), "ks_32_48": (2, [(7001, 768, 40), (2049, 256, 130)]),
+         "mm_64_32": (3, [(2049, 1024, 200), (8200, 768, 40), (1001, 3328, 403)]), "mm_64_64": (4, [(4100, 256, 130), (7001, 768, 257)]),
+         "mm_128_64": (5, [(8200, 512, 400), (4100, 2048, 257)]), "mm_128_128": (6, [(8200, 256, 601), (7001, 768, 400), (7001, 1280, 403)])}
+
+
+@pytest.mark.parametrize("name", SIZES)
+def test_sizes_that_reach_each_kernel(rules, name):
+    kernel, sizes = SIZES[name]
+    assert all(rules.pick(n, R, K, 1) == kernel for R, K, n in sizes), [rules.pick(n, R, K, 1) for R, K, n in sizes]
+
+
+def test_launches_fit_a_grid(rules):
+    """workgroups of 256 or 512 lanes along x below 2^32 lanes, along z (16 .. 48 tokens each) at most 65535, at every size that the
+    entry point takes (2^26 rows, 2^19 tokens) and 300 GB hold"""
+    n = 1
+    while n <= 1 << 19:
+        R = 1
+        while R <= 1 << 26:
+            for K in KS:
+                if max(4.0 * n * R, 0.5625 * R * K, 1.0 * n * K) < 3e11:
+                    k = rules.pick(n, R, K, 1)
+                    t, r = (rules.toks(k), rules.rows(k)) if k < rules.count() else (n, 1)
+                    tt, rt = -(-n // t), -(-R // r)
+                    if rules.tiled(k):
+                        assert rt * tt * 512 < 1 << 32, (n, R, K, k)
+                    else:
+                        assert tt <= 65535 and rt * (512 if k < rules.count() else 32) < 1 << 32, (n, R, K, k)
+            R = R + 1 if R < 16 else min(R * 3 // 2 + 1, 1 << 26) if R < 1 << 26 else R + 1
+        n = n + 1 if n < 20 else min(n * 4 // 3 + 1, 1 << 19) if n < 1 << 19 else n + 1
