@@ -50,25 +50,25 @@ constexpr int kq_shared_tok(int n) { return n <= 128 ? 16 : n <= 256 ? 32 : KQ_T
 // of rows x tokens, G of them, and with nb blocks a row a launch takes about
 //   max(s0 + s1 nb, ceil(G / 256) (p0 + p1 nb)) us:
 // what one workgroup needs from start to end, or the rounds of workgroups a CU goes through at its steady rate. The constants are
-// fitted to 223 sizes (512 .. 65536 rows, 4 .. 64 blocks, 4 .. 2000 tokens, weights from memory): 6 to 14 % rms a kernel, and
-// the pick is within 1.5 % of the best kernel on average. Examples, us: 40 tokens through 16384 -> 7168 39 (K split, 48
-// tokens a workgroup) against 46 (64 x 32 tiles), 59 (32 tokens, split); 128 through 7168 -> 16384 46 (128 x 64) against 51 (64 x 64)
-// and 75 (128 x 128); 2048 through it 485 (128 x 128) against 658 and 722.
+// fitted to 247 sizes (512 .. 65536 rows, 4 .. 64 blocks, 1 .. 2000 tokens, weights from memory): 5 to 13 % rms a kernel, and the pick
+// is within 1 % of the best kernel on average, 20 % at worst. Examples, us: 16 tokens through 16384 -> 7168 19 (K split, 32 rows x 16 tokens)
+// against 24 (16 x 16); 37 through it 33 (K split, 32 x 48) against 43 (32 x 16) and 46 (64 x 32 tiles); 128 through 7168 -> 16384 46
+// (128 x 64) against 51 (64 x 64) and 75 (128 x 128); 2048 through it 485 (128 x 128) against 658 and 722.
 struct Q4Kernel { int rows, toks; float s0, s1, p0, p1; };
-enum { Q4_KS_16_16, Q4_KS_32_32, Q4_KS_32_48, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_128_128, Q4_KERNELS, Q4_VEC = Q4_KERNELS };
+enum { Q4_KS_16_16, Q4_KS_32_16, Q4_KS_32_32, Q4_KS_32_48, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_128_128, Q4_KERNELS, Q4_VEC = Q4_KERNELS };
 constexpr Q4Kernel Q4_KERNEL[Q4_KERNELS] = {
-    { 16, 16, 3.8f, 0.13f, 1.1f, 0.14f }, { 32, 32, 4.1f, 0.37f, 2.9f, 0.39f }, { 32, 48, 4.7f, 0.48f, 3.5f, 0.50f }, { 64, 32, 5.8f, 0.62f, 1.5f, 0.58f },
-    { 64, 64, 5.1f, 0.90f, 1.9f, 0.77f }, { 128, 64, 5.5f, 1.28f, 4.2f, 1.32f }, { 128, 128, 6.5f, 2.33f, 4.0f, 2.15f } };
+    { 16, 16, 3.5f, 0.122f, 1.1f, 0.138f }, { 32, 16, 3.3f, 0.208f, 2.3f, 0.224f }, { 32, 32, 4.1f, 0.325f, 2.9f, 0.335f }, { 32, 48, 5.2f, 0.305f, 3.4f, 0.455f },
+    { 64, 32, 5.3f, 0.635f, 2.0f, 0.564f }, { 64, 64, 5.1f, 0.90f, 2.1f, 0.757f }, { 128, 64, 5.4f, 1.26f, 4.4f, 1.30f }, { 128, 128, 6.3f, 2.31f, 4.2f, 2.07f } };
 constexpr float q4k_us(const Q4Kernel & k, int n, int64_t R, int K) {
     const int64_t g = (R + k.rows - 1) / k.rows * ((n + k.toks - 1) / k.toks), q = (g + 255) / 256;
     const float nb = (float) (K / 256), one = k.s0 + k.s1 * nb, all = (float) q * (k.p0 + k.p1 * nb);
     return one > all ? one : all;
 }
-// R: rows of all matrices of the call; tiles: the tiled kernels may be taken (their scratch is there). One token: the mat-vec for very
-// many rows (65536 of 7168: 51 us against 67) and for few (512 of 16384: 7.2 against 10.4), the K-split kernel between (7168 of 16384: 17.7
-// against 19.4).
+// R: rows of all matrices of the call; tiles: the tiled kernels may be taken (their scratch is there). One token: the mat-vec for very many
+// rows (65536 of 7168: 53 us against 63, 65536 of 1024: 15 against 25), the K-split kernels below (16384 of 7168: 18 against 21, 2048 of 2048:
+// 3.7 against 6.1).
 constexpr int q4k_kernel(int n, int64_t R, int K, bool tiles) {
-    if (n <= 1 && (R > 24576 || R <= 1024)) { return Q4_VEC; }
+    if (n <= 1 && R > 24576) { return Q4_VEC; }
     int best = Q4_KS_16_16;
     for (int k = 1; k < (tiles && n > 16 ? (int) Q4_KERNELS : (int) Q4_MM_64_32); ++k) {   // (the tiled ones' times are of more than 16 tokens)
         if (q4k_us(Q4_KERNEL[k], n, R, K) < q4k_us(Q4_KERNEL[best], n, R, K)) { best = k; }

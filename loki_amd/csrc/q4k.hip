@@ -198,10 +198,13 @@ __device__ __forceinline__ void q4_mins(const u32x4 & hd, uint32_t (&mm)[2]) {
 
 // Few tokens: a workgroup's 8 waves share its rows and tokens and split K, wave w taking blocks w, w + 8, ... of the rows. A round's 8
 // blocks of a row are 1152 consecutive bytes: they are copied into LDS in whole, a round ahead (a wave's lanes fetching 16 rows'
-// pieces of 64 bytes themselves make twice the cache accesses, 37 a load instead of 19, and those bound the kernel: 32 tokens through
-// 7168 rows of 16384 36.6 us instead of 31.8, 16 tokens through 65536 rows of 7168 95 instead of 86). Activations come into registers straight from the caches, also a round ahead. Each round leaves the
-// blocks' terms in LDS, and the workgroup's lanes run the chains over them, an output or two a lane. summ comes from a third
-// product with the step's min in every byte (here the matrix cores have time to spare).
+// pieces of 64 bytes themselves make twice the cache accesses, 37 a load instead of 19: 16 tokens through 65536 rows of 7168 95 us instead
+// of 86). A wave's activations come into registers straight from the caches, each round's loads issued as soon as the last round's
+// products are done with the registers (a second set, filled a round earlier, holds every wave up at the round's start behind the
+// others' loads: 37 tokens through 7168 rows of 16384 39 us instead of 33). Each round leaves the blocks' terms in LDS, and the
+// workgroup's lanes run the chains over them, an output or two a lane. summ comes from a third product with the step's min in every
+// byte (here the matrix cores have time to spare). Of those 33 us, found by leaving out one part at a time: the copies and loads that
+// the products wait for 7, products and digits 14, the barriers, LDS reads and terms of the 8 rounds 7, the launch and first fetch 4.
 constexpr int KS_W = 8, KS_PITCH = 9 * KS_W + 1;   // 16-byte chunks from row to row in LDS: 16 rows start in 16 different quads of banks
 // copy i of a wave (past the last one: an earlier one of its own again, the same bytes, so that every wave has as many out)
 template <int ALLC> __device__ __forceinline__ int q4_copy(int wave, int i) { const int k = wave + KS_W * i; return k < ALLC ? k : wave; }
@@ -211,7 +214,7 @@ template <int RT, int NT> struct KsLds {
     static constexpr int T0 = 2 * WB, D0 = T0 + KS_W * RT * TT * 4, ALL = D0 + KS_W * TOK * 4;
 };
 template <int RT, int NT>
-__global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
+__global__ void __launch_bounds__(64 * KS_W, RT * NT == 1 ? 4 : 2) k_q4k_ks(KqArgs a) {
 #pragma clang fp contract(off)
     using L = KsLds<RT, NT>;
     constexpr int BS = 144, TOK = L::TOK, TT = L::TT;
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
         constexpr int NO = sizeof(acc) / sizeof(acc[0]);
 #pragma unroll
         for (int i = 0; i < NO; ++i) { acc[i] = 0.f; }
-        auto round = [&](const Act & v, int j0, int s) {
+        auto round = [&](Act & v, int j0, int s) {
             if (j0 + wave < nb) {
 #pragma unroll
                 for (int i = 0; i < RT; ++i) {
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
                 }
                 if (lane < TOK) { s_d[wave * TOK + lane] = __builtin_bit_cast(float, v.d); }
             }
+            load_x(j0 + KS_W + wave, v);   // the next round's, into the registers that the products are done with
             q4_barrier<63>();
             const int m = min(KS_W, nb - j0);
 #pragma unroll
@@ -325,18 +329,17 @@ __global__ void __launch_bounds__(64 * KS_W, 2) k_q4k_ks(KqArgs a) {
                 }
             }
         };
-        Act x[2];
+        Act x;
         constexpr int XL = 4 * NT + 1;   // the next round's activations may still be out when a round starts
         copy(0, 0);
-        load_x(wave, x[0]);
+        load_x(wave, x);
         for (int j0 = 0;;) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 q4_barrier<XL>();   // the round's copies have landed, this wave's and so everyone's; the last round's buffer and the terms are free
                 copy(j0 + KS_W, i ^ 1);
-                load_x(j0 + KS_W + wave, x[i ^ 1]);
                 __builtin_amdgcn_sched_barrier(0);
-                round(x[i], j0, i);
+                round(x, j0, i);
                 if ((j0 += KS_W) >= nb) { goto done; }
             }
         }
@@ -554,6 +557,7 @@ hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStre
     switch (kernel) {
     case Q4_VEC: return vec(a, gy, st);
     case Q4_KS_16_16: return ks<1, 1>(a, gy, st);
+    case Q4_KS_32_16: return ks<2, 1>(a, gy, st);
     case Q4_KS_32_32: return ks<2, 2>(a, gy, st);
     case Q4_KS_32_48: return ks<2, 3>(a, gy, st);
     case Q4_MM_64_32: return mm<1, 2, 4, 5>(a, st);

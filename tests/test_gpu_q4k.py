@@ -112,7 +112,7 @@ def test_every_kernel(ctx, name):
     """ragged sizes that the launch rule gives each of the kernels for many tokens (test_q4k_rules.py holds it to that), the matrix 4
     bytes off a 16-byte boundary; the largest block sums in three rows and two tokens"""
     import torch
-    for R, K, n in SIZES[name][1]:
+    for R, K, n in SIZES[name]:
         w = matrix(R + 7, R, K).reshape(R, K // 256, 144).copy()
         for r in (0, 17, R - 1):
             w[r, :, 4:] = 0xFF

@@ -60,20 +60,22 @@ def test_estimates_grow_with_the_work(rules):
 def test_few_tokens_do_not_take_many_token_tiles(rules):
     for R in RS:
         for K in KS:
-            assert rules.pick(1, R, K, 1) in (0, rules.count())
+            k = rules.pick(1, R, K, 1)
+            assert k == rules.count() or rules.toks(k) == 16
             assert not rules.tiled(rules.pick(16, R, K, 1))
 
 
-# rows, columns, tokens of the device tests that go through each kernel (test_gpu_q4k.py), ragged in rows and tokens: 1 to 13 blocks a row
-SIZES = {"ks_32_32": (1, [(1001, 1024, 200), (7001, 512, 17)]), "ks_32_48": (2, [(7001, 768, 40), (2049, 256, 130)]),
-         "mm_64_32": (3, [(2049, 1024, 200), (8200, 768, 40), (1001, 3328, 403)]), "mm_64_64": (4, [(4100, 256, 130), (7001, 768, 257)]),
-         "mm_128_64": (5, [(8200, 512, 400), (4100, 2048, 257)]), "mm_128_128": (6, [(8200, 256, 601), (7001, 768, 400), (7001, 1280, 403)])}
+# rows, columns, tokens of the device tests that go through each kernel (test_gpu_q4k.py), ragged in rows and tokens: 1 to 28 blocks a row
+SIZES = {"ks_32_16": [(7001, 512, 12), (7001, 7168, 13)], "ks_32_32": [(1001, 1024, 200), (7001, 512, 20)],
+         "ks_32_48": [(7001, 768, 40), (2049, 768, 130)], "mm_64_32": [(2049, 1024, 200), (8200, 768, 40), (1001, 3328, 403)],
+         "mm_64_64": [(4100, 256, 257), (7001, 768, 257), (1001, 3328, 601)], "mm_128_64": [(8200, 512, 400), (4100, 2048, 257), (7001, 3328, 130)],
+         "mm_128_128": [(8200, 256, 601), (7001, 768, 400), (7001, 1280, 403)]}
+KERNELS = ["ks_16_16", *SIZES]
 
 
 @pytest.mark.parametrize("name", SIZES)
 def test_sizes_that_reach_each_kernel(rules, name):
-    kernel, sizes = SIZES[name]
-    assert all(rules.pick(n, R, K, 1) == kernel for R, K, n in sizes), [rules.pick(n, R, K, 1) for R, K, n in sizes]
+    assert [KERNELS[rules.pick(n, R, K, 1)] for R, K, n in SIZES[name]] == [name] * len(SIZES[name])
 
 
 def test_launches_fit_a_grid(rules):
