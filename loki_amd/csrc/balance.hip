@@ -17,7 +17,7 @@ namespace {
 
 #pragma clang fp contract(fast)   // (no bit contract here: fewer and larger steps)
 
-constexpr int BL_B = 4;                      // rows a wave takes at a time: their loads and reductions overlap
+constexpr int BL_B = 4, BL_W = 16;           // rows a wave takes at a time (their loads and reductions overlap), waves of the sums' workgroups
 constexpr int BL_JOIN = 1024;                // threads of the joining workgroups
 constexpr float BL_TINY = 1e-10f;            // a row's sigmoid sum below which 1 + exp(-z) is exp(-z) to fp32 in every column
 
@@ -121,7 +121,10 @@ __device__ __forceinline__ void bl_finish(const BalanceArgs & g, int s, int T, f
     }
 }
 
-template <int J, int BL_W>
+// The sums: one read of the logits, P's parts in registers, counts by integer LDS atomics (exact in any order). Bound by memory
+// where the rows are many: 65536 rows of 256 experts in 16 sequences 17.5 us with the join, 3.8 TB/s; by its launches where they are few
+// (70 rows 5.0 us).
+template <int J>
 __global__ void __launch_bounds__(64 * BL_W) k_balance(BalanceArgs g) {
     constexpr int BL_T = 64 * BL_W;
     __shared__ float s_p[BL_W][64 * J];
@@ -167,8 +170,10 @@ __global__ void __launch_bounds__(64 * BL_W) k_balance(BalanceArgs g) {
     }
 }
 
-// chunks > 1: a sequence's sums over its chunks, four slices of them side by side and then in order, and its loss
+// chunks > 1: a sequence's sums over its chunks, four slices of them side by side and then in order, and its loss. A slice's loads
+// are AHEAD chunks at once: one after the other they took 17 us for the 256 chunks of one sequence of 16384 rows, now 6.
 __global__ void __launch_bounds__(BL_JOIN) k_balance_join(BalanceArgs g) {
+    constexpr int AHEAD = 8;
     __shared__ float s_p[4][NEXP_MAX];
     __shared__ int s_c[4][NEXP_MAX];
     __shared__ float s_f[BL_JOIN / 64];
@@ -177,9 +182,18 @@ __global__ void __launch_bounds__(BL_JOIN) k_balance_join(BalanceArgs g) {
     bl_rows(g, s, 0, a, b, T);
     float psum = 0.f; int cnt = 0;
     if (e < g.n_exp) {
-        for (int c = k; c < g.chunks; c += 4) {
-            const size_t o = ((size_t) s * g.chunks + c) * g.n_exp + e;
-            psum += g.part[o]; cnt += g.pcnt[o];
+        for (int c0 = k; c0 < g.chunks; c0 += 4 * AHEAD) {
+            float p[AHEAD]; int n[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {   // (past the last chunk: it again, left out below)
+                const size_t o = ((size_t) s * g.chunks + min(c0 + 4 * i, g.chunks - 1)) * g.n_exp + e;
+                p[i] = g.part[o]; n[i] = g.pcnt[o];
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const bool in = c0 + 4 * i < g.chunks;
+                psum += in ? p[i] : 0.f; cnt += in ? n[i] : 0;
+            }
         }
     }
     s_p[k][e] = psum; s_c[k][e] = cnt;
@@ -190,9 +204,11 @@ __global__ void __launch_bounds__(BL_JOIN) k_balance_join(BalanceArgs g) {
     bl_finish(g, s, T, k == 0 ? psum : 0.f, cnt, s_f);
 }
 
-template <int J, int BL_W>
-__global__ void __launch_bounds__(64 * BL_W) k_balance_grad(BalanceArgs g) {
-    constexpr int BL_T = 64 * BL_W;
+// The gradient: a row's sigmoids once more (reading them back would cost what reading the logits costs, and the sums would have to
+// write them), its weighted sum of f by the wave, one write. 65536 rows of 256 in 16 sequences 24.7 us, 5.4 TB/s read and written.
+template <int J, int W>
+__global__ void __launch_bounds__(64 * W) k_balance_grad(BalanceArgs g) {
+    constexpr int BL_T = 64 * W;
     const int s = blockIdx.y, lane = lane_id(), w = threadIdx.x >> 6, ne = g.n_exp;
     if (s == g.nseq) {   // rows of no sequence: their gradient is 0
         const int64_t lo = min(max(g.seq[0], 0), g.n), hi = min(max(g.seq[g.nseq], 0), g.n);
@@ -209,7 +225,7 @@ __global__ void __launch_bounds__(64 * BL_W) k_balance_grad(BalanceArgs g) {
     float f[J];
 #pragma unroll
     for (int j = 0; j < J; ++j) { const int e = lane + 64 * j; f[j] = e < ne ? bl_f(g.counts[(size_t) s * ne + e], g, T) : 0.f; }
-    for (int t = a + __builtin_amdgcn_readfirstlane(w) * BL_B; t < b; t += BL_W * BL_B) {
+    for (int t = a + __builtin_amdgcn_readfirstlane(w) * BL_B; t < b; t += W * BL_B) {
         float z[BL_B][J], q[BL_B][J], om[BL_B][J], inv[BL_B], d[BL_B];
         bl_load<J, BL_B>(g, t, b, z);
         bl_sigmoids<J, BL_B>(z, q, om, inv);
@@ -239,40 +255,31 @@ __global__ void __launch_bounds__(64 * BL_W) k_balance_grad(BalanceArgs g) {
 
 }  // namespace
 
-// Waves of a workgroup (a batch of BL_B rows each at a time) and workgroups a sequence, for the sums and for the gradient, which has
-// nothing to join. One sequence of 4100 rows: 4 waves 23.2 us (257 partial sums to join), 16 waves 10.8; 128 rows in one workgroup of
-// 16 waves 7.0, cut in 8 of 4 waves 10.2. The gradient of 4100 rows: 4 waves 5.5, 16 waves 6.4; of 16384 11.4 and 8.8.
-static int balance_waves(int n, bool grad) { return grad && n <= 8192 ? 4 : 16; }
+// Workgroups a sequence, each wave with a batch of BL_B rows at a time. Sums: 16 waves, so that there are few partial sums to join; up to
+// 128 rows one workgroup, which needs no second launch (128 rows 7.0 us, 256 rows in 4 workgroups 7.7). The gradient has nothing to
+// join: 4 waves up to 8192 rows (4100 rows 5.5 us, with 16 waves 6.4), 16 above (16384 rows 8.8 us, with 4 waves 11.4).
+static int grad_waves(int n) { return n <= 8192 ? 4 : 16; }
 static int chunks_of(int n, int nseq, bool grad) {
-    const int w = balance_waves(n, grad), rows = w * BL_B, most = w == 4 ? BALANCE_PARTS : BALANCE_PARTS / 2;
+    const int w = grad ? grad_waves(n) : BL_W, rows = w * BL_B, most = w == 4 ? BALANCE_PARTS : BALANCE_PARTS / 2;
     if (!grad && n <= 128 * nseq) { return 1; }
     return std::max(1, std::min({ (int) (((int64_t) n + (int64_t) nseq * rows - 1) / ((int64_t) nseq * rows)), most / nseq, 256 }));
 }
 int balance_chunks(int n, int nseq) { return chunks_of(n, nseq, false); }
 
-template <class F> static hipError_t by_shape(const BalanceArgs & a, bool grad, F && go) {
-    const int j = (a.n_exp + 63) / 64;
-    if (balance_waves(a.n, grad) == 4) {
-        switch (j) {
-        case 1: go(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{}); break;
-        case 2: go(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{}); break;
-        case 3: go(std::integral_constant<int, 3>{}, std::integral_constant<int, 4>{}); break;
-        default: go(std::integral_constant<int, 4>{}, std::integral_constant<int, 4>{}); break;
-        }
-    } else {
-        switch (j) {
-        case 1: go(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{}); break;
-        case 2: go(std::integral_constant<int, 2>{}, std::integral_constant<int, 16>{}); break;
-        case 3: go(std::integral_constant<int, 3>{}, std::integral_constant<int, 16>{}); break;
-        default: go(std::integral_constant<int, 4>{}, std::integral_constant<int, 16>{}); break;
-        }
+// go at the columns a lane holds
+template <class F> static hipError_t by_columns(int n_exp, F && go) {
+    switch ((n_exp + 63) / 64) {
+    case 1: go(std::integral_constant<int, 1>{}); break;
+    case 2: go(std::integral_constant<int, 2>{}); break;
+    case 3: go(std::integral_constant<int, 3>{}); break;
+    default: go(std::integral_constant<int, 4>{}); break;
     }
     return hipGetLastError();
 }
 
 hipError_t launch_balance(const BalanceArgs & a, hipStream_t st) {
     if (a.n < 0 || a.nseq < 1 || a.nseq > 65535 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.topk < 1 || a.chunks < 1 || (!a.seq && a.nseq != 1)) { return hipErrorInvalidValue; }
-    const hipError_t e = by_shape(a, false, [&](auto j, auto w) { k_balance<decltype(j)::value, decltype(w)::value><<<dim3(a.chunks, a.nseq), 64 * decltype(w)::value, 0, st>>>(a); });
+    const hipError_t e = by_columns(a.n_exp, [&](auto j) { k_balance<decltype(j)::value><<<dim3(a.chunks, a.nseq), 64 * BL_W, 0, st>>>(a); });
     if (e != hipSuccess || a.chunks == 1) { return e; }
     k_balance_join<<<a.nseq, BL_JOIN, 0, st>>>(a);
     return hipGetLastError();
@@ -284,7 +291,8 @@ hipError_t launch_balance_grad(const BalanceArgs & args, hipStream_t st) {
     if (a.n < 0 || a.nseq < 1 || a.nseq >= 65535 || a.n_exp < 1 || a.n_exp > NEXP_MAX || a.topk < 1 || a.chunks < 1 || (!a.seq && a.nseq != 1)) { return hipErrorInvalidValue; }
     if (a.n == 0) { return hipSuccess; }
     const dim3 grid(a.chunks, a.nseq + (a.seq && !a.accumulate ? 1 : 0));
-    return by_shape(a, true, [&](auto j, auto w) { k_balance_grad<decltype(j)::value, decltype(w)::value><<<grid, 64 * decltype(w)::value, 0, st>>>(a); });
+    if (grad_waves(a.n) == 4) { return by_columns(a.n_exp, [&](auto j) { k_balance_grad<decltype(j)::value, 4><<<grid, 64 * 4, 0, st>>>(a); }); }
+    return by_columns(a.n_exp, [&](auto j) { k_balance_grad<decltype(j)::value, 16><<<grid, 64 * 16, 0, st>>>(a); });
 }
 
 }  // namespace lk
