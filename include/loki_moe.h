@@ -182,6 +182,10 @@ int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, 
  * n_exp * 8 + n_exp * E * 4 bytes and dW's partial sums, kept until fl_free. */
 int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
+/* Workspaces of fl_balance_loss_dev, fl_route_grad_dev and Q4_K products are the context's. They grow in the call that needs more
+ * (hipMalloc; FL_ENOMEM when that fails, as it does under graph capture) and no block is freed before fl_free, so a captured call stays
+ * valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured from one context share
+ * its workspaces and must not run at the same time. The context's device has to be the current one (FL_EINVAL). */
 /* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device) */
 int fl_dispatch_dev(FLCtx *, const int * sel, int n, int topk, int n_exp, int * counts, int * offsets, int * perm, int * inv, int * act, int * nact);
 /* Q8_K of nrows x K floats (device): q [nrows][K] int8, d [nrows][K/256] */
@@ -191,7 +195,9 @@ int fl_quant_q8k_dev(FLCtx *, const float * x, int nrows, int K, int8_t * q, flo
  * FL_Q4K, the format of attention, dense layers and heads, K <= 65536).
  * The per-format mat-vec behind fl_moe / fl_ffn_begin (the reference's tc_matvec<F>, src/fused_layer.cu:102-158,
  * 203-254): integer sub-block sums exact, fp32 over the blocks in order (Q2_K bit-identical to ggml's scalar dot).
- * FL_Q4K: y = fma(d8, fma(-dmin, summ, d * isum), y) per block, whatever n and R: a row's output has the same bits in any batch. */
+ * FL_Q4K: y = fma(d8, fma(-dmin, summ, d * isum), y) per block, whatever n and R: a row's output has the same bits in any batch. R at
+ * most 2^26, n at most 2^19, q 16-byte aligned; batches that run on tiles (above 16 rows) take n * K / 8 bytes of the context's, see
+ * "Workspaces" below. */
 int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y);
 /* IQ2_XXS ggml layout <-> tiled layout for nmat matrices of R x K at byte strides (device, may not alias) */
 int fl_pack_iq2xxs(FLCtx *, const void * src_ggml, size_t src_stride, void * dst_tiled, size_t dst_stride, int R, int K, int nmat);

@@ -255,6 +255,7 @@ class Context:
         self.ctx = lib().fl_init(0, 0)
         if not self.ctx:
             raise LokiError("fl_init failed")
+        self._device = torch.cuda.current_device()
         # share torch's current stream so library kernels and torch ops on the same buffers stay ordered
         self.check(lib().fl_set_stream(self.ctx, torch.cuda.current_stream().cuda_stream))
 
@@ -444,11 +445,11 @@ class Context:
         return dl, dW, dx
 
     def _need(self, who, *args):
-        """Each (tensor, dtype, shape): contiguous on the GPU as the library reads it (None passes)."""
+        """Each (tensor, dtype, shape): contiguous on the context's GPU as the library reads it (None passes)."""
         for t, dtype, shape in args:
-            if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda):
-                raise LokiError("%s: a contiguous %s tensor of shape %s on the GPU is needed, not %s %s on %s" %
-                                (who, dtype, shape, t.dtype, tuple(t.shape), t.device))
+            if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == self._device):
+                raise LokiError("%s: a contiguous %s tensor of shape %s on GPU %d is needed, not %s %s on %s" %
+                                (who, dtype, shape, self._device, t.dtype, tuple(t.shape), t.device))
 
     def dispatch(self, sel, n_exp=N_EXPERT):
         t = self.torch

@@ -257,3 +257,112 @@ def test_layer_formats(ctx, fm):
     finally:
         ctx.set_layer_formats()
     torch.cuda.empty_cache()
+
+
+def test_gguf_layer(ctx, tmp_path):
+    """a layer of Q4_K routed down and shared matrices from a GGUF file: loaded tiled it runs through fl_moe_layer within the K-quants'
+    bar of the checker; the layout that fl_moe reads refuses the format"""
+    import torch
+    from loki_amd import FL_LAYOUT_GGML, FL_LAYOUT_TILED, Gguf, LokiError, lib
+    from tests import _gguf
+    from tests.golden import gen
+    from tests.test_gpu_gguf import layer_tensors
+    from tests.test_gpu_kquant import bar_close
+    ne, n = 16, 20
+    W, b, gate, up, _, _ = gen.layer(302, ne, E, H)
+    down = [matrix(303 + e, E, H) for e in range(ne)]
+    sh = (matrix(330, H, E), matrix(331, H, E), matrix(332, E, H))
+    path = str(tmp_path / "q4.gguf")
+    _gguf.write(path, layer_tensors(4, W, b, gate, up, down, sh, ["IQ2_XXS", "IQ2_XXS", "Q4_K", "Q4_K", "Q4_K", "Q4_K"]))
+    g = Gguf(path)
+    gl = ctx.load_gguf_layer(g, 4, FL_LAYOUT_TILED)
+    try:
+        fm = (gl.fmt_down, gl.fmt_sh_gate, gl.fmt_sh_up, gl.fmt_sh_down)
+        assert fm == (orc.Q4K,) * 4
+        ctx.set_experts(ne); ctx.set_routing(8, 4, 8, 2.5); ctx.set_layer_formats(*fm)
+        x = gen.uniform(12, 304, (n, E), 2.0)
+        xt = torch.from_numpy(x).cuda(); y = torch.empty_like(xt)
+        ctx.check(lib().fl_moe_layer(ctx.ctx, ctypes.byref(gl.L), ctypes.c_void_p(xt.data_ptr()), n, ctypes.c_void_p(y.data_ptr())))
+        ctx.sync()
+        _, _, so, wo = orc.router(W, b, x, 8, 4, 8, 2.5)
+        ok, err = bar_close(y.cpu().numpy(), orc.moe_experts(x, so, wo, gate, up, down, *sh, n_exp=ne, fmts=fm)["y"])
+        assert ok, err
+        with pytest.raises(LokiError, match="Q4_K"):
+            ctx.load_gguf_layer(g, 4, FL_LAYOUT_GGML)
+    finally:
+        ctx.set_layer_formats(); ctx.set_experts()
+        ctx.free_gguf_layer(gl)
+        g.close()
+
+
+# ---------------------------------------------------------------- graphs and streams
+def test_captured_products_outlive_a_larger_scratch(ctx):
+    """two captured products of one context (tiled: their scratch is the context's), an eager one that outgrows the scratch between
+    their replays, and changed rows: every replay has the bits of its rows' eager product"""
+    import torch
+    from loki_amd import Context, lib
+    R, K = 2049, 1024
+    w = torch.from_numpy(matrix(61, R, K)).cuda()
+    rows = [[torch.from_numpy(a).cuda() for a in q8k_rows(200, K, seed=62 + i)[:2]] for i in range(3)]
+    big = [torch.from_numpy(a).cuda() for a in q8k_rows(3000, K, seed=66)[:2]]
+    want = [ctx.kq_matvec(orc.Q4K, w, R, K, q, d).clone() for q, d in rows]
+    want_big = ctx.kq_matvec(orc.Q4K, w, R, K, *big)
+    ctx.sync()
+    c = Context()
+    try:
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        c.check(lib().fl_set_stream(c.ctx, side.cuda_stream))
+        ins = [[t.clone() for t in rows[0]] for _ in range(2)]
+        outs = [torch.empty((200, R), device="cuda") for _ in range(2)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            c.kq_matvec(orc.Q4K, w, R, K, *ins[0], outs[0])   # (the scratch is allocated here, before the captures)
+        torch.cuda.synchronize()
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        for i, g in enumerate(graphs):
+            with torch.cuda.graph(g, stream=side):
+                c.kq_matvec(orc.Q4K, w, R, K, *ins[i], outs[i])
+        for rep in range(3):
+            for i, g in enumerate(graphs):
+                pick = (rep + 2 * i) % 3
+                for dst, src in zip(ins[i], rows[pick]):
+                    dst.copy_(src)
+                outs[i].fill_(-1.0)
+                torch.cuda.synchronize()
+                with torch.cuda.stream(side):
+                    g.replay()
+                    y = c.kq_matvec(orc.Q4K, w, R, K, *big)
+                torch.cuda.synchronize()
+                assert torch.equal(outs[i].view(torch.int32), want[pick].view(torch.int32)), (rep, i)
+                assert torch.equal(y.view(torch.int32), want_big.view(torch.int32)), (rep, i)
+        del graphs, g
+    finally:
+        torch.cuda.synchronize()
+        c.close()
+
+
+def test_two_contexts_at_once(ctx):
+    """products on two contexts and streams in flight together, each with its own scratch: the bits that they have alone"""
+    import torch
+    from loki_amd import Context, lib
+    R, K = 7168, 2048
+    ws = [torch.from_numpy(matrix(71 + i, R, K)).cuda() for i in range(2)]
+    rows = [[torch.from_numpy(a).cuda() for a in q8k_rows(300, K, seed=73 + i)[:2]] for i in range(2)]
+    want = [ctx.kq_matvec(orc.Q4K, ws[i], R, K, *rows[i]) for i in range(2)]
+    ctx.sync()
+    cs, streams = [Context(), Context()], [torch.cuda.Stream(), torch.cuda.Stream()]
+    try:
+        for c, s in zip(cs, streams):
+            c.check(lib().fl_set_stream(c.ctx, s.cuda_stream))
+        outs = [[torch.full((300, R), -1.0, device="cuda") for _ in range(6)] for _ in range(2)]
+        torch.cuda.synchronize()
+        for k in range(6):
+            for i in range(2):
+                cs[i].kq_matvec(orc.Q4K, ws[i], R, K, *rows[i], outs[i][k])
+        torch.cuda.synchronize()
+        assert all(torch.equal(o.view(torch.int32), want[i].view(torch.int32)) for i in range(2) for o in outs[i])
+    finally:
+        torch.cuda.synchronize()
+        for c in cs:
+            c.close()
