@@ -364,8 +364,8 @@ template <int RT, int NT> hipError_t ks(const KqArgs & a, unsigned gy, hipStream
 // (copied there by the loads themselves, 16-byte chunks swizzled so that a tile's reads meet no bank twice). Each weight is decoded
 // once per workgroup and each activation read from LDS serves RT tiles, so the largest tile, 128 x 128, does the most work an
 // instruction; smaller ones are for calls that it would leave CUs without a workgroup (launch_rules.h). 2048 tokens through 16384 rows of
-// 7168 502 us, 958 TFLOP/s of the real product: the matrix cores are busy 52 % of the cycles and the vector units with digits and terms
-// 46 %, at the 1.9 GHz that the card then holds; 501 tokens through 7000 rows of 7168 75 us, 220 workgroups and so one wave a SIMD, whose
+// 7168 502 us, 958 TFLOP/s of the real product: the matrix cores are busy 53 % of the cycles and the vector units with digits and terms
+// 48 %, at the 1.9 GHz that the card then holds; 501 tokens through 7000 rows of 7168 75 us, 220 workgroups and so one wave a SIMD, whose
 // products (40 %) and vector work (35 %) follow each other.
 template <int RT, int NT, int W, int D>
 __global__ void __launch_bounds__(64 * W, 2) k_q4k_mm(Q4Args a) {
