@@ -378,10 +378,9 @@ class Context:
 
     def kq_matvec(self, fmt, w, R, K, q, d, y=None):
         """y [n][R] = K-quant matrix w (uint8 device tensor, R x K/256 ggml blocks) . Q8_K rows (q [n][K], d [n][K/256])."""
-        t = self.torch
         n = q.shape[0]
         if y is None:
-            y = t.empty((n, R), dtype=t.float32, device=q.device)
+            y = d.new_empty(n, R)
         self.check(lib().fl_kq_matvec_dev(self.ctx, fmt, _ptr(w), R, K, _ptr(q), _ptr(d), n, _ptr(y)))
         return y
 
@@ -404,8 +403,7 @@ class Context:
         topk = sel.shape[1]
         nseq = 1 if seq is None else seq.numel() - 1
         self._need("balance_loss", (logits, t.float32, (n, ne)), (sel, t.int32, (n, topk)), (seq, t.int32, (nseq + 1,)))
-        counts = t.empty((nseq, ne), dtype=t.int32, device=logits.device)
-        loss = t.empty(nseq, dtype=t.float32, device=logits.device)
+        counts, loss = sel.new_empty(nseq, ne), logits.new_empty(nseq)
         self.check(lib().fl_balance_loss_dev(self.ctx, _ptr(logits), _ptr(sel), _ptr(seq), n, nseq, ne, topk, alpha, _ptr(counts), _ptr(loss)))
         return counts, loss
 
@@ -447,9 +445,9 @@ class Context:
     def _need(self, who, *args):
         """Each (tensor, dtype, shape): contiguous on the context's GPU as the library reads it (None passes)."""
         for t, dtype, shape in args:
-            if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == self._device):
-                raise LokiError("%s: a contiguous %s tensor of shape %s on GPU %d is needed, not %s %s on %s" %
-                                (who, dtype, shape, self._device, t.dtype, tuple(t.shape), t.device))
+            if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda and t.get_device() == self._device):
+                raise LokiError("%s: a contiguous %s tensor of shape %s on the context's GPU is needed, not %s %s on %s" %
+                                (who, dtype, shape, t.dtype, tuple(t.shape), t.device))
 
     def dispatch(self, sel, n_exp=N_EXPERT):
         t = self.torch

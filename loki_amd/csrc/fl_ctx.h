@@ -29,7 +29,7 @@ template <class T> struct DBuf {
 // a workspace that a captured graph may hold on to: growing it keeps the older allocations until the context ends, and
 // sizes go up in powers of two, so all of them together are at most twice the largest
 struct KeptBuf {
-    void * p = nullptr; size_t cap = 0; std::vector<void *> old;
+    void * p = nullptr; size_t cap = 0; void * old[64] = {}; int olds = 0;
     hipError_t ensure(size_t bytes) {
         if (p && bytes <= cap) { return hipSuccess; }
         size_t want = 1 << 16;
@@ -37,14 +37,14 @@ struct KeptBuf {
         void * q = nullptr;
         const hipError_t e = hipMalloc(&q, want);
         if (e != hipSuccess) { return e; }
-        if (p) { old.push_back(p); }
+        if (p) { old[olds++] = p; }   // (one a power of two at most)
         p = q; cap = want;
         return hipSuccess;
     }
     void release() {
-        for (void * q : old) { (void) hipFree(q); }
+        while (olds > 0) { (void) hipFree(old[--olds]); }
         if (p) { (void) hipFree(p); }
-        old.clear(); p = nullptr; cap = 0;
+        p = nullptr; cap = 0;
     }
 };
 
