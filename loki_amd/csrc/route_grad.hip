@@ -42,6 +42,18 @@ __device__ __forceinline__ float rg_wave_max(float v) {
     v = fmaxf(v, rg_dpp<DPP_XOR1>(v)); v = fmaxf(v, rg_dpp<DPP_XOR2>(v)); v = fmaxf(v, rg_dpp<DPP_HALF_MIRROR>(v)); v = fmaxf(v, rg_dpp<DPP_MIRROR>(v));
     return fmaxf(fmaxf(rg_lane(v, 0), rg_lane(v, 16)), fmaxf(rg_lane(v, 32), rg_lane(v, 48)));
 }
+// the largest of the four lanes that share lane % 16
+__device__ __forceinline__ float rg_max_rows(float v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t a = __builtin_bit_cast(uint32_t, v);
+    const auto p = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+    const uint32_t b = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, (uint32_t) p[0]), __builtin_bit_cast(float, (uint32_t) p[1])));
+    const auto q = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t) q[0]), __builtin_bit_cast(float, (uint32_t) q[1]));
+#else
+    return v;
+#endif
+}
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rg_rsrc(const void * p, uint32_t bytes) {
     const uint64_t v = (uint64_t) p;
     const uint32_t hi = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) (v >> 32)), lo = (uint32_t) __builtin_amdgcn_readfirstlane((int) (uint32_t) v);
@@ -57,7 +69,7 @@ __device__ __forceinline__ void rg_lds16(__amdgpu_buffer_rsrc_t r, LK_LOCAL uint
 }
 
 // The operands in memory, halves of 16 bytes = 8 consecutive K values:
-//   zs [t][hi, lo][kp]          dz of row t, K = experts (kp: n_exp up to a multiple of 32, zeros)
+//   zs [t / 16][K / 32][hi, lo][K / 8 % 4][t % 16][8]   dz, K = experts (n_exp up to a multiple of 32, zeros): the order of a wave's lanes
 //   zt [t / 8][hi, lo][ea][8]   dz of 8 rows, K = rows (ea: n_exp up to 64, 128 or 256, zeros; rows up to a multiple of 32, zeros)
 //   kt [t]                      the rows' k
 //   wt [hi, lo][kp / 8][E][8]   W, K = experts; kw [E / 64] its k
@@ -164,19 +176,21 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
     }
     const int nc = o.kp / 8;
     for (int p = threadIdx.x; p < 16 * nc; p += 256) {    // 8 experts of a row
-        const int i = p / (2 * nc), c = p % (2 * nc);
-        if (t0 + i < g.n) { *reinterpret_cast<gh8 *>(o.zs + (size_t) (t0 + i) * 2 * o.kp + c * 8) = *reinterpret_cast<const gh8 *>(&s_h[c / nc][i][8 * (c % nc)]); }
+        const int i = p % 8, c = p / 8;
+        const int h = c / nc, b = c % nc, t = t0 + i;
+        *reinterpret_cast<gh8 *>(o.zs + ((((size_t) (t >> 4) * (nc / 4) + b / 4) * 2 + h) * 64 + (b % 4) * 16 + (t & 15)) * 8) = *reinterpret_cast<const gh8 *>(&s_h[h][i][8 * b]);
     }
 }
 
 constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128, RG_RT = 2;
 
 // dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 32 rows at a time,
-// whose dz comes straight from memory, the next 32 experts' in flight; no barrier after the first. The product runs with the columns
+// whose dz comes straight from the caches, D - 1 steps of 32 experts ahead; no barrier after the first. The product runs with the columns
 // as rows of the matrix core's tile, so a lane stores 4 consecutive columns. 64 rows a wave read LDS half as often and are 1 to 2 %
 // faster from 12000 rows on, but leave waves idle before: 1001 rows of 7168, 256 experts, both products 62 us instead of 51.
+template <int D>
 __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int part, int parts) {
-    constexpr int RT = RG_RT;
+    constexpr int RT = RG_RT, AH = 2;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
     const int j0 = ct * RG_COLS, nb = o.kp / 8, ns = o.kp / 32;
     const __amdgpu_buffer_rsrc_t rw = rg_rsrc(o.wt, (uint32_t) ((size_t) 2 * nb * g.E * 16));
@@ -187,23 +201,29 @@ __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o,
     __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
     __syncthreads();
     const uint32_t lo_off = (uint32_t) nb * 2048, lb = (uint32_t) (size_t) lds + (uint32_t) (q * 2048 + r * 16);
-    const int tiles = (g.n + 16 * RT - 1) / (16 * RT);
-    for (int tt = part * RG_W + wave; tt < tiles; tt += parts * RG_W) {
-        const int t0 = tt * 16 * RT, nt = min(16 * RT, g.n - t0);
-        // rows past the batch's end read 0
-        const __amdgpu_buffer_rsrc_t rz = rg_rsrc(o.zs + (size_t) t0 * 2 * o.kp, (uint32_t) nt * (uint32_t) o.kp * 4);
-        uint32_t vz[RT];
+    const int tiles = (g.n + 16 * RT - 1) / (16 * RT), stride = parts * RG_W, tt0 = part * RG_W + wave, nsp = (ns + D - 1) / D * D;
+    if (tt0 >= tiles) { return; }
+    uint32_t vz[RT];
 #pragma unroll
-        for (int i = 0; i < RT; ++i) { vz[i] = (uint32_t) (16 * i + r) * (uint32_t) (o.kp * 4) + 16u * q; }
-        gh8 z[2][RT][2];
-        auto load = [&](int s, gh8 (&d)[RT][2]) {
-            const uint32_t so = (uint32_t) (min(s, ns - 1) * 64);
+    for (int i = 0; i < RT; ++i) { vz[i] = (uint32_t) (i * ns * 2048 + lane * 16); }
+    // the loads' place, D - 1 steps ahead of the products' and into the next tile (after the last one: it again, unread)
+    auto rsrc = [&](int tt) { return rg_rsrc(o.zs + (size_t) tt * RT * ns * 1024, (uint32_t) (RT * ns * 2048)); };
+    int lt = tt0, ls = 0;
+    __amdgpu_buffer_rsrc_t rz = rsrc(lt);
+    gh8 z[D][RT][2];
+    auto load = [&](gh8 (&d)[RT][2]) {
+        const uint32_t so = (uint32_t) (min(ls, ns - 1) * 2048);
 #pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                d[i][0] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i], so, 0));
-                d[i][1] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i] + (uint32_t) (o.kp * 2), so, 0));
-            }
-        };
+        for (int i = 0; i < RT; ++i) {
+            d[i][0] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i], so, 0));
+            d[i][1] = __builtin_bit_cast(gh8, __builtin_amdgcn_raw_buffer_load_b128(rz, vz[i] + 1024u, so, 0));
+        }
+        if (++ls == nsp) { ls = 0; lt = lt + stride < tiles ? lt + stride : lt; rz = rsrc(lt); }
+    };
+#pragma unroll
+    for (int k = 0; k < D - 1; ++k) { load(z[k]); }
+    for (int tt = tt0; tt < tiles; tt += stride) {
+        const int t0 = tt * 16 * RT;
         gf4 acc[8][RT];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -212,25 +232,31 @@ __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o,
         }
         auto step = [&](int s, const gh8 (&d)[RT][2]) {
             const uint32_t a = lb + (uint32_t) s * 8192;   // 4 x 8 experts
+            __builtin_amdgcn_sched_barrier(0);
+            gh8 w[AH + 1][2];   // W's operands, AH column tiles ahead
+            auto ld = [&](int c) { w[c % (AH + 1)][0] = *(const LK_LOCAL gh8 *) (size_t) (a + c * 256); w[c % (AH + 1)][1] = *(const LK_LOCAL gh8 *) (size_t) (a + lo_off + c * 256); };
+#pragma unroll
+            for (int c = 0; c < AH; ++c) { ld(c); }
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                const gh8 wh = *(const LK_LOCAL gh8 *) (size_t) (a + c * 256), wl = *(const LK_LOCAL gh8 *) (size_t) (a + lo_off + c * 256);
+                if (c + AH < 8) { ld(c + AH); }
+                __builtin_amdgcn_sched_barrier(0);
+                const gh8 wh = w[c % (AH + 1)][0], wl = w[c % (AH + 1)][1];
 #pragma unroll
                 for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, d[i][0], acc[c][i], 0, 0, 0); }
 #pragma unroll
                 for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wh, d[i][1], acc[c][i], 0, 0, 0); }
 #pragma unroll
                 for (int i = 0; i < RT; ++i) { acc[c][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wl, d[i][0], acc[c][i], 0, 0, 0); }
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        load(0, z[0]);
-        for (int s = 0;;) {
-            load(s + 1, z[1]);
-            step(s, z[0]);
-            if (++s == ns) { break; }
-            load(s + 1, z[0]);
-            step(s, z[1]);
-            if (++s == ns) { break; }
+        for (int s = 0; s < nsp; s += D) {
+#pragma unroll
+            for (int k = 0; k < D; ++k) {
+                load(z[(k + D - 1) % D]);
+                if (s + k < ns) { step(s + k, z[k]); }
+            }
         }
 #pragma unroll
         for (int i = 0; i < RT; ++i) {
@@ -244,7 +270,7 @@ __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o,
                     gf4 v;
 #pragma unroll
                     for (int u = 0; u < 4; ++u) { v[u] = ldexpf(acc[c][i][u], k); }
-                    *reinterpret_cast<gf4 *>(row + 16 * c) = v;
+                    __builtin_nontemporal_store(v, reinterpret_cast<gf4 *>(row + 16 * c));
                 }
             }
         }
@@ -292,7 +318,7 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
         float y[8], m = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { y[i] = ldexpf(sl.x[i], K0 - (int) sl.k[i]); m = fmaxf(m, fabsf(y[i])); }
-        m = fmaxf(m, __shfl_xor(m, 16)); m = fmaxf(m, __shfl_xor(m, 32));
+        m = rg_max_rows(m);
         kc = min(kc, m > 0.f ? rg_k(m) : kc);   // (a column with an infinity is non-finite in every expert, whatever its k)
         const float sc = rg_pow2(kc);
         gh8 hi, lo;
@@ -320,26 +346,34 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
             copy_z(s + 1, b ^ 1);
             __builtin_amdgcn_sched_barrier(0);
             const uint32_t lb = (uint32_t) (size_t) lds + (uint32_t) (b * BUF);
+            int kn[JW];
+            gh8 xh[JW], xl[JW], z[2][2];
+            auto load_z = [&](int i) {
+                const uint32_t a = lb + (uint32_t) ((q * 2 * EA + 64 * we + 16 * i + r) * 16);
+                z[i & 1][0] = *(const LK_LOCAL gh8 *) (size_t) a; z[i & 1][1] = *(const LK_LOCAL gh8 *) (size_t) (a + EA * 16);
+            };
 #pragma unroll
-            for (int c = 0; c < JW; ++c) {   // columns whose k went down: what is summed so far follows
-                const int k = *(const LK_LOCAL int *) (size_t) (lb + AB + BB + (uint32_t) ((16 * JW * wj + 16 * c + r) * 4));
-                if (__ballot(k != cur[c])) {
-                    const float f = rg_pow2(k - cur[c]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { acc[i][c] = acc[i][c] * f; }
-                    cur[c] = k;
-                }
-            }
-            gh8 xh[JW], xl[JW];
+            for (int c = 0; c < JW; ++c) { kn[c] = *(const LK_LOCAL int *) (size_t) (lb + AB + BB + (uint32_t) ((16 * JW * wj + 16 * c + r) * 4)); }
+            load_z(0);
 #pragma unroll
             for (int c = 0; c < JW; ++c) {
                 const uint32_t a = lb + AB + (uint32_t) ((q * 2 * RG_COLS + 16 * JW * wj + 16 * c + r) * 16);
                 xh[c] = *(const LK_LOCAL gh8 *) (size_t) a; xl[c] = *(const LK_LOCAL gh8 *) (size_t) (a + RG_COLS * 16);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int c = 0; c < JW; ++c) {   // columns whose k went down: what is summed so far follows
+                if (__ballot(kn[c] != cur[c])) {
+                    const float f = rg_pow2(kn[c] - cur[c]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { acc[i][c] = acc[i][c] * f; }
+                    cur[c] = kn[c];
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t a = lb + (uint32_t) ((q * 2 * EA + 64 * we + 16 * i + r) * 16);
-                const gh8 zh = *(const LK_LOCAL gh8 *) (size_t) a, zl = *(const LK_LOCAL gh8 *) (size_t) (a + EA * 16);
+                if (i < 3) { load_z(i + 1); }
+                const gh8 zh = z[i & 1][0], zl = z[i & 1][1];
 #pragma unroll
                 for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, xh[c], acc[i][c], 0, 0, 0); }
 #pragma unroll
@@ -350,7 +384,10 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
             convert(next, b ^ 1);
             load_x(s + 4, next);
 #pragma unroll
-            for (int i = 0; i < 12 * JW; ++i) { __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x002, 2, 0); }
+            for (int i = 0; i < 12 * JW; ++i) {
+                if (i % (3 * JW) == 0 && i < 9 * JW) { __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
     };
     load_x(s0, sl[0]);
@@ -390,7 +427,7 @@ __global__ void __launch_bounds__(RG_T, 2) k_route_mm(RouteGradArgs g, Ops o, in
     extern __shared__ __attribute__((aligned(16))) uint8_t rg_dyn[];
     const int ct = g.E / RG_COLS, b = (int) blockIdx.x, dw = g.dW ? ct * splits : 0;
     if (b < dw) { route_dw<WR>(g, o, (LK_LOCAL uint8_t *) rg_dyn, b % ct, b / ct, splits, part); }
-    else { route_dx(g, o, (LK_LOCAL uint8_t *) rg_dyn, (b - dw) % ct, (b - dw) / ct, parts); }
+    else { route_dx<WR == 1 ? 2 : 4>(g, o, (LK_LOCAL uint8_t *) rg_dyn, (b - dw) % ct, (b - dw) / ct, parts); }
 }
 // the runs' sums, in order
 __global__ void __launch_bounds__(256) k_route_join(const float * __restrict__ part, int splits, int64_t n4, int accumulate, float * __restrict__ dW) {
@@ -408,7 +445,7 @@ struct Sizes { int kp, ea, np; size_t zs, zt, kt, wt, kw, part, all; };
 Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
     Sizes z{};
     z.kp = (ne + 31) / 32 * 32; z.ea = ne <= 64 ? 64 : ne <= 128 ? 128 : 256; z.np = (n + 31) / 32 * 32;
-    z.zs = up256((size_t) n * 2 * z.kp * 2); z.zt = up256((size_t) z.np * 2 * z.ea * 2); z.kt = up256((size_t) z.np * 2);
+    z.zs = up256((size_t) z.np * 2 * z.kp * 2); z.zt = up256((size_t) z.np * 2 * z.ea * 2); z.kt = up256((size_t) z.np * 2);
     z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = up256((size_t) (E / 64) * 4);
     const int sp = rg_splits(n, E);
     z.part = dW && sp > 1 ? (size_t) sp * ne * E * 4 : 0;
