@@ -185,12 +185,15 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
 constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128, RG_RT = 2;
 
 // dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 32 rows at a time,
-// whose dz comes straight from the caches, D - 1 steps of 32 experts ahead; no barrier after the first. The product runs with the columns
-// as rows of the matrix core's tile, so a lane stores 4 consecutive columns. 64 rows a wave read LDS half as often and are 1 to 2 %
-// faster from 12000 rows on, but leave waves idle before: 1001 rows of 7168, 256 experts, both products 62 us instead of 51.
+// whose dz comes straight from the caches, D - 1 steps of 32 experts ahead and into the wave's next tile; no barrier after the first.
+// The product runs with the columns as rows of the matrix core's tile, so a lane stores 4 consecutive columns. dz's layout has each
+// load's 64 lanes side by side: rows apart, with 64 bytes each, cost 8192 rows of 7168, 256 experts, 12 of their 112 us. 64 rows a
+// wave need half the LDS reads but leave waves idle (both products, 1001 rows: 57 us instead of 48; 8192 rows: 203 instead of 205).
+// Workgroups: one a CU, and four beside dW above 4096 rows, which fill the CUs that dW leaves (16384 rows 405 us instead of 432; 256 rows
+// 29.7 and 28.8; dx alone, 8192 rows, 116 and 98: each loads its W again).
 template <int D>
 __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int part, int parts) {
-    constexpr int RT = RG_RT, AH = 2;
+    constexpr int RT = RG_RT, AH = 1;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
     const int j0 = ct * RG_COLS, nb = o.kp / 8, ns = o.kp / 32;
     const __amdgpu_buffer_rsrc_t rw = rg_rsrc(o.wt, (uint32_t) ((size_t) 2 * nb * g.E * 16));
@@ -280,7 +283,9 @@ __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o,
 // dW: a workgroup takes 128 columns of x, all experts (64 WR) and a run of 32-row steps. dz of a step is copied into LDS as it is
 // stored; x is read once, each wave 16 columns x 32 rows of it into registers (8 consecutive rows a lane), scaled, split and
 // written to LDS as 16-byte halves. Both are double-buffered: a step's barrier, the next step's copies and conversion, its products.
-// Waves: WR along the experts (64 each), 8 / WR along the columns (16 WR each).
+// Waves: WR along the experts (64 each), 8 / WR along the columns (16 WR each). x's conversion is spread between the products, one in
+// three instructions, and dz's operands are read one row tile ahead. 8192 rows of 7168, 256 experts: 64 steps of 1.8 us in a run, of
+// which the products with their LDS reads and barriers take 1.1 (the matrix cores are busy 43 % of the cycles).
 template <int WR>
 __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int run, int splits, float * part) {
     constexpr int EA = 64 * WR, AB = 4 * 2 * EA * 16, BB = 4 * 2 * RG_COLS * 16, BUF = AB + BB + RG_COLS * 4, JW = WR;
@@ -456,7 +461,7 @@ template <int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, int sp, 
     constexpr int DW = 2 * (4 * 2 * 64 * WR * 16 + 4 * 2 * RG_COLS * 16 + RG_COLS * 4), DX = 2 * 64 * WR * RG_COLS * 2;
     static LdsLimit limit;
     if (const hipError_t e = limit((const void *) k_route_mm<WR>, std::max(DW, DX))) { return e; }
-    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RG_RT - 1) / (16 * RG_RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, 256 / ct));
+    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RG_RT - 1) / (16 * RG_RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, (a.dW && a.n > 4096 ? 1024 : 256) / ct));
     k_route_mm<WR><<<(unsigned) (ct * ((a.dW ? sp : 0) + (a.dx ? parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, sp, parts, part);
     return hipGetLastError();
 }
