@@ -88,7 +88,12 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) { const int e = 8 * (wv + 4 * i) + u; v[i][u] = e < ne ? g.W[(size_t) e * g.E + c] : 0.f; }
+            for (int u = 0; u < 8; ++u) { const int e = 8 * (wv + 4 * i) + u; v[i][u] = g.W[(size_t) min(e, ne - 1) * g.E + c]; }   // (all loads out before the first use)
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { v[i][u] = 8 * (wv + 4 * i) + u < ne ? v[i][u] : 0.f; }
         }
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
