@@ -1,6 +1,6 @@
 // q4k.hip -- products of Q4_K matrices (ggml's 4-bit blocks with 6-bit group scales and mins, read in place) with Q8_K
-// rows. Q4_K is the format of the reference's attention and dense-layer matrices (tc_matvec<F_Q4K>,
-// src/fused_layer.cu:71-101).
+// rows. Q4_K is the format of the reference's attention and dense-layer matrices
+// (src/fused_layer.cu:71-101).
 //
 // A block is 256 weights in 144 bytes: fp16 d and dmin, 12 bytes of 6-bit scales s_j and mins m_j (8 sub-blocks of 32), 128
 // bytes of quants; group jj = 0..3 of 32 quant bytes holds sub-block 2 jj in its low nibbles and 2 jj + 1 in its high ones.

@@ -1,6 +1,6 @@
 """GPU: products of Q4_K matrices (fl_kq_matvec_dev with FL_Q4K, and as a format of the device-resident block) against the CPU
-checker, bit for bit: the integer sums are exact and the fp32 chain over the blocks is the same in every kernel, so a row's output
-has the same bits whatever n and R. The checker itself is held to a 64-bit product on the CPU (test_oracle_q4k.py)."""
+oracle, bit for bit: the integer sums are exact and the fp32 chain over the blocks is the same in every kernel, so a row's output
+has the same bits whatever n and R. The oracle itself is held to a 64-bit product on the CPU (test_oracle_q4k.py)."""
 import ctypes
 
 import numpy as np
@@ -63,7 +63,7 @@ def test_extremes(ctx):
 
 
 def test_non_finite_scales_stay_in_their_rows(ctx):
-    """a row of infinite d or NaN d8: its outputs as the checker's, the others' untouched"""
+    """a row of infinite d or NaN d8: its outputs as the oracle's, the others' untouched"""
     R, K = 20, 1024
     w = matrix(12, R, K).reshape(R, -1).copy()
     w[5, 0:2] = np.frombuffer(np.float16(np.inf).tobytes(), np.uint8)
@@ -211,7 +211,7 @@ def test_layer_of_many_rows(ctx):
                                 (orc.Q4K, 4, 4, 4)], ids=["all", "down", "shared", "down_iq2_shared"])
 def test_layer_formats(ctx, fm):
     """fl_moe_layer with Q4_K routed down and shared matrices at decode and prefill sizes: picks bit-identical, outputs within the
-    K-quants' bar of the checker, and each row's bits the same in a batch and alone (the per-pass kernels and the GEMMs)"""
+    K-quants' bar of the oracle, and each row's bits the same in a batch and alone (the per-pass kernels and the GEMMs)"""
     import torch
     from loki_amd import MoeLayerWeights
     from tests._helpers import host_matrix, make_x
@@ -261,7 +261,7 @@ def test_layer_formats(ctx, fm):
 
 def test_gguf_layer(ctx, tmp_path):
     """a layer of Q4_K routed down and shared matrices from a GGUF file: loaded tiled it runs through fl_moe_layer within the K-quants'
-    bar of the checker; the layout that fl_moe reads refuses the format"""
+    bar of the oracle; the layout that fl_moe reads refuses the format"""
     import torch
     from loki_amd import FL_LAYOUT_GGML, FL_LAYOUT_TILED, Gguf, LokiError, lib
     from tests import _gguf

@@ -1,4 +1,4 @@
-"""CPU: the checker's Q4_K against a 64-bit product of the dequantised matrix, built here from the format's definition."""
+"""CPU: the oracle's Q4_K against a 64-bit product of the dequantised matrix, built here from the format's definition."""
 import numpy as np
 import pytest
 
@@ -9,7 +9,7 @@ U = 2.0 ** -24
 
 
 @pytest.mark.parametrize("R,K,n", [(3, 256, 2), (5, 2048, 3), (2, 7168, 1), (2, 18432, 2)])
-def test_checker_matches_the_definition(R, K, n):
+def test_oracle_matches_the_definition(R, K, n):
     w = matrix(K + R, R, K)
     q, d, bs = q8k_rows(n, K, seed=K + n)
     y = orc.matvec_kq(orc.Q4K, w, R, K, q, d, bs)
@@ -18,7 +18,7 @@ def test_checker_matches_the_definition(R, K, n):
     assert np.all(np.abs(y - want) <= error_bound(w, R, K, q, d)), np.abs(y - want).max()
 
 
-def test_checker_dequantises():
+def test_oracle_dequantises():
     w = matrix(7, 4, 512)
     got = orc.dequant_kq(orc.Q4K, w, 512).astype(np.float64)
     want = dequant(w, 4, 512)
