@@ -51,14 +51,16 @@ constexpr int kq_shared_tok(int n) { return n <= 128 ? 16 : n <= 256 ? 32 : KQ_T
 //   max(s0 + s1 nb, ceil(G / 256) (p0 + p1 nb)) us:
 // what one workgroup needs from start to end, or the rounds of workgroups a CU goes through at its steady rate. The constants are
 // fitted to 247 sizes (512 .. 65536 rows, 4 .. 64 blocks, 1 .. 2000 tokens, weights from memory): 5 to 13 % rms a kernel, and the pick
-// is within 1 % of the best kernel on average, 20 % at worst. Examples, us: 16 tokens through 16384 -> 7168 19 (K split, 32 rows x 16 tokens)
-// against 24 (16 x 16); 37 through it 33 (K split, 32 x 48) against 43 (32 x 16) and 46 (64 x 32 tiles); 128 through 7168 -> 16384 46
-// (128 x 64) against 51 (64 x 64) and 75 (128 x 128); 2048 through it 485 (128 x 128) against 658 and 722.
+// is within 1 % of the best kernel on average, 16 % at worst from 3 tokens on. Examples, us: 16 tokens through 16384 -> 7168 19 (K split, 32 rows
+// x 16 tokens) against 24 (16 x 16); 37 through it 33 (K split, 32 x 48) against 43 (32 x 16) and 46 (64 x 32 tiles); 64 through 7168 ->
+// 65536 85 (256 x 64) against 99 (128 x 64); 501 through 7168 -> 7000, which leaves each CU one workgroup, 68 (128 x 128 on 8 waves) against
+// 75 (on 4); 2048 through 7168 -> 16384 502 (128 x 128 on 4 waves, two workgroups a CU) against 569 (8 waves) and 668 (128 x 64).
 struct Q4Kernel { int rows, toks; float s0, s1, p0, p1; };
-enum { Q4_KS_16_16, Q4_KS_32_16, Q4_KS_32_32, Q4_KS_32_48, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_128_128, Q4_KERNELS, Q4_VEC = Q4_KERNELS };
+enum { Q4_KS_16_16, Q4_KS_32_16, Q4_KS_32_32, Q4_KS_32_48, Q4_MM_64_32, Q4_MM_64_64, Q4_MM_128_64, Q4_MM_256_64, Q4_MM_128_128_8, Q4_MM_128_128, Q4_KERNELS, Q4_VEC = Q4_KERNELS };
 constexpr Q4Kernel Q4_KERNEL[Q4_KERNELS] = {
-    { 16, 16, 3.5f, 0.122f, 1.1f, 0.138f }, { 32, 16, 3.3f, 0.208f, 2.3f, 0.224f }, { 32, 32, 4.1f, 0.325f, 2.9f, 0.335f }, { 32, 48, 5.2f, 0.305f, 3.4f, 0.455f },
-    { 64, 32, 5.3f, 0.635f, 2.0f, 0.564f }, { 64, 64, 5.1f, 0.90f, 2.1f, 0.757f }, { 128, 64, 5.4f, 1.26f, 4.4f, 1.30f }, { 128, 128, 6.3f, 2.31f, 4.2f, 2.07f } };
+    { 16, 16, 4.0f, 0.113f, 1.1f, 0.138f }, { 32, 16, 3.8f, 0.194f, 2.3f, 0.226f }, { 32, 32, 4.2f, 0.325f, 2.9f, 0.344f }, { 32, 48, 5.2f, 0.311f, 3.4f, 0.471f },
+    { 64, 32, 5.4f, 0.639f, 1.9f, 0.573f }, { 64, 64, 5.2f, 0.91f, 2.1f, 0.749f }, { 128, 64, 5.4f, 1.27f, 4.6f, 1.29f }, { 256, 64, 7.2f, 2.25f, 7.2f, 2.25f },
+    { 128, 128, 6.3f, 2.06f, 6.3f, 2.06f }, { 128, 128, 6.3f, 2.33f, 5.1f, 1.93f } };
 constexpr float q4k_us(const Q4Kernel & k, int n, int64_t R, int K) {
     const int64_t g = (R + k.rows - 1) / k.rows * ((n + k.toks - 1) / k.toks), q = (g + 255) / 256;
     const float nb = (float) (K / 256), one = k.s0 + k.s1 * nb, all = (float) q * (k.p0 + k.p1 * nb);

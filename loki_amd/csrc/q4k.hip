@@ -365,8 +365,9 @@ template <int RT, int NT> hipError_t ks(const KqArgs & a, unsigned gy, hipStream
 // once per workgroup and each activation read from LDS serves RT tiles, so the largest tile, 128 x 128, does the most work an
 // instruction; smaller ones are for calls that it would leave CUs without a workgroup (launch_rules.h). 2048 tokens through 16384 rows of
 // 7168 502 us, 958 TFLOP/s of the real product: the matrix cores are busy 53 % of the cycles and the vector units with digits and terms
-// 48 %, at the 1.9 GHz that the card then holds; 501 tokens through 7000 rows of 7168 75 us, 220 workgroups and so one wave a SIMD, whose
-// products (40 %) and vector work (35 %) follow each other.
+// 48 %, at the 1.9 GHz that the card then holds. Where a CU gets one workgroup, one wave a SIMD does its products (40 % of the cycles) and
+// its vector work (35 %) one after the other; 8 waves of one row tile then overlap the two, at twice the LDS reads: 501 tokens through
+// 7000 rows of 7168 68 us instead of 75.
 template <int RT, int NT, int W, int D>
 __global__ void __launch_bounds__(64 * W, 2) k_q4k_mm(Q4Args a) {
 #pragma clang fp contract(off)
@@ -571,6 +572,8 @@ hipError_t launch_q4k(const KqArgs & a, int max_slots, int grid_experts, hipStre
     case Q4_MM_64_32: return mm<1, 2, 4, 5>(a, st);
     case Q4_MM_64_64: return mm<1, 4, 4, 3>(a, st);
     case Q4_MM_128_64: return mm<1, 4, 8, 3>(a, st);
+    case Q4_MM_256_64: return mm<2, 4, 8, 3>(a, st);
+    case Q4_MM_128_128_8: return mm<1, 8, 8, 3>(a, st);
     default: return mm<2, 8, 4, 2>(a, st);
     }
 }

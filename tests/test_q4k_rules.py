@@ -68,8 +68,9 @@ def test_few_tokens_do_not_take_many_token_tiles(rules):
 # rows, columns, tokens of the device tests that go through each kernel (test_gpu_q4k.py), ragged in rows and tokens: 1 to 28 blocks a row
 SIZES = {"ks_32_16": [(7001, 512, 12), (7001, 7168, 13)], "ks_32_32": [(1001, 1024, 200), (7001, 512, 20)],
          "ks_32_48": [(7001, 768, 40), (2049, 768, 130)], "mm_64_32": [(2049, 1024, 200), (8200, 768, 40), (1001, 3328, 403)],
-         "mm_64_64": [(4100, 256, 257), (7001, 768, 257), (1001, 3328, 601)], "mm_128_64": [(8200, 512, 400), (4100, 2048, 257), (7001, 3328, 130)],
-         "mm_128_128": [(8200, 256, 601), (7001, 768, 400), (7001, 1280, 403)]}
+         "mm_64_64": [(4100, 256, 257), (7001, 768, 130), (1001, 3328, 601)], "mm_128_64": [(4100, 2048, 257), (7001, 3328, 130)],
+         "mm_256_64": [(8200, 256, 403), (8200, 2048, 403), (33000, 768, 130)], "mm_128_128_8": [(2049, 256, 1000), (7001, 768, 403), (4100, 3328, 601)],
+         "mm_128_128": [(8200, 256, 601), (16000, 768, 333), (7001, 1280, 1000)]}
 KERNELS = ["ks_16_16", *SIZES]
 
 
