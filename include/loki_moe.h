@@ -183,8 +183,8 @@ int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, 
 int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
 /* Workspaces of fl_balance_loss_dev, fl_route_grad_dev and Q4_K products are the context's. They grow in the call that needs more
- * (hipMalloc; FL_ENOMEM when that fails, as it does under graph capture) and no block is freed before fl_free, so a captured call stays
- * valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured from one context share
+ * (hipMalloc; FL_ENOMEM when that fails, and under graph capture, where nothing is allocated and the capture goes on) and no block is
+ * freed before fl_free, so a captured call stays valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured from one context share
  * its workspaces and must not run at the same time. The context's device has to be the current one (FL_EINVAL). */
 /* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device) */
 int fl_dispatch_dev(FLCtx *, const int * sel, int n, int topk, int n_exp, int * counts, int * offsets, int * perm, int * inv, int * act, int * nact);

@@ -284,11 +284,20 @@ static int need_device(FLCtx * c) {
     TRY(c, hipGetDevice(&dev));
     return dev == c->dev ? FL_OK : fail(c, FL_EINVAL, "the current device is %d, the context's %d", dev, c->dev);
 }
+// a workspace of at least `bytes`; under graph capture it has to be there already (nothing is allocated, the capture stays valid)
+static int grow(FLCtx * c, KeptBuf & b, size_t bytes) {
+    if (b.p && bytes <= b.cap) { return FL_OK; }
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    TRY(c, hipStreamIsCapturing(c->st, &cap));
+    if (cap != hipStreamCaptureStatusNone) { return fail(c, FL_ENOMEM, "%zu bytes of workspace are needed under graph capture: make one call of this size before it", bytes); }
+    if (b.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
+    return FL_OK;
+}
 // Q4_K products of many rows take a scratch (their rows' sub-block sums)
 static int q4_scratch(FLCtx * c, KqArgs & k, int fmt) {
     const size_t bytes = fmt == FL_Q4K ? q4k_scratch_bytes(k.n, (int64_t) k.R * (k.w2 ? 2 : 1), k.K) : 0;
     if (bytes == 0) { return FL_OK; }
-    if (c->q4.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
+    if (int rc = grow(c, c->q4, bytes)) { return rc; }
     k.xs = c->q4.p;
     return FL_OK;
 }
@@ -344,7 +353,7 @@ extern "C" int fl_balance_loss_dev(FLCtx * c, const float * logits, const int * 
     if (!loss || (n > 0 && !sel)) { return fail(c, FL_EINVAL, "null pointer"); }
     if ((n > 0 && !covers(sel, (size_t) n * topk * 4)) || !covers(loss, (size_t) nseq * 4)) { return fail(c, FL_EINVAL, "sel's or loss's allocation is smaller than its shape"); }
     if (b.chunks > 1) {   // (the workspace has one size)
-        if (c->bal.ensure((size_t) BALANCE_PARTS * NEXP_MAX * 8) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation failed"); }
+        if (int rc = grow(c, c->bal, (size_t) BALANCE_PARTS * NEXP_MAX * 8)) { return rc; }
         b.part = (float *) c->bal.p; b.pcnt = (int *) c->bal.p + BALANCE_PARTS * NEXP_MAX;
     }
     TRY(c, launch_balance(b, c->st));
@@ -391,7 +400,7 @@ extern "C" int fl_route_grad_dev(FLCtx * c, const float * W, const float * x, co
         return FL_OK;
     }
     const size_t bytes = route_grad_scratch(n, n_exp, E, dW != nullptr, dx != nullptr);
-    if (c->rg.ensure(bytes) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", bytes); }
+    if (int rc = grow(c, c->rg, bytes)) { return rc; }
     TRY(c, launch_route_grad(a, c->rg.p, c->st));
     return FL_OK;
 }
@@ -712,7 +721,7 @@ static int moe_layer(FLCtx * c, const FLMoeLayer * L, const float * x, int n, fl
     {   // the shared expert's Q4_K matrices on tiles
         const size_t gu = q4k_scratch_bytes(n, lf[1] == lf[2] ? 2 * (int64_t) H : H, E), dn = q4k_scratch_bytes(n, E, H);
         const size_t q4 = std::max(lf[1] == FL_Q4K || lf[2] == FL_Q4K ? gu : 0, lf[3] == FL_Q4K ? dn : 0);
-        if (q4 > 0 && c->q4.ensure(q4) != hipSuccess) { (void) hipGetLastError(); return fail(c, FL_ENOMEM, "device allocation of %zu bytes failed", q4); }
+        if (q4 > 0) { if (int rc = grow(c, c->q4, q4)) { return rc; } }
     }
     c->last_n = n; c->last_P = P; c->last_fused = fused ? 1 : 0; c->last_kernel = 0;
     hipStream_t st = c->st;

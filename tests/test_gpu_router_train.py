@@ -385,3 +385,38 @@ def test_training_step_eager_and_captured(ctx):
     finally:
         torch.cuda.synchronize()
         other.close()
+
+
+def test_workspace_is_not_grown_under_capture(ctx):
+    """a captured call that would have to allocate is refused by its code, and the capture goes on: the graph holds what came before
+    and after it"""
+    import torch
+    from loki_amd import FL_ENOMEM, Context, lib
+    n, ne = 4000, 64
+    z = torch.randn((n, ne), device="cuda"); sel = torch.zeros((n, 8), dtype=torch.int32, device="cuda")
+    counts = torch.empty((1, ne), dtype=torch.int32, device="cuda"); loss = torch.empty(1, device="cuda")
+    x = torch.zeros(1000, device="cuda")
+    c = Context()
+    try:
+        side = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        c.check(lib().fl_set_stream(c.ctx, side.cuda_stream))
+        call = lambda: lib().fl_balance_loss_dev(c.ctx, z.data_ptr(), sel.data_ptr(), None, n, 1, ne, 8, 1e-3, counts.data_ptr(), loss.data_ptr())   # noqa: E731
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            x += 1
+            rc = call()
+            x += 1
+        assert rc == FL_ENOMEM and b"capture" in lib().fl_last_error(c.ctx)
+        for rep in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.all(x == 2 * (rep + 1))
+        with torch.cuda.stream(side):
+            assert call() == 0
+        torch.cuda.synchronize()
+        assert counts[0, 0].item() == 8 * n
+        del graph
+    finally:
+        torch.cuda.synchronize()
+        c.close()
