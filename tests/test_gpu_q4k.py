@@ -131,6 +131,27 @@ def test_every_kernel(ctx, name):
         assert same(o[16:16 + n * R].reshape(n, R), orc.matvec_kq(orc.Q4K, w, R, K, q, d, bs)), (R, K, n)
 
 
+def test_offsets_past_32_bits(ctx):
+    """the last rows of a 4.8 GB matrix, and outputs behind 2^32 bytes of others, as from those rows alone"""
+    import torch
+    R, K, T = 1200007, 7168, 45
+    rb = K // 256 * 144
+    tail = matrix(81, T, K)
+    w = torch.zeros(R * rb + 1, dtype=torch.uint8, device="cuda")[:R * rb]
+    w[(R - T) * rb:] = torch.from_numpy(tail).cuda()
+    for n in (1, 5, 40, 1000):
+        q, d, bs = q8k_rows(n, K, seed=82 + n)
+        print("q4_K 4.8 GB n %d" % n, flush=True)
+        y = ctx.kq_matvec(orc.Q4K, w, R, K, torch.from_numpy(q).cuda(), torch.from_numpy(d).cuda())
+        ctx.sync()
+        want = orc.matvec_kq(orc.Q4K, tail, T, K, q, d, bs)
+        assert same(np.ascontiguousarray(y[:, R - T:].cpu().numpy()), want), n
+        assert not torch.any(y[:, :R - T]), n
+        del y
+    del w
+    torch.cuda.empty_cache()
+
+
 def test_refusals(ctx):
     import torch
     from loki_amd import FL_EINVAL, FL_OK, FL_Q4K, lib

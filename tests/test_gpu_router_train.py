@@ -420,3 +420,50 @@ def test_workspace_is_not_grown_under_capture(ctx):
     finally:
         torch.cuda.synchronize()
         c.close()
+
+
+# several tiles of rows a wave, with experts that fill their steps of 32 or do not, and dx's parts beside dW for many rows
+@pytest.mark.parametrize("n,ne,topk,E", [(3001, 130, 4, 7168), (2100, 100, 8, 16384), (5003, 64, 6, 8192), (4100, 256, 8, 7168)])
+def test_route_grad_many_rows(ctx, rule, n, ne, topk, E):
+    rule(topk)
+    W, x, z, sel, dw, dz = inputs(n, ne, topk, E, n + ne + E)
+    print("route_grad n %d ne %d E %d" % (n, ne, E), flush=True)
+    dl, dW, dx = run_grad(ctx, W, x, z, sel, dw, dz)
+    check_products(W, x, dl, dW, dx)
+    _, _, alone = run_grad(ctx, W, x, z, sel, dw, dz, need_dW=False)
+    assert np.array_equal(alone.view(np.uint32), dx.view(np.uint32))   # a row's dx has the same bits however the rows are shared out
+    _, _, tail = run_grad(ctx, W, x[-70:], z[-70:], sel[-70:], dw[-70:], dz[-70:], need_dW=False)
+    assert np.array_equal(tail.view(np.uint32), dx[-70:].view(np.uint32))
+
+
+def test_offsets_past_32_bits(ctx, rule):
+    """rows behind 2^32 bytes of logits, gradients, x and dx: as the same rows alone"""
+    import torch
+    rule(2)
+    n, ne, T = 1 << 23, 160, 100   # 5.4 GB of logits
+    g = torch.Generator(device="cuda").manual_seed(4)
+    z = torch.randn((T, ne), device="cuda", generator=g); sel = torch.topk(z, 2, dim=1).indices.to(torch.int32).contiguous()
+    big = torch.zeros((n, ne), device="cuda"); big[-T:] = z
+    bsel = torch.zeros((n, 2), dtype=torch.int32, device="cuda"); bsel[-T:] = sel
+    seq = torch.tensor([n - T - 5, n - T, n], dtype=torch.int32, device="cuda")
+    counts, loss = ctx.balance_loss(big, bsel, 0.5, seq=seq)
+    grad = ctx.balance_loss_grad(big, counts, 2, 0.5, seq=seq)
+    c1, l1 = ctx.balance_loss(z, sel, 0.5)
+    g1 = ctx.balance_loss_grad(z, c1, 2, 0.5)
+    ctx.sync()
+    assert torch.equal(counts[1], c1[0])
+    check_balance((c1.cpu().numpy(), l1.cpu().numpy(), g1.cpu().numpy()), z.cpu().numpy(), sel.cpu().numpy(), np.float32(0.5), [0, T])
+    assert abs(loss[1].item() - l1.item()) <= 460 * U * l1.item()   # two orders of the same sum, (130 + 100) u each
+    assert torch.equal(grad[-T:].view(torch.int32), g1.view(torch.int32)) and not torch.any(grad[:-T - 5])
+    del big, bsel, grad
+    n, ne, E, T = 65536, 8, 20480, 64   # 5.4 GB of x and of dx
+    W = 0.02 * torch.randn((ne, E), device="cuda", generator=g)
+    x = torch.zeros((n, E), device="cuda"); x[-T:] = torch.randn((T, E), device="cuda", generator=g)
+    z = torch.randn((n, ne), device="cuda", generator=g); sel = torch.topk(z, 2, dim=1).indices.to(torch.int32).contiguous()
+    dz = torch.zeros((n, ne), device="cuda"); dz[-T:] = 1e-3 * torch.randn((T, ne), device="cuda", generator=g)
+    dl, dW, dx = ctx.route_grad(W, x, z, sel, dz=dz)
+    ctx.sync()
+    assert not torch.any(dx[:-T]) and torch.equal(dl, dz)
+    check_products(W.cpu().numpy(), x[-T:].cpu().numpy(), dz[-T:].cpu().numpy(), dW.cpu().numpy(), dx[-T:].cpu().numpy())
+    del x, dx
+    torch.cuda.empty_cache()
