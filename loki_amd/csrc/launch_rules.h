@@ -1,5 +1,5 @@
 // launch_rules.h -- which kernel a call's sizes get: plain functions of the sizes, without HIP, so that a CPU test can hold
-// them against each other (tests/test_launch_rules.py).
+// them against each other (tests/test_launch_rules.py, test_q4k_rules.py, test_route_rules.py).
 #pragma once
 #include <stdint.h>
 
@@ -78,5 +78,26 @@ constexpr int q4k_kernel(int n, int64_t R, int K, bool tiles) {
     return best;
 }
 constexpr bool q4k_tiled(int kernel) { return kernel >= Q4_MM_64_32 && kernel < Q4_KERNELS; }
+
+// ---------------------------------------------------------------- the router's backward products (route_grad.hip)
+// Runs of rows that a tile of ROUTE_COLS columns of dW is split into, and parts of dx (ROUTE_ROWS rows at a time). One of the two products
+// alone: one workgroup a CU. Both: one a CU together, three fifths of them dW's, whose rows cost more (5000 rows of 4096, 256 experts, 5 + 3
+// 85 us, 8 + 8 89; 3000 rows of 6144, 160 experts, 3 + 2 67, 5 + 5 83); where that leaves more than a tenth of the CUs idle and x is large,
+// several rounds of workgroups pay instead, dx's in small pieces (8192 rows of 7168: 4 + 18 207 us, 2 + 2 229; 700 rows: 39 and 37). Over
+// 141 sizes (200 .. 16000 rows of 1024 .. 16384, 64 .. 256 experts) the pick is within 3 % of the best measured on average.
+constexpr int ROUTE_COLS = 128, ROUTE_ROWS = 256;
+struct RouteCut { int splits, parts; };
+constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {
+    const int ct = E / ROUTE_COLS, one = 256 / ct;   // workgroups a column tile, one a CU
+    int splits = one, parts = one;
+    if (dW && dx) {
+        const int both = one > 2 ? one : 2;
+        if (one * ct < 230 && (int64_t) n * E >= 25000000) { parts = 1024 / ct; }
+        else { splits = (3 * both + 2) / 5; parts = both - splits; }
+    }
+    const int ms = n / 128, mp = (n + ROUTE_ROWS - 1) / ROUTE_ROWS;   // a run of at least 128 rows, a part that has rows
+    splits = splits < ms ? splits : ms; parts = parts < mp ? parts : mp;
+    return { splits > 1 ? splits : 1, parts > 1 ? parts : 1 };
+}
 
 }  // namespace lk

@@ -187,15 +187,14 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
     }
 }
 
-constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = 128, RG_RT = 2;
+constexpr int RG_W = 8, RG_T = 64 * RG_W, RG_COLS = ROUTE_COLS, RG_RT = 2;
+static_assert(16 * RG_RT * RG_W == ROUTE_ROWS, "rows that a workgroup of dx takes at a time");
 
 // dx: a workgroup keeps 128 columns of W, all experts, both halves, in LDS (at most 128 KB) and its waves take 32 rows at a time,
 // whose dz comes straight from the caches, D - 1 steps of 32 experts ahead and into the wave's next tile; no barrier after the first.
 // The product runs with the columns as rows of the matrix core's tile, so a lane stores 4 consecutive columns. dz's layout has each
 // load's 64 lanes side by side: rows apart, with 64 bytes each, cost 8192 rows of 7168, 256 experts, 12 of their 112 us. 64 rows a
 // wave need half the LDS reads but leave waves idle (both products, 1001 rows: 57 us instead of 48; 8192 rows: 203 instead of 205).
-// Workgroups: one a CU, and four beside dW above 4096 rows, which fill the CUs that dW leaves (16384 rows 405 us instead of 432; 256 rows
-// 29.7 and 28.8; dx alone, 8192 rows, 116 and 98: each loads its W again).
 template <int D>
 __device__ __forceinline__ void route_dx(const RouteGradArgs & g, const Ops & o, LK_LOCAL uint8_t * lds, int ct, int part, int parts) {
     constexpr int RT = RG_RT, AH = 1;
@@ -449,7 +448,6 @@ __global__ void __launch_bounds__(256) k_route_join(const float * __restrict__ p
     *d = accumulate ? *d + v : v;
 }
 
-int rg_splits(int n, int E) { return std::max(1, std::min((n + 127) / 128, 256 / (E / RG_COLS))); }
 constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 struct Sizes { int kp, ea, np; size_t zs, zt, kt, wt, kw, part, all; };
 Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
@@ -457,17 +455,17 @@ Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
     z.kp = (ne + 31) / 32 * 32; z.ea = ne <= 64 ? 64 : ne <= 128 ? 128 : 256; z.np = (n + 31) / 32 * 32;
     z.zs = up256((size_t) z.np * 2 * z.kp * 2); z.zt = up256((size_t) z.np * 2 * z.ea * 2); z.kt = up256((size_t) z.np * 2);
     z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = up256((size_t) (E / 64) * 4);
-    const int sp = rg_splits(n, E);
+    const int sp = route_cut(n, E, dW, dx).splits;
     z.part = dW && sp > 1 ? (size_t) sp * ne * E * 4 : 0;
     z.all = z.zs + z.zt + z.kt + z.wt + z.kw + z.part;
     return z;
 }
-template <int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, int sp, float * part, hipStream_t st) {
+template <int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, RouteCut cut, float * part, hipStream_t st) {
     constexpr int DW = 2 * (4 * 2 * 64 * WR * 16 + 4 * 2 * RG_COLS * 16 + RG_COLS * 4), DX = 2 * 64 * WR * RG_COLS * 2;
     static LdsLimit limit;
     if (const hipError_t e = limit((const void *) k_route_mm<WR>, std::max(DW, DX))) { return e; }
-    const int ct = a.E / RG_COLS, tiles = (a.n + 16 * RG_RT - 1) / (16 * RG_RT), parts = std::max(1, std::min((tiles + RG_W - 1) / RG_W, (a.dW && a.n > 4096 ? 1024 : 256) / ct));
-    k_route_mm<WR><<<(unsigned) (ct * ((a.dW ? sp : 0) + (a.dx ? parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, sp, parts, part);
+    const int ct = a.E / RG_COLS;
+    k_route_mm<WR><<<(unsigned) (ct * ((a.dW ? cut.splits : 0) + (a.dx ? cut.parts : 0))), RG_T, std::max(a.dW ? DW : 0, a.dx ? 2 * o.kp * RG_COLS * 2 : 0), st>>>(a, o, cut.splits, cut.parts, part);
     return hipGetLastError();
 }
 
@@ -484,10 +482,11 @@ hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_
     o.kp = z.kp; o.ea = z.ea; o.np = z.np;
     o.zs = (_Float16 *) p; p += z.zs; o.zt = (_Float16 *) p; p += z.zt; o.kt = (short *) p; p += z.kt; o.wt = (_Float16 *) p; p += z.wt; o.kw = (int *) p; p += z.kw;
     float * part = (float *) p;
-    const int nw = a.dx ? a.E / 64 : 0, sp = rg_splits(a.n, a.E);
+    const RouteCut cut = route_cut(a.n, a.E, a.dW != nullptr, a.dx != nullptr);
+    const int nw = a.dx ? a.E / 64 : 0, sp = cut.splits;
     k_route_prep<<<nw + z.np / 8, 256, 0, st>>>(a, o, nw);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && (a.dW || a.dx)) { e = o.ea == 64 ? go<1>(a, o, sp, part, st) : o.ea == 128 ? go<2>(a, o, sp, part, st) : go<4>(a, o, sp, part, st); }
+    if (e == hipSuccess && (a.dW || a.dx)) { e = o.ea == 64 ? go<1>(a, o, cut, part, st) : o.ea == 128 ? go<2>(a, o, cut, part, st) : go<4>(a, o, cut, part, st); }
     if (e == hipSuccess && a.dW && sp > 1) {
         const int64_t n4 = (int64_t) a.n_exp * a.E / 4;
         k_route_join<<<(unsigned) ((n4 + 255) / 256), 256, 0, st>>>(part, sp, n4, a.accumulate, a.dW);

@@ -423,7 +423,7 @@ def test_workspace_is_not_grown_under_capture(ctx):
 
 
 # several tiles of rows a wave, with experts that fill their steps of 32 or do not, and dx's parts beside dW for many rows
-@pytest.mark.parametrize("n,ne,topk,E", [(3001, 130, 4, 7168), (2100, 100, 8, 16384), (5003, 64, 6, 8192), (4100, 256, 8, 7168)])
+@pytest.mark.parametrize("n,ne,topk,E", [(3001, 130, 4, 7168), (2100, 100, 8, 16384), (5003, 64, 6, 8192), (4100, 256, 8, 7168), (2900, 30, 5, 2048)])
 def test_route_grad_many_rows(ctx, rule, n, ne, topk, E):
     rule(topk)
     W, x, z, sel, dw, dz = inputs(n, ne, topk, E, n + ne + E)
