@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
         }
     }
     __syncthreads();
-    for (int p = threadIdx.x; p < 2 * o.ea; p += 256) {   // 8 rows of an expert
+    for (int p = threadIdx.x; p < (g.dW ? 2 * o.ea : 0); p += 256) {   // 8 rows of an expert
         const int q = p / o.ea, c = p % o.ea;
         gh8 h;
 #pragma unroll
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
         *reinterpret_cast<gh8 *>(o.zt + (((size_t) tb * 2 + q) * o.ea + c) * 8) = h;
     }
     const int nc = o.kp / 8;
-    for (int p = threadIdx.x; p < 16 * nc; p += 256) {    // 8 experts of a row
+    for (int p = threadIdx.x; p < (g.dx ? 16 * nc : 0); p += 256) {    // 8 experts of a row
         const int i = p % 8, c = p / 8;
         const int h = c / nc, b = c % nc, t = t0 + i;
         *reinterpret_cast<gh8 *>(o.zs + ((((size_t) (t >> 4) * (nc / 4) + b / 4) * 2 + h) * 64 + (b % 4) * 16 + (t & 15)) * 8) = *reinterpret_cast<const gh8 *>(&s_h[h][i][8 * b]);
@@ -453,7 +453,7 @@ struct Sizes { int kp, ea, np; size_t zs, zt, kt, wt, kw, part, all; };
 Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
     Sizes z{};
     z.kp = (ne + 31) / 32 * 32; z.ea = ne <= 64 ? 64 : ne <= 128 ? 128 : 256; z.np = (n + 31) / 32 * 32;
-    z.zs = up256((size_t) z.np * 2 * z.kp * 2); z.zt = up256((size_t) z.np * 2 * z.ea * 2); z.kt = up256((size_t) z.np * 2);
+    z.zs = dx ? up256((size_t) z.np * 2 * z.kp * 2) : 0; z.zt = dW ? up256((size_t) z.np * 2 * z.ea * 2) : 0; z.kt = up256((size_t) z.np * 2);
     z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = up256((size_t) (E / 64) * 4);
     const int sp = route_cut(n, E, dW, dx).splits;
     z.part = dW && sp > 1 ? (size_t) sp * ne * E * 4 : 0;

@@ -432,6 +432,10 @@ def test_route_grad_many_rows(ctx, rule, n, ne, topk, E):
     check_products(W, x, dl, dW, dx)
     _, _, alone = run_grad(ctx, W, x, z, sel, dw, dz, need_dW=False)
     assert np.array_equal(alone.view(np.uint32), dx.view(np.uint32))   # a row's dx has the same bits however the rows are shared out
+    for kw in ({"need_dx": False}, {"need_dW": False, "need_dx": False}):   # dW alone (cut into runs of its own), dlogits alone
+        dl2, dW2, _ = run_grad(ctx, W, x, z, sel, dw, dz, **kw)
+        assert np.array_equal(dl2.view(np.uint32), dl.view(np.uint32))
+        check_products(W, x, dl, dW2, None)
     _, _, tail = run_grad(ctx, W, x[-70:], z[-70:], sel[-70:], dw[-70:], dz[-70:], need_dW=False)
     assert np.array_equal(tail.view(np.uint32), dx[-70:].view(np.uint32))
 
