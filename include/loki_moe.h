@@ -178,8 +178,13 @@ int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, 
  *   dW [n_exp][E] = (accumulate: +=) dlogits^T x,   dx [n][E] = dlogits W
  * (each of the three may be NULL: not computed). logits and sel are fl_route_dev's; the bias has no gradient; entries of sel
  * outside 0 .. n_exp - 1 are skipped. n <= 65536, E a multiple of 1024 up to 65536, dW and dx 16-byte aligned. Deterministic, no
- * atomics. The products are exact to about 2^-22 of each term (route_grad.hip); the operands' split copies are the context's, n *
- * n_exp * 8 + n_exp * E * 4 bytes and dW's partial sums, kept until fl_free. */
+ * atomics. The products take their operands in two fp16 halves and sum in fp32: a term is exact to about 2^-22 of itself as long as
+ * its operands are not far below the largest ones that share their scale. Below, an operand's error is at most
+ *   dx  2^-39 of row t's largest |dlogits|; 2^-39 of the largest |W| of 64 columns
+ *   dW  2^-27 of expert e's largest |dlogits| in 8 rows and 2^-36 of its largest in all; 2^-39 of the largest |x| of the column, of rows
+ *       with a gradient (rows whose dlogits are all 0 have no part in it, whatever finite values x holds there)
+ * The operands' split copies are the context's: for n_exp up to kp (a multiple of 32) and ea (64, 128 or 256) about n * (4 kp + 4.25 ea)
+ * + kp * E * 4 bytes and dW's partial sums, rounded up to a power of two. */
 int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
 /* Workspaces of fl_balance_loss_dev, fl_route_grad_dev and Q4_K products are the context's. They grow in the call that needs more

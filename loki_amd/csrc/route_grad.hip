@@ -7,14 +7,18 @@
 // The bias only takes part in the selection and has no gradient.
 //
 // The two products run on the fp16 matrix cores at fp32's precision: an operand v is taken as v 2^k = hi + lo, two fp16 of 11 bits
-// each, and a product is hi hi + hi lo + lo hi in fp32 sums; what is left out, lo lo, and lo's own rounding are below 2^-22 of the
-// product. Three fp16 products cost a third of what the fp32 matrix cores take. k puts the largest finite |v| at 2^14 .. 2^15, so
-// that values down to 2^-18 of it keep both halves whole and smaller ones an absolute error of 2^-39 of it:
-//   dz   one k per row t, which both products can take: dx's row t is scaled back by 2^-k_t, and in dW's sum over t the factor
-//        goes to x (x 2^(K0 - k_t), K0 the smallest k of the rows summed, so no factor exceeds 1)
-//   W    one k per 64 columns, found by the kernel that splits it
-//   x    one k per column, running: a slab's maximum that passes the present range lowers k, and the accumulators of that column
-//        follow (as the running maximum of an online softmax)
+// each, and a product is hi hi + hi lo + lo hi in fp32 sums; what is left out, lo lo, and each half's own rounding are below 2^-22 of
+// the product. Three fp16 products cost a third of what the fp32 matrix cores take. k puts the largest finite |v| of those that share
+// it at 2^14 .. 2^15, so that values down to 2^-18 of it keep both halves whole and smaller ones an absolute error of 2^-39 of it:
+//   dx   dz: one k per row t (dx's row t is scaled back by 2^-k_t). W: one k per 64 columns, found by the kernel that splits it
+//   dW   dz: one k per expert. What a row's picks get is a million times and more what the balance loss gives the other experts, and
+//        an expert that is picked in few rows or none gets nothing else: on the row's scale its whole row of dW would be lost. It
+//        comes in two steps, since nobody knows an expert's maximum when dz is split: the halves are made with a k per expert and 8
+//        rows (the maximum at 2^2 .. 2^3: below it an absolute error of 2^-27 of these 8 rows' maximum), and a lane brings its operands
+//        to the smallest k of its run's rows by one fp16 factor of 2^12 .. 2^-24 (rows below 2^-36 of the expert's largest become 0).
+//        x: one k per column, running: a slab's maximum that passes the present range lowers k, and the accumulators of that column
+//        follow (as the running maximum of an online softmax). Rows without any gradient have no part in it: what padding holds
+//        there must not cost the others their bits.
 // Non-finite values take no part in the maxima of dz and W; they make the outputs that they enter non-finite.
 #include "moe_device.h"
 #include "moe_kernels.h"
@@ -26,13 +30,13 @@ namespace lk {
 namespace {
 
 constexpr float RG_CLAMP = 0x1p-14f;   // select_token_p's
-constexpr int RG_NONE = 1000;          // k of a row without gradient: its factor is 0
+constexpr int RG_NONE = 1000;          // k of a row without gradient: dx's is 0
+constexpr int RG_ZK = 113, RG_ZNONE = 142, RG_ZUP = 12;   // dW's dz: k + RG_ZK is a byte; k of 8 rows without gradient; halves are made with k - RG_ZUP
 typedef float gf4 __attribute__((ext_vector_type(4)));
 typedef _Float16 gh8 __attribute__((ext_vector_type(8)));
-typedef short gs8 __attribute__((ext_vector_type(8)));
 
-// the k that puts m > 0 at 2^14 .. 2^15 (m finite; subnormals as the smallest normal number)
-__device__ __forceinline__ int rg_k(float m) { return min(126, 141 - max(1, (int) (__builtin_bit_cast(uint32_t, m) >> 23))); }
+// the k that puts m > 0 at 2^14 .. 2^15 (m finite; subnormals as the smallest normal number), at most MOST
+template <int MOST = 126> __device__ __forceinline__ int rg_k(float m) { return min(MOST, 141 - max(1, (int) (__builtin_bit_cast(uint32_t, m) >> 23))); }
 __device__ __forceinline__ float rg_pow2(int k) { return __builtin_bit_cast(float, (uint32_t) (min(max(k, -126), 127) + 127) << 23); }
 __device__ __forceinline__ float rg_mag(float v) { const float a = fabsf(v); return a < INFINITY ? a : 0.f; }
 __device__ __forceinline__ void rg_split(float v, _Float16 & hi, _Float16 & lo) { hi = (_Float16) v; lo = (_Float16) (v - (float) hi); }
@@ -70,16 +74,18 @@ __device__ __forceinline__ void rg_lds16(__amdgpu_buffer_rsrc_t r, LK_LOCAL uint
 
 // The operands in memory, halves of 16 bytes = 8 consecutive K values:
 //   zs [t / 16][K / 32][hi, lo][K / 8 % 4][t % 16][8]   dz, K = experts (n_exp up to a multiple of 32, zeros): the order of a wave's lanes
+//   kt [t]                      the rows' k (zs)
 //   zt [t / 8][hi, lo][ea][8]   dz of 8 rows, K = rows (ea: n_exp up to 64, 128 or 256, zeros; rows up to a multiple of 32, zeros)
-//   kt [t]                      the rows' k
+//   zk [t / 8][ea / 64][16]     x: the k of experts r, r + 16, r + 32, r + 48 of the 64, bytes; y: bit i: row i of the 8 has a gradient
 //   wt [hi, lo][kp / 8][E][8]   W, K = experts; kw [E / 64] its k
-struct Ops { _Float16 * zs, * zt, * wt; short * kt; int * kw; int kp, ea, np; };
+struct Ops { _Float16 * zs, * zt, * wt; short * kt; uint2 * zk; int * kw; int kp, ea, np; };
 
 // The first nw workgroups split 64 columns of W each (all experts in registers between the maximum and the split). The others take 8
 // rows, two a wave: lane k < topk holds pick k, then the columns e = lane + 64 j of the row.
 __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int nw) {
     __shared__ _Float16 s_h[2][8][NEXP_MAX];
-    __shared__ float s_m[4];
+    __shared__ float s_v[8][NEXP_MAX], s_m[4];
+    __shared__ uint8_t s_k[NEXP_MAX], s_on[8];
     const int lane = lane_id(), wv = threadIdx.x >> 6, ne = g.n_exp;
     if ((int) blockIdx.x < nw) {
         constexpr int NB = NEXP_MAX / 32;   // experts 8 (wv + 4 i) .. + 7 a wave
@@ -161,7 +167,7 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
         const bool none = m == 0.f && __ballot(odd) == 0;
         const int k = none ? RG_NONE : rg_k(m);
         const float sc = none ? 1.f : rg_pow2(k);
-        if (lane == 0) { o.kt[t] = (short) k; }
+        if (lane == 0) { s_on[wv + 4 * h] = none ? 0 : 1; if (g.dx) { o.kt[t] = (short) k; } }
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int c = lane + 64 * j;
@@ -169,15 +175,33 @@ __global__ void __launch_bounds__(256) k_route_prep(RouteGradArgs g, Ops o, int 
             _Float16 a, l;
             rg_split(v[h][j] * sc, a, l);
             s_h[0][wv + 4 * h][c] = a; s_h[1][wv + 4 * h][c] = l;
+            s_v[wv + 4 * h][c] = v[h][j];
         }
     }
     __syncthreads();
-    for (int p = threadIdx.x; p < (g.dW ? 2 * o.ea : 0); p += 256) {   // 8 rows of an expert
-        const int q = p / o.ea, c = p % o.ea;
-        gh8 h;
+    if (g.dW) {   // 8 rows of expert threadIdx.x
+        const int c = (int) threadIdx.x;
+        if (c < o.ea) {
+            float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { h[i] = s_h[q][i][c]; }
-        *reinterpret_cast<gh8 *>(o.zt + (((size_t) tb * 2 + q) * o.ea + c) * 8) = h;
+            for (int i = 0; i < 8; ++i) { m = fmaxf(m, rg_mag(s_v[i][c])); }
+            const int k = m > 0.f ? rg_k<RG_ZNONE - 2>(m) : RG_ZNONE;
+            gh8 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { _Float16 h, l; rg_split(ldexpf(s_v[i][c], k - RG_ZUP), h, l); hi[i] = h; lo[i] = l; }
+            *reinterpret_cast<gh8 *>(o.zt + ((size_t) tb * 2 * o.ea + c) * 8) = hi;
+            *reinterpret_cast<gh8 *>(o.zt + (((size_t) tb * 2 + 1) * o.ea + c) * 8) = lo;
+            s_k[c] = (uint8_t) (k + RG_ZK);
+        }
+        __syncthreads();
+        if (c < o.ea / 4) {
+            uint2 w = { 0u, 0u };
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { w.x |= (uint32_t) s_k[64 * (c >> 4) + 16 * i + (c & 15)] << (8 * i); }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { w.y |= (uint32_t) s_on[i] << i; }
+            o.zk[(size_t) tb * (o.ea / 4) + c] = w;
+        }
     }
     const int nc = o.kp / 8;
     for (int p = threadIdx.x; p < (g.dx ? 16 * nc : 0); p += 256) {    // 8 experts of a row
@@ -296,25 +320,14 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), r = lane & 15, q = lane >> 4;
     const int j0 = ct * RG_COLS, we = wave % WR, wj = wave / WR;
     const int steps = o.np / 32, s0 = (int) ((int64_t) steps * run / splits), s1 = (int) ((int64_t) steps * (run + 1) / splits);
-    // K0: the smallest k of the run's rows
-    int K0 = RG_NONE;
-    for (int t = 32 * s0 + (int) threadIdx.x; t < 32 * s1; t += RG_T) { K0 = min(K0, (int) o.kt[t]); }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { K0 = min(K0, __shfl_xor(K0, d)); }
-    if (lane == 0) { *(LK_LOCAL int *) (lds + 4 * wave) = K0; }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < RG_W; ++i) { K0 = min(K0, *(const LK_LOCAL int *) (lds + 4 * i)); }
-    __syncthreads();
-
-    struct Slab { float x[8]; gs8 k; };
-    auto load_x = [&](int s, Slab & d) {   // rows 32 s + 8 q .. + 7, column j0 + 16 wave + r; rows past the batch's end read 0
+    struct Slab { float x[8]; uint2 k; };
+    auto load_x = [&](int s, Slab & d) {   // rows 32 s + 8 q .. + 7, column j0 + 16 wave + r; rows past the batch's end read 0. Their dz's k
         const int t = 32 * min(s, s1 - 1), nt = min(32, g.n - t);
         const __amdgpu_buffer_rsrc_t rx = rg_rsrc(g.x + (size_t) t * g.E, (uint32_t) nt * (uint32_t) g.E * 4);
         const uint32_t v = ((uint32_t) (8 * q) * (uint32_t) g.E + (uint32_t) (j0 + 16 * wave + r)) * 4;
 #pragma unroll
         for (int i = 0; i < 8; ++i) { d.x[i] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rx, v + (uint32_t) i * (uint32_t) g.E * 4, 0, 0)); }
-        d.k = *reinterpret_cast<const gs8 *>(o.kt + t + 8 * q);
+        d.k = o.zk[(size_t) (t / 8 + q) * (EA / 4) + 16 * we + r];
     };
     auto copy_z = [&](int s, int b) {   // 4 x 8 rows' halves, as they are stored
         const int st = min(s, s1 - 1);
@@ -323,10 +336,13 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
         for (int i = 0; i < AB / 1024 / RG_W; ++i) { rg_lds16(rz, lds + b * BUF + (wave + i * RG_W) * 1024, (uint32_t) (lane * 16), (uint32_t) ((wave + i * RG_W) * 1024)); }
     };
     int kc = 200;   // the wave's columns' k (column r, the same in the four lane groups)
+    uint32_t zk = 0;   // the k of the converted rows' dz
+    int kr[4];         // the smallest k of experts 64 we + 16 i + r in the run's rows, + RG_ZK + RG_ZUP
     auto convert = [&](const Slab & sl, int b) {
         float y[8], m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) { y[i] = ldexpf(sl.x[i], K0 - (int) sl.k[i]); m = fmaxf(m, fabsf(y[i])); }
+        for (int i = 0; i < 8; ++i) { y[i] = sl.x[i] * (float) ((sl.k.y >> i) & 1u); m = fmaxf(m, fabsf(y[i])); }
+        zk = sl.k.x;
         m = rg_max_rows(m);
         kc = min(kc, m > 0.f ? rg_k(m) : kc);   // (a column with an infinity is non-finite in every expert, whatever its k)
         const float sc = rg_pow2(kc);
@@ -364,6 +380,9 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
 #pragma unroll
             for (int c = 0; c < JW; ++c) { kn[c] = *(const LK_LOCAL int *) (size_t) (lb + AB + BB + (uint32_t) ((16 * JW * wj + 16 * c + r) * 4)); }
             load_z(0);
+            _Float16 fz[4];   // of experts 64 we + 16 i + r, rows 8 q .. + 7: to the run's k (a row group far below it: 0)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { fz[i] = (_Float16) ldexpf(1.f, kr[i] - (int) ((zk >> (8 * i)) & 255u)); }
 #pragma unroll
             for (int c = 0; c < JW; ++c) {
                 const uint32_t a = lb + AB + (uint32_t) ((q * 2 * RG_COLS + 16 * JW * wj + 16 * c + r) * 16);
@@ -382,7 +401,7 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (i < 3) { load_z(i + 1); }
-                const gh8 zh = z[i & 1][0], zl = z[i & 1][1];
+                const gh8 zh = z[i & 1][0] * fz[i], zl = z[i & 1][1] * fz[i];
 #pragma unroll
                 for (int c = 0; c < JW; ++c) { acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, xh[c], acc[i][c], 0, 0, 0); }
 #pragma unroll
@@ -401,6 +420,31 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
     };
     load_x(s0, sl[0]);
     copy_z(s0, 0);
+    // kr: the waves that share the experts take the groups of 8 rows in turn, 8 loads at once; their minima meet in the second buffer,
+    // which is free until the first step's barrier
+    {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 lo = { 255, 255 }, hi = lo;   // experts i = 0, 2 and 1, 3
+        auto low = [&](uint32_t w) {
+            lo = __builtin_elementwise_min(lo, __builtin_bit_cast(us2, w & 0x00FF00FFu));
+            hi = __builtin_elementwise_min(hi, __builtin_bit_cast(us2, (w >> 8) & 0x00FF00FFu));
+        };
+        constexpr int G = 4 * RG_W / WR, AHEAD = 8;
+        for (int t = 4 * s0 + 4 * wj + q; t < 4 * s1; t += G * AHEAD) {
+            uint32_t w[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) { w[i] = o.zk[(size_t) min(t + G * i, 4 * s1 - 1) * (EA / 4) + 16 * we + r].x; }   // (past the run's end: its last again)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) { low(w[i]); }
+        }
+        auto word = [&]() { return __builtin_bit_cast(uint32_t, lo) | (__builtin_bit_cast(uint32_t, hi) << 8); };
+        low((uint32_t) __shfl_xor((int) word(), 16)); low((uint32_t) __shfl_xor((int) word(), 32));
+        if (q == 0) { *(LK_LOCAL uint32_t *) (lds + BUF + 64 * wave + 4 * r) = word(); }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < RG_W / WR; ++i) { low(*(const LK_LOCAL uint32_t *) (lds + BUF + 64 * (we + WR * i) + 4 * r)); }
+        kr[0] = lo.x + RG_ZUP; kr[1] = hi.x + RG_ZUP; kr[2] = lo.y + RG_ZUP; kr[3] = hi.y + RG_ZUP;
+    }
     convert(sl[0], 0);
     load_x(s0 + 1, sl[0]); load_x(s0 + 2, sl[1]); load_x(s0 + 3, sl[2]);
     for (int s = s0;;) {   // (past the run's end: its last rows again, unread)
@@ -414,13 +458,13 @@ __device__ __forceinline__ void route_dw(const RouteGradArgs & g, const Ops & o,
     __builtin_amdgcn_s_waitcnt(0x0f70);   // no copy into LDS outlives the workgroup
     float * out = splits > 1 ? part + (size_t) run * g.n_exp * g.E : g.dW;
 #pragma unroll
-    for (int c = 0; c < JW; ++c) {
-        const int k = cur[c] == 200 || K0 == RG_NONE ? 0 : -cur[c] - K0;   // (200: nothing but zeros in the column)
+    for (int i = 0; i < 4; ++i) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int u = 0; u < 4; ++u) {
+            const int e = 64 * we + 16 * i + 4 * q + u, ke = __shfl(kr[i], 4 * q + u) - RG_ZUP - RG_ZK;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int e = 64 * we + 16 * i + 4 * q + u;
+            for (int c = 0; c < JW; ++c) {
+                const int k = cur[c] == 200 ? 0 : -cur[c] - ke;   // (200: nothing but zeros in the column)
                 if (e < g.n_exp) {
                     float * d = out + (size_t) e * g.E + j0 + 16 * JW * wj + 16 * c + r;
                     const float v = ldexpf(acc[i][c][u], k);
@@ -449,15 +493,16 @@ __global__ void __launch_bounds__(256) k_route_join(const float * __restrict__ p
 }
 
 constexpr size_t up256(size_t v) { return (v + 255) / 256 * 256; }
-struct Sizes { int kp, ea, np; size_t zs, zt, kt, wt, kw, part, all; };
+struct Sizes { int kp, ea, np; size_t zs, zt, kt, zk, wt, kw, part, all; };
 Sizes rg_sizes(int n, int ne, int E, bool dW, bool dx) {
     Sizes z{};
     z.kp = (ne + 31) / 32 * 32; z.ea = ne <= 64 ? 64 : ne <= 128 ? 128 : 256; z.np = (n + 31) / 32 * 32;
-    z.zs = dx ? up256((size_t) z.np * 2 * z.kp * 2) : 0; z.zt = dW ? up256((size_t) z.np * 2 * z.ea * 2) : 0; z.kt = up256((size_t) z.np * 2);
-    z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = up256((size_t) (E / 64) * 4);
+    z.zs = dx ? up256((size_t) z.np * 2 * z.kp * 2) : 0; z.zt = dW ? up256((size_t) z.np * 2 * z.ea * 2) : 0; z.kt = dx ? up256((size_t) z.np * 2) : 0;
+    z.zk = dW ? up256((size_t) z.np / 8 * (z.ea / 4) * 8) : 0;
+    z.wt = dx ? up256((size_t) 2 * z.kp * E * 2) : 0; z.kw = dx ? up256((size_t) (E / 64) * 4) : 0;
     const int sp = route_cut(n, E, dW, dx).splits;
     z.part = dW && sp > 1 ? (size_t) sp * ne * E * 4 : 0;
-    z.all = z.zs + z.zt + z.kt + z.wt + z.kw + z.part;
+    z.all = std::max<size_t>(256, z.zs + z.zt + z.kt + z.zk + z.wt + z.kw + z.part);   // (256: a call for dlogits alone takes none of it)
     return z;
 }
 template <int WR> hipError_t go(const RouteGradArgs & a, const Ops & o, RouteCut cut, float * part, hipStream_t st) {
@@ -480,7 +525,7 @@ hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_
     Ops o{};
     uint8_t * p = (uint8_t *) scratch;
     o.kp = z.kp; o.ea = z.ea; o.np = z.np;
-    o.zs = (_Float16 *) p; p += z.zs; o.zt = (_Float16 *) p; p += z.zt; o.kt = (short *) p; p += z.kt; o.wt = (_Float16 *) p; p += z.wt; o.kw = (int *) p; p += z.kw;
+    o.zs = (_Float16 *) p; p += z.zs; o.zt = (_Float16 *) p; p += z.zt; o.kt = (short *) p; p += z.kt; o.zk = (uint2 *) p; p += z.zk; o.wt = (_Float16 *) p; p += z.wt; o.kw = (int *) p; p += z.kw;
     float * part = (float *) p;
     const RouteCut cut = route_cut(a.n, a.E, a.dW != nullptr, a.dx != nullptr);
     const int nw = a.dx ? a.E / 64 : 0, sp = cut.splits;
