@@ -377,11 +377,22 @@ class Context:
         lib().fl_gguf_free_layer(ctypes.byref(gl))
 
     def kq_matvec(self, fmt, w, R, K, q, d, y=None):
-        """y [n][R] = K-quant matrix w (uint8 device tensor, R x K/256 ggml blocks) . Q8_K rows (q [n][K], d [n][K/256])."""
-        n = q.shape[0]
+        """y [n][R] float32 = K-quant matrix w (uint8 device tensor, R x K/256 ggml blocks) . Q8_K rows (q [n][K] int8,
+        d [n][K/256] float32); contiguous tensors on the context's GPU. A given y has n * R elements."""
+        t, dev, n = self.torch, self._device, q.shape[0]
+        if not (q.dtype is t.int8 and d.dtype is t.float32 and q.is_contiguous() and d.is_contiguous() and w.is_contiguous() and
+                q.get_device() == dev and d.get_device() == dev and w.get_device() == dev and
+                q.nbytes == n * K == d.nbytes * (QK_K // 4) and w.nbytes * QK_K >= R * K * KQ_BYTES.get(fmt, 0)):
+            raise LokiError("kq_matvec: on the context's GPU and contiguous, q [n][%d] int8, d [n][%d] float32 and w of %d rows are needed, not %s" %
+                            (K, K // QK_K, R, ", ".join("%s %s on %s" % (a.dtype, tuple(a.shape), a.device) for a in (q, d, w))))
         if y is None:
             y = d.new_empty(n, R)
-        self.check(lib().fl_kq_matvec_dev(self.ctx, fmt, _ptr(w), R, K, _ptr(q), _ptr(d), n, _ptr(y)))
+        elif not (y.dtype is t.float32 and y.is_contiguous() and y.get_device() == dev and y.nbytes == 4 * n * R):
+            raise LokiError("kq_matvec: y must be a contiguous float32 tensor of %d x %d elements on the context's GPU, not %s %s on %s" %
+                            (n, R, y.dtype, tuple(y.shape), y.device))
+        rc = lib().fl_kq_matvec_dev(self.ctx, fmt, w.data_ptr(), R, K, q.data_ptr(), d.data_ptr(), n, y.data_ptr())
+        if rc:
+            self.check(rc)
         return y
 
     def route(self, W, bias, x, topk=8):
