@@ -202,7 +202,7 @@ int fl_quant_q8k_dev(FLCtx *, const float * x, int nrows, int K, int8_t * q, flo
  * 203-254): integer sub-block sums exact, fp32 over the blocks in order (Q2_K bit-identical to ggml's scalar dot).
  * FL_Q4K: y = fma(d8, fma(-dmin, summ, d * isum), y) per block, whatever n and R: a row's output has the same bits in any batch. R at
  * most 2^26, n at most 2^19, q 16-byte aligned; batches that run on tiles (above 16 rows) take n * K / 8 bytes of the context's, see
- * "Workspaces" below. */
+ * "Workspaces" above. */
 int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y);
 /* IQ2_XXS ggml layout <-> tiled layout for nmat matrices of R x K at byte strides (device, may not alias) */
 int fl_pack_iq2xxs(FLCtx *, const void * src_ggml, size_t src_stride, void * dst_tiled, size_t dst_stride, int R, int K, int nmat);

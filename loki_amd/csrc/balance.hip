@@ -121,9 +121,10 @@ __device__ __forceinline__ void bl_finish(const BalanceArgs & g, int s, int T, f
     }
 }
 
-// The sums: one read of the logits, P's parts in registers, counts by integer LDS atomics (exact in any order). Bound by memory
-// where the rows are many: 65536 rows of 256 experts in 16 sequences 17.5 us with the join, 3.8 TB/s; by its launches where they are few
-// (70 rows 5.0 us).
+// The sums: one read of the logits, P's parts in registers, counts by integer LDS atomics (exact in any order). 65536 rows of 256
+// experts in 16 sequences, logits from memory: 21 us, 3.2 TB/s, and 4 for the join (17.8 together when the same call runs again and
+// again, its logits then in the last-level cache). The vector units are busy 76 % of the cycles, and a wave has no load out while
+// they are. Few rows: the launch (70 rows 5.5 us).
 template <int J>
 __global__ void __launch_bounds__(64 * BL_W) k_balance(BalanceArgs g) {
     constexpr int BL_T = 64 * BL_W;
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(BL_JOIN) k_balance_join(BalanceArgs g) {
 }
 
 // The gradient: a row's sigmoids once more (reading them back would cost what reading the logits costs, and the sums would have to
-// write them), its weighted sum of f by the wave, one write. 65536 rows of 256 in 16 sequences 24.7 us, 5.4 TB/s read and written.
+// write them), its weighted sum of f by the wave, one write. 65536 rows of 256 in 16 sequences, from memory: 29.5 us, 4.6 TB/s read and
+// written (25 when the same call is repeated), vector units 76 % busy.
 template <int J, int W>
 __global__ void __launch_bounds__(64 * W) k_balance_grad(BalanceArgs g) {
     constexpr int BL_T = 64 * W;
@@ -256,8 +258,10 @@ __global__ void __launch_bounds__(64 * W) k_balance_grad(BalanceArgs g) {
 }  // namespace
 
 // Workgroups a sequence, each wave with a batch of BL_B rows at a time. Sums: 16 waves, so that there are few partial sums to join; up to
-// 128 rows one workgroup, which needs no second launch (128 rows 7.0 us, 256 rows in 4 workgroups 7.7). The gradient has nothing to
-// join: 4 waves up to 8192 rows (4100 rows 5.5 us, with 16 waves 6.4), 16 above (16384 rows 8.8 us, with 4 waves 11.4).
+// 128 rows one workgroup, which needs no second launch (128 rows 6.9 us, and so 256 rows in 4 workgroups). The gradient has nothing to
+// join: 4 waves up to 8192 rows (4100 rows 5.3 us, with 16 waves 6.3), 16 above (16384 rows 8.4 us, with 4 waves 10.9). (One sequence, the
+// same call repeated.) The sequences' lengths are known on the device alone, so the cut is by their mean: one sequence with nine tenths
+// of the rows is slow (8192 rows in 64 sequences: loss 8.8 -> 288 us, gradient 7.9 -> 88).
 static int grad_waves(int n) { return n <= 8192 ? 4 : 16; }
 static int chunks_of(int n, int nseq, bool grad) {
     const int w = grad ? grad_waves(n) : BL_W, rows = w * BL_B, most = w == 4 ? BALANCE_PARTS : BALANCE_PARTS / 2;

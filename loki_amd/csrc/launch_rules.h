@@ -84,7 +84,8 @@ constexpr bool q4k_tiled(int kernel) { return kernel >= Q4_MM_64_32 && kernel < 
 // alone: one workgroup a CU. Both: one a CU together, three fifths of them dW's, whose rows cost more (5000 rows of 4096, 256 experts, 5 + 3
 // 85 us, 8 + 8 89; 3000 rows of 6144, 160 experts, 3 + 2 67, 5 + 5 83); where that leaves more than a tenth of the CUs idle and x is large,
 // several rounds of workgroups pay instead, dx's in small pieces (8192 rows of 7168: 4 + 18 207 us, 2 + 2 229; 700 rows: 39 and 37). Over
-// 141 sizes (200 .. 16000 rows of 1024 .. 16384, 64 .. 256 experts) the pick is within 3 % of the best measured on average.
+// 141 sizes (200 .. 16000 rows of 1024 .. 16384, 64 .. 256 experts) the pick is within 3 % of the best measured on average. (Times of these
+// cuts side by side; dW's scale per expert has added up to 3 % to all of them since.)
 constexpr int ROUTE_COLS = 128, ROUTE_ROWS = 256;
 struct RouteCut { int splits, parts; };
 constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {

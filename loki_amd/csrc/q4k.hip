@@ -203,7 +203,7 @@ __device__ __forceinline__ void q4_mins(const u32x4 & hd, uint32_t (&mm)[2]) {
 // products are done with the registers (a second set, filled a round earlier, holds every wave up at the round's start behind the
 // others' loads: 37 tokens through 7168 rows of 16384 39 us instead of 33). Each round leaves the blocks' terms in LDS, and the
 // workgroup's lanes run the chains over them, an output or two a lane. summ comes from a third product with the step's min in every
-// byte (here the matrix cores have time to spare). Of those 33 us, found by leaving out one part at a time: the copies and loads that
+// byte (here the matrix cores have time to spare). 37 tokens through 7168 rows of 16384 take 31 us a call. Of 33, found by leaving out one part at a time: the copies and loads that
 // the products wait for 7, products and digits 14, the barriers, LDS reads and terms of the 8 rounds 7, the launch and first fetch 4.
 constexpr int KS_W = 8, KS_PITCH = 9 * KS_W + 1;   // 16-byte chunks from row to row in LDS: 16 rows start in 16 different quads of banks
 // copy i of a wave (past the last one: an earlier one of its own again, the same bytes, so that every wave has as many out)
@@ -364,8 +364,8 @@ template <int RT, int NT> hipError_t ks(const KqArgs & a, unsigned gy, hipStream
 // (copied there by the loads themselves, 16-byte chunks swizzled so that a tile's reads meet no bank twice). Each weight is decoded
 // once per workgroup and each activation read from LDS serves RT tiles, so the largest tile, 128 x 128, does the most work an
 // instruction; smaller ones are for calls that it would leave CUs without a workgroup (launch_rules.h). 2048 tokens through 16384 rows of
-// 7168 502 us, 958 TFLOP/s of the real product: the matrix cores are busy 53 % of the cycles and the vector units with digits and terms
-// 48 %, at the 1.9 GHz that the card then holds. Where a CU gets one workgroup, one wave a SIMD does its products (40 % of the cycles) and
+// 7168 505 us, 953 TFLOP/s of the real product: the matrix cores are busy 55 % of the cycles and the vector units with digits and terms
+// 50 %, at the 1.9 GHz that the card then holds. Where a CU gets one workgroup, one wave a SIMD does its products (40 % of the cycles) and
 // its vector work (35 %) one after the other; 8 waves of one row tile then overlap the two, at twice the LDS reads: 501 tokens through
 // 7000 rows of 7168 68 us instead of 75.
 template <int RT, int NT, int W, int D>
