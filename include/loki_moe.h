@@ -187,7 +187,7 @@ int fl_balance_loss_grad_dev(FLCtx *, const float * logits, const int * counts, 
  * + kp * E * 4 bytes and dW's partial sums, rounded up to a power of two. */
 int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * logits, const int * sel, const float * dw, const float * dz, int n,
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
-/* Workspaces of fl_balance_loss_dev, fl_route_grad_dev and Q4_K products are the context's. They grow in the call that needs more
+/* Workspaces of fl_balance_loss_dev, fl_route_grad_dev, Q4_K and 16-bit products are the context's. They grow in the call that needs more
  * (hipMalloc; FL_ENOMEM when that fails, and under graph capture, where nothing is allocated and the capture goes on) and no block is
  * freed before fl_free, so a captured call stays valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured from one context share
  * its workspaces and must not run at the same time. The context's device has to be the current one (FL_EINVAL). */
@@ -204,6 +204,43 @@ int fl_quant_q8k_dev(FLCtx *, const float * x, int nrows, int K, int8_t * q, flo
  * most 2^26, n at most 2^19, q 16-byte aligned; batches that run on tiles (above 16 rows) take n * K / 8 bytes of the context's, see
  * "Workspaces" above. */
 int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_t * q, const float * d, int n, float * y);
+/* ---------------------------------------------------------------- additive: 16-bit products, and what trains with them
+ * (no counterpart in the reference, whose matrices are all quantised and which does not train). type: FL_BF16 or FL_F16, of every
+ * operand and result that is not named float or int; products are exact and summed in fp32, each result rounded once. R and K are
+ * multiples of 8 (R at most 2^20, K 65536), n at most 2^24, pointers 16-byte aligned, tensors contiguous.
+ * Groups: with offsets [n_exp + 1] (device, ascending, as fl_dispatch_dev leaves them) expert e has the rows ("slots") offsets[e] ..
+ * offsets[e + 1] - 1 of the n and a matrix of its own; slots of no expert are not read and their results stay as they were. Offsets
+ * are clamped to 0 .. n; ones that are not ascending give unspecified values. Without offsets (NULL) n_exp is 1 and takes all n rows.
+ * With perm [n] (fl_dispatch_dev's) slot s reads row perm[s] / topk of the xrows rows of x, at most 2^31 - 2^16 values; a row outside
+ * them counts as zeros. Without it slot s reads row s, and topk and xrows are not looked at. */
+enum { FL_F32 = 16, FL_F16 = 17, FL_BF16 = 18 };
+/* silu(z) = z / (1 + e^-z); gelu in its tanh form, z / (1 + e^(-2 sqrt(2 / pi) (z + 0.044715 z^3))) */
+enum { FL_ACT_NONE = 0, FL_ACT_SILU = 1, FL_ACT_GELU = 2 };
+/* y [n][R] = act(x W^T + bias) + residual, W [n_exp][R][K], bias [n_exp][R] floats, residual [n][R]; or, with a second matrix W2 of
+ * W's shape, the gated form y = act(x W^T) * (x W2^T) + residual (no bias). bias, residual and W2 may be NULL. y is of `type` or
+ * FL_F32 (y_type); it may be the residual's buffer when their types are the same. z and z2 [n][R] (may be NULL) get x W^T + bias and
+ * x W2^T, for the backward pass. */
+int fl_matmul_dev(FLCtx *, int type, int act, const void * x, const void * W, const void * W2, const float * bias, const void * residual,
+                  int n, int R, int K, int n_exp, const int * offsets, const int * perm, int topk, int xrows, void * y, int y_type, void * z, void * z2);
+/* the epilogue's backward pass: from dy [n][R] and fl_matmul_dev's z and z2 (z2 NULL: not gated; z may be NULL without an activation)
+ *   dz = dy act'(z) (* z2),   dz2 = dy act(z),   dbias [n_exp][R] = (accumulate: +=) sum over the expert's rows of dz, before rounding
+ * (each may be NULL: not computed). dz and dz2 may be the buffers of dy, z or z2. */
+int fl_act_grad_dev(FLCtx *, int type, int act, const void * dy, const void * z, const void * z2, int n, int R, int n_exp, const int * offsets,
+                    void * dz, void * dz2, float * dbias, int accumulate);
+/* the products' backward pass: dx [n][K] = dz W (+ dz2 W2), of each slot (with perm too: a row's slots are summed by fl_combine_dev with
+ * w NULL), dW [n_exp][R][K] = (accumulate: +=) dz^T x of the expert's slots, dW2 = dz2^T x likewise; each may be NULL: not computed.
+ * dW and dW2 are of `type` or FL_F32 (dw_type). An expert without slots gets 0 (accumulate: stays). Deterministic, no atomics. */
+int fl_matmul_grad_dev(FLCtx *, int type, const void * dz, const void * dz2, const void * x, const void * W, const void * W2, int n, int R, int K, int n_exp,
+                       const int * offsets, const int * perm, int topk, int xrows, void * dx, void * dW, void * dW2, int dw_type, int accumulate);
+/* the picks' sum: y [n][E] = residual + sum over k of w[t][k] o[inv[t][k]], fp32 in k's order; o [P][E] the slots' rows, inv and sel
+ * [n][topk] as fl_dispatch_dev takes and leaves them, w NULL: ones. Picks outside 0 .. n_exp - 1 (sel NULL: none), or with a slot
+ * outside 0 .. P - 1, are skipped. y is of `type` or FL_F32 (y_type), and may be the residual's buffer in the same type. */
+int fl_combine_dev(FLCtx *, int type, const void * o, const int * inv, const float * w, const int * sel, const void * residual, int n, int topk, int n_exp,
+                   int P, int E, void * y, int y_type);
+/* its gradients: d_o[inv[t][k]] = w[t][k] dy[t] (slots of no pick stay; may be o's buffer) and dw [n][topk] = <o[inv[t][k]], dy[t]> in fp32
+ * (0 for a skipped pick), which fl_route_grad_dev takes; either may be NULL */
+int fl_combine_grad_dev(FLCtx *, int type, const void * dy, const void * o, const int * inv, const float * w, const int * sel, int n, int topk, int n_exp,
+                        int P, int E, void * d_o, float * dw);
 /* IQ2_XXS ggml layout <-> tiled layout for nmat matrices of R x K at byte strides (device, may not alias) */
 int fl_pack_iq2xxs(FLCtx *, const void * src_ggml, size_t src_stride, void * dst_tiled, size_t dst_stride, int R, int K, int nmat);
 int fl_unpack_iq2xxs(FLCtx *, const void * src_tiled, size_t src_stride, void * dst_ggml, size_t dst_stride, int R, int K, int nmat);

@@ -23,6 +23,9 @@ KQ_BYTES = {FL_Q2K: 84, FL_Q3K: 110, FL_Q4K: 144, FL_Q5K: 176, FL_Q6K: 210}
 FL_LAYOUT_GGML, FL_LAYOUT_TILED = 0, 1
 FL_OK, FL_EINVAL, FL_ENOMEM, FL_EHIP, FL_ERANGE, FL_ESCOPE = 0, -1, -2, -3, -4, -5
 
+FL_F32, FL_F16, FL_BF16 = 16, 17, 18
+FL_ACT = {None: 0, "silu": 1, "gelu": 2}
+
 P_ = ctypes.c_void_p
 
 
@@ -127,7 +130,7 @@ ABI_SYMBOLS = [
     "fl_wide_outs", "fl_wide_skip", "fl_spec", "fl_sketch", "fl_fetch", "fl_moe", "fl_skip", "fl_h2d", "fl_h2d_bytes", "fl_wait_event",
     "fl_gpu_ms", "fl_ffn_begin", "fl_set_experts", "fl_set_routing", "fl_set_keep", "fl_set_share_experts", "fl_set_shared_formats", "fl_set_layer_formats", "fl_kq_matvec_dev",
     "fl_gguf_open", "fl_gguf_close", "fl_gguf_n_tensors", "fl_gguf_tensor_name", "fl_gguf_tensor", "fl_gguf_tensor_at",
-    "fl_gguf_get_int", "fl_gguf_get_float", "fl_gguf_get_str", "fl_gguf_read", "fl_gguf_load_moe_layer", "fl_gguf_free_layer", "fl_moe_layer", "fl_moe_layer_normed", "fl_moe_layer_noalloc", "fl_route_dev", "fl_balance_loss_dev", "fl_balance_loss_grad_dev", "fl_route_grad_dev", "fl_dispatch_dev", "fl_quant_q8k_dev",
+    "fl_gguf_get_int", "fl_gguf_get_float", "fl_gguf_get_str", "fl_gguf_read", "fl_gguf_load_moe_layer", "fl_gguf_free_layer", "fl_moe_layer", "fl_moe_layer_normed", "fl_moe_layer_noalloc", "fl_route_dev", "fl_balance_loss_dev", "fl_balance_loss_grad_dev", "fl_route_grad_dev", "fl_matmul_dev", "fl_act_grad_dev", "fl_matmul_grad_dev", "fl_combine_dev", "fl_combine_grad_dev", "fl_dispatch_dev", "fl_quant_q8k_dev",
     "fl_pack_iq2xxs", "fl_unpack_iq2xxs", "fl_register_tiled", "fl_unregister_tiled", "fl_rmsnorm_dev", "fl_synth_iq2xxs", "fl_synth_normal", "fl_probe_exp",
     "fl_debug", "fl_set_debug", "fl_set_fused", "fl_set_decode1", "fl_set_prefill_mfma", "fl_stream", "fl_set_stream", "fl_d2h", "fl_set_profile", "fl_stage_ms", "fl_sync", "fl_last_error", "fl_free",
 ]
@@ -185,6 +188,11 @@ def lib():
             "fl_balance_loss_dev": (I, [P_, P_, P_, P_, I, I, I, I, F, P_, P_]),
             "fl_balance_loss_grad_dev": (I, [P_, P_, P_, P_, P_, I, I, I, I, F, I, P_]),
             "fl_route_grad_dev": (I, [P_, P_, P_, P_, P_, P_, P_, I, I, I, P_, P_, I, P_]),
+            "fl_matmul_dev": (I, [P_, I, I, P_, P_, P_, P_, P_, I, I, I, I, P_, P_, I, I, P_, I, P_, P_]),
+            "fl_act_grad_dev": (I, [P_, I, I, P_, P_, P_, I, I, I, P_, P_, P_, P_, I]),
+            "fl_matmul_grad_dev": (I, [P_, I, P_, P_, P_, P_, P_, I, I, I, I, P_, P_, I, I, P_, P_, P_, I, I]),
+            "fl_combine_dev": (I, [P_, I, P_, P_, P_, P_, P_, I, I, I, I, I, P_, I]),
+            "fl_combine_grad_dev": (I, [P_, I, P_, P_, P_, P_, P_, I, I, I, I, I, P_, P_]),
             "fl_dispatch_dev": (I, [P_, P_, I, I, I, P_, P_, P_, P_, P_, P_]),
             "fl_quant_q8k_dev": (I, [P_, P_, I, I, P_, P_]),
             "fl_pack_iq2xxs": (I, [P_, P_, S, P_, S, I, I, I]),
@@ -459,6 +467,153 @@ class Context:
             if t is not None and not (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda and t.get_device() == self._device):
                 raise LokiError("%s: a contiguous %s tensor of shape %s on the context's GPU is needed, not %s %s on %s" %
                                 (who, dtype, shape, t.dtype, tuple(t.shape), t.device))
+
+    # ---- 16-bit products (bfloat16 or float16), dense and by expert, and their backward pass
+    def _type(self, who, t):
+        code = {self.torch.bfloat16: FL_BF16, self.torch.float16: FL_F16, self.torch.float32: FL_F32}.get(t)
+        if code is None:
+            raise LokiError("%s: bfloat16 or float16 is needed, not %s" % (who, t))
+        return code
+
+    def _mm(self, who, x, W, up, offsets, perm, topk):
+        """(type code, slots, R, K, experts, rows of x) of a product's operands, checked"""
+        T = x.dtype
+        code = self._type(who, T)
+        if code == FL_F32 or x.dim() != 2 or W.dim() != (2 if offsets is None else 3):
+            raise LokiError("%s: x [rows][K] and W %s of bfloat16 or float16 are needed, not %s %s and %s" %
+                            (who, "[R][K]" if offsets is None else "[n_exp][R][K]", T, tuple(x.shape), tuple(W.shape)))
+        R, K = W.shape[-2:]
+        ne = 1 if offsets is None else W.shape[0]
+        n = x.shape[0] if perm is None else perm.numel()
+        self._need(who, (x, T, (x.shape[0], K)), (W, T, W.shape), (up, T, W.shape))
+        if offsets is not None:
+            self._need(who, (offsets, self.torch.int32, (ne + 1,)), (perm, self.torch.int32, (n,)))
+        elif perm is not None:
+            raise LokiError("%s: perm goes with offsets" % who)
+        return code, n, R, K, ne, x.shape[0]
+
+    def _product(self, who, x, W, offsets, up, bias, act, residual, perm, topk, dtype, keep, y, z, z2):
+        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm, topk)
+        T = x.dtype
+        if act not in FL_ACT:
+            raise LokiError("%s: act is None, 'silu' or 'gelu', not %r" % (who, act))
+        if y is None:
+            y = x.new_empty(n, R, dtype=dtype or T)
+        if keep:
+            z = x.new_empty(n, R) if z is None else z
+            z2 = x.new_empty(n, R) if z2 is None and up is not None else z2
+        self._need(who, (bias, self.torch.float32, (R,) if offsets is None else (ne, R)), (residual, T, (n, R)), (y, dtype or y.dtype, (n, R)), (z, T, (n, R)), (z2, T, (n, R)))
+        rc = lib().fl_matmul_dev(self.ctx, code, FL_ACT[act], x.data_ptr(), W.data_ptr(), _ptr(up), _ptr(bias), _ptr(residual), n, R, K, ne, _ptr(offsets),
+                                 _ptr(perm), topk, xr, y.data_ptr(), self._type(who, y.dtype), _ptr(z), _ptr(z2))
+        if rc:
+            self.check(rc)
+        return y if z is None and z2 is None else (y, z) if up is None else (y, z, z2)
+
+    def matmul(self, x, W, up=None, bias=None, act=None, residual=None, dtype=None, keep=False, y=None, z=None, z2=None):
+        """y [n][R] = act(x W^T + bias) + residual for x [n][K], W [R][K] in bfloat16 or float16 (bias float32 [R]); with a second
+        matrix `up`, act(x W^T) * (x up^T) + residual. act: None, 'silu' or 'gelu' (tanh form). dtype: y's, the operands' (default) or
+        float32. keep, or tensors z (and z2): also returns x W^T + bias (and x up^T), for act_grad."""
+        return self._product("matmul", x, W, None, up, bias, act, residual, None, 1, dtype, keep, y, z, z2)
+
+    def expert_matmul(self, x, W, offsets, up=None, bias=None, act=None, residual=None, perm=None, topk=1, dtype=None, keep=False, y=None, z=None, z2=None):
+        """matmul() grouped by expert: W [n_exp][R][K], bias [n_exp][R]; expert e's slots offsets[e] .. offsets[e + 1] - 1 (dispatch()'s).
+        With perm (dispatch()'s) and topk, slot s reads row perm[s] // topk of x; else row s. Slots of no expert keep what y holds (new
+        tensors: anything)."""
+        return self._product("expert_matmul", x, W, offsets, up, bias, act, residual, perm, topk, dtype, keep, y, z, z2)
+
+    def act_grad(self, dy, z, act, z2=None, bias=False, offsets=None, dz=None, dz2=None, dbias=None):
+        """(dz, dz2, dbias) from dy [n][R] and the kept z (and z2) of act(z) (* z2): dz2 is None without z2, dbias [R] (offsets: [n_exp][R])
+        without `bias`; a dbias tensor is added to in place. Without an activation and z2, dz is dy itself (z may be None)."""
+        t, T = self.torch, dy.dtype
+        code = self._type("act_grad", T)
+        if code == FL_F32 or dy.dim() != 2 or act not in FL_ACT:
+            raise LokiError("act_grad: dy [n][R] of bfloat16 or float16 and act None, 'silu' or 'gelu' are needed, not %s %s and %r" % (T, tuple(dy.shape), act))
+        n, R = dy.shape
+        ne = 1 if offsets is None else offsets.numel() - 1
+        plain = act is None and z2 is None
+        add = dbias is not None
+        if plain and dz is None:
+            out = None
+        else:
+            out = t.empty_like(dy) if dz is None else dz
+        if z2 is not None and dz2 is None:
+            dz2 = t.empty_like(dy)
+        bshape = (R,) if offsets is None else (ne, R)
+        if bias and dbias is None:
+            dbias = dy.new_empty(bshape, dtype=t.float32)
+        self._need("act_grad", (dy, T, (n, R)), (z, T, (n, R)), (z2, T, (n, R)), (out, T, (n, R)), (dz2, T, (n, R)), (dbias, t.float32, bshape), (offsets, t.int32, (ne + 1,)))
+        if out is not None or dbias is not None:
+            rc = lib().fl_act_grad_dev(self.ctx, code, FL_ACT[act], dy.data_ptr(), _ptr(z), _ptr(z2), n, R, ne, _ptr(offsets), _ptr(out), _ptr(dz2), _ptr(dbias), 1 if add else 0)
+            if rc:
+                self.check(rc)
+        return dy if out is None else out, dz2, dbias
+
+    def _product_grad(self, who, dz, x, W, offsets, dz2, up, perm, topk, dW, dW2, dw_dtype, need_dx, need_dW, dx):
+        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm, topk)
+        T = x.dtype
+        if (dz2 is None) != (up is None):
+            raise LokiError("%s: dz2 and up go together" % who)
+        add = dW is not None or dW2 is not None
+        if add and (dW is None or (dW2 is None) != (up is None)):
+            raise LokiError("%s: dW and dW2 are added to together" % who)
+        if add:
+            dw_dtype = dW.dtype
+        elif need_dW:
+            dW = x.new_empty(W.shape, dtype=dw_dtype or T)
+            dW2 = None if up is None else self.torch.empty_like(dW)
+        if need_dx and dx is None:
+            dx = x.new_empty(n, K)
+        self._need(who, (dz, T, (n, R)), (dz2, T, (n, R)), (dx, T, (n, K)), (dW, dw_dtype or T, W.shape), (dW2, dw_dtype or T, W.shape))
+        rc = lib().fl_matmul_grad_dev(self.ctx, code, dz.data_ptr(), _ptr(dz2), x.data_ptr(), W.data_ptr(), _ptr(up), n, R, K, ne, _ptr(offsets), _ptr(perm), topk, xr,
+                                      _ptr(dx), _ptr(dW), _ptr(dW2), self._type(who, dw_dtype or T), 1 if add else 0)
+        if rc:
+            self.check(rc)
+        return (dx, dW) if up is None else (dx, dW, dW2)
+
+    def matmul_grad(self, dz, x, W, dz2=None, up=None, dW=None, dW2=None, dw_dtype=None, need_dx=True, need_dW=True, dx=None):
+        """(dx, dW), with `up` (dx, dW, dW2): dx = dz W (+ dz2 up), dW = dz^T x, dW2 = dz2^T x, from act_grad's dz (and dz2). dW (and dW2)
+        tensors are added to in place; new ones are of dw_dtype, the operands' type (default) or float32."""
+        return self._product_grad("matmul_grad", dz, x, W, None, dz2, up, None, 1, dW, dW2, dw_dtype, need_dx, need_dW, dx)
+
+    def expert_matmul_grad(self, dz, x, W, offsets, dz2=None, up=None, perm=None, topk=1, dW=None, dW2=None, dw_dtype=None, need_dx=True, need_dW=True, dx=None):
+        """matmul_grad() grouped by expert, as expert_matmul(). dx is each slot's; combine(dx, inv) sums a row's. An expert without slots
+        gets zeros; slots of no expert keep what dx holds."""
+        return self._product_grad("expert_matmul_grad", dz, x, W, offsets, dz2, up, perm, topk, dW, dW2, dw_dtype, need_dx, need_dW, dx)
+
+    def combine(self, o, inv, w=None, sel=None, n_exp=N_EXPERT, residual=None, topk=None, dtype=None, y=None):
+        """y [n][E] = residual + sum_k w[t][k] o[inv[t][k]] for the slots' rows o [P][E], dispatch()'s inv and route()'s w [n][topk] float32
+        (None: ones; topk then from sel, or given). Picks of sel outside 0 .. n_exp - 1 are skipped. dtype: o's (default) or float32."""
+        P, E, n, k, T = self._picks("combine", o, inv, w, sel, topk)
+        if y is None:
+            y = o.new_empty(n, E, dtype=dtype or T)
+        self._need("combine", (residual, T, (n, E)), (y, dtype or y.dtype, (n, E)))
+        rc = lib().fl_combine_dev(self.ctx, self._type("combine", T), o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), _ptr(residual), n, k, n_exp, P, E,
+                                  y.data_ptr(), self._type("combine", y.dtype))
+        if rc:
+            self.check(rc)
+        return y
+
+    def combine_grad(self, dy, o, inv, w=None, sel=None, n_exp=N_EXPERT, topk=None, do=None, need_do=True, need_dw=True):
+        """(do, dw): the gradients of combine() to the slots' rows (w[t][k] dy[t]; slots of no pick keep what `do` holds) and to the routing
+        weights (float32 [n][topk], for route_grad)."""
+        P, E, n, k, T = self._picks("combine_grad", o, inv, w, sel, topk)
+        if do is None and need_do:
+            do = o.new_empty(P, E)
+        dw = o.new_empty(n, k, dtype=self.torch.float32) if need_dw else None
+        self._need("combine_grad", (dy, T, (n, E)), (do, T, (P, E)))
+        rc = lib().fl_combine_grad_dev(self.ctx, self._type("combine_grad", T), dy.data_ptr(), o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), n, k, n_exp, P, E, _ptr(do), _ptr(dw))
+        if rc:
+            self.check(rc)
+        return do, dw
+
+    def _picks(self, who, o, inv, w, sel, topk):
+        t = self.torch
+        k = topk or (w.shape[1] if w is not None else sel.shape[1] if sel is not None else 0)
+        if o.dim() != 2 or o.dtype is t.float32 or k < 1 or inv.numel() % k:
+            raise LokiError("%s: o [P][E] of bfloat16 or float16, and w, sel or topk that tells the picks a row, are needed" % who)
+        (P, E), n = o.shape, inv.numel() // k
+        self._need(who, (o, o.dtype, (P, E)), (inv, t.int32, inv.shape), (w, t.float32, (n, k)), (sel, t.int32, (n, k)))
+        return P, E, n, k, o.dtype
 
     def dispatch(self, sel, n_exp=N_EXPERT):
         t = self.torch

@@ -95,7 +95,7 @@ struct FLCtx {
     DBuf<unsigned> rcnt;                       // the one-launch routing's self-resetting counter (launch_router_fused)
     DBuf<double> rpart;                        // the matrix-core router's parts [router_parts][n][n_exp]
     DBuf<int> dscr;                            // the multi-workgroup dispatch's per-round counts and bases
-    KeptBuf bal, rg, q4;                       // fl_balance_loss_dev's partial sums, fl_route_grad_dev's operands, Q4_K's row sums
+    KeptBuf bal, rg, q4, mm;                   // fl_balance_loss_dev's partial sums, fl_route_grad_dev's operands, Q4_K's row sums, the 16-bit products' partial sums
     size_t h2d_zc = 0, h2d_ce = 0; int h2d_said = 0;   // fl_h2d bytes by kernel (mapped pinned) / by copy engine
     // fl_ffn_begin's event pairs (recorded, not yet folded into ms_ffn by fl_gpu_ms) and the reusable ones
     std::vector<std::pair<hipEvent_t, hipEvent_t>> ffn_ev_pending, ffn_ev_free; double ms_ffn = 0.0;

@@ -405,6 +405,178 @@ extern "C" int fl_route_grad_dev(FLCtx * c, const float * W, const float * x, co
     return FL_OK;
 }
 
+// ---------------------------------------------------------------- 16-bit products and what trains with them
+static bool misaligned(std::initializer_list<const void *> ps) {
+    uintptr_t all = 0;
+    for (const void * p : ps) { all |= reinterpret_cast<uintptr_t>(p); }
+    return (all & 15u) != 0;
+}
+// [a, a + na) and [b, b + nb) share a byte
+static bool overlap(const void * a, size_t na, const void * b, size_t nb) {
+    return a && b && (const char *) a < (const char *) b + nb && (const char *) b < (const char *) a + na;
+}
+// sizes, groups and gather of a product; rows: the rows of x
+static int mm_shape(FLCtx * c, int type, int n, int R, int K, int n_exp, const int * offsets, const int * perm, int topk, int xrows, uint32_t & magic) {
+    if (type != FL_BF16 && type != FL_F16) { return fail(c, FL_EINVAL, "type %d is not FL_BF16 or FL_F16", type); }
+    if (n < 0 || n > MM_MAXN) { return fail(c, FL_ERANGE, "n = %d outside 0..%d", n, MM_MAXN); }
+    if (R <= 0 || R % 8 || R > MM_MAXR || K <= 0 || K % 8 || K > MM_MAXK) {
+        return fail(c, FL_EINVAL, "R %d, K %d: positive multiples of 8, at most %d and %d", R, K, MM_MAXR, MM_MAXK);
+    }
+    if (n_exp < 1 || n_exp > NEXP_MAX || (!offsets && n_exp != 1)) { return fail(c, FL_EINVAL, "n_exp %d outside 1..%d, or not 1 without offsets", n_exp, NEXP_MAX); }
+    if (offsets && !covers(offsets, (size_t) (n_exp + 1) * 4)) { return fail(c, FL_EINVAL, "offsets' allocation is smaller than its shape (n_exp %d)", n_exp); }
+    magic = 0;
+    if (perm) {
+        if (!offsets) { return fail(c, FL_EINVAL, "perm goes with offsets"); }
+        if (topk < 1 || topk > MAXK) { return fail(c, FL_EINVAL, "topk %d outside 1..%d", topk, MAXK); }
+        if (xrows < 0 || (int64_t) xrows * K > 2147418112) { return fail(c, FL_ERANGE, "x has %d rows of %d: rows picked through perm are at most 2^31 - 2^16 values", xrows, K); }
+        if (!covers(perm, (size_t) n * 4)) { return fail(c, FL_EINVAL, "perm's allocation is smaller than its shape (n %d)", n); }
+        if (topk > 1) { magic = (uint32_t) ((((uint64_t) 1 << 32) + (uint64_t) topk - 1) / (uint64_t) topk); }
+    }
+    return need_device(c);
+}
+extern "C" int fl_matmul_dev(FLCtx * c, int type, int act, const void * x, const void * W, const void * W2, const float * bias, const void * residual,
+                             int n, int R, int K, int n_exp, const int * offsets, const int * perm, int topk, int xrows, void * y, int y_type, void * z, void * z2) {
+    if (!c) { return FL_EINVAL; }
+    MatmulArgs a{};
+    if (int rc = mm_shape(c, type, n, R, K, n_exp, offsets, perm, topk, xrows, a.magic)) { return rc; }
+    if (act < FL_ACT_NONE || act > FL_ACT_GELU) { return fail(c, FL_EINVAL, "activation %d", act); }
+    if (y_type != type && y_type != FL_F32) { return fail(c, FL_EINVAL, "y's type %d is neither the operands' nor FL_F32", y_type); }
+    if (n == 0) { return FL_OK; }
+    if (!x || !W || !y) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (W2 && bias) { return fail(c, FL_EINVAL, "a gated product takes no bias"); }
+    if (z2 && !W2) { return fail(c, FL_EINVAL, "z2 is the second matrix's product"); }
+    if (misaligned({ x, W, W2, bias, residual, y, z, z2 })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
+    const size_t xb = (size_t) (perm ? xrows : n) * K * 2, wb = (size_t) n_exp * R * K * 2, out = (size_t) n * R, yb = out * (y_type == FL_F32 ? 4 : 2);
+    if (!covers(x, xb) || !covers(W, wb) || (W2 && !covers(W2, wb)) || (bias && !covers(bias, (size_t) n_exp * R * 4)) || (residual && !covers(residual, out * 2)) ||
+        !covers(y, yb) || (z && !covers(z, out * 2)) || (z2 && !covers(z2, out * 2))) {
+        return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, R %d, K %d, n_exp %d)", n, R, K, n_exp);
+    }
+    const void * outs[3] = { y, z, z2 };
+    const size_t ob[3] = { yb, out * 2, out * 2 };
+    for (int i = 0; i < 3; ++i) {
+        if (overlap(outs[i], ob[i], x, xb) || overlap(outs[i], ob[i], W, wb) || overlap(outs[i], ob[i], W2, wb) || overlap(outs[i], ob[i], outs[(i + 1) % 3], ob[(i + 1) % 3]) ||
+            (!(i == 0 && y == residual && y_type == type) && overlap(outs[i], ob[i], residual, out * 2))) {
+            return fail(c, FL_EINVAL, "results must not overlap the operands or each other (y may be the residual's buffer in the operands' type)");
+        }
+    }
+    a.type = type; a.act = act; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
+    a.x = x; a.W = W; a.W2 = W2; a.bias = bias; a.residual = residual; a.y = y; a.z = z; a.z2 = z2; a.y_f32 = y_type == FL_F32;
+    TRY(c, launch_matmul(a, c->st));
+    return FL_OK;
+}
+extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const void * dz2, const void * x, const void * W, const void * W2, int n, int R, int K, int n_exp,
+                                  const int * offsets, const int * perm, int topk, int xrows, void * dx, void * dW, void * dW2, int dw_type, int accumulate) {
+    if (!c) { return FL_EINVAL; }
+    MatmulGradArgs a{};
+    if (int rc = mm_shape(c, type, n, R, K, n_exp, offsets, perm, topk, xrows, a.magic)) { return rc; }
+    if (dw_type != type && dw_type != FL_F32) { return fail(c, FL_EINVAL, "dW's type %d is neither the operands' nor FL_F32", dw_type); }
+    if (!dx && !dW && !dW2) { return fail(c, FL_EINVAL, "nothing to compute: dx, dW and dW2 are all null"); }
+    if ((n > 0 && (((dx || dW) && !dz) || ((dW || dW2) && !x) || (dx && (!W || (dz2 && !W2))) || (dW2 && !dz2)))) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (misaligned({ dz, dz2, x, W, W2, dx, dW, dW2 })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
+    const size_t xb = (size_t) (perm ? xrows : n) * K * 2, wn = (size_t) n_exp * R * K, wb = wn * (dw_type == FL_F32 ? 4 : 2), zb = (size_t) n * R * 2, dxb = (size_t) n * K * 2;
+    if ((n > 0 && ((dz && !covers(dz, zb)) || (dz2 && !covers(dz2, zb)) || (x && !covers(x, xb)) || (W && !covers(W, wn * 2)) || (W2 && !covers(W2, wn * 2)))) ||
+        (dx && !covers(dx, dxb)) || (dW && !covers(dW, wb)) || (dW2 && !covers(dW2, wb))) {
+        return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, R %d, K %d, n_exp %d)", n, R, K, n_exp);
+    }
+    const void * outs[3] = { dx, dW, dW2 };
+    const size_t ob[3] = { dxb, wb, wb };
+    for (int i = 0; i < 3; ++i) {
+        if (overlap(outs[i], ob[i], x, xb) || overlap(outs[i], ob[i], W, wn * 2) || overlap(outs[i], ob[i], W2, wn * 2) || overlap(outs[i], ob[i], dz, zb) ||
+            overlap(outs[i], ob[i], dz2, zb) || overlap(outs[i], ob[i], outs[(i + 1) % 3], ob[(i + 1) % 3])) {
+            return fail(c, FL_EINVAL, "results must not overlap the operands or each other");
+        }
+    }
+    a.type = type; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
+    a.dz = dz; a.dz2 = dz2; a.x = x; a.W = W; a.W2 = W2; a.dx = dx; a.dW = dW; a.dW2 = dW2; a.dw_f32 = dw_type == FL_F32; a.accumulate = accumulate ? 1 : 0;
+    if (dx && n > 0) { TRY(c, launch_matmul_dx(a, c->st)); }
+    if (dW || dW2) { TRY(c, launch_matmul_dw(a, c->st)); }   // (no rows: 0, or it stays)
+    return FL_OK;
+}
+extern "C" int fl_act_grad_dev(FLCtx * c, int type, int act, const void * dy, const void * z, const void * z2, int n, int R, int n_exp, const int * offsets,
+                               void * dz, void * dz2, float * dbias, int accumulate) {
+    if (!c) { return FL_EINVAL; }
+    ActGradArgs a{};
+    uint32_t magic;
+    if (int rc = mm_shape(c, type, n, R, 8, n_exp, offsets, nullptr, 1, 0, magic)) { return rc; }
+    if (act < FL_ACT_NONE || act > FL_ACT_GELU) { return fail(c, FL_EINVAL, "activation %d", act); }
+    if (!dz && !dz2 && !dbias) { return fail(c, FL_EINVAL, "nothing to compute: dz, dz2 and dbias are all null"); }
+    if ((z2 != nullptr || dz2 != nullptr) && dbias) { return fail(c, FL_EINVAL, "a gated product has no bias"); }
+    if (n > 0 && (!dy || ((act != FL_ACT_NONE || z2) && !z) || (dz2 && !z2))) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (misaligned({ dy, z, z2, dz, dz2, dbias })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
+    const size_t b = (size_t) n * R * 2;
+    for (const void * p : { dy, z, z2, (const void *) dz, (const void *) dz2 }) {
+        if (p && n > 0 && !covers(p, b)) { return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, R %d)", n, R); }
+    }
+    if (dbias && !covers(dbias, (size_t) n_exp * R * 4)) { return fail(c, FL_EINVAL, "dbias' allocation is smaller than its shape (n_exp %d, R %d)", n_exp, R); }
+    for (const void * q : { (const void *) dz, (const void *) dz2 }) {   // a thread reads its values before it writes them: whole buffers may be the same
+        for (const void * p : { dy, z, z2 }) { if (q != p && overlap(q, b, p, b)) { return fail(c, FL_EINVAL, "a result may be an operand's buffer, not overlap it in part"); } }
+        if (overlap(q, b, dbias, (size_t) n_exp * R * 4)) { return fail(c, FL_EINVAL, "results must not overlap each other"); }
+    }
+    if (overlap(dz, b, dz2, b)) { return fail(c, FL_EINVAL, "results must not overlap each other"); }
+    for (const void * p : { dy, z, z2 }) { if (overlap(dbias, (size_t) n_exp * R * 4, p, b)) { return fail(c, FL_EINVAL, "dbias must not overlap the operands"); } }
+    if (n == 0 && !dbias) { return FL_OK; }
+    a.type = type; a.act = act; a.n = n; a.R = R; a.n_exp = n_exp; a.offsets = offsets; a.dy = dy; a.z = z; a.z2 = z2; a.dz = dz; a.dz2 = dz2; a.dbias = dbias;
+    a.accumulate = accumulate ? 1 : 0; a.chunks = 1;
+    if (dbias) {
+        a.chunks = act_grad_chunks(n, R, n_exp);
+        if (a.chunks > 1) {
+            if (int rc = grow(c, c->mm, (size_t) n_exp * a.chunks * R * 4)) { return rc; }
+            a.part = (float *) c->mm.p;
+        }
+    }
+    TRY(c, launch_act_grad(a, c->st));
+    return FL_OK;
+}
+static int combine_args(FLCtx * c, const CombineArgs & a) {
+    if (a.type != FL_BF16 && a.type != FL_F16) { return fail(c, FL_EINVAL, "type %d is not FL_BF16 or FL_F16", a.type); }
+    if (a.topk < 1 || a.topk > MAXK || a.n < 0 || a.P < 0 || a.P > MM_MAXN || (int64_t) a.n * a.topk > MM_MAXN) {
+        return fail(c, FL_ERANGE, "n %d, topk %d (1..%d), P %d: n * topk and P at most %d", a.n, a.topk, MAXK, a.P, MM_MAXN);
+    }
+    if (a.E <= 0 || a.E % 8 || a.E > MM_MAXK) { return fail(c, FL_EINVAL, "E %d: a positive multiple of 8, at most %d", a.E, MM_MAXK); }
+    if (a.sel && (a.n_exp < 1 || a.n_exp > NEXP_MAX)) { return fail(c, FL_EINVAL, "n_exp %d outside 1..%d", a.n_exp, NEXP_MAX); }
+    const size_t pairs = (size_t) a.n * a.topk;
+    if (a.n > 0 && (!a.inv || !covers(a.inv, pairs * 4) || (a.sel && !covers(a.sel, pairs * 4)) || (a.w && !covers(a.w, pairs * 4)) || (a.o && !covers(a.o, (size_t) a.P * a.E * 2)))) {
+        return fail(c, FL_EINVAL, "inv is null, or an allocation is smaller than its shape (n %d, topk %d, P %d, E %d)", a.n, a.topk, a.P, a.E);
+    }
+    return need_device(c);
+}
+extern "C" int fl_combine_dev(FLCtx * c, int type, const void * o, const int * inv, const float * w, const int * sel, const void * residual, int n, int topk, int n_exp,
+                              int P, int E, void * y, int y_type) {
+    if (!c) { return FL_EINVAL; }
+    CombineArgs a{};
+    a.type = type; a.n = n; a.topk = topk; a.n_exp = n_exp; a.P = P; a.E = E; a.inv = inv; a.sel = sel; a.w = w; a.o = o; a.residual = residual; a.y = y; a.y_f32 = y_type == FL_F32;
+    if (int rc = combine_args(c, a)) { return rc; }
+    if (y_type != type && y_type != FL_F32) { return fail(c, FL_EINVAL, "y's type %d is neither the operands' nor FL_F32", y_type); }
+    if (n == 0) { return FL_OK; }
+    if (!y || (P > 0 && !o)) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (misaligned({ o, residual, y })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
+    const size_t yn = (size_t) n * E, yb = yn * (a.y_f32 ? 4 : 2);
+    if (!covers(y, yb) || (residual && !covers(residual, yn * 2))) { return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, E %d)", n, E); }
+    if (overlap(y, yb, o, (size_t) P * E * 2) || (!(y == residual && !a.y_f32) && overlap(y, yb, residual, yn * 2))) {
+        return fail(c, FL_EINVAL, "y must not overlap the operands (it may be the residual's buffer in the operands' type)");
+    }
+    TRY(c, launch_combine16(a, c->st));
+    return FL_OK;
+}
+extern "C" int fl_combine_grad_dev(FLCtx * c, int type, const void * dy, const void * o, const int * inv, const float * w, const int * sel, int n, int topk, int n_exp,
+                                   int P, int E, void * d_o, float * dw) {
+    if (!c) { return FL_EINVAL; }
+    CombineArgs a{};
+    a.type = type; a.n = n; a.topk = topk; a.n_exp = n_exp; a.P = P; a.E = E; a.inv = inv; a.sel = sel; a.w = w; a.o = o; a.dy = dy; a.d_o = d_o; a.dw = dw;
+    if (int rc = combine_args(c, a)) { return rc; }
+    if (!d_o && !dw) { return fail(c, FL_EINVAL, "nothing to compute: d_o and dw are both null"); }
+    if (n == 0) { return FL_OK; }
+    if (!dy || (dw && P > 0 && !o)) { return fail(c, FL_EINVAL, "null pointer"); }
+    if (misaligned({ dy, o, d_o })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
+    const size_t ob = (size_t) P * E * 2, yb = (size_t) n * E * 2, wb = (size_t) n * topk * 4;
+    if (!covers(dy, yb) || (d_o && !covers(d_o, ob)) || (dw && !covers(dw, wb))) { return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, topk %d, P %d, E %d)", n, topk, P, E); }
+    if (overlap(d_o, ob, dy, yb) || (d_o != o && overlap(d_o, ob, o, ob)) || overlap(dw, wb, w, wb) || overlap(dw, wb, d_o, ob) || overlap(dw, wb, o, ob) || overlap(dw, wb, dy, yb)) {
+        return fail(c, FL_EINVAL, "results must not overlap the operands or each other (d_o may be o's buffer)");
+    }
+    TRY(c, launch_combine16_grad(a, c->st));
+    return FL_OK;
+}
+
 static int pack_args(FLCtx * c, const void * s, const void * d, int R, int K, int nmat) {
     if (!s || !d) { return fail(c, FL_EINVAL, "null pointer"); }
     if (R <= 0 || R % 4 || K <= 0 || K % 1024 || nmat <= 0) { return fail(c, FL_EINVAL, "tiled layout needs R %% 4 == 0 and K %% 1024 == 0 (R %d, K %d)", R, K); }

@@ -1,0 +1,63 @@
+// matmul_device.h -- what the kernels of the 16-bit products share: types, activations, expert lookup, epilogues.
+#pragma once
+#include "moe_common.h"
+#include "moe_kernels.h"
+
+namespace lk {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+template <class T> struct Vec;
+template <> struct Vec<__bf16> { typedef bf16x8 v8; typedef bf16x4 v4; };
+template <> struct Vec<_Float16> { typedef f16x8 v8; typedef f16x4 v4; };
+template <class T> using V8 = typename Vec<T>::v8;
+template <class T> using V4 = typename Vec<T>::v4;
+
+// D[16][16] += A[16][32] B[32][16]: lane (r, g) = 16 g + r holds A[r][8 g ..] and B[8 g ..][r], and D[4 g + i][r]
+__device__ __forceinline__ f32x4 mfma32(bf16x8 a, bf16x8 b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+#else
+    (void) a; (void) b; return c;
+#endif
+}
+__device__ __forceinline__ f32x4 mfma32(f16x8 a, f16x8 b, f32x4 c) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+#else
+    (void) a; (void) b; return c;
+#endif
+}
+
+// ---------------------------------------------------------------- activations z s(g(z)), s(t) = 1 / (1 + e^-t)
+// silu: g = z; gelu: g = 2 sqrt(2 / pi) (z + 0.044715 z^3), the tanh form. In fp32: e^-t by the exp2 instruction, whose argument's
+// rounding costs |t| 2^-24 of it; where |t| is large the factor is near 0 or 1 and the error falls away or reaches 100 * 2^-24 of values
+// below e^-100. A factor below 2^-126 is 0.
+constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;
+__device__ __forceinline__ float sigma(float t) { return 1.f / (1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)); }
+template <int ACT> __device__ __forceinline__ float act_arg(float z) { return ACT == ACT_GELU ? GELU_C * (z + GELU_A * z * z * z) : z; }
+template <int ACT> __device__ __forceinline__ float act_fn(float z) { return ACT == ACT_NONE ? z : z * sigma(act_arg<ACT>(z)); }
+// the derivative: s(g) + z g' s(g) s(-g)
+template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+    if (ACT == ACT_NONE) { return 1.f; }
+    const float t = act_arg<ACT>(z), s = sigma(t), r = sigma(-t), d = ACT == ACT_GELU ? GELU_C * (1.f + 3.f * GELU_A * z * z) : 1.f;
+    const float q = s * r;
+    return q > 0.f ? s + z * d * q : s;   // (z d may be infinite where s or r has vanished)
+}
+
+// ---------------------------------------------------------------- slots
+struct Span { int begin, end; };
+// expert e's slots, inside 0 .. n whatever the offsets say
+__device__ __forceinline__ Span span_of(const int * offsets, int n, int e) {
+    if (!offsets) { return { 0, n }; }
+    const int a = min(max(offsets[e], 0), n), b = min(max(offsets[e + 1], 0), n);
+    return { a, max(a, b) };
+}
+// the pair's row: perm[slot] / topk by a product with 2^32 / topk rounded up (exact below 2^28 for topk <= 8); rows outside 0 .. xrows - 1
+// come out as xrows or more
+__device__ __forceinline__ uint32_t pair_row(uint32_t pair, uint32_t magic) { return magic ? __umulhi(pair, magic) : pair; }
+
+}  // namespace lk

@@ -294,6 +294,39 @@ struct RouteGradArgs {
 };
 size_t route_grad_scratch(int n, int n_exp, int E, bool dW, bool dx);
 hipError_t launch_route_grad(const RouteGradArgs & a, void * scratch, hipStream_t st);   // (n == 0: nothing is done)
+// ---------------------------------------------------------------- 16-bit products (matmul.hip, matmul_rows.hip)
+enum { TYPE_F32 = 16, TYPE_F16 = 17, TYPE_BF16 = 18 };
+enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU = 2 };
+constexpr int MM_MAXN = 1 << 24, MM_MAXK = 65536, MM_MAXR = 1 << 20;
+struct MatmulArgs {
+    int type, act, n, R, K, n_exp;           // n: slots (rows without offsets, n_exp 1)
+    const int * offsets; const int * perm; uint32_t magic; int xrows;   // perm may be null: slot s reads row s of x
+    const void * x, * W, * W2; const float * bias; const void * residual;
+    void * y, * z, * z2; int y_f32;
+};
+struct MatmulGradArgs {
+    int type, n, R, K, n_exp;
+    const int * offsets; const int * perm; uint32_t magic; int xrows;
+    const void * dz, * dz2, * x, * W, * W2;
+    void * dx, * dW, * dW2; int dw_f32, accumulate;
+};
+struct ActGradArgs {
+    int type, act, n, R, n_exp; const int * offsets;
+    const void * dy, * z, * z2; void * dz, * dz2; float * dbias, * part; int accumulate, chunks;
+};
+struct CombineArgs {
+    int type, n, topk, n_exp, P, E; const int * inv, * sel; const float * w;
+    const void * o, * residual; void * y; int y_f32;    // combine
+    const void * dy; void * d_o; float * dw;            // its gradient
+};
+hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st);
+hipError_t launch_matmul_dx(const MatmulGradArgs & a, hipStream_t st);
+hipError_t launch_matmul_dw(const MatmulGradArgs & a, hipStream_t st);
+int act_grad_chunks(int n, int R, int n_exp);             // row chunks an expert's bias gradient is summed in
+hipError_t launch_act_grad(const ActGradArgs & a, hipStream_t st);
+hipError_t launch_combine16(const CombineArgs & a, hipStream_t st);
+hipError_t launch_combine16_grad(const CombineArgs & a, hipStream_t st);
+
 // h = silu(g) * u, element-wise under the exp contract
 hipError_t launch_swiglu(const float * g, const float * u, int64_t n, float * h, hipStream_t st);
 // the same h for nrows rows of K (K % 256 == 0) and its Q8_K (q [nrows][K], d [nrows][K/256]) in one pass
