@@ -1,173 +1,485 @@
 // matmul.hip -- products of bfloat16 / float16 matrices, dense or grouped by expert, and their backward pass.
 //
-//   forward  y[s][r]  = sum_k x[row(s)][k] W[e][r][k], with an epilogue     s: expert e's slots
-//   dx       dx[s][k] = sum_r dz[s][r] W[e][r][k] (+ dz2 W2)
+//   forward  y[s][r]     = sum_k x[row(s)][k] W[e][r][k], with an epilogue     s: expert e's slots
+//   dx       dx[s][k]    = sum_r dz[s][r] W[e][r][k] (+ dz2 W2)
 //   dW       dW[e][r][k] = sum over e's slots of dz[s][r] x[row(s)][k]
 //
 // All three are D[m][n] = sum_k A[m][k] B[n][k] with D's rows along n in memory. The matrix cores take B as their first operand, so that a
 // lane's four results lie next to each other in a row of D.
+//
+// A workgroup takes tiles of BM x BN, BK = 32 of the sum's terms a step. A step's operands are copied straight into LDS, 16 bytes a lane, S
+// steps ahead; what lies outside an operand is not read and arrives as 0 (the buffer's range), so that no row of another expert, infinite
+// or not, takes part. While a step's products run, the next step's operands go from LDS into the other set of registers. One barrier a step.
+//
+// In LDS an operand whose terms are next to each other in memory ("row" operand) has 64 bytes a row, chunk c of 16 at c ^ (row / 4 % 4): a
+// ds_read_b128 takes its 16 lanes of a pass from different bank quads. One whose terms are rows of memory ("col" operand) has a row a
+// term, segments of 32 bytes at segment ^ (term % 4 + term / 8 % 2 * 4), and is transposed by ds_read_b64_tr_b16: 16 lanes read 4 terms x 16
+// columns and each gets its column's 4.
 #include "matmul_device.h"
 
 namespace lk {
 namespace {
 
-constexpr int TM = 64, TN = 64, TK = 32, LDK = TK + 8;
+enum { FWD, DX, DW };
+constexpr int BK = 32;
+constexpr uint32_t FAR = 0xFFFF0000u, WINDOW = 0xFFFE0000u;   // an offset outside every buffer; the largest range of one
 
-// the expert and first slot of the launch's m-tile `mt` of `tm` slots; false: there is no such tile
-__device__ bool find_tile(const int * offsets, int n, int n_exp, int tm, int mt, int & e, Span & s) {
-    for (e = 0; e < n_exp; ++e) {
-        s = span_of(offsets, n, e);
-        const int tiles = (s.end - s.begin + tm - 1) / tm;
-        if (mt < tiles) { s.begin += mt * tm; return true; }
-        mt -= tiles;
-    }
-    return false;
+// one step's copy instruction: 16 bytes a lane to m0 + 16 * lane; nothing of it is known to the compiler, which would wait for all
+// copies before each ds_read_b64_tr_b16: the waits below are counted by hand
+__device__ __forceinline__ void copy16(uint32_t lds, uint32_t voff, u32x4 rsrc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+#endif
+}
+template <int N> __device__ __forceinline__ void wait_copies() {   // all but the last N, and all LDS reads
+    __asm__ volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ void meet() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ u32x4 buffer(uint64_t base, uint32_t bytes) { return (u32x4) { (uint32_t) base, (uint32_t) (base >> 32) & 0xFFFFu, bytes, 0x00020000u }; }
+__device__ __forceinline__ uint64_t uni64(const void * p) {
+    const uint64_t v = (uint64_t) p;
+    return ((uint64_t) (uint32_t) uni((int) (uint32_t) (v >> 32)) << 32) | (uint32_t) uni((int) (uint32_t) v);
 }
 
-// rows 0 .. nr - 1 of `p` (row i at p + at(i) * ld), columns k0 .. min(k0 + TK, K) - 1, as lds[i][k]; what is not there is 0
-template <class T, class At> __device__ __forceinline__ void stage_rows(T (*lds)[LDK], const T * p, size_t ld, int nr, int k0, int K, At at) {
-    for (int i = threadIdx.x; i < 64 * TK; i += 256) {
-        const int r = i / TK, k = i % TK;
-        T v = (T) 0.f;
-        if (r < nr && k0 + k < K) { const int64_t row = at(r); if (row >= 0) { v = p[(size_t) row * ld + k0 + k]; } }
-        lds[r][k] = v;
+// a row operand's lane: it copies chunk `chunk` of row `lane / 4` of 16, and reads row lane % 16, chunk lane / 16
+struct RowLane {
+    uint32_t chunk, read;
+    __device__ __forceinline__ RowLane() {
+        const int l = lane_id();
+        chunk = (uint32_t) ((l & 3) ^ ((l >> 4) & 3));
+        read = (uint32_t) ((l & 15) * 64 + (((l >> 4) ^ ((l >> 2) & 3)) * 16));
     }
-}
-// rows k0 .. min(k0 + TK, K) - 1 of `p`, columns c0 .. c0 + nc - 1, as lds[column][row]
-template <class T, class At> __device__ __forceinline__ void stage_cols(T (*lds)[LDK], const T * p, size_t ld, int c0, int nc, int k0, int K, At at) {
-    for (int i = threadIdx.x; i < 64 * TK; i += 256) {
-        const int k = i / 64, c = i % 64;
-        T v = (T) 0.f;
-        if (c < nc && k0 + k < K) { const int64_t row = at(k0 + k); if (row >= 0) { v = p[(size_t) row * ld + c0 + c]; } }
-        lds[c][k] = v;
+};
+// a col operand's: of an instruction's 1024 bytes = 512 / COLS terms
+template <int COLS> struct ColLane {
+    static constexpr int TERMS = 512 / COLS;   // terms an instruction copies
+    __device__ __forceinline__ static int term(int j) { return j * TERMS + lane_id() / (COLS / 8); }
+    __device__ __forceinline__ static int column(int j) {   // first of the 8 columns it copies
+        const int k = term(j), p = lane_id() % (COLS / 8);
+        return 8 * ((((p >> 1) ^ swz(k)) << 1) | (p & 1));
     }
+    __device__ __forceinline__ static int swz(int k) { return (k & 3) | ((k >> 1) & 4); }
+    // the address of columns 16 j .. 16 j + 15 (j = 0 .. 7, + 8 i: + 256 i bytes), terms 8 (lane / 16) .. + 3; + 4: + 4 rows
+    __device__ __forceinline__ static uint32_t read(int j) {
+        const int l = lane_id(), k = 8 * (l >> 4) + ((l >> 2) & 3);
+        return (uint32_t) (k * COLS * 2 + ((j ^ swz(k)) & 7) * 32 + (l & 3) * 8);
+    }
+};
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <class T> __device__ __forceinline__ V8<T> lds_row(uint32_t a) { return *(const LK_LOCAL V8<T> *) (size_t) a; }
+template <class T, int COLS> __device__ __forceinline__ V8<T> lds_col(uint32_t a) {
+    union { s16x4 s[2]; V8<T> v; } u;
+#if defined(__HIP_DEVICE_COMPILE__)
+    u.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LK_LOCAL s16x4 *) (size_t) a);
+    u.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LK_LOCAL s16x4 *) (size_t) (a + 4 * COLS * 2));
+#else
+    u.v = (V8<T>) {};
+#endif
+    return u.v;
 }
-// a wave's 64 x 16 of the tile's products of one TK: n-rows 16 w .. of lb, all m of la
-template <class T> __device__ __forceinline__ void products(const T (*la)[LDK], const T (*lb)[LDK], f32x4 (&acc)[4]) {
-    const int w = threadIdx.x >> 6, lane = lane_id(), r = lane & 15, g = lane >> 4;
-    const V8<T> b = *reinterpret_cast<const V8<T> *>(&lb[16 * w + r][8 * g]);
+
+// ---------------------------------------------------------------- the launch's tiles
+struct Tiles { int first[NEXP_MAX + 1]; };   // m-tiles of the experts before e; [n_exp]: all of them
+__device__ __forceinline__ void count_tiles(Tiles & t, const int * offsets, int n, int n_exp, int bm) {   // (all threads; ends with a barrier)
+    if (threadIdx.x < 64) {
+        const int l = threadIdx.x;
+        int c[4], s = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { acc[i] = mfma32(b, *reinterpret_cast<const V8<T> *>(&la[16 * i + r][8 * g]), acc[i]); }
+        for (int j = 0; j < 4; ++j) {
+            const int e = 4 * l + j;
+            c[j] = 0;
+            if (e < n_exp) { const Span sp = span_of(offsets, n, e); c[j] = (sp.end - sp.begin + bm - 1) / bm; }
+            s += c[j];
+        }
+        int si = s;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(si, o); if (l >= o) { si += v; } }
+        int at = si - s;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { t.first[4 * l + j] = at; at += c[j]; }
+        if (l == 63) { t.first[NEXP_MAX] = at; }
+    }
+    __syncthreads();
+}
+// the expert of tile `i`, i < the sum: the last one whose tiles begin at or before it
+__device__ __forceinline__ int expert_of(const Tiles & t, int i) {
+    int e = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { e += __popcll(__ballot(t.first[4 * lane_id() + j] <= i)); }
+    return uni(e) - 1;
+}
+struct Spot { int e, slot, nm, n0; };   // expert, first slot, its slots in the tile, first column
+// tile i of the launch, i < first[NEXP_MAX] * nt: an expert's tiles are next to each other, in bands of `band` m-tiles, m fastest
+__device__ __forceinline__ Spot spot_of(const Tiles & t, const int * offsets, int n, int nt, int bm, int bn, int band, int i) {
+    Spot s;
+    s.e = expert_of(t, i / nt);   // (first[e] * nt <= i exactly when first[e] <= i / nt)
+    const Span sp = span_of(offsets, n, s.e);
+    const int mt = uni(t.first[s.e + 1]) - uni(t.first[s.e]), in = i - uni(t.first[s.e]) * nt, b = in / (band * nt), rows = min(band, mt - b * band), r = in - b * band * nt;
+    s.slot = uni(sp.begin) + (b * band + r % rows) * bm;
+    s.nm = min(bm, uni(sp.end) - s.slot);
+    s.n0 = r / rows * bn;
+    return s;
 }
 
-template <class T, int ACT> __global__ void __launch_bounds__(256) k_mm(MatmulArgs a) {
-    __shared__ __attribute__((aligned(16))) T la[TM][LDK], lb[TN][LDK], lc[TN][LDK];
-    int e; Span s;
-    if (!find_tile(a.offsets, a.n, a.n_exp, TM, blockIdx.x, e, s)) { return; }
-    const int n0 = blockIdx.y * TN, nm = min(TM, s.end - s.begin), nn = min(TN, a.R - n0);
-    const T * W = (const T *) a.W + ((size_t) e * a.R + n0) * a.K, * W2 = a.W2 ? (const T *) a.W2 + ((size_t) e * a.R + n0) * a.K : nullptr;
-    auto row = [&](int i) -> int64_t {
-        if (!a.perm) { return s.begin + i; }
-        const uint32_t t = pair_row((uint32_t) a.perm[s.begin + i], a.magic);
-        return t < (uint32_t) a.xrows ? (int64_t) t : -1;
+// ---------------------------------------------------------------- a tile's sums
+// NW = WM * WN waves, a wave BM / WM x BN / WN. A: m side, B: n side; AC, BC: whether they are col operands
+template <class T, bool AC, bool BC, int BM_, int BN_, int WM_, int WN_, int S_> struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, S = S_, NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+    static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, STAGE = AB + BB, LDS = S * STAGE;
+    static constexpr int IA = AB / 1024 < NW ? 1 : AB / 1024 / NW, IB = BB / 1024 < NW ? 1 : BB / 1024 / NW, NI = IA + IB;   // copies a wave and step
+    static constexpr int threads = 64 * NW;
+    typedef V8<T> F;
+};
+template <class H> struct Frags { typename H::F a[H::FM], b[H::FN]; };
+
+// which of an operand's 1024-byte pieces copy i of wave w takes (fewer pieces than waves: some copy the same one)
+template <int BYTES, int I> __device__ __forceinline__ int piece(int w, int i) { return (w * I + i) % (BYTES / 1024); }
+
+// the loop over the sum's steps. issue(j, slot address, t): copy j (0 .. NI - 1) of step t; it is called for t past the end too, and then
+// copies nothing (zeros)
+template <class T, bool AC, bool BC, class H, class Issue>
+__device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, int steps, Issue issue) {
+    const int wave = uni(threadIdx.x >> 6), wm = wave / H::WN, wn = wave % H::WN;
+    const RowLane row;
+    constexpr int RA = AC ? (H::FM < 8 ? H::FM : 8) : 1, RB = BC ? (H::FN < 8 ? H::FN : 8) : 1;
+    uint32_t ra[RA], rb[RB];   // a lane's addresses in a stage
+    if constexpr (AC) {
+#pragma unroll
+        for (int j = 0; j < RA; ++j) { ra[j] = ColLane<H::BM>::read(wm * H::FM + j) + (uint32_t) (wm * H::FM + j) / 8 * 256; }
+    } else { ra[0] = row.read + (uint32_t) (wm * H::FM * 1024); }
+    if constexpr (BC) {
+#pragma unroll
+        for (int j = 0; j < RB; ++j) { rb[j] = ColLane<H::BN>::read(wn * H::FN + j) + (uint32_t) (wn * H::FN + j) / 8 * 256 + H::AB; }
+    } else { rb[0] = row.read + (uint32_t) (wn * H::FN * 1024) + H::AB; }
+    auto read_a = [&](Frags<H> & f, uint32_t at, int i) {
+        if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at + ra[i % RA] + (uint32_t) (i / RA * 256)); } else { f.a[i] = lds_row<T>(at + ra[0] + (uint32_t) (i * 1024)); }
     };
-    f32x4 acc[4] = {}, acc2[4] = {};
-    for (int k0 = 0; k0 < a.K; k0 += TK) {
-        __syncthreads();
-        stage_rows(la, (const T *) a.x, a.K, nm, k0, a.K, row);
-        stage_rows(lb, W, a.K, nn, k0, a.K, [](int i) -> int64_t { return i; });
-        if (W2) { stage_rows(lc, W2, a.K, nn, k0, a.K, [](int i) -> int64_t { return i; }); }
-        __syncthreads();
-        products<T>(la, lb, acc);
-        if (W2) { products<T>(la, lc, acc2); }
-    }
-    const int w = threadIdx.x >> 6, lane = lane_id(), r = lane & 15, g = lane >> 4;
-    for (int i = 0; i < 4; ++i) {
-        for (int u = 0; u < 4; ++u) {
-            const int m = 16 * i + r, nc = n0 + 16 * w + 4 * g + u;
-            if (m >= nm || nc >= a.R) { continue; }
-            const size_t at = (size_t) (s.begin + m) * a.R + nc;
-            const float z = acc[i][u] + (a.bias ? a.bias[(size_t) e * a.R + nc] : 0.f), z2 = acc2[i][u];
-            float y = act_fn<ACT>(z);
-            if (W2) { y *= z2; }
-            if (a.residual) { y += (float) ((const T *) a.residual)[at]; }
-            if (a.y_f32) { ((float *) a.y)[at] = y; } else { ((T *) a.y)[at] = (T) y; }
-            if (a.z) { ((T *) a.z)[at] = (T) z; }
-            if (a.z2) { ((T *) a.z2)[at] = (T) z2; }
-        }
-    }
-}
-
-template <class T> __global__ void __launch_bounds__(256) k_mm_dx(MatmulGradArgs a) {
-    __shared__ __attribute__((aligned(16))) T la[TM][LDK], lb[TN][LDK];
-    int e; Span s;
-    if (!find_tile(a.offsets, a.n, a.n_exp, TM, blockIdx.x, e, s)) { return; }
-    const int n0 = blockIdx.y * TN, nm = min(TM, s.end - s.begin), nn = min(TN, a.K - n0);
-    auto same = [](int i) -> int64_t { return i; };
-    f32x4 acc[4] = {};
-    for (int src = 0; src < (a.dz2 ? 2 : 1); ++src) {
-        const T * dz = (const T *) (src ? a.dz2 : a.dz) + (size_t) s.begin * a.R, * W = (const T *) (src ? a.W2 : a.W) + (size_t) e * a.R * a.K;
-        for (int k0 = 0; k0 < a.R; k0 += TK) {
-            __syncthreads();
-            stage_rows(la, dz, a.R, nm, k0, a.R, same);
-            stage_cols(lb, W, a.K, n0, nn, k0, a.R, same);
-            __syncthreads();
-            products<T>(la, lb, acc);
-        }
-    }
-    const int w = threadIdx.x >> 6, lane = lane_id(), r = lane & 15, g = lane >> 4;
-    for (int i = 0; i < 4; ++i) {
-        for (int u = 0; u < 4; ++u) {
-            const int m = 16 * i + r, nc = n0 + 16 * w + 4 * g + u;
-            if (m < nm && nc < a.K) { ((T *) a.dx)[(size_t) (s.begin + m) * a.K + nc] = (T) acc[i][u]; }
-        }
-    }
-}
-
-template <class T> __global__ void __launch_bounds__(256) k_mm_dw(MatmulGradArgs a) {
-    __shared__ __attribute__((aligned(16))) T la[TM][LDK], lb[TN][LDK];
-    const int e = blockIdx.z % a.n_exp, second = blockIdx.z / a.n_exp;
-    const Span s = span_of(a.offsets, a.n, e);
-    const int m0 = blockIdx.y * TM, n0 = blockIdx.x * TN, nm = min(TM, a.R - m0), nn = min(TN, a.K - n0), len = s.end - s.begin;
-    const T * dz = (const T *) (second ? a.dz2 : a.dz) + (size_t) s.begin * a.R;
-    auto row = [&](int i) -> int64_t {
-        if (!a.perm) { return s.begin + i; }
-        const uint32_t t = pair_row((uint32_t) a.perm[s.begin + i], a.magic);
-        return t < (uint32_t) a.xrows ? (int64_t) t : -1;
+    auto read_b = [&](Frags<H> & f, uint32_t at, int i) {
+        if constexpr (BC) { f.b[i] = lds_col<T, H::BN>(at + rb[i % RB] + (uint32_t) (i / RB * 256)); } else { f.b[i] = lds_row<T>(at + rb[0] + (uint32_t) (i * 1024)); }
     };
-    f32x4 acc[4] = {};
-    for (int k0 = 0; k0 < len; k0 += TK) {
-        __syncthreads();
-        stage_cols(la, dz, a.R, m0, nm, k0, len, [](int i) -> int64_t { return i; });
-        stage_cols(lb, (const T *) a.x, a.K, n0, nn, k0, len, row);
-        __syncthreads();
-        products<T>(la, lb, acc);
+    constexpr int MF = H::FM * H::FN, RD = H::FM + H::FN, G = MF < 8 ? MF : 8;
+    int slot = 0;   // of step t
+    auto step = [&](Frags<H> & cur, Frags<H> & nxt, int t) {
+        wait_copies<(H::S - 2) * H::NI>();   // step t + 1 is there, and this wave has read step t
+        meet();                              // and everyone's: step t's place is free
+        const uint32_t here = lds + (uint32_t) (slot * H::STAGE);
+        slot = slot + 1 == H::S ? 0 : slot + 1;
+        const uint32_t next = lds + (uint32_t) (slot * H::STAGE);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+#pragma unroll
+            for (int j = g * H::NI / G; j < (g + 1) * H::NI / G; ++j) { issue(j, here, t + H::S); }
+            constexpr int GR = G > 2 ? G - 2 : 1;   // the reads end two groups early
+#pragma unroll
+            for (int j = g * RD / GR; j < (g + 1) * RD / GR && j < RD; ++j) { if (j < H::FN) { read_b(nxt, next, j); } else { read_a(nxt, next, j - H::FN); } }
+#pragma unroll
+            for (int j = g * MF / G; j < (g + 1) * MF / G; ++j) { acc[j / H::FN][j % H::FN] = mfma32(cur.b[j % H::FN], cur.a[j / H::FN], acc[j / H::FN][j % H::FN]); }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < H::FM; ++i) {
+#pragma unroll
+        for (int j = 0; j < H::FN; ++j) { acc[i][j] = (f32x4) { 0.f, 0.f, 0.f, 0.f }; }
     }
-    const int w = threadIdx.x >> 6, lane = lane_id(), r = lane & 15, g = lane >> 4;
+    for (int t = 0; t < H::S; ++t) {
+#pragma unroll
+        for (int j = 0; j < H::NI; ++j) { issue(j, lds + (uint32_t) (t * H::STAGE), t); }
+    }
+    Frags<H> f0, f1;
+    wait_copies<(H::S - 1) * H::NI>();
+    meet();
+#pragma unroll
+    for (int j = 0; j < H::FN; ++j) { read_b(f0, lds, j); }
+#pragma unroll
+    for (int j = 0; j < H::FM; ++j) { read_a(f0, lds, j); }
+    for (int t = 0; t < steps; t += 2) {   // (an odd number of steps: one more, of zeros)
+        step(f0, f1, t);
+        step(f1, f0, t + 1);
+    }
+    wait_copies<0>();   // nothing is written to LDS after the tile
+    meet();
+}
+
+// 8 results next to each other in a row: lane (r, g) of fragments j and j + 1 gets row r, columns 16 (g % 2) + 8 (g / 2) .. + 7 of the 32
+__device__ __forceinline__ void eight(f32x4 a, f32x4 b, float (&v)[8]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
     for (int i = 0; i < 4; ++i) {
-        for (int u = 0; u < 4; ++u) {
-            const int m = m0 + 16 * i + r, nc = n0 + 16 * w + 4 * g + u;
-            if (m >= a.R || nc >= a.K) { continue; }
-            const size_t at = ((size_t) e * a.R + m) * a.K + nc;
-            float v = acc[i][u];
-            if (a.dw_f32) { float * d = (float *) (second ? a.dW2 : a.dW) + at; *d = a.accumulate ? *d + v : v; }
-            else { T * d = (T *) (second ? a.dW2 : a.dW) + at; *d = (T) (a.accumulate ? (float) *d + v : v); }
+        const float p = a[i], o = b[i];   // (a bit cast of a vector's element would take the first)
+        const auto q = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, p), __builtin_bit_cast(uint32_t, o), false, false);
+        v[i] = __builtin_bit_cast(float, (uint32_t) q[0]); v[4 + i] = __builtin_bit_cast(float, (uint32_t) q[1]);
+    }
+#endif
+}
+template <class T> __device__ __forceinline__ void put8(T * p, const float (&v)[8]) {
+    V8<T> u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { u[i] = (T) v[i]; }
+    *(LK_GLOBAL V8<T> *) p = u;
+}
+__device__ __forceinline__ void put8(float * p, const float (&v)[8]) {
+    *(LK_GLOBAL f32x4 *) p = (f32x4) { v[0], v[1], v[2], v[3] };
+    *(LK_GLOBAL f32x4 *) (p + 4) = (f32x4) { v[4], v[5], v[6], v[7] };
+}
+template <class T> __device__ __forceinline__ void add8(const T * p, float (&v)[8]) {
+    const V8<T> u = *(const LK_GLOBAL V8<T> *) p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { v[i] += (float) u[i]; }
+}
+__device__ __forceinline__ void add8(const float * p, float (&v)[8]) {
+    const f32x4 a = *(const LK_GLOBAL f32x4 *) p, b = *(const LK_GLOBAL f32x4 *) (p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] += a[i]; v[4 + i] += b[i]; }
+}
+
+// the range [first, last) of tiles of this workgroup's XCD (workgroups go round the 8 XCDs), and where it begins in it
+struct Share { int first, last, step; };
+__device__ __forceinline__ Share share_of(int tiles) {
+    const int x = blockIdx.x % 8, per = gridDim.x / 8;   // (the grid is a multiple of 8)
+    return { (int) ((int64_t) tiles * x / 8) + (int) blockIdx.x / 8, (int) ((int64_t) tiles * (x + 1) / 8), per };
+}
+
+// ---------------------------------------------------------------- forward
+// GATED: of a wave's columns of the tile the first half are W's rows, the second the same rows of W2
+template <class T, int ACT, bool GATED, class H> __global__ void __launch_bounds__(H::threads) k_mm(MatmulArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    __shared__ Tiles tiles;
+    constexpr int CN = GATED ? H::BN / 2 : H::BN, WC = CN / H::WN;   // result columns of a tile, of a wave
+    const int nt = (a.R + CN - 1) / CN;
+    count_tiles(tiles, a.offsets, a.n, a.n_exp, H::BM);
+    const Share sh = share_of(uni(tiles.first[NEXP_MAX]) * nt);
+    const uint32_t lds = lds_addr(dyn);
+    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
+    const RowLane row;
+    for (int i = sh.first; i < sh.last; i += sh.step) {
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, CN, 4, i);
+        uint32_t va[H::IA], vb[H::IB];
+#pragma unroll
+        for (int j = 0; j < H::IA; ++j) {
+            const int m = piece<H::AB, H::IA>(wave, j) * 16 + (lane >> 2);
+            uint32_t r = (uint32_t) m;
+            bool ok = m < s.nm;
+            if (a.perm && ok) { r = pair_row((uint32_t) a.perm[s.slot + m], a.magic); ok = r < (uint32_t) a.xrows; }
+            va[j] = ok ? r * (uint32_t) a.K * 2 + row.chunk * 16 : FAR;
+        }
+#pragma unroll
+        for (int j = 0; j < H::IB; ++j) {
+            const int rr = piece<H::BB, H::IB>(wave, j) * 16 + (lane >> 2);
+            const int c = GATED ? rr / (2 * WC) * WC + rr % WC : rr;
+            vb[j] = s.n0 + c < a.R ? (uint32_t) c * (uint32_t) a.K * 2 + row.chunk * 16 : FAR;
+        }
+        const size_t w0 = ((size_t) s.e * a.R + s.n0) * a.K;
+        const uint64_t pa = uni64((const T *) a.x + (a.perm ? 0 : (size_t) s.slot * a.K)), pb = uni64((const T *) a.W + w0), pb2 = GATED ? uni64((const T *) a.W2 + w0) : 0;
+        f32x4 acc[H::FM][H::FN];
+        sums<T, false, false, H>(acc, lds, (a.K + BK - 1) / BK, [&](int j, uint32_t at, int t) {
+            const int left = a.K - t * BK;   // terms from this step on
+            const uint32_t bytes = left > 0 ? WINDOW : 0;
+            const bool in = left >= BK || (int) row.chunk * 8 < left;
+            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, buffer(pa + (uint64_t) (uint32_t) t * (BK * 2), bytes)); }
+            else {
+                const int p = piece<H::BB, H::IB>(wave, j - H::IA);
+                const uint64_t b = GATED && p * 16 % (2 * WC) >= WC ? pb2 : pb;
+                copy16(at + H::AB + (uint32_t) (p * 1024), in ? vb[j - H::IA] : FAR, buffer(b + (uint64_t) (uint32_t) t * (BK * 2), bytes));
+            }
+        });
+        constexpr int FC = GATED ? H::FN / 2 : H::FN;
+#pragma unroll
+        for (int m = 0; m < H::FM; ++m) {
+            const int sr = (wm * H::FM + m) * 16 + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < FC; j += 2) {
+                const int c = s.n0 + wn * WC + 16 * (j + ((lane >> 4) & 1)) + 8 * (lane >> 5);
+                float z[8], y[8], z2[8];
+                eight(acc[m][j], acc[m][j + 1], z);
+                if (GATED) { eight(acc[m][FC + j], acc[m][FC + j + 1], z2); }
+                if (sr >= s.nm || c >= a.R) { continue; }
+                const size_t at = (size_t) (s.slot + sr) * a.R + c;
+                if (a.bias) { add8(a.bias + (size_t) s.e * a.R + c, z); }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) { y[u] = act_fn<ACT>(z[u]); if (GATED) { y[u] *= z2[u]; } }
+                if (a.residual) { add8((const T *) a.residual + at, y); }
+                if (a.y_f32) { put8((float *) a.y + at, y); } else { put8((T *) a.y + at, y); }
+                if (a.z) { put8((T *) a.z + at, z); }
+                if (GATED && a.z2) { put8((T *) a.z2 + at, z2); }
+            }
         }
     }
 }
 
-constexpr unsigned ceil_div(int64_t a, int64_t b) { return (unsigned) ((a + b - 1) / b); }
+// ---------------------------------------------------------------- dx
+template <class T, class H> __global__ void __launch_bounds__(H::threads) k_mm_dx(MatmulGradArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    __shared__ Tiles tiles;
+    const int nt = (a.K + H::BN - 1) / H::BN;
+    count_tiles(tiles, a.offsets, a.n, a.n_exp, H::BM);
+    const Share sh = share_of(uni(tiles.first[NEXP_MAX]) * nt);
+    const uint32_t lds = lds_addr(dyn);
+    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
+    const RowLane row;
+    const int half = (a.R + BK - 1) / BK, steps = a.dz2 ? 2 * half : half;
+    for (int i = sh.first; i < sh.last; i += sh.step) {
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, i);
+        uint32_t va[H::IA], vb[H::IB];
+#pragma unroll
+        for (int j = 0; j < H::IA; ++j) {
+            const int m = piece<H::AB, H::IA>(wave, j) * 16 + (lane >> 2);
+            va[j] = m < s.nm ? (uint32_t) m * (uint32_t) a.R * 2 + row.chunk * 16 : FAR;
+        }
+#pragma unroll
+        for (int j = 0; j < H::IB; ++j) {
+            const int p = piece<H::BB, H::IB>(wave, j), c = ColLane<H::BN>::column(p);
+            vb[j] = s.n0 + c < a.K ? (uint32_t) ColLane<H::BN>::term(p) * (uint32_t) a.K * 2 + (uint32_t) c * 2 : FAR;
+        }
+        const size_t a0 = (size_t) s.slot * a.R, w0 = (size_t) s.e * a.R * a.K + s.n0;
+        const uint64_t pa = uni64((const T *) a.dz + a0), pb = uni64((const T *) a.W + w0);
+        const uint64_t pa2 = a.dz2 ? uni64((const T *) a.dz2 + a0) : 0, pb2 = a.dz2 ? uni64((const T *) a.W2 + w0) : 0;
+        f32x4 acc[H::FM][H::FN];
+        sums<T, false, true, H>(acc, lds, steps, [&](int j, uint32_t at, int t) {
+            const bool second = t >= half;   // (t < steps: the second pair's)
+            const int u = second ? t - half : t, left = t < steps ? a.R - u * BK : 0;
+            if (j < H::IA) {
+                const bool in = left >= BK || (int) row.chunk * 8 < left;
+                copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, buffer((second ? pa2 : pa) + (uint64_t) (uint32_t) u * (BK * 2), left > 0 ? WINDOW : 0));
+            } else {   // the range ends with the last term's row
+                const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) s.n0 * 2 : 0;
+                copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, j - H::IA) * 1024), vb[j - H::IA],
+                       buffer((second ? pb2 : pb) + (uint64_t) (uint32_t) u * ((uint64_t) (uint32_t) a.K * (BK * 2)), bytes));
+            }
+        });
+#pragma unroll
+        for (int m = 0; m < H::FM; ++m) {
+            const int sr = (wm * H::FM + m) * 16 + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < H::FN; j += 2) {
+                const int c = s.n0 + (wn * H::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+                float v[8];
+                eight(acc[m][j], acc[m][j + 1], v);
+                if (sr < s.nm && c < a.K) { put8((T *) a.dx + (size_t) (s.slot + sr) * a.K + c, v); }
+            }
+        }
+    }
+}
 
-template <class T> hipError_t go_fwd(const MatmulArgs & a, hipStream_t st) {
-    const dim3 grid(ceil_div(a.n, TM) + (a.offsets ? a.n_exp : 0), ceil_div(a.R, TN));
-    if (a.act == ACT_SILU) { k_mm<T, ACT_SILU><<<grid, 256, 0, st>>>(a); }
-    else if (a.act == ACT_GELU) { k_mm<T, ACT_GELU><<<grid, 256, 0, st>>>(a); }
-    else { k_mm<T, ACT_NONE><<<grid, 256, 0, st>>>(a); }
+// ---------------------------------------------------------------- dW
+// one workgroup a tile: [second][expert][m-tile band][n][m]
+template <class T, bool F32, class H> __global__ void __launch_bounds__(H::threads) k_mm_dw(MatmulGradArgs a, int mt, int nt) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    const uint32_t lds = lds_addr(dyn);
+    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
+    const int all = (int) gridDim.x, b = (int) ((int64_t) all / 8 * (blockIdx.x % 8) + min((int) blockIdx.x % 8, all % 8)) + (int) blockIdx.x / 8;   // an XCD's share is a run
+    const int per = mt * nt, which = b / per, e = which % a.n_exp, in = b % per;
+    const bool second = which >= a.n_exp ? true : a.dW == nullptr;
+    const Span sp = span_of(a.offsets, a.n, e);
+    const int begin = uni(sp.begin), len = uni(sp.end) - begin, m0 = in % mt * H::BM, n0 = in / mt * H::BN;
+    const T * dz = (const T *) (second ? a.dz2 : a.dz) + (size_t) begin * a.R + m0;
+    uint32_t va[H::IA], vb[H::IB];
+#pragma unroll
+    for (int j = 0; j < H::IA; ++j) {
+        const int p = piece<H::AB, H::IA>(wave, j), c = ColLane<H::BM>::column(p);
+        va[j] = m0 + c < a.R ? (uint32_t) ColLane<H::BM>::term(p) * (uint32_t) a.R * 2 + (uint32_t) c * 2 : FAR;
+    }
+#pragma unroll
+    for (int j = 0; j < H::IB; ++j) {
+        const int p = piece<H::BB, H::IB>(wave, j), c = ColLane<H::BN>::column(p);
+        vb[j] = n0 + c < a.K ? (a.perm ? 0 : (uint32_t) ColLane<H::BN>::term(p) * (uint32_t) a.K * 2) + (uint32_t) c * 2 : FAR;
+    }
+    const uint64_t pa = uni64(dz), pb = uni64((const T *) a.x + (a.perm ? 0 : (size_t) begin * a.K) + n0);
+    f32x4 acc[H::FM][H::FN];
+    sums<T, true, true, H>(acc, lds, (len + BK - 1) / BK, [&](int j, uint32_t at, int t) {
+        const int left = len - t * BK;
+        if (j < H::IA) {
+            const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.R * 2 - (uint32_t) m0 * 2 : 0;
+            copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), va[j], buffer(pa + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.R * (BK * 2)), bytes));
+        } else {
+            const int p = piece<H::BB, H::IB>(wave, j - H::IA);
+            if (a.perm) {
+                const int k = ColLane<H::BN>::term(p);
+                uint32_t v = FAR;
+                if (k < left && vb[j - H::IA] != FAR) {
+                    const uint32_t r = pair_row((uint32_t) a.perm[begin + t * BK + k], a.magic);
+                    if (r < (uint32_t) a.xrows) { v = vb[j - H::IA] + r * (uint32_t) a.K * 2; }
+                }
+                copy16(at + H::AB + (uint32_t) (p * 1024), v, buffer(pb, WINDOW));
+            } else {
+                const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) n0 * 2 : 0;
+                copy16(at + H::AB + (uint32_t) (p * 1024), vb[j - H::IA], buffer(pb + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.K * (BK * 2)), bytes));
+            }
+        }
+    });
+#pragma unroll
+    for (int m = 0; m < H::FM; ++m) {
+        const int r = m0 + (wm * H::FM + m) * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < H::FN; j += 2) {
+            const int c = n0 + (wn * H::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+            float v[8];
+            eight(acc[m][j], acc[m][j + 1], v);
+            if (r >= a.R || c >= a.K) { continue; }
+            const size_t at = ((size_t) e * a.R + r) * a.K + c;
+            if (F32) { float * d = (float *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
+            else { T * d = (T *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
+        }
+    }
+}
+
+constexpr int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int CUS = 256;
+// m-tiles of `bm` slots at most
+int64_t most_tiles(int n, int n_exp, bool groups, int bm) { return ceil_div(n, bm) + (groups ? n_exp : 0); }
+unsigned grid_of(int64_t tiles, int per_cu) { return (unsigned) std::min<int64_t>(CUS * per_cu, ceil_div(tiles, 8) * 8); }
+
+template <class T, int ACT, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hipStream_t st, int per_cu) {
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_mm<T, ACT, GATED, H>, H::LDS)) { return e; }
+    const int64_t tiles = most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.R, GATED ? H::BN / 2 : H::BN);
+    k_mm<T, ACT, GATED, H><<<grid_of(tiles, per_cu), H::threads, H::LDS, st>>>(a);
     return hipGetLastError();
+}
+template <class T, int ACT, bool GATED> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
+    const int per = a.n / a.n_exp;
+    if (per > 96) { return fwd<T, ACT, GATED, Shape<T, false, false, 256, 256, 2, 2, 4>>(a, st, 1); }
+    return fwd<T, ACT, GATED, Shape<T, false, false, 64, 128, 2, 2, 4>>(a, st, 3);
+}
+template <class T> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
+    if (a.W2) { return a.act == ACT_SILU ? fwd<T, ACT_SILU, true>(a, st) : a.act == ACT_GELU ? fwd<T, ACT_GELU, true>(a, st) : fwd<T, ACT_NONE, true>(a, st); }
+    return a.act == ACT_SILU ? fwd<T, ACT_SILU, false>(a, st) : a.act == ACT_GELU ? fwd<T, ACT_GELU, false>(a, st) : fwd<T, ACT_NONE, false>(a, st);
+}
+template <class T, class H> hipError_t dx(const MatmulGradArgs & a, hipStream_t st, int per_cu) {
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_mm_dx<T, H>, H::LDS)) { return e; }
+    k_mm_dx<T, H><<<grid_of(most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.K, H::BN), per_cu), H::threads, H::LDS, st>>>(a);
+    return hipGetLastError();
+}
+template <class T> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
+    if (a.n / a.n_exp > 96) { return dx<T, Shape<T, false, true, 256, 256, 2, 2, 4>>(a, st, 1); }
+    return dx<T, Shape<T, false, true, 64, 128, 2, 2, 4>>(a, st, 3);
+}
+template <class T, bool F32, class H> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
+    static LdsLimit limit;
+    if (const hipError_t e = limit((const void *) k_mm_dw<T, F32, H>, H::LDS)) { return e; }
+    const int mt = (int) ceil_div(a.R, H::BM), nt = (int) ceil_div(a.K, H::BN);
+    k_mm_dw<T, F32, H><<<(unsigned) (mt * nt * a.n_exp * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0))), H::threads, H::LDS, st>>>(a, mt, nt);
+    return hipGetLastError();
+}
+template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
+    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, Shape<T, true, true, 256, 256, 2, 2, 4>>(a, st); }
+    return dw<T, F32, Shape<T, true, true, 128, 128, 2, 2, 4>>(a, st);
 }
 
 }  // namespace
 
-hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st) { return a.type == TYPE_BF16 ? go_fwd<__bf16>(a, st) : go_fwd<_Float16>(a, st); }
-hipError_t launch_matmul_dx(const MatmulGradArgs & a, hipStream_t st) {
-    const dim3 grid(ceil_div(a.n, TM) + (a.offsets ? a.n_exp : 0), ceil_div(a.K, TN));
-    if (a.type == TYPE_BF16) { k_mm_dx<__bf16><<<grid, 256, 0, st>>>(a); } else { k_mm_dx<_Float16><<<grid, 256, 0, st>>>(a); }
-    return hipGetLastError();
-}
+hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st) { return a.type == TYPE_BF16 ? fwd<__bf16>(a, st) : fwd<_Float16>(a, st); }
+hipError_t launch_matmul_dx(const MatmulGradArgs & a, hipStream_t st) { return a.type == TYPE_BF16 ? dx<__bf16>(a, st) : dx<_Float16>(a, st); }
 hipError_t launch_matmul_dw(const MatmulGradArgs & a, hipStream_t st) {
-    const dim3 grid(ceil_div(a.K, TN), ceil_div(a.R, TM), a.n_exp * (a.dW2 ? 2 : 1));
-    if (a.type == TYPE_BF16) { k_mm_dw<__bf16><<<grid, 256, 0, st>>>(a); } else { k_mm_dw<_Float16><<<grid, 256, 0, st>>>(a); }
-    return hipGetLastError();
+    if (a.dw_f32) { return a.type == TYPE_BF16 ? dw<__bf16, true>(a, st) : dw<_Float16, true>(a, st); }
+    return a.type == TYPE_BF16 ? dw<__bf16, false>(a, st) : dw<_Float16, false>(a, st);
 }
 
 }  // namespace lk
