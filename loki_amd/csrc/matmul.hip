@@ -140,46 +140,57 @@ template <class H> struct Frags { typename H::F a[H::FM], b[H::FN]; };
 // which of an operand's 1024-byte pieces copy i of wave w takes (fewer pieces than waves: some copy the same one)
 template <int BYTES, int I> __device__ __forceinline__ int piece(int w, int i) { return (w * I + i) % (BYTES / 1024); }
 
-// the loop over the sum's steps. issue(j, slot address, t): copy j (0 .. NI - 1) of step t; it is called for t past the end too, and then
-// copies nothing (zeros)
-template <class T, bool AC, bool BC, class H, class Issue>
-__device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, int steps, Issue issue) {
+// the loop over the sum's steps. begin(t) and then copy(j, slot address), j = 0 .. NI - 1, copy step t's operands; they are called for t past
+// the end too, and then copy nothing (zeros). A wave has its SIMD to itself and its products follow each other without a gap only if
+// between two of them (16 cycles each) go no more than three other instructions: the copies and reads are dealt out one to each two
+// products, in this order (the compiler's own puts them in clumps: 8192 x 16384 x 7168 @MIX@)
+template <class T, bool AC, bool BC, class H, class Begin, class Copy>
+__device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, int steps, Begin begin, Copy copy) {
     const int wave = uni(threadIdx.x >> 6), wm = wave / H::WN, wn = wave % H::WN;
     const RowLane row;
     constexpr int RA = AC ? (H::FM < 8 ? H::FM : 8) : 1, RB = BC ? (H::FN < 8 ? H::FN : 8) : 1;
     uint32_t ra[RA], rb[RB];   // a lane's addresses in a stage
     if constexpr (AC) {
 #pragma unroll
-        for (int j = 0; j < RA; ++j) { ra[j] = ColLane<H::BM>::read(wm * H::FM + j) + (uint32_t) (wm * H::FM + j) / 8 * 256; }
-    } else { ra[0] = row.read + (uint32_t) (wm * H::FM * 1024); }
+        for (int j = 0; j < RA; ++j) { ra[j] = ColLane<H::BM>::read(wm * H::FM + j) + (uint32_t) (wm * H::FM + j) / 8 * 256 + lds; }
+    } else { ra[0] = row.read + (uint32_t) (wm * H::FM * 1024) + lds; }
     if constexpr (BC) {
 #pragma unroll
-        for (int j = 0; j < RB; ++j) { rb[j] = ColLane<H::BN>::read(wn * H::FN + j) + (uint32_t) (wn * H::FN + j) / 8 * 256 + H::AB; }
-    } else { rb[0] = row.read + (uint32_t) (wn * H::FN * 1024) + H::AB; }
-    auto read_a = [&](Frags<H> & f, uint32_t at, int i) {
-        if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at + ra[i % RA] + (uint32_t) (i / RA * 256)); } else { f.a[i] = lds_row<T>(at + ra[0] + (uint32_t) (i * 1024)); }
+        for (int j = 0; j < RB; ++j) { rb[j] = ColLane<H::BN>::read(wn * H::FN + j) + (uint32_t) (wn * H::FN + j) / 8 * 256 + H::AB + lds; }
+    } else { rb[0] = row.read + (uint32_t) (wn * H::FN * 1024) + H::AB + lds; }
+    struct At { uint32_t a[RA], b[RB]; };
+    auto at_slot = [&](At & at, uint32_t off) {
+#pragma unroll
+        for (int j = 0; j < RA; ++j) { at.a[j] = ra[j] + off; __asm__ volatile("" : "+v"(at.a[j])); }   // (one register each, the fragments by immediate offsets)
+#pragma unroll
+        for (int j = 0; j < RB; ++j) { at.b[j] = rb[j] + off; __asm__ volatile("" : "+v"(at.b[j])); }
     };
-    auto read_b = [&](Frags<H> & f, uint32_t at, int i) {
-        if constexpr (BC) { f.b[i] = lds_col<T, H::BN>(at + rb[i % RB] + (uint32_t) (i / RB * 256)); } else { f.b[i] = lds_row<T>(at + rb[0] + (uint32_t) (i * 1024)); }
+    auto read_a = [&](Frags<H> & f, const At & at, int i) {
+        if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at.a[i % RA] + (uint32_t) (i / RA * 256)); } else { f.a[i] = lds_row<T>(at.a[0] + (uint32_t) (i * 1024)); }
     };
-    constexpr int MF = H::FM * H::FN, RD = H::FM + H::FN, G = MF < 8 ? MF : 8;
+    auto read_b = [&](Frags<H> & f, const At & at, int i) {
+        if constexpr (BC) { f.b[i] = lds_col<T, H::BN>(at.b[i % RB] + (uint32_t) (i / RB * 256)); } else { f.b[i] = lds_row<T>(at.b[0] + (uint32_t) (i * 1024)); }
+    };
+    constexpr int MF = H::FM * H::FN, RD = H::FM + H::FN, G = MF < 4 ? 1 : MF / 2, GR = G < 4 ? G : G - G / 4;   // the reads end a quarter early
     int slot = 0;   // of step t
     auto step = [&](Frags<H> & cur, Frags<H> & nxt, int t) {
         wait_copies<(H::S - 2) * H::NI>();   // step t + 1 is there, and this wave has read step t
         meet();                              // and everyone's: step t's place is free
         const uint32_t here = lds + (uint32_t) (slot * H::STAGE);
         slot = slot + 1 == H::S ? 0 : slot + 1;
-        const uint32_t next = lds + (uint32_t) (slot * H::STAGE);
+        begin(t + H::S);
+        At at;
+        at_slot(at, (uint32_t) (slot * H::STAGE));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < G; ++g) {
 #pragma unroll
-            for (int j = g * H::NI / G; j < (g + 1) * H::NI / G; ++j) { issue(j, here, t + H::S); }
-            constexpr int GR = G > 2 ? G - 2 : 1;   // the reads end two groups early
-#pragma unroll
-            for (int j = g * RD / GR; j < (g + 1) * RD / GR && j < RD; ++j) { if (j < H::FN) { read_b(nxt, next, j); } else { read_a(nxt, next, j - H::FN); } }
-#pragma unroll
             for (int j = g * MF / G; j < (g + 1) * MF / G; ++j) { acc[j / H::FN][j % H::FN] = mfma32(cur.b[j % H::FN], cur.a[j / H::FN], acc[j / H::FN][j % H::FN]); }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = g * RD / GR; j < (g + 1) * RD / GR && j < RD; ++j) { if (j < H::FN) { read_b(nxt, at, j); } else { read_a(nxt, at, j - H::FN); } }
+#pragma unroll
+            for (int j = g * H::NI / G; j < (g + 1) * H::NI / G; ++j) { copy(j, here); }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -189,16 +200,19 @@ __device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, i
         for (int j = 0; j < H::FN; ++j) { acc[i][j] = (f32x4) { 0.f, 0.f, 0.f, 0.f }; }
     }
     for (int t = 0; t < H::S; ++t) {
+        begin(t);
 #pragma unroll
-        for (int j = 0; j < H::NI; ++j) { issue(j, lds + (uint32_t) (t * H::STAGE), t); }
+        for (int j = 0; j < H::NI; ++j) { copy(j, lds + (uint32_t) (t * H::STAGE)); }
     }
     Frags<H> f0, f1;
     wait_copies<(H::S - 1) * H::NI>();
     meet();
+    At at;
+    at_slot(at, 0);
 #pragma unroll
-    for (int j = 0; j < H::FN; ++j) { read_b(f0, lds, j); }
+    for (int j = 0; j < H::FN; ++j) { read_b(f0, at, j); }
 #pragma unroll
-    for (int j = 0; j < H::FM; ++j) { read_a(f0, lds, j); }
+    for (int j = 0; j < H::FM; ++j) { read_a(f0, at, j); }
     for (int t = 0; t < steps; t += 2) {   // (an odd number of steps: one more, of zeros)
         step(f0, f1, t);
         step(f1, f0, t + 1);
@@ -278,15 +292,19 @@ template <class T, int ACT, bool GATED, class H> __global__ void __launch_bounds
         const size_t w0 = ((size_t) s.e * a.R + s.n0) * a.K;
         const uint64_t pa = uni64((const T *) a.x + (a.perm ? 0 : (size_t) s.slot * a.K)), pb = uni64((const T *) a.W + w0), pb2 = GATED ? uni64((const T *) a.W2 + w0) : 0;
         f32x4 acc[H::FM][H::FN];
-        sums<T, false, false, H>(acc, lds, (a.K + BK - 1) / BK, [&](int j, uint32_t at, int t) {
+        u32x4 ba, bb, bb2;
+        bool in = true;   // the lane's chunk of the step is there (a branch for the last step costs registers, this one instruction a copy)
+        sums<T, false, false, H>(acc, lds, (a.K + BK - 1) / BK, [&](int t) {
             const int left = a.K - t * BK;   // terms from this step on
             const uint32_t bytes = left > 0 ? WINDOW : 0;
-            const bool in = left >= BK || (int) row.chunk * 8 < left;
-            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, buffer(pa + (uint64_t) (uint32_t) t * (BK * 2), bytes)); }
+            const uint64_t off = (uint64_t) (uint32_t) t * (BK * 2);
+            ba = buffer(pa + off, bytes); bb = buffer(pb + off, bytes); bb2 = buffer(pb2 + off, bytes);
+            in = left >= BK || (int) row.chunk * 8 < left;
+        }, [&](int j, uint32_t at) {
+            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, ba); }
             else {
                 const int p = piece<H::BB, H::IB>(wave, j - H::IA);
-                const uint64_t b = GATED && p * 16 % (2 * WC) >= WC ? pb2 : pb;
-                copy16(at + H::AB + (uint32_t) (p * 1024), in ? vb[j - H::IA] : FAR, buffer(b + (uint64_t) (uint32_t) t * (BK * 2), bytes));
+                copy16(at + H::AB + (uint32_t) (p * 1024), in ? vb[j - H::IA] : FAR, GATED && p * 16 % (2 * WC) >= WC ? bb2 : bb);
             }
         });
         constexpr int FC = GATED ? H::FN / 2 : H::FN;
@@ -341,17 +359,18 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads) k_mm_d
         const uint64_t pa = uni64((const T *) a.dz + a0), pb = uni64((const T *) a.W + w0);
         const uint64_t pa2 = a.dz2 ? uni64((const T *) a.dz2 + a0) : 0, pb2 = a.dz2 ? uni64((const T *) a.W2 + w0) : 0;
         f32x4 acc[H::FM][H::FN];
-        sums<T, false, true, H>(acc, lds, steps, [&](int j, uint32_t at, int t) {
+        u32x4 ba, bb;
+        bool in = true;
+        sums<T, false, true, H>(acc, lds, steps, [&](int t) {
             const bool second = t >= half;   // (t < steps: the second pair's)
             const int u = second ? t - half : t, left = t < steps ? a.R - u * BK : 0;
-            if (j < H::IA) {
-                const bool in = left >= BK || (int) row.chunk * 8 < left;
-                copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, buffer((second ? pa2 : pa) + (uint64_t) (uint32_t) u * (BK * 2), left > 0 ? WINDOW : 0));
-            } else {   // the range ends with the last term's row
-                const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) s.n0 * 2 : 0;
-                copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, j - H::IA) * 1024), vb[j - H::IA],
-                       buffer((second ? pb2 : pb) + (uint64_t) (uint32_t) u * ((uint64_t) (uint32_t) a.K * (BK * 2)), bytes));
-            }
+            ba = buffer((second ? pa2 : pa) + (uint64_t) (uint32_t) u * (BK * 2), left > 0 ? WINDOW : 0);
+            bb = buffer((second ? pb2 : pb) + (uint64_t) (uint32_t) u * ((uint64_t) (uint32_t) a.K * (BK * 2)),   // the range ends with the last term's row
+                        left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) s.n0 * 2 : 0);
+            in = left >= BK || (int) row.chunk * 8 < left;
+        }, [&](int j, uint32_t at) {
+            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, ba); }
+            else { copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, j - H::IA) * 1024), vb[j - H::IA], bb); }
         });
 #pragma unroll
         for (int m = 0; m < H::FM; ++m) {
@@ -369,7 +388,7 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads) k_mm_d
 
 // ---------------------------------------------------------------- dW
 // one workgroup a tile: [second][expert][m-tile band][n][m]
-template <class T, bool F32, class H> __global__ void __launch_bounds__(H::threads) k_mm_dw(MatmulGradArgs a, int mt, int nt) {
+template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads) k_mm_dw(MatmulGradArgs a, int mt, int nt) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     const uint32_t lds = lds_addr(dyn);
     const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
@@ -388,29 +407,55 @@ template <class T, bool F32, class H> __global__ void __launch_bounds__(H::threa
 #pragma unroll
     for (int j = 0; j < H::IB; ++j) {
         const int p = piece<H::BB, H::IB>(wave, j), c = ColLane<H::BN>::column(p);
-        vb[j] = n0 + c < a.K ? (a.perm ? 0 : (uint32_t) ColLane<H::BN>::term(p) * (uint32_t) a.K * 2) + (uint32_t) c * 2 : FAR;
+        vb[j] = n0 + c < a.K ? (PERM ? 0 : (uint32_t) ColLane<H::BN>::term(p) * (uint32_t) a.K * 2) + (uint32_t) c * 2 : FAR;
     }
-    const uint64_t pa = uni64(dz), pb = uni64((const T *) a.x + (a.perm ? 0 : (size_t) begin * a.K) + n0);
+    const uint64_t pa = uni64(dz), pb = uni64((const T *) a.x + (PERM ? 0 : (size_t) begin * a.K) + n0);
     f32x4 acc[H::FM][H::FN];
-    sums<T, true, true, H>(acc, lds, (len + BK - 1) / BK, [&](int j, uint32_t at, int t) {
-        const int left = len - t * BK;
-        if (j < H::IA) {
-            const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.R * 2 - (uint32_t) m0 * 2 : 0;
-            copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), va[j], buffer(pa + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.R * (BK * 2)), bytes));
-        } else {
-            const int p = piece<H::BB, H::IB>(wave, j - H::IA);
-            if (a.perm) {
-                const int k = ColLane<H::BN>::term(p);
-                uint32_t v = FAR;
-                if (k < left && vb[j - H::IA] != FAR) {
-                    const uint32_t r = pair_row((uint32_t) a.perm[begin + t * BK + k], a.magic);
-                    if (r < (uint32_t) a.xrows) { v = vb[j - H::IA] + r * (uint32_t) a.K * 2; }
-                }
-                copy16(at + H::AB + (uint32_t) (p * 1024), v, buffer(pb, WINDOW));
-            } else {
-                const uint32_t bytes = left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) n0 * 2 : 0;
-                copy16(at + H::AB + (uint32_t) (p * 1024), vb[j - H::IA], buffer(pb + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.K * (BK * 2)), bytes));
+    u32x4 ba, bb;
+    constexpr int Q = ColLane<H::BN>::TERMS, NR = PERM ? H::IB * Q : 1;
+    int pair[NR];        // PERM: the next step's pairs of this wave's copies, by scalar loads
+    uint32_t off[NR];    // and the step's rows, as offsets
+    auto load_pairs = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < H::IB; ++j) {
+#pragma unroll
+            for (int q = 0; q < Q; ++q) {   // (past the end: its last one again, or any)
+                const int i = min(t * BK + piece<H::BB, H::IB>(wave, j) * Q + q, len - 1);
+                pair[j * Q + q] = ((const LK_CONST int *) a.perm)[uni(max(begin + i, 0))];
             }
+        }
+    };
+    if constexpr (PERM) { load_pairs(0); }
+    sums<T, true, true, H>(acc, lds, (len + BK - 1) / BK, [&](int t) {
+        const int left = len - t * BK;
+        ba = buffer(pa + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.R * (BK * 2)), left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.R * 2 - (uint32_t) m0 * 2 : 0);
+        if constexpr (PERM) {
+            bb = buffer(pb, WINDOW);
+#pragma unroll
+            for (int j = 0; j < H::IB; ++j) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q) {
+                    const uint32_t r = pair_row((uint32_t) pair[j * Q + q], a.magic);
+                    off[j * Q + q] = piece<H::BB, H::IB>(wave, j) * Q + q < left && r < (uint32_t) a.xrows ? r * (uint32_t) a.K * 2 : WINDOW;   // (and a column: still outside)
+                }
+            }
+            load_pairs(t + 1);
+        } else {
+            bb = buffer(pb + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.K * (BK * 2)), left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) n0 * 2 : 0);
+        }
+    }, [&](int j, uint32_t at) {
+        if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), va[j], ba); }
+        else {
+            const int i = j - H::IA;
+            uint32_t v = vb[i];
+            if constexpr (PERM) {
+                const int q = lane / (64 / Q);
+                uint32_t o = off[i * Q];
+#pragma unroll
+                for (int u = 1; u < Q; ++u) { o = q == u ? off[i * Q + u] : o; }
+                v = v == FAR ? FAR : v + o;
+            }
+            copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, i) * 1024), v, bb);
         }
     });
 #pragma unroll
@@ -461,17 +506,18 @@ template <class T> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
     if (a.n / a.n_exp > 96) { return dx<T, Shape<T, false, true, 256, 256, 2, 2, 4>>(a, st, 1); }
     return dx<T, Shape<T, false, true, 64, 128, 2, 2, 4>>(a, st, 3);
 }
-template <class T, bool F32, class H> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
+template <class T, bool F32, bool PERM, class H> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
     static LdsLimit limit;
-    if (const hipError_t e = limit((const void *) k_mm_dw<T, F32, H>, H::LDS)) { return e; }
+    if (const hipError_t e = limit((const void *) k_mm_dw<T, F32, PERM, H>, H::LDS)) { return e; }
     const int mt = (int) ceil_div(a.R, H::BM), nt = (int) ceil_div(a.K, H::BN);
-    k_mm_dw<T, F32, H><<<(unsigned) (mt * nt * a.n_exp * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0))), H::threads, H::LDS, st>>>(a, mt, nt);
+    k_mm_dw<T, F32, PERM, H><<<(unsigned) (mt * nt * a.n_exp * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0))), H::threads, H::LDS, st>>>(a, mt, nt);
     return hipGetLastError();
 }
-template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
-    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, Shape<T, true, true, 256, 256, 2, 2, 4>>(a, st); }
-    return dw<T, F32, Shape<T, true, true, 128, 128, 2, 2, 4>>(a, st);
+template <class T, bool F32, bool PERM> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
+    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, PERM, Shape<T, true, true, 256, 256, 2, 2, 4>>(a, st); }
+    return dw<T, F32, PERM, Shape<T, true, true, 128, 128, 2, 2, 4>>(a, st);
 }
+template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) { return a.perm && a.n > 0 ? dw<T, F32, true>(a, st) : dw<T, F32, false>(a, st); }
 
 }  // namespace
 
