@@ -11,8 +11,9 @@
 // steps ahead; what lies outside an operand is not read and arrives as 0 (the buffer's range), so that no row of another expert, infinite
 // or not, takes part. While a step's products run, the next step's operands go from LDS into the other set of registers. One barrier a step.
 //
-// In LDS an operand whose terms are next to each other in memory ("row" operand) has 64 bytes a row, chunk c of 16 at c ^ (row / 4 % 4): a
-// ds_read_b128 takes its 16 lanes of a pass from different bank quads. One whose terms are rows of memory ("col" operand) has a row a
+// In LDS an operand whose terms are next to each other in memory ("row" operand) has 64 bytes a row, chunk c of 16 at c ^ f(row / 4 % 4), f
+// = 0, 2, 3, 1: a ds_read_b128 is served in passes of 16 lanes (0-3, 12-15, 20-23, 24-27; 4-11, 16-19, 28-31; and 32 on), and so each pass
+// has 16 different bank quads (with f the identity half of the cycles of the LDS were conflicts). One whose terms are rows of memory ("col" operand) has a row a
 // term, segments of 32 bytes at segment ^ (term % 4 + term / 8 % 2 * 4), and is transposed by ds_read_b64_tr_b16: 16 lanes read 4 terms x 16
 // columns and each gets its column's 4.
 #include "matmul_device.h"
@@ -24,11 +25,18 @@ enum { FWD, DX, DW };
 constexpr int BK = 32;
 constexpr uint32_t FAR = 0xFFFF0000u, WINDOW = 0xFFFE0000u;   // an offset outside every buffer; the largest range of one
 
-// one step's copy instruction: 16 bytes a lane to m0 + 16 * lane; nothing of it is known to the compiler, which would wait for all
-// copies before each ds_read_b64_tr_b16: the waits below are counted by hand
-__device__ __forceinline__ void copy16(uint32_t lds, uint32_t voff, u32x4 rsrc) {
+// one step's copy instruction: 16 bytes a lane to m0 + 16 * lane; nothing of it is known to the compiler, which would wait for all copies
+// before each ds_read_b64_tr_b16: the waits below are counted by hand. m0 is set at least one instruction before.
+__device__ __forceinline__ uint32_t copy_to(uint32_t lds, uint32_t off) {
+    uint32_t m = 0;
 #if defined(__HIP_DEVICE_COMPILE__)
-    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(voff), "s"(rsrc) : "memory");
+    __asm__ volatile("s_add_u32 %0, %1, %2" : "={m0}"(m) : "s"(lds), "s"(off) : "scc");
+#endif
+    return m;
+}
+__device__ __forceinline__ void copy16(uint32_t m, uint32_t voff, u32x4 rsrc) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __asm__ volatile("buffer_load_dwordx4 %1, %2, 0 offen lds" :: "{m0}"(m), "v"(voff), "s"(rsrc) : "memory");
 #endif
 }
 template <int N> __device__ __forceinline__ void wait_copies() {   // all but the last N, and all LDS reads
@@ -51,9 +59,10 @@ struct RowLane {
     uint32_t chunk, read;
     __device__ __forceinline__ RowLane() {
         const int l = lane_id();
-        chunk = (uint32_t) ((l & 3) ^ ((l >> 4) & 3));
-        read = (uint32_t) ((l & 15) * 64 + (((l >> 4) ^ ((l >> 2) & 3)) * 16));
+        chunk = (uint32_t) ((l & 3) ^ swz((l >> 4) & 3));
+        read = (uint32_t) ((l & 15) * 64 + (((l >> 4) ^ swz((l >> 2) & 3)) * 16));
     }
+    __device__ __forceinline__ static int swz(int b) { return (((b ^ (b >> 1)) & 1) << 1) | (b >> 1); }
 };
 // a col operand's: of an instruction's 1024 bytes = 512 / COLS terms
 template <int COLS> struct ColLane {
@@ -140,15 +149,17 @@ template <class H> struct Frags { typename H::F a[H::FM], b[H::FN]; };
 // which of an operand's 1024-byte pieces copy i of wave w takes (fewer pieces than waves: some copy the same one)
 template <int BYTES, int I> __device__ __forceinline__ int piece(int w, int i) { return (w * I + i) % (BYTES / 1024); }
 
-// the loop over the sum's steps. begin(t) and then copy(j, slot address), j = 0 .. NI - 1, copy step t's operands; they are called for t past
-// the end too, and then copy nothing (zeros). A wave has its SIMD to itself and its products follow each other without a gap only if
-// between two of them (16 cycles each) go no more than three other instructions: the copies and reads are dealt out one to each two
-// products, in this order (the compiler's own puts them in clumps: 8192 x 16384 x 7168 @MIX@)
-template <class T, bool AC, bool BC, class H, class Begin, class Copy>
-__device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, int steps, Begin begin, Copy copy) {
+// the loop over the sum's steps. begin(t) and then set(j, slot address) and copy(j), j = 0 .. NI - 1, copy step t's operands; they are called for
+// t past the end too, and then copy nothing (zeros).
+// A wave has its SIMD to itself, and its products (16 cycles each) follow each other without a gap only if no more than three other
+// instructions go between two of them: the copies and reads are dealt out among the products in this order, and what the next step needs
+// in scalars and addresses is made among the last ones. The barrier comes after the step's first products, whose operands are in registers.
+template <class T, bool AC, bool BC, class H, class Begin, class Set, class Copy>
+__device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, int steps, Begin begin, Set set, Copy copy) {
     const int wave = uni(threadIdx.x >> 6), wm = wave / H::WN, wn = wave % H::WN;
     const RowLane row;
     constexpr int RA = AC ? (H::FM < 8 ? H::FM : 8) : 1, RB = BC ? (H::FN < 8 ? H::FN : 8) : 1;
+    static_assert(!AC || (H::FM & (H::FM - 1)) == 0, "addresses of a col operand"); static_assert(!BC || (H::FN & (H::FN - 1)) == 0, "addresses of a col operand");
     uint32_t ra[RA], rb[RB];   // a lane's addresses in a stage
     if constexpr (AC) {
 #pragma unroll
@@ -158,41 +169,52 @@ __device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, i
 #pragma unroll
         for (int j = 0; j < RB; ++j) { rb[j] = ColLane<H::BN>::read(wn * H::FN + j) + (uint32_t) (wn * H::FN + j) / 8 * 256 + H::AB + lds; }
     } else { rb[0] = row.read + (uint32_t) (wn * H::FN * 1024) + H::AB + lds; }
-    struct At { uint32_t a[RA], b[RB]; };
-    auto at_slot = [&](At & at, uint32_t off) {
+    struct At { uint32_t a[RA], b[RB]; } at;
+    auto at_slot = [&](uint32_t off) {
 #pragma unroll
-        for (int j = 0; j < RA; ++j) { at.a[j] = ra[j] + off; __asm__ volatile("" : "+v"(at.a[j])); }   // (one register each, the fragments by immediate offsets)
+        for (int j = 0; j < RA; ++j) { at.a[j] = ra[j] + off; __asm__("" : "+v"(at.a[j])); }   // (one register each, the fragments by immediate offsets)
 #pragma unroll
-        for (int j = 0; j < RB; ++j) { at.b[j] = rb[j] + off; __asm__ volatile("" : "+v"(at.b[j])); }
+        for (int j = 0; j < RB; ++j) { at.b[j] = rb[j] + off; __asm__("" : "+v"(at.b[j])); }
     };
-    auto read_a = [&](Frags<H> & f, const At & at, int i) {
+    auto read_a = [&](Frags<H> & f, int i) {
         if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at.a[i % RA] + (uint32_t) (i / RA * 256)); } else { f.a[i] = lds_row<T>(at.a[0] + (uint32_t) (i * 1024)); }
     };
-    auto read_b = [&](Frags<H> & f, const At & at, int i) {
+    auto read_b = [&](Frags<H> & f, int i) {
         if constexpr (BC) { f.b[i] = lds_col<T, H::BN>(at.b[i % RB] + (uint32_t) (i / RB * 256)); } else { f.b[i] = lds_row<T>(at.b[0] + (uint32_t) (i * 1024)); }
     };
-    constexpr int MF = H::FM * H::FN, RD = H::FM + H::FN, G = MF < 4 ? 1 : MF / 2, GR = G < 4 ? G : G - G / 4;   // the reads end a quarter early
-    int slot = 0;   // of step t
+    // G groups of products; the first has none of the rest, then come RG groups with reads and copies, then those with the next step's set-up
+    constexpr int MF = H::FM * H::FN, RD = H::FM + H::FN, G = MF, RG = G - G / 4 - 1;
+    static_assert(RG > H::NI, "a group between two copies");
+    int slot = 0;            // of step t
+    uint32_t here = lds;     // its place
     auto step = [&](Frags<H> & cur, Frags<H> & nxt, int t) {
-        wait_copies<(H::S - 2) * H::NI>();   // step t + 1 is there, and this wave has read step t
-        meet();                              // and everyone's: step t's place is free
-        const uint32_t here = lds + (uint32_t) (slot * H::STAGE);
-        slot = slot + 1 == H::S ? 0 : slot + 1;
-        begin(t + H::S);
-        At at;
-        at_slot(at, (uint32_t) (slot * H::STAGE));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g <= RG; ++g) {
 #pragma unroll
             for (int j = g * MF / G; j < (g + 1) * MF / G; ++j) { acc[j / H::FN][j % H::FN] = mfma32(cur.b[j % H::FN], cur.a[j / H::FN], acc[j / H::FN][j % H::FN]); }
             __builtin_amdgcn_sched_barrier(0);
+            if (g == 0) {
+                wait_copies<(H::S - 2) * H::NI>();   // step t + 1 is there, and this wave has read step t
+                meet();                              // and everyone's: step t's place is free
+            } else {
 #pragma unroll
-            for (int j = g * RD / GR; j < (g + 1) * RD / GR && j < RD; ++j) { if (j < H::FN) { read_b(nxt, at, j); } else { read_a(nxt, at, j - H::FN); } }
+                for (int j = (g - 1) * RD / RG; j < g * RD / RG; ++j) { if (j < H::FN) { read_b(nxt, j); } else { read_a(nxt, j - H::FN); } }
 #pragma unroll
-            for (int j = g * H::NI / G; j < (g + 1) * H::NI / G; ++j) { copy(j, here); }
+                for (int j = 0; j < H::NI; ++j) {   // copy j: its address, a group later the copy
+                    if ((j + 1) * (RG - 1) / H::NI == g) { set(j, here); }
+                    if ((j + 1) * (RG - 1) / H::NI == g - 1) { copy(j); }
+                }
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+        slot = slot + 1 == H::S ? 0 : slot + 1;
+        here = lds + (uint32_t) (slot * H::STAGE);
+        at_slot((uint32_t) ((slot + 1 == H::S ? 0 : slot + 1) * H::STAGE));
+        begin(t + H::S + 1);
+#pragma unroll
+        for (int j = (RG + 1) * MF / G; j < MF; ++j) { acc[j / H::FN][j % H::FN] = mfma32(cur.b[j % H::FN], cur.a[j / H::FN], acc[j / H::FN][j % H::FN]); }
+        __builtin_amdgcn_sched_barrier(0);
     };
 #pragma unroll
     for (int i = 0; i < H::FM; ++i) {
@@ -202,17 +224,18 @@ __device__ __forceinline__ void sums(f32x4 (&acc)[H::FM][H::FN], uint32_t lds, i
     for (int t = 0; t < H::S; ++t) {
         begin(t);
 #pragma unroll
-        for (int j = 0; j < H::NI; ++j) { copy(j, lds + (uint32_t) (t * H::STAGE)); }
+        for (int j = 0; j < H::NI; ++j) { set(j, lds + (uint32_t) (t * H::STAGE)); __asm__ volatile("s_nop 0"); copy(j); }
     }
     Frags<H> f0, f1;
     wait_copies<(H::S - 1) * H::NI>();
     meet();
-    At at;
-    at_slot(at, 0);
+    at_slot(0);
 #pragma unroll
-    for (int j = 0; j < H::FN; ++j) { read_b(f0, at, j); }
+    for (int j = 0; j < H::FN; ++j) { read_b(f0, j); }
 #pragma unroll
-    for (int j = 0; j < H::FM; ++j) { read_a(f0, at, j); }
+    for (int j = 0; j < H::FM; ++j) { read_a(f0, j); }
+    at_slot(H::STAGE);
+    begin(H::S);
     for (int t = 0; t < steps; t += 2) {   // (an odd number of steps: one more, of zeros)
         step(f0, f1, t);
         step(f1, f0, t + 1);
@@ -293,6 +316,7 @@ template <class T, int ACT, bool GATED, class H> __global__ void __launch_bounds
         const uint64_t pa = uni64((const T *) a.x + (a.perm ? 0 : (size_t) s.slot * a.K)), pb = uni64((const T *) a.W + w0), pb2 = GATED ? uni64((const T *) a.W2 + w0) : 0;
         f32x4 acc[H::FM][H::FN];
         u32x4 ba, bb, bb2;
+        uint32_t dst, voff;
         bool in = true;   // the lane's chunk of the step is there (a branch for the last step costs registers, this one instruction a copy)
         sums<T, false, false, H>(acc, lds, (a.K + BK - 1) / BK, [&](int t) {
             const int left = a.K - t * BK;   // terms from this step on
@@ -301,12 +325,10 @@ template <class T, int ACT, bool GATED, class H> __global__ void __launch_bounds
             ba = buffer(pa + off, bytes); bb = buffer(pb + off, bytes); bb2 = buffer(pb2 + off, bytes);
             in = left >= BK || (int) row.chunk * 8 < left;
         }, [&](int j, uint32_t at) {
-            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, ba); }
-            else {
-                const int p = piece<H::BB, H::IB>(wave, j - H::IA);
-                copy16(at + H::AB + (uint32_t) (p * 1024), in ? vb[j - H::IA] : FAR, GATED && p * 16 % (2 * WC) >= WC ? bb2 : bb);
-            }
-        });
+            dst = copy_to(at, j < H::IA ? (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024) : (uint32_t) (H::AB + piece<H::BB, H::IB>(wave, j - H::IA) * 1024));
+            voff = in ? j < H::IA ? va[j] : vb[j - H::IA] : FAR;
+            __asm__ volatile("" : "+v"(voff));
+        }, [&](int j) { copy16(dst, voff, j < H::IA ? ba : GATED && piece<H::BB, H::IB>(wave, j - H::IA) * 16 % (2 * WC) >= WC ? bb2 : bb); });
         constexpr int FC = GATED ? H::FN / 2 : H::FN;
 #pragma unroll
         for (int m = 0; m < H::FM; ++m) {
@@ -360,6 +382,7 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads) k_mm_d
         const uint64_t pa2 = a.dz2 ? uni64((const T *) a.dz2 + a0) : 0, pb2 = a.dz2 ? uni64((const T *) a.W2 + w0) : 0;
         f32x4 acc[H::FM][H::FN];
         u32x4 ba, bb;
+        uint32_t dst, voff;
         bool in = true;
         sums<T, false, true, H>(acc, lds, steps, [&](int t) {
             const bool second = t >= half;   // (t < steps: the second pair's)
@@ -369,9 +392,10 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads) k_mm_d
                         left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) s.n0 * 2 : 0);
             in = left >= BK || (int) row.chunk * 8 < left;
         }, [&](int j, uint32_t at) {
-            if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), in ? va[j] : FAR, ba); }
-            else { copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, j - H::IA) * 1024), vb[j - H::IA], bb); }
-        });
+            dst = copy_to(at, j < H::IA ? (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024) : (uint32_t) (H::AB + piece<H::BB, H::IB>(wave, j - H::IA) * 1024));
+            voff = j < H::IA ? in ? va[j] : FAR : vb[j - H::IA];
+            __asm__ volatile("" : "+v"(voff));
+        }, [&](int j) { copy16(dst, voff, j < H::IA ? ba : bb); });
 #pragma unroll
         for (int m = 0; m < H::FM; ++m) {
             const int sr = (wm * H::FM + m) * 16 + (lane & 15);
@@ -412,6 +436,7 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
     const uint64_t pa = uni64(dz), pb = uni64((const T *) a.x + (PERM ? 0 : (size_t) begin * a.K) + n0);
     f32x4 acc[H::FM][H::FN];
     u32x4 ba, bb;
+    uint32_t dst, voff;
     constexpr int Q = ColLane<H::BN>::TERMS, NR = PERM ? H::IB * Q : 1;
     int pair[NR];        // PERM: the next step's pairs of this wave's copies, by scalar loads
     uint32_t off[NR];    // and the step's rows, as offsets
@@ -426,7 +451,7 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
         }
     };
     if constexpr (PERM) { load_pairs(0); }
-    sums<T, true, true, H>(acc, lds, (len + BK - 1) / BK, [&](int t) {
+    sums<T, true, true, H>(acc, lds, (len + BK - 1) / BK, [&](int t) {   // (what lies behind the last slot is outside the buffer)
         const int left = len - t * BK;
         ba = buffer(pa + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.R * (BK * 2)), left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.R * 2 - (uint32_t) m0 * 2 : 0);
         if constexpr (PERM) {
@@ -444,20 +469,21 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
             bb = buffer(pb + (uint64_t) (uint32_t) t * ((uint64_t) (uint32_t) a.K * (BK * 2)), left > 0 ? (uint32_t) min(left, BK) * (uint32_t) a.K * 2 - (uint32_t) n0 * 2 : 0);
         }
     }, [&](int j, uint32_t at) {
-        if (j < H::IA) { copy16(at + (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024), va[j], ba); }
+        dst = copy_to(at, j < H::IA ? (uint32_t) (piece<H::AB, H::IA>(wave, j) * 1024) : (uint32_t) (H::AB + piece<H::BB, H::IB>(wave, j - H::IA) * 1024));
+        if (j < H::IA) { voff = va[j]; }
         else {
             const int i = j - H::IA;
-            uint32_t v = vb[i];
+            voff = vb[i];
             if constexpr (PERM) {
                 const int q = lane / (64 / Q);
                 uint32_t o = off[i * Q];
 #pragma unroll
                 for (int u = 1; u < Q; ++u) { o = q == u ? off[i * Q + u] : o; }
-                v = v == FAR ? FAR : v + o;
+                voff = voff == FAR ? FAR : voff + o;
             }
-            copy16(at + H::AB + (uint32_t) (piece<H::BB, H::IB>(wave, i) * 1024), v, bb);
         }
-    });
+        __asm__ volatile("" : "+v"(voff));
+    }, [&](int j) { copy16(dst, voff, j < H::IA ? ba : bb); });
 #pragma unroll
     for (int m = 0; m < H::FM; ++m) {
         const int r = m0 + (wm * H::FM + m) * 16 + (lane & 15);
