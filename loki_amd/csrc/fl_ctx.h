@@ -96,6 +96,7 @@ struct FLCtx {
     DBuf<double> rpart;                        // the matrix-core router's parts [router_parts][n][n_exp]
     DBuf<int> dscr;                            // the multi-workgroup dispatch's per-round counts and bases
     KeptBuf bal, rg, q4, mm;                   // fl_balance_loss_dev's partial sums, fl_route_grad_dev's operands, Q4_K's row sums, the 16-bit products' partial sums
+    int * mm_queue = nullptr;                  // the 16-bit products' tile counters (16 ints, 0 between launches)
     size_t h2d_zc = 0, h2d_ce = 0; int h2d_said = 0;   // fl_h2d bytes by kernel (mapped pinned) / by copy engine
     // fl_ffn_begin's event pairs (recorded, not yet folded into ms_ffn by fl_gpu_ms) and the reusable ones
     std::vector<std::pair<hipEvent_t, hipEvent_t>> ffn_ev_pending, ffn_ev_free; double ms_ffn = 0.0;

@@ -117,6 +117,10 @@ extern "C" FLCtx * fl_init(int kvp, int sc_cap) {
     }
     (void) decode_ready(c);      // its set-up (attributes, XCD probe) here, not in a call that must not allocate
     (void) decode1_ready(c);
+    CK(hipMalloc((void **) &c->mm_queue, 64));
+    k_zero16<<<1, 64, 0, c->st>>>(reinterpret_cast<uint4 *>(c->mm_queue), 4);
+    CK(hipGetLastError());
+    CK(hipStreamSynchronize(c->st));
     return c;
 }
 
@@ -131,7 +135,8 @@ extern "C" void fl_free(FLCtx * c) {
     c->tab.release(); c->derr.release(); c->dlogit.release(); c->dth.release(); c->dto.release(); c->dxq.release();
     c->ptab.release(); c->pcols.release(); c->pcolsk.release(); c->pncols.release(); c->xh.release(); c->hh.release();
     c->ksg.release(); c->ksu.release(); c->rcnt.release(); c->rpart.release(); c->dscr.release();
-    c->bal.release(); c->rg.release(); c->q4.release();
+    c->bal.release(); c->rg.release(); c->q4.release(); c->mm.release();
+    if (c->mm_queue) { (void) hipFree(c->mm_queue); }
     for (auto & v : c->ev_free) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto & v : c->ev_pending) { for (auto e : v) { (void) hipEventDestroy(e); } }
     for (auto * l : { &c->ffn_ev_pending, &c->ffn_ev_free, &c->moe_ev_pending, &c->moe_ev_free }) { for (auto & e : *l) { (void) hipEventDestroy(e.first); (void) hipEventDestroy(e.second); } }
@@ -461,6 +466,7 @@ extern "C" int fl_matmul_dev(FLCtx * c, int type, int act, const void * x, const
     }
     a.type = type; a.act = act; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.x = x; a.W = W; a.W2 = W2; a.bias = bias; a.residual = residual; a.y = y; a.z = z; a.z2 = z2; a.y_f32 = y_type == FL_F32;
+    a.queue = c->mm_queue; a.shape = mm_shape_of(n, n_exp, W2 ? 2 * R : R);
     TRY(c, launch_matmul(a, c->st));
     return FL_OK;
 }
@@ -488,6 +494,7 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
     }
     a.type = type; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.dz = dz; a.dz2 = dz2; a.x = x; a.W = W; a.W2 = W2; a.dx = dx; a.dW = dW; a.dW2 = dW2; a.dw_f32 = dw_type == FL_F32; a.accumulate = accumulate ? 1 : 0;
+    a.queue = c->mm_queue; a.shape = mm_shape_of(n, n_exp, K);
     if (dx && n > 0) { TRY(c, launch_matmul_dx(a, c->st)); }
     if (dW || dW2) { TRY(c, launch_matmul_dw(a, c->st)); }   // (no rows: 0, or it stays)
     return FL_OK;

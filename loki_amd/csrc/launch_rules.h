@@ -101,4 +101,8 @@ constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {
     return { splits > 1 ? splits : 1, parts > 1 ? parts : 1 };
 }
 
+// ---------------------------------------------------------------- 16-bit products (matmul.hip)
+enum { MM_SMALL, MM_WIDE, MM_LARGE };
+constexpr int mm_shape_of(int n, int n_exp, int cols) { return n / n_exp > 96 ? MM_LARGE : MM_SMALL; }
+
 }  // namespace lk

@@ -137,33 +137,53 @@ __device__ __forceinline__ Spot spot_of(const Tiles & t, const int * offsets, in
 }
 
 // ---------------------------------------------------------------- a tile's sums
-// NW = WM * WN waves, a wave BM / WM x BN / WN. A: m side, B: n side. PER_CU workgroups a CU
-template <int BM_, int BN_, int WM_, int WN_, int SA_, int SB_, int PER_CU_> struct Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, SA = SA_, SB = SB_, PER_CU = PER_CU_, NW = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
+// 4 waves. A: m side, B: n side. PER_CU workgroups a CU
+template <int BM_, int BN_, int SA_, int SB_, int PER_CU_> struct Shape {
+    static constexpr int BM = BM_, BN = BN_, SA = SA_, SB = SB_, PER_CU = PER_CU_, NW = 4;
     static constexpr int AB = BM * BK * 2, BB = BN * BK * 2, LB = SA * AB, LDS = LB + SB * BB;   // a round's bytes; B's place
     static constexpr int CA = AB / 1024 < NW ? 1 : AB / 1024 / NW, CB = BB / 1024 < NW ? 1 : BB / 1024 / NW;   // copies a wave and round
     static constexpr int threads = 64 * NW;
 };
-template <class T, class H> struct Frags { V8<T> a[H::FM], b[H::FN]; };
+// how the waves share a tile's first ROWS rows: WM x 4 / WM of them, FM x FN fragments of 16 x 16 each. A tile that is not full takes the one
+// of as few rows as hold it (an expert's last tile: 256 experts of 256 slots on average leave a third of their rows empty)
+template <class H, int ROWS_, int WM_> struct Waves {
+    static constexpr int ROWS = ROWS_, WM = WM_, WN = H::NW / WM, FM = ROWS / WM / 16, FN = H::BN / WN / 16;
+};
+template <class T, class V> struct Frags { V8<T> a[V::FM], b[V::FN]; };
 
 // which of an operand's 1024-byte pieces copy i of wave w takes (fewer pieces than waves: some copy the same one)
 template <int BYTES, int I> __device__ __forceinline__ int piece(int w, int i) { return (w * I + i) % (BYTES / 1024); }
 
 // The loop over the sum's rounds. `c` copies: c.begin_a(d) and then c.set_a(j, address), c.copy_a(j) for j = 0 .. CA - 1 copy A's round d, _b
-// B's; they are called for rounds past the end too, and then copy nothing (zeros). start() is called before, on its own, so that the
-// first copies can be out while the last tile's results are written.
+// B's; they are called for rounds past the end too, and then copy nothing (zeros). start() comes before.
 // A wave has its SIMD to itself, and its products (16 cycles each) follow each other without a gap only if no more than three other
 // instructions go between two of them: the copies and reads are dealt out among the products in this order, and what comes next is
 // prepared in scalars and addresses among the last ones. In a round's first half A of round d + SA - 1 is copied, in its second B of round
 // d + SB, behind the barrier that comes after the half's first product: it says that round d + 1 is there and that round d's last half is
 // in registers.
-template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
-    static constexpr int FM = H::FM, FN = H::FN, RA = AC ? (FM < 8 ? FM : 8) : 2, RB = BC ? (FN < 8 ? FN : 8) : 2;
+// a tile's first copies, before run(): A of rounds 0 .. SA - 2, B of 0 .. SB - 1
+template <class H, class Copies> __device__ __forceinline__ void start(Copies & c, uint32_t lds) {
+#pragma unroll
+    for (int d = 0; d < (H::SA - 1 > H::SB ? H::SA - 1 : H::SB); ++d) {
+        if (d < H::SA - 1) {
+            c.begin_a(d);
+#pragma unroll
+            for (int j = 0; j < H::CA; ++j) { c.set_a(j, lds + (uint32_t) (d * H::AB)); c.copy_a(j); }
+        }
+        if (d < H::SB) {
+            c.begin_b(d);
+#pragma unroll
+            for (int j = 0; j < H::CB; ++j) { c.set_b(j, lds + (uint32_t) (H::LB + d * H::BB)); c.copy_b(j); }
+        }
+    }
+}
+template <class T, bool AC, bool BC, class H, class V, class Copies> struct Sums {
+    static constexpr int FM = V::FM, FN = V::FN, RA = AC ? (FM < 8 ? FM : 8) : 2, RB = BC ? (FN < 8 ? FN : 8) : 2;
     static_assert(!AC || (FM & (FM - 1)) == 0, "addresses of a col operand"); static_assert(!BC || (FN & (FN - 1)) == 0, "addresses of a col operand");
-    typedef Frags<T, H> F;
+    typedef Frags<T, V> F;
     uint32_t lds, ra[RA], rb[RB];   // a lane's addresses in a round
     __device__ __forceinline__ Sums(uint32_t lds_) : lds(lds_) {
-        const int wave = uni(threadIdx.x >> 6), wm = wave / H::WN, wn = wave % H::WN;
+        const int wave = uni((int) threadIdx.x >> 6), wm = wave / V::WN, wn = wave % V::WN;
         const RowLane row;
 #pragma unroll
         for (int j = 0; j < RA; ++j) {
@@ -175,6 +195,11 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
             if constexpr (BC) { rb[j] = ColLane<H::BN>::read(wn * FN + j) + (uint32_t) ((wn * FN + j) / 8 * 256) + lds + H::LB; }
             else { rb[j] = (row.read ^ (uint32_t) (64 * j)) + (uint32_t) (wn * FN * 2048) + lds + H::LB; }
         }
+    }
+    static __device__ __forceinline__ void pin_sum(f32x4 & v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        __asm__ volatile("" : "+a"(v));
+#endif
     }
     static __device__ __forceinline__ void pin(uint32_t & v) { __asm__("" : "+v"(v)); }   // (a register of its own, the fragments by immediate offsets)
     struct At { uint32_t a[RA], b[RB]; };
@@ -193,21 +218,6 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
             if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at.a[i % RA] + (uint32_t) (i / RA * 256 + h * 32 * H::BM * 2)); } else { f.a[i] = lds_row<T>(at.a[h] + (uint32_t) (i * 2048)); }
         }
     }
-    __device__ __forceinline__ void start(Copies & c) const {   // A of rounds 0 .. SA - 2, B of 0 .. SB - 1
-#pragma unroll
-        for (int d = 0; d < (H::SA - 1 > H::SB ? H::SA - 1 : H::SB); ++d) {
-            if (d < H::SA - 1) {
-                c.begin_a(d);
-#pragma unroll
-                for (int j = 0; j < H::CA; ++j) { c.set_a(j, lds + (uint32_t) (d * H::AB)); c.copy_a(j); }
-            }
-            if (d < H::SB) {
-                c.begin_b(d);
-#pragma unroll
-                for (int j = 0; j < H::CB; ++j) { c.set_b(j, lds + (uint32_t) (H::LB + d * H::BB)); c.copy_b(j); }
-            }
-        }
-    }
     __device__ __forceinline__ void run(f32x4 (&acc)[FM][FN], int rounds, Copies & c) const {
         constexpr int MF = FM * FN, RD = FM + FN, RG = MF - MF / 4 - 1;   // groups of one product: the first, RG with reads and copies, the rest
         constexpr int LATER = (H::SB - 1) * H::CA + (H::SB - 2) * H::CB < (H::SA - 2) * (H::CA + H::CB) ? (H::SB - 1) * H::CA + (H::SB - 2) * H::CB : (H::SA - 2) * (H::CA + H::CB);
@@ -220,8 +230,8 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
         F f0, f1;
         At at;
         int sa = 0, sb = 0;                  // round d's places
-        auto product = [&](const F & f, int j) { acc[j / FN][j % FN] = mfma32(f.b[j % FN], f.a[j / FN], acc[j / FN][j % FN]); };
-        auto half = [&](auto second, const F & cur, F & nxt, uint32_t to) {
+        auto product = [&](const F & f, int j) __attribute__((always_inline)) { acc[j / FN][j % FN] = mfma32(f.b[j % FN], f.a[j / FN], acc[j / FN][j % FN]); };
+        auto half = [&](auto second, const F & cur, F & nxt, uint32_t to) __attribute__((always_inline)) {
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g <= RG; ++g) {
@@ -235,7 +245,7 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
                     constexpr int CN = decltype(second)::value ? H::CB : H::CA;
 #pragma unroll
                     for (int j = 0; j < CN; ++j) {   // copy j: its lane's offset, a group later the copy
-                        const int when = 1 + j * (RG - 1) / CN;
+                        const int when = second && RG > 2 * CN ? 1 + 2 * j : 1 + j * (RG - 1) / CN;   // (B has a round to arrive, A more: 2 % of dx and dW)
                         if (g == when) { if (second) { c.set_b(j, to); } else { c.set_a(j, to); } }
                         if (g == when + 1) { if (second) { c.copy_b(j); } else { c.copy_a(j); } }
                     }
@@ -243,7 +253,7 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto rest = [&](const F & cur) {
+        auto rest = [&](const F & cur) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = RG + 1; j < MF; ++j) { product(cur, j); }
             __builtin_amdgcn_sched_barrier(0);
@@ -269,6 +279,13 @@ template <class T, bool AC, bool BC, class H, class Copies> struct Sums {
         }
         wait_copies<0>();   // nothing is written to LDS after the tile
         meet();
+        if constexpr (FM * FN == 64) {   // the sums fill one half of the registers: what follows must not move them inside the loop
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+#pragma unroll
+                for (int j = 0; j < FN; ++j) { pin_sum(acc[i][j]); }
+            }
+        }
     }
 };
 
@@ -304,12 +321,33 @@ __device__ __forceinline__ void add8(const float * p, float (&v)[8]) {
     for (int i = 0; i < 4; ++i) { v[i] += a[i]; v[4 + i] += b[i]; }
 }
 
-// the range [first, last) of tiles of this workgroup's XCD (workgroups go round the 8 XCDs), and where it begins in it
-struct Share { int first, last, step; };
-__device__ __forceinline__ Share share_of(int tiles) {
-    const int x = blockIdx.x % 8, per = gridDim.x / 8;   // (the grid is a multiple of 8)
-    return { (int) ((int64_t) tiles * x / 8) + (int) blockIdx.x / 8, (int) ((int64_t) tiles * (x + 1) / 8), per };
-}
+// The workgroups (a multiple of 8) go round the 8 XCDs; an XCD's tiles are a run of the launch's, so that what runs at a time there shares
+// panels in its L2. Tiles differ in cost, so after its first a workgroup takes the XCD's next one (queue[x]); the last to find none
+// sets the two counters back to 0 for the next launch.
+struct Queue {
+    int * next, * gone; int first, last, per;
+    __device__ __forceinline__ Queue(int * queue, int tiles) {
+        const int x = (int) blockIdx.x % 8;
+        per = (int) gridDim.x / 8;
+        next = queue + x; gone = queue + 8 + x;
+        first = (int) ((int64_t) tiles * x / 8); last = (int) ((int64_t) tiles * (x + 1) / 8);
+    }
+    __device__ __forceinline__ int begin() const { return first + (int) blockIdx.x / 8; }
+    __device__ __forceinline__ int ask() const { return threadIdx.x == 0 ? atomicAdd(next, 1) : 0; }   // (called before a tile's sums, answered by then)
+    // every thread: the answer, through LDS, which nothing else uses now
+    __device__ __forceinline__ int told(int asked, uint32_t lds) const {
+        if (threadIdx.x == 0) { *(LK_LOCAL int *) (size_t) lds = asked; }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        meet();
+        const int v = uni(*(const LK_LOCAL int *) (size_t) lds);
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        meet();
+        return first + per + v;
+    }
+    __device__ __forceinline__ void leave() const {
+        if (threadIdx.x == 0 && atomicAdd(gone, 1) == per - 1) { *next = 0; *gone = 0; }
+    }
+};
 
 // ---------------------------------------------------------------- the operands' copies
 // A row operand of `rows` rows of `ld` values from base on; row r of the tile is row at(r) of it (< 0: not there). Terms 0 .. K - 1
@@ -333,7 +371,7 @@ template <class H, int COLS, int BYTES, int C> struct ColCopies {
     uint64_t base; uint32_t v[C], voff; Place dst; u32x4 buf;
     __device__ __forceinline__ void init(const void * p, int ld, int first) {
         base = uni64(p);
-        const int wave = uni(threadIdx.x >> 6);
+        const int wave = uni((int) threadIdx.x >> 6);
 #pragma unroll
         for (int j = 0; j < C; ++j) {
             const int q = piece<BYTES, C>(wave, j), c = ColLane<COLS>::column(q);
@@ -351,13 +389,27 @@ template <class H, int COLS, int BYTES, int C> struct ColCopies {
     __device__ __forceinline__ void copy() const { copy16(dst, voff, buf); }
 };
 
+// f on the sharing of a tile with nm rows
+template <class H, class F> __device__ __forceinline__ void by_rows(int nm, F f) {
+    if constexpr (H::BM == 256) { if (nm > 128) { f(Waves<H, 256, 2>()); return; } }
+    if constexpr (H::BM >= 128 && H::BN == 256) { if (nm > 64) { f(Waves<H, 128, 1>()); return; } f(Waves<H, 64, 1>()); }
+    else if constexpr (H::BM == 128) { f(Waves<H, 128, 2>()); }
+    else { f(Waves<H, 64, 2>()); }
+}
+
 // ---------------------------------------------------------------- forward
 // GATED: of a wave's columns of the tile the first half are W's rows, the second the same rows of W2
 template <class T, bool GATED, class H> struct FwdCopies {
-    static constexpr int CN = GATED ? H::BN / 2 : H::BN, WC = CN / H::WN;   // result columns of a tile, of a wave
-    RowCopies<H, H::AB, H::CA> a; RowCopies<H, H::BB, H::CB> b; uint64_t base2; u32x4 buf2; int K, wave;
-    __device__ __forceinline__ void init(const MatmulArgs & g, const Spot & s) {
-        K = g.K; wave = uni(threadIdx.x >> 6);
+    static constexpr int CN = GATED ? H::BN / 2 : H::BN, WC = 32;   // result columns of a tile; GATED: W's and W2's rows take turns so many at a time
+    RowCopies<H, H::AB, H::CA> a; RowCopies<H, H::BB, H::CB> b; uint64_t base2; u32x4 buf2; const int K, wave;
+    // GATED: a wave's first copies are of W's pieces, the others of W2's
+    static __device__ __forceinline__ int piece_b(int w, int j) {
+        if (!GATED) { return piece<H::BB, H::CB>(w, j); }
+        static_assert(!GATED || (H::CB % 4 == 0 && WC % 16 == 0), "half a wave's copies, of even and odd pieces in turn");
+        const int q = w * (H::CB / 2) + j % (H::CB / 2);
+        return q / (WC / 8) * (WC / 4) + q % (WC / 8) + (j < H::CB / 2 ? 0 : WC / 8);
+    }
+    __device__ __forceinline__ FwdCopies(const MatmulArgs & g, const Spot & s) : K(g.K), wave(uni((int) threadIdx.x >> 6)) {
         const int lane = lane_id();
 #pragma unroll
         for (int j = 0; j < H::CA; ++j) {
@@ -369,7 +421,7 @@ template <class T, bool GATED, class H> struct FwdCopies {
         }
 #pragma unroll
         for (int j = 0; j < H::CB; ++j) {
-            const int p = piece<H::BB, H::CB>(wave, j), rr = p * 8 + (lane >> 3), c = GATED ? rr / (2 * WC) * WC + rr % WC : rr;
+            const int p = piece_b(wave, j), rr = p * 8 + (lane >> 3), c = GATED ? rr / (2 * WC) * WC + rr % WC : rr;
             b.v[j] = s.n0 + c < g.R ? (uint32_t) c * (uint32_t) K * 2 + RowLane::chunk(p) * 16 : FAR;
         }
         const size_t w0 = ((size_t) s.e * g.R + s.n0) * K;
@@ -380,59 +432,68 @@ template <class T, bool GATED, class H> struct FwdCopies {
     __device__ __forceinline__ void begin_a(int d) { a.begin(d, K); }
     __device__ __forceinline__ void begin_b(int d) { b.begin(d, K); if (GATED) { buf2 = buffer(base2 + (uint64_t) (uint32_t) d * (BK * 2), b.buf[2]); } }
     __device__ __forceinline__ void set_a(int j, uint32_t to) { a.set(wave, j, to); }
-    __device__ __forceinline__ void set_b(int j, uint32_t to) { b.set(wave, j, to); }
+    __device__ __forceinline__ void set_b(int j, uint32_t to) { b.set(wave, j, to); b.dst.off = (uint32_t) (piece_b(wave, j) * 1024); }
     __device__ __forceinline__ void copy_a(int) const { a.copy(); }
-    __device__ __forceinline__ void copy_b(int j) const {
-        if (GATED && piece<H::BB, H::CB>(wave, j) * 8 % (2 * WC) >= WC) { copy16(b.dst, b.voff, buf2); } else { b.copy(); }
-    }
+    __device__ __forceinline__ void copy_b(int j) const { if (GATED && j >= H::CB / 2) { copy16(b.dst, b.voff, buf2); } else { b.copy(); } }
 };
-template <class T, int ACT, bool GATED, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm(MatmulArgs a) {
+// the epilogue of a tile's results
+template <class T, bool GATED, class H, class V> __device__ __forceinline__ void fwd_results(const MatmulArgs & a, const Spot & s, f32x4 (&acc)[V::FM][V::FN]) {
+    constexpr int FC = GATED ? V::FN / 2 : V::FN;
+    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
+#pragma unroll
+    for (int m = 0; m < V::FM; ++m) {
+        const int sr = (wm * V::FM + m) * 16 + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < FC; j += 2) {
+            const int col = s.n0 + (wn * FC + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+            const int f = GATED ? 2 * j : j;   // (W's 2 fragments, W2's 2, and so on)
+            float z[8], y[8], z2[8];
+            eight(acc[m][f], acc[m][f + 1], z);
+            if (GATED) { eight(acc[m][f + 2], acc[m][f + 3], z2); }
+            if (sr >= s.nm || col >= a.R) { continue; }
+            const size_t at = (size_t) (s.slot + sr) * a.R + col;
+            if (a.bias) { add8(a.bias + (size_t) s.e * a.R + col, z); }
+            activate8(a.act, z, y);
+            if (GATED) {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) { y[u] *= z2[u]; }
+            }
+            if (a.residual) { add8((const T *) a.residual + at, y); }
+            if (a.y_f32) { put8((float *) a.y + at, y); } else { put8((T *) a.y + at, y); }
+            if (a.z) { put8((T *) a.z + at, z); }
+            if (GATED && a.z2) { put8((T *) a.z2 + at, z2); }
+        }
+    }
+}
+template <class T, bool GATED, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm(MatmulArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef FwdCopies<T, GATED, H> C;
     const int nt = (a.R + C::CN - 1) / C::CN;
     const Tiles tiles(a.offsets, a.n, a.n_exp, H::BM);
-    const Share sh = share_of(tiles.all * nt);
-    const Sums<T, false, false, H, C> sums(lds_addr(dyn));
-    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
-    C c;
-    Spot next;
-    auto take = [&](int i) { next = spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, i); c.init(a, next); sums.start(c); };
-    if (sh.first < sh.last) { take(sh.first); }
-    for (int i = sh.first; i < sh.last; i += sh.step) {
-        const Spot s = next;
-        f32x4 acc[H::FM][H::FN];
-        sums.run(acc, (a.K + BK - 1) / BK, c);
-        if (i + sh.step < sh.last) { take(i + sh.step); }
-        constexpr int FC = GATED ? H::FN / 2 : H::FN;
-#pragma unroll
-        for (int m = 0; m < H::FM; ++m) {
-            const int sr = (wm * H::FM + m) * 16 + (lane & 15);
-#pragma unroll
-            for (int j = 0; j < FC; j += 2) {
-                const int col = s.n0 + wn * C::WC + 16 * (j + ((lane >> 4) & 1)) + 8 * (lane >> 5);
-                float z[8], y[8], z2[8];
-                eight(acc[m][j], acc[m][j + 1], z);
-                if (GATED) { eight(acc[m][FC + j], acc[m][FC + j + 1], z2); }
-                if (sr >= s.nm || col >= a.R) { continue; }
-                const size_t at = (size_t) (s.slot + sr) * a.R + col;
-                if (a.bias) { add8(a.bias + (size_t) s.e * a.R + col, z); }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) { y[u] = act_fn<ACT>(z[u]); if (GATED) { y[u] *= z2[u]; } }
-                if (a.residual) { add8((const T *) a.residual + at, y); }
-                if (a.y_f32) { put8((float *) a.y + at, y); } else { put8((T *) a.y + at, y); }
-                if (a.z) { put8((T *) a.z + at, z); }
-                if (GATED && a.z2) { put8((T *) a.z2 + at, z2); }
-            }
-        }
+    const Queue queue(a.queue, tiles.all * nt);
+    const uint32_t lds = lds_addr(dyn);
+    for (int i = queue.begin(); i < queue.last;) {
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, i);
+        const int asked = queue.ask();
+        by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
+            typedef decltype(v) V;
+            const Sums<T, false, false, H, V, C> sums(lds);
+            C c(a, s);
+            start<H>(c, lds);
+            f32x4 acc[V::FM][V::FN];
+            sums.run(acc, (a.K + BK - 1) / BK, c);
+            fwd_results<T, GATED, H, V>(a, s, acc);
+        });
+        i = queue.told(asked, lds);
     }
+    queue.leave();
 }
 
 // ---------------------------------------------------------------- dx
 // the sum goes over dz's columns and then, with a second pair, over dz2's: rounds 0 .. half - 1 and half .. 2 half - 1
 template <class T, class H> struct DxCopies {
-    RowCopies<H, H::AB, H::CA> a; ColCopies<H, H::BN, H::BB, H::CB> b; uint64_t a1, a2, b1, b2; int R, K, n0, half, rounds, wave;
-    __device__ __forceinline__ void init(const MatmulGradArgs & g, const Spot & s) {
-        R = g.R; K = g.K; n0 = s.n0; wave = uni(threadIdx.x >> 6); half = (R + BK - 1) / BK; rounds = g.dz2 ? 2 * half : half;
+    RowCopies<H, H::AB, H::CA> a; ColCopies<H, H::BN, H::BB, H::CB> b; uint64_t a1, a2, b1, b2; const int R, K, wave, half, rounds, n0;
+    __device__ __forceinline__ DxCopies(const MatmulGradArgs & g, const Spot & s) : R(g.R), K(g.K), wave(uni((int) threadIdx.x >> 6)), half((g.R + BK - 1) / BK), rounds(g.dz2 ? 2 * half : half), n0(s.n0) {
         const int lane = lane_id();
 #pragma unroll
         for (int j = 0; j < H::CA; ++j) {
@@ -456,30 +517,34 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads, H::PER
     typedef DxCopies<T, H> C;
     const int nt = (a.K + H::BN - 1) / H::BN;
     const Tiles tiles(a.offsets, a.n, a.n_exp, H::BM);
-    const Share sh = share_of(tiles.all * nt);
-    const Sums<T, false, true, H, C> sums(lds_addr(dyn));
-    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
-    C c;
-    Spot next;
-    auto take = [&](int i) { next = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, i); c.init(a, next); sums.start(c); };
-    if (sh.first < sh.last) { take(sh.first); }
-    for (int i = sh.first; i < sh.last; i += sh.step) {
-        const Spot s = next;
-        f32x4 acc[H::FM][H::FN];
-        sums.run(acc, c.rounds, c);
-        if (i + sh.step < sh.last) { take(i + sh.step); }
+    const Queue queue(a.queue, tiles.all * nt);
+    const uint32_t lds = lds_addr(dyn);
+    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id();
+    for (int i = queue.begin(); i < queue.last;) {
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, i);
+        const int asked = queue.ask();
+        by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
+            typedef decltype(v) V;
+            const Sums<T, false, true, H, V, C> sums(lds);
+            C c(a, s);
+            start<H>(c, lds);
+            f32x4 acc[V::FM][V::FN];
+            sums.run(acc, c.rounds, c);
 #pragma unroll
-        for (int m = 0; m < H::FM; ++m) {
-            const int sr = (wm * H::FM + m) * 16 + (lane & 15);
+            for (int m = 0; m < V::FM; ++m) {
+                const int sr = (wave / V::WN * V::FM + m) * 16 + (lane & 15);
 #pragma unroll
-            for (int j = 0; j < H::FN; j += 2) {
-                const int col = s.n0 + (wn * H::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
-                float v[8];
-                eight(acc[m][j], acc[m][j + 1], v);
-                if (sr < s.nm && col < a.K) { put8((T *) a.dx + (size_t) (s.slot + sr) * a.K + col, v); }
+                for (int j = 0; j < V::FN; j += 2) {
+                    const int col = s.n0 + (wave % V::WN * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+                    float v[8];
+                    eight(acc[m][j], acc[m][j + 1], v);
+                    if (sr < s.nm && col < a.K) { put8((T *) a.dx + (size_t) (s.slot + sr) * a.K + col, v); }
+                }
             }
-        }
+        });
+        i = queue.told(asked, lds);
     }
+    queue.leave();
 }
 
 // ---------------------------------------------------------------- dW
@@ -490,7 +555,7 @@ template <class T, bool PERM, class H> struct DwCopies {
     uint32_t off[NR];    // and the round's rows, as offsets
     const int * perm; uint32_t magic, xrows; int R, K, m0, n0, begin, len, wave;
     __device__ __forceinline__ void init(const MatmulGradArgs & g, const void * dz, int begin_, int len_, int m0_, int n0_) {
-        perm = g.perm; magic = g.magic; xrows = (uint32_t) g.xrows; R = g.R; K = g.K; m0 = m0_; n0 = n0_; begin = begin_; len = len_; wave = uni(threadIdx.x >> 6);
+        perm = g.perm; magic = g.magic; xrows = (uint32_t) g.xrows; R = g.R; K = g.K; m0 = m0_; n0 = n0_; begin = begin_; len = len_; wave = uni((int) threadIdx.x >> 6);
         a.init((const T *) dz + (size_t) begin * R + m0, R, m0);
         b.init((const T *) g.x + (PERM ? 0 : (size_t) begin * K) + n0, K, n0);
         if constexpr (PERM) {
@@ -501,12 +566,9 @@ template <class T, bool PERM, class H> struct DwCopies {
     }
     __device__ __forceinline__ void load_pairs(int d) {
 #pragma unroll
-        for (int j = 0; j < H::CB; ++j) {
-#pragma unroll
-            for (int q = 0; q < Q; ++q) {   // (past the end: its last one again, or any)
-                const int i = min(d * BK + piece<H::BB, H::CB>(wave, j) * Q + q, len - 1);
-                pair[j * Q + q] = ((const LK_CONST int *) perm)[uni(max(begin + i, 0))];
-            }
+        for (int i = 0; i < NR; ++i) {   // (past the end: its last one again, or any)
+            const int at = min(d * BK + piece<H::BB, H::CB>(wave, i / Q) * Q + i % Q, len - 1);
+            pair[i] = ((const LK_CONST int *) perm)[uni(max(begin + at, 0))];
         }
     }
     __device__ __forceinline__ void begin_a(int d) { a.begin(d, len, R, m0); }
@@ -514,12 +576,9 @@ template <class T, bool PERM, class H> struct DwCopies {
         if constexpr (PERM) {
             b.buf = buffer(b.base, WINDOW);
 #pragma unroll
-            for (int j = 0; j < H::CB; ++j) {
-#pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    const uint32_t r = pair_row((uint32_t) pair[j * Q + q], magic);
-                    off[j * Q + q] = d * BK + piece<H::BB, H::CB>(wave, j) * Q + q < len && r < xrows ? r * (uint32_t) K * 2 : WINDOW;   // (and a column: still outside)
-                }
+            for (int i = 0; i < NR; ++i) {
+                const uint32_t r = pair_row((uint32_t) pair[i], magic);
+                off[i] = d * BK + piece<H::BB, H::CB>(wave, i / Q) * Q + i % Q < len && r < xrows ? r * (uint32_t) K * 2 : WINDOW;   // (and a column: still outside)
             }
             load_pairs(d + 1);
         } else { b.begin(d, len, K, n0); }
@@ -529,9 +588,14 @@ template <class T, bool PERM, class H> struct DwCopies {
         b.set(wave, j, to);
         if constexpr (PERM) {
             const int q = lane_id() / (64 / Q);
+            static_assert(Q == 2 || Q == 4, "tiles of 256 or 128 columns");
             uint32_t o = off[j * Q];
 #pragma unroll
-            for (int u = 1; u < Q; ++u) { o = q == u ? off[j * Q + u] : o; }
+            for (int u = 1; u < Q; ++u) {
+                uint32_t w = off[j * Q + u];
+                __asm__("" : "+s"(w));   // (else the choice becomes an indexed load from scratch memory)
+                o = q == u ? w : o;
+            }
             b.voff = b.voff == FAR ? FAR : b.voff + o;
             __asm__ volatile("" : "+v"(b.voff));
         }
@@ -544,24 +608,26 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef DwCopies<T, PERM, H> C;
     constexpr int BAND = 4;
-    const int wave = uni(threadIdx.x >> 6), lane = lane_id(), wm = wave / H::WN, wn = wave % H::WN;
+    typedef Waves<H, H::BM, 2> V;
+    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
     const int all = (int) gridDim.x, x = (int) blockIdx.x % 8, t = all / 8 * x + min(x, all % 8) + (int) blockIdx.x / 8;
     const int per = mt * nt, which = t / per, e = which % a.n_exp, in = t % per, band = in / (BAND * nt), rows = min(BAND, mt - band * BAND), r = in - band * BAND * nt;
     const bool second = which >= a.n_exp || !a.dW;
     const Span sp = span_of(a.offsets, a.n, e);
     const int begin = uni(sp.begin), len = uni(sp.end) - begin, m0 = (band * BAND + r % rows) * H::BM, n0 = r / rows * H::BN;
-    const Sums<T, true, true, H, C> sums(lds_addr(dyn));
+    const uint32_t lds = lds_addr(dyn);
+    const Sums<T, true, true, H, V, C> sums(lds);
     C c;
     c.init(a, second ? a.dz2 : a.dz, begin, len, m0, n0);
-    f32x4 acc[H::FM][H::FN];
-    sums.start(c);
+    f32x4 acc[V::FM][V::FN];
+    start<H>(c, lds);
     sums.run(acc, (len + BK - 1) / BK, c);
 #pragma unroll
-    for (int m = 0; m < H::FM; ++m) {
-        const int row = m0 + (wm * H::FM + m) * 16 + (lane & 15);
+    for (int m = 0; m < V::FM; ++m) {
+        const int row = m0 + (wm * V::FM + m) * 16 + (lane & 15);
 #pragma unroll
-        for (int j = 0; j < H::FN; j += 2) {
-            const int col = n0 + (wn * H::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+        for (int j = 0; j < V::FN; j += 2) {
+            const int col = n0 + (wn * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
             float v[8];
             eight(acc[m][j], acc[m][j + 1], v);
             if (row >= a.R || col >= a.K) { continue; }
@@ -578,22 +644,24 @@ constexpr int CUS = 256;
 int64_t most_tiles(int n, int n_exp, bool groups, int bm) { return ceil_div(n, bm) + (groups ? n_exp : 0); }
 unsigned grid_of(int64_t tiles, int per_cu) { return (unsigned) std::min<int64_t>(CUS * per_cu, ceil_div(tiles, 8) * 8); }
 
-template <class T, int ACT, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
+template <class T, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
     static LdsLimit limit;
-    if (const hipError_t e = limit((const void *) k_mm<T, ACT, GATED, H>, H::LDS)) { return e; }
+    if (const hipError_t e = limit((const void *) k_mm<T, GATED, H>, H::LDS)) { return e; }
     const int64_t tiles = most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.R, GATED ? H::BN / 2 : H::BN);
-    k_mm<T, ACT, GATED, H><<<grid_of(tiles, H::PER_CU), H::threads, H::LDS, st>>>(a);
+    k_mm<T, GATED, H><<<grid_of(tiles, H::PER_CU), H::threads, H::LDS, st>>>(a);
     return hipGetLastError();
 }
-template <class T, int ACT, bool GATED> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
-    const int per = a.n / a.n_exp;
-    if (per > 96) { return fwd<T, ACT, GATED, Shape<256, 256, 2, 2, 3, 2, 1>>(a, st); }
-    return fwd<T, ACT, GATED, Shape<64, 128, 2, 2, 3, 2, 2>>(a, st);
+typedef Shape<256, 256, 3, 2, 1> Large;
+typedef Shape<128, 256, 3, 2, 1> Wide;
+typedef Shape<64, 128, 3, 2, 2> Small;
+template <class T, bool GATED> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
+    switch (a.shape) {
+        case MM_LARGE: return fwd<T, GATED, Large>(a, st);
+        case MM_WIDE: return fwd<T, GATED, Wide>(a, st);
+        default: return fwd<T, GATED, Small>(a, st);
+    }
 }
-template <class T> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
-    if (a.W2) { return a.act == ACT_SILU ? fwd<T, ACT_SILU, true>(a, st) : a.act == ACT_GELU ? fwd<T, ACT_GELU, true>(a, st) : fwd<T, ACT_NONE, true>(a, st); }
-    return a.act == ACT_SILU ? fwd<T, ACT_SILU, false>(a, st) : a.act == ACT_GELU ? fwd<T, ACT_GELU, false>(a, st) : fwd<T, ACT_NONE, false>(a, st);
-}
+template <class T> hipError_t fwd(const MatmulArgs & a, hipStream_t st) { return a.W2 ? fwd<T, true>(a, st) : fwd<T, false>(a, st); }
 template <class T, class H> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
     static LdsLimit limit;
     if (const hipError_t e = limit((const void *) k_mm_dx<T, H>, H::LDS)) { return e; }
@@ -601,8 +669,11 @@ template <class T, class H> hipError_t dx(const MatmulGradArgs & a, hipStream_t 
     return hipGetLastError();
 }
 template <class T> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
-    if (a.n / a.n_exp > 96) { return dx<T, Shape<256, 256, 2, 2, 3, 2, 1>>(a, st); }
-    return dx<T, Shape<64, 128, 2, 2, 3, 2, 2>>(a, st);
+    switch (a.shape) {
+        case MM_LARGE: return dx<T, Large>(a, st);
+        case MM_WIDE: return dx<T, Wide>(a, st);
+        default: return dx<T, Small>(a, st);
+    }
 }
 template <class T, bool F32, bool PERM, class H> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
     static LdsLimit limit;
@@ -612,8 +683,8 @@ template <class T, bool F32, bool PERM, class H> hipError_t dw(const MatmulGradA
     return hipGetLastError();
 }
 template <class T, bool F32, bool PERM> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
-    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, PERM, Shape<256, 256, 2, 2, 3, 2, 1>>(a, st); }
-    return dw<T, F32, PERM, Shape<128, 128, 2, 2, 3, 2, 2>>(a, st);
+    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, PERM, Large>(a, st); }
+    return dw<T, F32, PERM, Shape<128, 128, 3, 2, 2>>(a, st);
 }
 template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) { return a.perm && a.n > 0 ? dw<T, F32, true>(a, st) : dw<T, F32, false>(a, st); }
 

@@ -40,6 +40,18 @@ constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;
 __device__ __forceinline__ float sigma(float t) { return 1.f / (1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)); }
 template <int ACT> __device__ __forceinline__ float act_arg(float z) { return ACT == ACT_GELU ? GELU_C * (z + GELU_A * z * z * z) : z; }
 template <int ACT> __device__ __forceinline__ float act_fn(float z) { return ACT == ACT_NONE ? z : z * sigma(act_arg<ACT>(z)); }
+__device__ __forceinline__ void activate8(int act, const float (&z)[8], float (&y)[8]) {   // (act is the launch's)
+    if (act == ACT_SILU) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { y[u] = act_fn<ACT_SILU>(z[u]); }
+    } else if (act == ACT_GELU) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { y[u] = act_fn<ACT_GELU>(z[u]); }
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { y[u] = z[u]; }
+    }
+}
 // the derivative: s(g) + z g' s(g) s(-g)
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
     if (ACT == ACT_NONE) { return 1.f; }
