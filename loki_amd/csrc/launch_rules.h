@@ -102,7 +102,47 @@ constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {
 }
 
 // ---------------------------------------------------------------- 16-bit products (matmul.hip)
+// Tiles of bm x bn, `slots` of them at a time on the chip. A tile takes fixed + rounds * (a round of 64 terms) us, a round `one` where
+// few CUs have work and `full` where all have (the clock falls with the power, and Small's two workgroups share a CU). A sum can be split into
+// parts, whose results a second launch adds up. The constants are fitted to 112 sizes (16 .. 2048 rows, 512 .. 16384 columns and
+// terms, weights from memory). Examples, us, Small / Wide / Large, then the best split: 64 rows, 7168 terms -> 2048 columns 54 / 74 / -, 17 (Small, 8
+// parts); 501, 7168 -> 2048 53 / 75 / 141, 33 (Wide, 4); 501, 2048 -> 7168 29 / 29 / 57; 1024, 7168 -> 7168 137 / 93 / 144; 2048, 7168 -> 7168
+// 302 / 203 / 173; 2048, 2048 -> 2048 33 / 31 / 58; 512 rows, columns and terms 7.6 / 13 / 25.
 enum { MM_SMALL, MM_WIDE, MM_LARGE };
-constexpr int mm_shape_of(int n, int n_exp, int cols) { return n / n_exp > 96 ? MM_LARGE : MM_SMALL; }
+struct MmPlan { int shape, parts; };
+struct MmCost { int bm, bn, slots; float fixed, one, full; };
+constexpr MmCost MM_COST[3] = { { 64, 128, 512, 3.7f, 0.40f, 0.69f }, { 128, 256, 256, 5.4f, 0.55f, 0.86f }, { 256, 256, 256, 10.0f, 1.07f, 1.33f } };
+constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int terms) {
+    const MmCost k = MM_COST[shape];
+    const float per = (float) n / (float) n_exp;
+    // m-tiles: an expert's last one is half full on average (and costs less: the waves share as many rows as it has)
+    const float mt = n_exp == 1 ? (float) ((n + k.bm - 1) / k.bm) : (float) n / (float) k.bm + 0.5f * (float) (n < n_exp ? n : n_exp);
+    const float fill = per / ((float) n_exp >= 2.f ? mt * (float) k.bm / (float) n_exp : per);
+    const float items = mt * (float) ((cols + k.bn - 1) / k.bn) * (float) parts;
+    const int rounds = (terms + 63) / 64, r = (rounds + parts - 1) / parts;
+    float waves = items / (float) k.slots;
+    const float busy = waves >= 1.f ? 1.f : shape == MM_SMALL ? (waves > 0.5f ? 1.f : 0.f) : waves;
+    if (n_exp == 1 || waves < 1.f) { const int w = (int) waves; waves = (float) w < waves ? (float) (w + 1) : (float) w; }
+    const float cost = (k.one + (k.full - k.one) * busy) * (shape == MM_LARGE && n_exp > 1 ? 0.4f + 0.6f * fill : 1.f);
+    const float sums = waves * (k.fixed + (float) r * cost);
+    const float used = n_exp == 1 ? 1.f : per / (0.6f + per) * (float) n_exp;   // experts with rows, about
+    const float memory = (float) cols * (float) terms * used * 3.1e-7f + (float) n * (float) cols * 4e-7f;         // the weights and the results
+    const float join = parts > 1 ? 4.f + 0.15f * (float) parts + (float) parts * (float) n * (float) cols * 1.2e-6f : 0.f;
+    return 2.5f + (sums > memory ? sums + 0.15f * memory : memory + 0.15f * sums) + join;
+}
+// n rows of n_exp experts, `cols` results a row (gated: of both matrices), sums of `terms`
+constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms) {
+    const int split[8] = { 1, 2, 3, 4, 6, 8, 12, 16 };
+    MmPlan best{ MM_SMALL, 1 };
+    float least = mm_time(MM_SMALL, 1, n, n_exp, cols, terms);
+    for (int s = 0; s < 3; ++s) {
+        for (int i = 0; i < 8; ++i) {
+            if (split[i] > 1 && split[i] * 128 > terms) { break; }   // two rounds a part at least
+            const float t = mm_time(s, split[i], n, n_exp, cols, terms);
+            if (t < least) { least = t; best = { s, split[i] }; }
+        }
+    }
+    return best;
+}
 
 }  // namespace lk

@@ -124,15 +124,21 @@ struct Tiles {
     }
 };
 struct Spot { int e, slot, nm, n0; };   // expert, first slot, its slots in the tile, first column
+// the sum's part of work item i: parts come one after the other, each with all tiles; rounds d0 .. d0 + rounds - 1
+struct Part { int tile, part, d0, rounds; };
+__device__ __forceinline__ Part part_of(int i, int tiles, int parts, int rounds) {
+    const int p = parts > 1 ? uni(i / tiles) : 0, d0 = parts > 1 ? uni(rounds * p / parts) : 0;   // (at most 2^15 rounds, 16 parts)
+    return { i - p * tiles, p, d0, (parts > 1 ? uni(rounds * (p + 1) / parts) : rounds) - d0 };
+}
 // tile i of the launch, i < all * nt: an expert's tiles are next to each other, in bands of `band` m-tiles, m fastest
 __device__ __forceinline__ Spot spot_of(const Tiles & t, const int * offsets, int n, int nt, int bm, int bn, int band, int i) {
     Spot s;
     s.e = t.expert(i / nt);   // (before(e) * nt <= i exactly when before(e) <= i / nt)
     const Span sp = span_of(offsets, n, s.e);
     const int f = t.before(s.e), mt = t.before(s.e + 1) - f, in = i - f * nt, b = in / (band * nt), rows = min(band, mt - b * band), r = in - b * band * nt;
-    s.slot = uni(sp.begin) + (b * band + r % rows) * bm;
-    s.nm = min(bm, uni(sp.end) - s.slot);
-    s.n0 = r / rows * bn;
+    s.slot = uni(sp.begin + (b * band + r % rows) * bm);
+    s.nm = uni(min(bm, sp.end - s.slot));
+    s.n0 = uni(r / rows * bn);
     return s;
 }
 
@@ -401,7 +407,7 @@ template <class H, class F> __device__ __forceinline__ void by_rows(int nm, F f)
 // GATED: of a wave's columns of the tile the first half are W's rows, the second the same rows of W2
 template <class T, bool GATED, class H> struct FwdCopies {
     static constexpr int CN = GATED ? H::BN / 2 : H::BN, WC = 32;   // result columns of a tile; GATED: W's and W2's rows take turns so many at a time
-    RowCopies<H, H::AB, H::CA> a; RowCopies<H, H::BB, H::CB> b; uint64_t base2; u32x4 buf2; const int K, wave;
+    RowCopies<H, H::AB, H::CA> a; RowCopies<H, H::BB, H::CB> b; uint64_t base2; u32x4 buf2; const int K, wave;   // K: the part's terms
     // GATED: a wave's first copies are of W's pieces, the others of W2's
     static __device__ __forceinline__ int piece_b(int w, int j) {
         if (!GATED) { return piece<H::BB, H::CB>(w, j); }
@@ -409,23 +415,23 @@ template <class T, bool GATED, class H> struct FwdCopies {
         const int q = w * (H::CB / 2) + j % (H::CB / 2);
         return q / (WC / 8) * (WC / 4) + q % (WC / 8) + (j < H::CB / 2 ? 0 : WC / 8);
     }
-    __device__ __forceinline__ FwdCopies(const MatmulArgs & g, const Spot & s) : K(g.K), wave(uni((int) threadIdx.x >> 6)) {
+    __device__ __forceinline__ FwdCopies(const MatmulArgs & g, const Spot & s, const Part & p) : K(min(g.K - p.d0 * BK, p.rounds * BK)), wave(uni((int) threadIdx.x >> 6)) {
         const int lane = lane_id();
 #pragma unroll
         for (int j = 0; j < H::CA; ++j) {
-            const int p = piece<H::AB, H::CA>(wave, j), m = p * 8 + (lane >> 3);
+            const int q = piece<H::AB, H::CA>(wave, j), m = q * 8 + (lane >> 3);
             uint32_t r = (uint32_t) m;
             bool ok = m < s.nm;
             if (g.perm && ok) { r = pair_row((uint32_t) g.perm[s.slot + m], g.magic); ok = r < (uint32_t) g.xrows; }
-            a.v[j] = ok ? r * (uint32_t) K * 2 + RowLane::chunk(p) * 16 : FAR;
+            a.v[j] = ok ? r * (uint32_t) g.K * 2 + RowLane::chunk(q) * 16 : FAR;
         }
 #pragma unroll
         for (int j = 0; j < H::CB; ++j) {
-            const int p = piece_b(wave, j), rr = p * 8 + (lane >> 3), c = GATED ? rr / (2 * WC) * WC + rr % WC : rr;
-            b.v[j] = s.n0 + c < g.R ? (uint32_t) c * (uint32_t) K * 2 + RowLane::chunk(p) * 16 : FAR;
+            const int q = piece_b(wave, j), rr = q * 8 + (lane >> 3), c = GATED ? rr / (2 * WC) * WC + rr % WC : rr;
+            b.v[j] = s.n0 + c < g.R ? (uint32_t) c * (uint32_t) g.K * 2 + RowLane::chunk(q) * 16 : FAR;
         }
-        const size_t w0 = ((size_t) s.e * g.R + s.n0) * K;
-        a.base = uni64((const T *) g.x + (g.perm ? 0 : (size_t) s.slot * K));
+        const size_t w0 = ((size_t) s.e * g.R + s.n0) * g.K + p.d0 * BK;
+        a.base = uni64((const T *) g.x + (g.perm ? 0 : (size_t) s.slot * g.K) + p.d0 * BK);
         b.base = uni64((const T *) g.W + w0);
         base2 = GATED ? uni64((const T *) g.W2 + w0) : 0;
     }
@@ -436,53 +442,79 @@ template <class T, bool GATED, class H> struct FwdCopies {
     __device__ __forceinline__ void copy_a(int) const { a.copy(); }
     __device__ __forceinline__ void copy_b(int j) const { if (GATED && j >= H::CB / 2) { copy16(b.dst, b.voff, buf2); } else { b.copy(); } }
 };
-// the epilogue of a tile's results
-template <class T, bool GATED, class H, class V> __device__ __forceinline__ void fwd_results(const MatmulArgs & a, const Spot & s, f32x4 (&acc)[V::FM][V::FN]) {
+// the epilogue of a tile's results. Addresses are the tile's (scalars) and a lane's 32-bit offset: a tile's last row is below 2^28 values away
+template <class T, bool GATED, class H, class V> __device__ __forceinline__ void fwd_results(const MatmulArgs & a, const Spot & s, int part, f32x4 (&acc)[V::FM][V::FN]) {
     constexpr int FC = GATED ? V::FN / 2 : V::FN;
     const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
-#pragma unroll
-    for (int m = 0; m < V::FM; ++m) {
-        const int sr = (wm * V::FM + m) * 16 + (lane & 15);
+    const size_t t0 = (size_t) s.slot * a.R + s.n0, all = (size_t) a.n * a.R;
+    const int c0 = wn * FC * 16 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);   // the lane's first column in the tile
+    auto each = [&](auto column, auto f) __attribute__((always_inline)) {   // column(c) and then f(offset, z, z2) on 8 results at a time
 #pragma unroll
         for (int j = 0; j < FC; j += 2) {
-            const int col = s.n0 + (wn * FC + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
-            const int f = GATED ? 2 * j : j;   // (W's 2 fragments, W2's 2, and so on)
-            float z[8], y[8], z2[8];
-            eight(acc[m][f], acc[m][f + 1], z);
-            if (GATED) { eight(acc[m][f + 2], acc[m][f + 3], z2); }
-            if (sr >= s.nm || col >= a.R) { continue; }
-            const size_t at = (size_t) (s.slot + sr) * a.R + col;
-            if (a.bias) { add8(a.bias + (size_t) s.e * a.R + col, z); }
-            activate8(a.act, z, y);
-            if (GATED) {
+            const int g = GATED ? 2 * j : j, c = c0 + 16 * j;   // (W's 2 fragments, W2's 2, and so on)
+            column(c);
 #pragma unroll
-                for (int u = 0; u < 8; ++u) { y[u] *= z2[u]; }
+            for (int m = 0; m < V::FM; ++m) {
+                const int sr = (wm * V::FM + m) * 16 + (lane & 15);
+                float z[8], z2[8];
+                eight(acc[m][g], acc[m][g + 1], z);
+                if (GATED) { eight(acc[m][g + 2], acc[m][g + 3], z2); }
+                if (sr < s.nm && s.n0 + c < a.R) { f((uint32_t) sr * (uint32_t) a.R + (uint32_t) c, z, z2); }
             }
-            if (a.residual) { add8((const T *) a.residual + at, y); }
-            if (a.y_f32) { put8((float *) a.y + at, y); } else { put8((T *) a.y + at, y); }
-            if (a.z) { put8((T *) a.z + at, z); }
-            if (GATED && a.z2) { put8((T *) a.z2 + at, z2); }
         }
+    };
+    auto none = [](int) {};
+    if (a.parts > 1) {   // (k_mm_join does the rest)
+        float * p = a.part + (size_t) part * all + t0, * p2 = p + (size_t) a.parts * all;
+        each(none, [&](uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) { put8(p + at, z); if (GATED) { put8(p2 + at, z2); } });
+        return;
     }
+    const float * bias = a.bias ? a.bias + (size_t) s.e * a.R + s.n0 : nullptr;
+    const T * res = a.residual ? (const T *) a.residual + t0 : nullptr;
+    T * y = (T *) a.y + (a.y_f32 ? 2 * t0 : t0), * pz = a.z ? (T *) a.z + t0 : nullptr, * pz2 = GATED && a.z2 ? (T *) a.z2 + t0 : nullptr;
+    if (!GATED && !bias && !res && !pz && !a.act && !a.y_f32) {
+        each(none, [&](uint32_t at, float (&z)[8], float (&)[8]) __attribute__((always_inline)) { put8(y + at, z); });
+        return;
+    }
+    float b8[8];
+    each([&](int c) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { b8[u] = 0.f; }
+        if (bias && s.n0 + c < a.R) { add8(bias + c, b8); }
+    }, [&](uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) { z[u] += b8[u]; }
+        activate8(a.act, z, v);
+        if (GATED) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { v[u] *= z2[u]; }
+        }
+        if (res) { add8(res + at, v); }
+        if (a.y_f32) { put8((float *) y + at, v); } else { put8(y + at, v); }
+        if (pz) { put8(pz + at, z); }
+        if (pz2) { put8(pz2 + at, z2); }
+    });
 }
 template <class T, bool GATED, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm(MatmulArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef FwdCopies<T, GATED, H> C;
     const int nt = (a.R + C::CN - 1) / C::CN;
     const Tiles tiles(a.offsets, a.n, a.n_exp, H::BM);
-    const Queue queue(a.queue, tiles.all * nt);
+    const Queue queue(a.queue, tiles.all * nt * a.parts);
     const uint32_t lds = lds_addr(dyn);
     for (int i = queue.begin(); i < queue.last;) {
-        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, i);
+        const Part p = part_of(i, tiles.all * nt, a.parts, (a.K + BK - 1) / BK);
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, p.tile);
         const int asked = queue.ask();
         by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
             typedef decltype(v) V;
             const Sums<T, false, false, H, V, C> sums(lds);
-            C c(a, s);
+            C c(a, s, p);
             start<H>(c, lds);
             f32x4 acc[V::FM][V::FN];
-            sums.run(acc, (a.K + BK - 1) / BK, c);
-            fwd_results<T, GATED, H, V>(a, s, acc);
+            sums.run(acc, p.rounds, c);
+            fwd_results<T, GATED, H, V>(a, s, p.part, acc);
         });
         i = queue.told(asked, lds);
     }
@@ -492,21 +524,21 @@ template <class T, bool GATED, class H> __global__ void __launch_bounds__(H::thr
 // ---------------------------------------------------------------- dx
 // the sum goes over dz's columns and then, with a second pair, over dz2's: rounds 0 .. half - 1 and half .. 2 half - 1
 template <class T, class H> struct DxCopies {
-    RowCopies<H, H::AB, H::CA> a; ColCopies<H, H::BN, H::BB, H::CB> b; uint64_t a1, a2, b1, b2; const int R, K, wave, half, rounds, n0;
-    __device__ __forceinline__ DxCopies(const MatmulGradArgs & g, const Spot & s) : R(g.R), K(g.K), wave(uni((int) threadIdx.x >> 6)), half((g.R + BK - 1) / BK), rounds(g.dz2 ? 2 * half : half), n0(s.n0) {
+    RowCopies<H, H::AB, H::CA> a; ColCopies<H, H::BN, H::BB, H::CB> b; uint64_t a1, a2, b1, b2; const int R, K, wave, half, d0, end, n0;
+    __device__ __forceinline__ DxCopies(const MatmulGradArgs & g, const Spot & s, const Part & p) : R(g.R), K(g.K), wave(uni((int) threadIdx.x >> 6)), half((g.R + BK - 1) / BK), d0(p.d0), end(p.d0 + p.rounds), n0(s.n0) {
         const int lane = lane_id();
 #pragma unroll
         for (int j = 0; j < H::CA; ++j) {
-            const int p = piece<H::AB, H::CA>(wave, j), m = p * 8 + (lane >> 3);
-            a.v[j] = m < s.nm ? (uint32_t) m * (uint32_t) R * 2 + RowLane::chunk(p) * 16 : FAR;
+            const int q = piece<H::AB, H::CA>(wave, j), m = q * 8 + (lane >> 3);
+            a.v[j] = m < s.nm ? (uint32_t) m * (uint32_t) R * 2 + RowLane::chunk(q) * 16 : FAR;
         }
         const size_t a0 = (size_t) s.slot * R, w0 = (size_t) s.e * R * K + s.n0;
         b.init((const T *) g.W + w0, K, n0);
         a1 = uni64((const T *) g.dz + a0); b1 = b.base;
         a2 = g.dz2 ? uni64((const T *) g.dz2 + a0) : a1; b2 = g.dz2 ? uni64((const T *) g.W2 + w0) : b1;
     }
-    __device__ __forceinline__ void begin_a(int d) { a.base = d < half ? a1 : a2; a.begin(d < half ? d : d - half, d < rounds ? R : 0); }
-    __device__ __forceinline__ void begin_b(int d) { b.base = d < half ? b1 : b2; b.begin(d < half ? d : d - half, d < rounds ? R : 0, K, n0); }
+    __device__ __forceinline__ void begin_a(int d) { d += d0; a.base = d < half ? a1 : a2; a.begin(d < half ? d : d - half, d < end ? R : 0); }
+    __device__ __forceinline__ void begin_b(int d) { d += d0; b.base = d < half ? b1 : b2; b.begin(d < half ? d : d - half, d < end ? R : 0, K, n0); }
     __device__ __forceinline__ void set_a(int j, uint32_t to) { a.set(wave, j, to); }
     __device__ __forceinline__ void set_b(int j, uint32_t to) { b.set(wave, j, to); }
     __device__ __forceinline__ void copy_a(int) const { a.copy(); }
@@ -517,34 +549,56 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads, H::PER
     typedef DxCopies<T, H> C;
     const int nt = (a.K + H::BN - 1) / H::BN;
     const Tiles tiles(a.offsets, a.n, a.n_exp, H::BM);
-    const Queue queue(a.queue, tiles.all * nt);
+    const Queue queue(a.queue, tiles.all * nt * a.parts);
     const uint32_t lds = lds_addr(dyn);
-    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id();
+    const int rounds = (a.R + BK - 1) / BK * (a.dz2 ? 2 : 1);
     for (int i = queue.begin(); i < queue.last;) {
-        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, i);
+        const Part p = part_of(i, tiles.all * nt, a.parts, rounds);
+        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, p.tile);
         const int asked = queue.ask();
         by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
             typedef decltype(v) V;
             const Sums<T, false, true, H, V, C> sums(lds);
-            C c(a, s);
+            C c(a, s, p);
             start<H>(c, lds);
             f32x4 acc[V::FM][V::FN];
-            sums.run(acc, c.rounds, c);
-#pragma unroll
-            for (int m = 0; m < V::FM; ++m) {
-                const int sr = (wave / V::WN * V::FM + m) * 16 + (lane & 15);
-#pragma unroll
-                for (int j = 0; j < V::FN; j += 2) {
-                    const int col = s.n0 + (wave % V::WN * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
-                    float v[8];
-                    eight(acc[m][j], acc[m][j + 1], v);
-                    if (sr < s.nm && col < a.K) { put8((T *) a.dx + (size_t) (s.slot + sr) * a.K + col, v); }
-                }
-            }
+            sums.run(acc, p.rounds, c);
+            MatmulArgs r{};   // the sums alone
+            r.n = a.n; r.R = a.K; r.y = a.dx; r.parts = a.parts; r.part = a.part;
+            fwd_results<T, false, H, V>(r, s, p.part, acc);
         });
         i = queue.told(asked, lds);
     }
     queue.leave();
+}
+
+// ---------------------------------------------------------------- the parts of split sums, in order, and what follows the sum
+template <class T> __global__ void __launch_bounds__(256) k_mm_join(MatmulArgs a) {
+    int first = 0, last = a.n;
+    if (a.offsets) { first = min(max(a.offsets[0], 0), a.n); last = min(max(a.offsets[a.n_exp], 0), a.n); }
+    const int64_t all = (int64_t) a.n * a.R, end = (int64_t) last * (a.R / 8);
+    for (int64_t i = (int64_t) first * (a.R / 8) + (int64_t) blockIdx.x * 256 + threadIdx.x; i < end; i += (int64_t) gridDim.x * 256) {
+        float z[8] = {}, z2[8] = {}, y[8];
+        for (int p = 0; p < a.parts; ++p) {
+            add8(a.part + p * all + 8 * i, z);
+            if (a.W2) { add8(a.part + (a.parts + p) * all + 8 * i, z2); }
+        }
+        if (a.bias) {
+            const int slot = (int) (i / (a.R / 8)), col = (int) (i % (a.R / 8)) * 8;
+            int e = 0;   // the last expert whose slots begin at or before this one
+            if (a.offsets) { for (int b = NEXP_MAX / 2; b > 0; b >>= 1) { if (e + b < a.n_exp && a.offsets[e + b] <= slot) { e += b; } } }
+            add8(a.bias + (size_t) e * a.R + col, z);
+        }
+        activate8(a.act, z, y);
+        if (a.W2) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { y[u] *= z2[u]; }
+        }
+        if (a.residual) { add8((const T *) a.residual + 8 * i, y); }
+        if (a.y_f32) { put8((float *) a.y + 8 * i, y); } else { put8((T *) a.y + 8 * i, y); }
+        if (a.z) { put8((T *) a.z + 8 * i, z); }
+        if (a.z2) { put8((T *) a.z2 + 8 * i, z2); }
+    }
 }
 
 // ---------------------------------------------------------------- dW
@@ -644,12 +698,18 @@ constexpr int CUS = 256;
 int64_t most_tiles(int n, int n_exp, bool groups, int bm) { return ceil_div(n, bm) + (groups ? n_exp : 0); }
 unsigned grid_of(int64_t tiles, int per_cu) { return (unsigned) std::min<int64_t>(CUS * per_cu, ceil_div(tiles, 8) * 8); }
 
+template <class T> hipError_t join(const MatmulArgs & a, hipStream_t st) {
+    k_mm_join<T><<<(unsigned) std::min<int64_t>(4096, ceil_div((int64_t) a.n * a.R, 2048)), 256, 0, st>>>(a);
+    return hipGetLastError();
+}
 template <class T, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
     static LdsLimit limit;
     if (const hipError_t e = limit((const void *) k_mm<T, GATED, H>, H::LDS)) { return e; }
-    const int64_t tiles = most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.R, GATED ? H::BN / 2 : H::BN);
+    const int64_t tiles = most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.R, GATED ? H::BN / 2 : H::BN) * a.parts;
     k_mm<T, GATED, H><<<grid_of(tiles, H::PER_CU), H::threads, H::LDS, st>>>(a);
-    return hipGetLastError();
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.parts > 1) { e = join<T>(a, st); }
+    return e;
 }
 typedef Shape<256, 256, 3, 2, 1> Large;
 typedef Shape<128, 256, 3, 2, 1> Wide;
@@ -665,8 +725,14 @@ template <class T> hipError_t fwd(const MatmulArgs & a, hipStream_t st) { return
 template <class T, class H> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
     static LdsLimit limit;
     if (const hipError_t e = limit((const void *) k_mm_dx<T, H>, H::LDS)) { return e; }
-    k_mm_dx<T, H><<<grid_of(most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.K, H::BN), H::PER_CU), H::threads, H::LDS, st>>>(a);
-    return hipGetLastError();
+    k_mm_dx<T, H><<<grid_of(most_tiles(a.n, a.n_exp, a.offsets, H::BM) * ceil_div(a.K, H::BN) * a.parts, H::PER_CU), H::threads, H::LDS, st>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.parts > 1) {
+        MatmulArgs j{};   // the sums alone
+        j.n = a.n; j.R = a.K; j.n_exp = a.n_exp; j.offsets = a.offsets; j.y = a.dx; j.parts = a.parts; j.part = a.part;
+        e = join<T>(j, st);
+    }
+    return e;
 }
 template <class T> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
     switch (a.shape) {

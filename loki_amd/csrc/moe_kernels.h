@@ -303,14 +303,15 @@ struct MatmulArgs {
     const int * offsets; const int * perm; uint32_t magic; int xrows;   // perm may be null: slot s reads row s of x
     const void * x, * W, * W2; const float * bias; const void * residual;
     void * y, * z, * z2; int y_f32;
-    int shape; int * queue;                  // MM_*; 16 counters, 0 between launches
+    int shape, parts; float * part;          // MM_*; the sums are split into so many parts [parts][n][R] (gated: and once more)
+    int * queue;                             // 16 counters, 0 between launches
 };
 struct MatmulGradArgs {
     int type, n, R, K, n_exp;
     const int * offsets; const int * perm; uint32_t magic; int xrows;
     const void * dz, * dz2, * x, * W, * W2;
     void * dx, * dW, * dW2; int dw_f32, accumulate;
-    int shape; int * queue;
+    int shape, parts; float * part; int * queue;   // (dx's)
 };
 struct ActGradArgs {
     int type, act, n, R, n_exp; const int * offsets;
