@@ -467,7 +467,7 @@ extern "C" int fl_matmul_dev(FLCtx * c, int type, int act, const void * x, const
     a.type = type; a.act = act; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.x = x; a.W = W; a.W2 = W2; a.bias = bias; a.residual = residual; a.y = y; a.z = z; a.z2 = z2; a.y_f32 = y_type == FL_F32;
     a.queue = c->mm_queue;
-    const MmPlan plan = mm_plan(n, n_exp, W2 ? 2 * R : R, K);
+    const MmPlan plan = mm_plan(n, n_exp, W2 ? 2 * R : R, K, true);
     a.shape = plan.shape; a.parts = plan.parts;
     if (plan.parts > 1) {
         if (int rc = grow(c, c->mm, (size_t) plan.parts * n * R * (W2 ? 8 : 4))) { return rc; }
@@ -502,7 +502,7 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
     a.dz = dz; a.dz2 = dz2; a.x = x; a.W = W; a.W2 = W2; a.dx = dx; a.dW = dW; a.dW2 = dW2; a.dw_f32 = dw_type == FL_F32; a.accumulate = accumulate ? 1 : 0;
     a.queue = c->mm_queue;
     if (dx && n > 0) {
-        const MmPlan plan = mm_plan(n, n_exp, K, dz2 ? 2 * R : R);
+        const MmPlan plan = mm_plan(n, n_exp, K, dz2 ? 2 * R : R, false);
         a.shape = plan.shape; a.parts = plan.parts;
         if (plan.parts > 1) {
             if (int rc = grow(c, c->mm, (size_t) plan.parts * n * K * 4)) { return rc; }

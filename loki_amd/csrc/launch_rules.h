@@ -108,10 +108,15 @@ constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {
 // terms, weights from memory). Examples, us, Small / Wide / Large, then the best split: 64 rows, 7168 terms -> 2048 columns 54 / 74 / -, 17 (Small, 8
 // parts); 501, 7168 -> 2048 53 / 75 / 141, 33 (Wide, 4); 501, 2048 -> 7168 29 / 29 / 57; 1024, 7168 -> 7168 137 / 93 / 144; 2048, 7168 -> 7168
 // 302 / 203 / 173; 2048, 2048 -> 2048 33 / 31 / 58; 512 rows, columns and terms 7.6 / 13 / 25.
-enum { MM_SMALL, MM_WIDE, MM_LARGE };
+enum { MM_SMALL, MM_WIDE, MM_LARGE, MM_FEW };
 struct MmPlan { int shape, parts; };
-struct MmCost { int bm, bn, slots; float fixed, one, full; };
-constexpr MmCost MM_COST[3] = { { 64, 128, 512, 3.7f, 0.40f, 0.69f }, { 128, 256, 256, 5.4f, 0.55f, 0.86f }, { 256, 256, 256, 10.0f, 1.07f, 1.33f } };
+struct MmCost { int bm, bn, slots; float fixed, one, full, stream; };
+constexpr MmCost MM_COST[3] = { { 64, 128, 512, 3.7f, 0.40f, 0.69f, 1.f }, { 128, 256, 256, 5.4f, 0.55f, 0.86f, 1.06f }, { 256, 256, 256, 10.0f, 1.07f, 1.33f, 1.08f } };
+// experts with rows, about: n_exp (1 - e^-x) for x rows an expert
+constexpr float mm_used(int n, int n_exp) {
+    const float x = (float) n / (float) n_exp;
+    return n_exp == 1 || x > 3.f ? (float) n_exp : (float) n_exp * x / (1.f + 0.5f * x + 0.0833f * x * x);
+}
 constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int terms) {
     const MmCost k = MM_COST[shape];
     const float per = (float) n / (float) n_exp;
@@ -125,13 +130,22 @@ constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int te
     if (n_exp == 1 || waves < 1.f) { const int w = (int) waves; waves = (float) w < waves ? (float) (w + 1) : (float) w; }
     const float cost = (k.one + (k.full - k.one) * busy) * (shape == MM_LARGE && n_exp > 1 ? 0.4f + 0.6f * fill : 1.f);
     const float sums = waves * (k.fixed + (float) r * cost);
-    const float used = n_exp == 1 ? 1.f : per / (0.6f + per) * (float) n_exp;   // experts with rows, about
-    const float memory = (float) cols * (float) terms * used * 3.1e-7f + (float) n * (float) cols * 4e-7f;         // the weights and the results
+    const float memory = ((float) cols * (float) terms * mm_used(n, n_exp) * 3.1e-7f + (float) n * (float) cols * 4e-7f) * k.stream;   // the weights and the results
     const float join = parts > 1 ? 4.f + 0.15f * (float) parts + (float) parts * (float) n * (float) cols * 1.2e-6f : 0.f;
     return 2.5f + (sums > memory ? sums + 0.15f * memory : memory + 0.15f * sums) + join;
 }
+// Few rows (matmul_few.hip; up to 16 of an expert with one reading of its matrix): 16 columns a workgroup, whose 8 waves take 64 terms each in turn.
+// Us against the best of the above: 1 row of 2048 terms -> 7168 columns 9.5 / 14, 7168 -> 7168 19 / 24, 7168 -> 131072 358 / 306; 8 rows 10.5 / 14,
+// 24 / 24, 461 / 307; 16 rows 11.5 / 15, 28 / 24; one token's 8 experts of 256, 7168 -> 2 x 2048, 90 / 89, two tokens' 171 / 150; 6 of 64, 2048 ->
+// 2 x 1024, 12 / 21, 48 51 / 60, 192 98 / 97.
+constexpr float mm_few_time(int n, int n_exp, int cols, int terms) {
+    const float used = mm_used(n, n_exp), rows = (float) n / used;
+    const float tiles = n_exp == 1 ? (float) ((n + 15) / 16) : rows < 8.f ? used : used * (0.5f + rows / 16.f), groups = tiles * (float) cols / 16.f;
+    const float memory = (float) cols * (float) terms * tiles * 2.9e-7f * (1.f + 0.036f * (rows < 16.f ? rows : 16.f)), waves = 0.53f * (float) ((terms + 511) / 512);
+    return 4.f + (memory > waves ? memory : waves) + (groups > 1024.f ? 0.01f * (groups - 1024.f) : 0.f);
+}
 // n rows of n_exp experts, `cols` results a row (gated: of both matrices), sums of `terms`
-constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms) {
+constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms, bool forward) {
     const int split[8] = { 1, 2, 3, 4, 6, 8, 12, 16 };
     MmPlan best{ MM_SMALL, 1 };
     float least = mm_time(MM_SMALL, 1, n, n_exp, cols, terms);
@@ -142,6 +156,7 @@ constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms) {
             if (t < least) { least = t; best = { s, split[i] }; }
         }
     }
+    if (forward && n <= 1 << 15 && mm_few_time(n, n_exp, cols, terms) < least) { return { MM_FEW, 1 }; }
     return best;
 }
 

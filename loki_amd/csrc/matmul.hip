@@ -18,7 +18,6 @@
 // of memory ("col" operand) has a row a term, segments of 32 bytes at segment ^ (term % 4 + term / 8 % 2 * 4), and is transposed by
 // ds_read_b64_tr_b16: 16 lanes read 4 terms x 16 columns and each gets its column's 4.
 #include "matmul_device.h"
-#include <type_traits>
 
 namespace lk {
 namespace {
@@ -43,13 +42,7 @@ __device__ __forceinline__ void meet() {
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
 }
-__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ u32x4 buffer(uint64_t base, uint32_t bytes) { return (u32x4) { (uint32_t) base, (uint32_t) (base >> 32) & 0xFFFFu, bytes, 0x00020000u }; }
-__device__ __forceinline__ uint64_t uni64(const void * p) {
-    const uint64_t v = (uint64_t) p;
-    return ((uint64_t) (uint32_t) uni((int) (uint32_t) (v >> 32)) << 32) | (uint32_t) uni((int) (uint32_t) v);
-}
-
 // a row operand's lane: of a piece of 8 rows it copies chunk(piece) of row lane / 8; it reads row lane % 16, chunk lane / 16 (second half: ^ 64)
 struct RowLane {
     uint32_t read;
@@ -88,41 +81,6 @@ template <class T, int COLS> __device__ __forceinline__ V8<T> lds_col(uint32_t a
 }
 
 // ---------------------------------------------------------------- the launch's tiles
-// m-tiles of the experts before e, lane l's of experts 4 l .. 4 l + 3 (LDS is the operands'); all: of all experts
-struct Tiles {
-    int first[4], all;
-    __device__ __forceinline__ Tiles(const int * offsets, int n, int n_exp, int bm) {
-        const int l = lane_id();
-        int c[4], s = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = 4 * l + j;
-            c[j] = 0;
-            if (e < n_exp) { const Span sp = span_of(offsets, n, e); c[j] = (sp.end - sp.begin + bm - 1) / bm; }
-            s += c[j];
-        }
-        int si = s;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(si, o); if (l >= o) { si += v; } }
-        int at = si - s;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { first[j] = at; at += c[j]; }
-        all = __builtin_amdgcn_readlane(at, 63);
-    }
-    __device__ __forceinline__ int before(int e) const {   // (e uniform)
-        int v = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { const int w = __builtin_amdgcn_readlane(first[j], (e >> 2) & 63); v = (e & 3) == j ? w : v; }
-        return e >= NEXP_MAX ? all : v;
-    }
-    // the expert of m-tile i, i < all: the last one whose tiles begin at or before it
-    __device__ __forceinline__ int expert(int i) const {
-        int e = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { e += __popcll(__ballot(first[j] <= i)); }
-        return uni(e) - 1;
-    }
-};
 struct Spot { int e, slot, nm, n0; };   // expert, first slot, its slots in the tile, first column
 // the sum's part of work item i: parts come one after the other, each with all tiles; rounds d0 .. d0 + rounds - 1
 struct Part { int tile, part, d0, rounds; };
@@ -306,27 +264,6 @@ __device__ __forceinline__ void eight(f32x4 a, f32x4 b, float (&v)[8]) {
     }
 #endif
 }
-template <class T> __device__ __forceinline__ void put8(T * p, const float (&v)[8]) {
-    V8<T> u;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { u[i] = (T) v[i]; }
-    *(LK_GLOBAL V8<T> *) p = u;
-}
-__device__ __forceinline__ void put8(float * p, const float (&v)[8]) {
-    *(LK_GLOBAL f32x4 *) p = (f32x4) { v[0], v[1], v[2], v[3] };
-    *(LK_GLOBAL f32x4 *) (p + 4) = (f32x4) { v[4], v[5], v[6], v[7] };
-}
-template <class T> __device__ __forceinline__ void add8(const T * p, float (&v)[8]) {
-    const V8<T> u = *(const LK_GLOBAL V8<T> *) p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) { v[i] += (float) u[i]; }
-}
-__device__ __forceinline__ void add8(const float * p, float (&v)[8]) {
-    const f32x4 a = *(const LK_GLOBAL f32x4 *) p, b = *(const LK_GLOBAL f32x4 *) (p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] += a[i]; v[4 + i] += b[i]; }
-}
-
 // The workgroups (a multiple of 8) go round the 8 XCDs; an XCD's tiles are a run of the launch's, so that what runs at a time there shares
 // panels in its L2. Tiles differ in cost, so after its first a workgroup takes the XCD's next one (queue[x]); the last to find none
 // sets the two counters back to 0 for the next launch.
@@ -756,7 +693,10 @@ template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t
 
 }  // namespace
 
-hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st) { return a.type == TYPE_BF16 ? fwd<__bf16>(a, st) : fwd<_Float16>(a, st); }
+hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st) {
+    if (a.shape == MM_FEW) { return launch_matmul_few(a, st); }
+    return a.type == TYPE_BF16 ? fwd<__bf16>(a, st) : fwd<_Float16>(a, st);
+}
 hipError_t launch_matmul_dx(const MatmulGradArgs & a, hipStream_t st) { return a.type == TYPE_BF16 ? dx<__bf16>(a, st) : dx<_Float16>(a, st); }
 hipError_t launch_matmul_dw(const MatmulGradArgs & a, hipStream_t st) {
     if (a.dw_f32) { return a.type == TYPE_BF16 ? dw<__bf16, true>(a, st) : dw<_Float16, true>(a, st); }

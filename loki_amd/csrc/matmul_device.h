@@ -2,6 +2,8 @@
 #pragma once
 #include "moe_common.h"
 #include "moe_kernels.h"
+#include <algorithm>
+#include <type_traits>
 
 namespace lk {
 
@@ -72,5 +74,69 @@ __device__ __forceinline__ Span span_of(const int * offsets, int n, int e) {
 // the pair's row: perm[slot] / topk by a product with 2^32 / topk rounded up (exact below 2^28 for topk <= 8); rows outside 0 .. xrows - 1
 // come out as xrows or more
 __device__ __forceinline__ uint32_t pair_row(uint32_t pair, uint32_t magic) { return magic ? __umulhi(pair, magic) : pair; }
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uni64(const void * p) {
+    const uint64_t v = (uint64_t) p;
+    return ((uint64_t) (uint32_t) uni((int) (uint32_t) (v >> 32)) << 32) | (uint32_t) uni((int) (uint32_t) v);
+}
+
+// m-tiles of the experts before e, lane l's of experts 4 l .. 4 l + 3 (no LDS: the operands may fill it); all: of all experts
+struct Tiles {
+    int first[4], all;
+    __device__ __forceinline__ Tiles(const int * offsets, int n, int n_exp, int bm) {
+        const int l = lane_id();
+        int c[4], s = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = 4 * l + j;
+            c[j] = 0;
+            if (e < n_exp) { const Span sp = span_of(offsets, n, e); c[j] = (sp.end - sp.begin + bm - 1) / bm; }
+            s += c[j];
+        }
+        int si = s;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) { const int v = __shfl_up(si, o); if (l >= o) { si += v; } }
+        int at = si - s;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { first[j] = at; at += c[j]; }
+        all = __builtin_amdgcn_readlane(at, 63);
+    }
+    __device__ __forceinline__ int before(int e) const {   // (e uniform)
+        int v = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { const int w = __builtin_amdgcn_readlane(first[j], (e >> 2) & 63); v = (e & 3) == j ? w : v; }
+        return e >= NEXP_MAX ? all : v;
+    }
+    // the expert of m-tile i, i < all: the last one whose tiles begin at or before it
+    __device__ __forceinline__ int expert(int i) const {
+        int e = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { e += __popcll(__ballot(first[j] <= i)); }
+        return uni(e) - 1;
+    }
+};
+
+// ---------------------------------------------------------------- 8 values next to each other
+template <class T> __device__ __forceinline__ void put8(T * p, const float (&v)[8]) {
+    V8<T> u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { u[i] = (T) v[i]; }
+    *(LK_GLOBAL V8<T> *) p = u;
+}
+__device__ __forceinline__ void put8(float * p, const float (&v)[8]) {
+    *(LK_GLOBAL f32x4 *) p = (f32x4) { v[0], v[1], v[2], v[3] };
+    *(LK_GLOBAL f32x4 *) (p + 4) = (f32x4) { v[4], v[5], v[6], v[7] };
+}
+template <class T> __device__ __forceinline__ void add8(const T * p, float (&v)[8]) {
+    const V8<T> u = *(const LK_GLOBAL V8<T> *) p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { v[i] += (float) u[i]; }
+}
+__device__ __forceinline__ void add8(const float * p, float (&v)[8]) {
+    const f32x4 a = *(const LK_GLOBAL f32x4 *) p, b = *(const LK_GLOBAL f32x4 *) (p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] += a[i]; v[4 + i] += b[i]; }
+}
 
 }  // namespace lk

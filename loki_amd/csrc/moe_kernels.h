@@ -322,7 +322,8 @@ struct CombineArgs {
     const void * o, * residual; void * y; int y_f32;    // combine
     const void * dy; void * d_o; float * dw;            // its gradient
 };
-hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st);
+hipError_t launch_matmul(const MatmulArgs & a, hipStream_t st);        // (MM_FEW: launch_matmul_few)
+hipError_t launch_matmul_few(const MatmulArgs & a, hipStream_t st);   // n at most 65535 * 16
 hipError_t launch_matmul_dx(const MatmulGradArgs & a, hipStream_t st);
 hipError_t launch_matmul_dw(const MatmulGradArgs & a, hipStream_t st);
 int act_grad_chunks(int n, int R, int n_exp);             // row chunks an expert's bias gradient is summed in
