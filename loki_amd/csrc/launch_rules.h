@@ -130,7 +130,7 @@ constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int te
     if (n_exp == 1 || waves < 1.f) { const int w = (int) waves; waves = (float) w < waves ? (float) (w + 1) : (float) w; }
     const float cost = (k.one + (k.full - k.one) * busy) * (shape == MM_LARGE && n_exp > 1 ? 0.4f + 0.6f * fill : 1.f);
     const float sums = waves * (k.fixed + (float) r * cost);
-    const float memory = ((float) cols * (float) terms * mm_used(n, n_exp) * 3.1e-7f + (float) n * (float) cols * 4e-7f) * k.stream;   // the weights and the results
+    const float memory = ((float) cols * (float) terms * mm_used(n, n_exp) * 3.1e-7f + (float) n * (float) cols * 4e-7f) * (shape == MM_SMALL && busy == 0.f ? 1.3f : k.stream);   // the weights and the results
     const float join = parts > 1 ? 4.f + 0.15f * (float) parts + (float) parts * (float) n * (float) cols * 1.2e-6f : 0.f;
     return 2.5f + (sums > memory ? sums + 0.15f * memory : memory + 0.15f * sums) + join;
 }

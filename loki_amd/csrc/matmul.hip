@@ -440,20 +440,27 @@ template <class T, bool GATED, class H> __global__ void __launch_bounds__(H::thr
     const Tiles tiles(a.offsets, a.n, a.n_exp, H::BM);
     const Queue queue(a.queue, tiles.all * nt * a.parts);
     const uint32_t lds = lds_addr(dyn);
-    for (int i = queue.begin(); i < queue.last;) {
-        const Part p = part_of(i, tiles.all * nt, a.parts, (a.K + BK - 1) / BK);
-        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, p.tile);
+    const int rounds = (a.K + BK - 1) / BK;
+    int i = queue.begin();
+    auto part = [&](int t) __attribute__((always_inline)) { return part_of(t, tiles.all * nt, a.parts, rounds); };
+    auto spot = [&](const Part & p) __attribute__((always_inline)) { return spot_of(tiles, a.offsets, a.n, nt, H::BM, C::CN, 4, p.tile); };
+    auto first = [&](int t) __attribute__((always_inline)) {
+        if (t < queue.last) { const Part p = part(t); C c(a, spot(p), p); start<H>(c, lds); }
+    };
+    for (first(i); i < queue.last;) {
         const int asked = queue.ask();
+        const Part p = part(i);
+        const Spot s = spot(p);
         by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
             typedef decltype(v) V;
             const Sums<T, false, false, H, V, C> sums(lds);
             C c(a, s, p);
-            start<H>(c, lds);
             f32x4 acc[V::FM][V::FN];
             sums.run(acc, p.rounds, c);
+            i = queue.told(asked, lds);
+            first(i);   // the next tile's first copies are out while this one's results are written
             fwd_results<T, GATED, H, V>(a, s, p.part, acc);
         });
-        i = queue.told(asked, lds);
     }
     queue.leave();
 }
@@ -489,22 +496,28 @@ template <class T, class H> __global__ void __launch_bounds__(H::threads, H::PER
     const Queue queue(a.queue, tiles.all * nt * a.parts);
     const uint32_t lds = lds_addr(dyn);
     const int rounds = (a.R + BK - 1) / BK * (a.dz2 ? 2 : 1);
-    for (int i = queue.begin(); i < queue.last;) {
-        const Part p = part_of(i, tiles.all * nt, a.parts, rounds);
-        const Spot s = spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, p.tile);
+    int i = queue.begin();
+    auto part = [&](int t) __attribute__((always_inline)) { return part_of(t, tiles.all * nt, a.parts, rounds); };
+    auto spot = [&](const Part & p) __attribute__((always_inline)) { return spot_of(tiles, a.offsets, a.n, nt, H::BM, H::BN, 4, p.tile); };
+    auto first = [&](int t) __attribute__((always_inline)) {
+        if (t < queue.last) { const Part p = part(t); C c(a, spot(p), p); start<H>(c, lds); }
+    };
+    for (first(i); i < queue.last;) {
         const int asked = queue.ask();
+        const Part p = part(i);
+        const Spot s = spot(p);
         by_rows<H>(s.nm, [&](auto v) __attribute__((always_inline)) {
             typedef decltype(v) V;
             const Sums<T, false, true, H, V, C> sums(lds);
             C c(a, s, p);
-            start<H>(c, lds);
             f32x4 acc[V::FM][V::FN];
             sums.run(acc, p.rounds, c);
+            i = queue.told(asked, lds);
+            first(i);
             MatmulArgs r{};   // the sums alone
             r.n = a.n; r.R = a.K; r.y = a.dx; r.parts = a.parts; r.part = a.part;
             fwd_results<T, false, H, V>(r, s, p.part, acc);
         });
-        i = queue.told(asked, lds);
     }
     queue.leave();
 }
