@@ -510,7 +510,17 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
         }
         TRY(c, launch_matmul_dx(a, c->st));
     }
-    if (dW || dW2) { TRY(c, launch_matmul_dw(a, c->st)); }   // (no rows: 0, or it stays)
+    if (dW || dW2) {   // (no rows: 0, or it stays)
+        const int mats = (dW ? 1 : 0) + (dW2 ? 1 : 0);
+        const MmPlan plan = dw_plan(n, n_exp, R, K, mats);
+        a.dw_shape = plan.shape; a.dw_parts = plan.parts;
+        if (n == 0) { a.perm = nullptr; }
+        if (plan.parts > 1) {
+            if (int rc = grow(c, c->mm, (size_t) plan.parts * mats * wn * 4)) { return rc; }
+            a.dw_part = (float *) c->mm.p;
+        }
+        TRY(c, launch_matmul_dw(a, c->st));
+    }
     return FL_OK;
 }
 extern "C" int fl_act_grad_dev(FLCtx * c, int type, int act, const void * dy, const void * z, const void * z2, int n, int R, int n_exp, const int * offsets,

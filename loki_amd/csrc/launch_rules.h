@@ -128,7 +128,7 @@ constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int te
     float waves = items / (float) k.slots;
     const float busy = waves >= 1.f ? 1.f : shape == MM_SMALL ? (waves > 0.5f ? 1.f : 0.f) : waves;
     if (n_exp == 1 || waves < 1.f) { const int w = (int) waves; waves = (float) w < waves ? (float) (w + 1) : (float) w; }
-    const float cost = (k.one + (k.full - k.one) * busy) * (shape == MM_LARGE && n_exp > 1 ? 0.4f + 0.6f * fill : 1.f);
+    const float cost = (k.one + (k.full - k.one) * busy) * (shape == MM_LARGE && n_exp > 1 ? 0.62f + 0.38f * fill : 1.f);
     const float sums = waves * (k.fixed + (float) r * cost);
     const float memory = ((float) cols * (float) terms * mm_used(n, n_exp) * 3.1e-7f + (float) n * (float) cols * 4e-7f) * (shape == MM_SMALL && busy == 0.f ? 1.3f : k.stream);   // the weights and the results
     const float join = parts > 1 ? 4.f + 0.15f * (float) parts + (float) parts * (float) n * (float) cols * 1.2e-6f : 0.f;
@@ -157,6 +157,37 @@ constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms, bool forward) {
         }
     }
     if (forward && n <= 1 << 15 && mm_few_time(n, n_exp, cols, terms) < least) { return { MM_FEW, 1 }; }
+    return best;
+}
+
+// dW of `mats` matrices [n_exp][R][K] from n rows: tiles of 256 x 256 (MM_LARGE), of 128 x 128 with two workgroups a CU (MM_SMALL) or four
+// that keep nothing ahead (MM_FEW); the rows can be split into parts. As above, fitted to 25 sizes. Us, MM_SMALL / MM_LARGE / MM_FEW: 16 rows,
+// 7168 x 7168 31 / 35 / 24; 501 68 / 74 / 64; 8192 943 / 673 / 1088; 8192 rows, 2048 x 2048 71 / - / -, 512 x 512 29 and 18 in 8 parts; 256 experts of
+// 4, 128 and 256 rows, 7168 x 2048, 1899 / 1928 / 1378, 2629 / 2487 / 2317, 3720 / 3370 / 3089.
+constexpr float dw_time(int shape, int parts, int n, int n_exp, int R, int K, int mats) {
+    const int b = shape == MM_LARGE ? 256 : 128, slots = shape == MM_LARGE ? 256 : shape == MM_FEW ? 1024 : 512;
+    const float fixed = shape == MM_LARGE ? 10.f : shape == MM_FEW ? 5.4f : 5.f, one = shape == MM_LARGE ? 0.92f : shape == MM_FEW ? 1.05f : 0.5f,
+                full = shape == MM_LARGE ? 1.28f : shape == MM_FEW ? 1.75f : 0.88f;
+    const float all = (float) ((R + b - 1) / b) * (float) ((K + b - 1) / b) * (float) n_exp * (float) mats * (float) parts;
+    const float rounds = n_exp == 1 ? (float) ((n + 63) / 64) : (float) n / (float) n_exp / 64.f + 0.5f;
+    const float r = parts == 1 ? rounds : (float) (int) (rounds / (float) parts + 0.999f);
+    float waves = all / (float) slots;
+    const float busy = waves >= 1.f ? 1.f : shape == MM_SMALL ? (waves > 0.5f ? 1.f : 0.f) : waves;
+    if (waves < 8.f) { const int w = (int) waves; waves = (float) w < waves ? (float) (w + 1) : (float) w; }
+    const float values = (float) R * (float) K * (float) n_exp * (float) mats, sums = waves * (fixed + r * (one + (full - one) * busy)), memory = values * 3.7e-7f;
+    return 2.5f + (sums > memory ? sums + 0.15f * memory : memory + 0.15f * sums) + (parts > 1 ? 4.f + 0.15f * (float) parts + (float) parts * values * 1.2e-6f : 0.f);
+}
+constexpr MmPlan dw_plan(int n, int n_exp, int R, int K, int mats) {
+    const int split[8] = { 1, 2, 4, 8, 16, 1, 1, 1 }, shapes[3] = { MM_SMALL, MM_LARGE, MM_FEW };
+    MmPlan best{ MM_SMALL, 1 };
+    float least = dw_time(MM_SMALL, 1, n, n_exp, R, K, mats);
+    for (int s = 0; s < 3; ++s) {
+        for (int i = 0; i < 5; ++i) {
+            if (split[i] > 1 && (long long) split[i] * 128 * n_exp > n) { break; }   // two rounds a part at least
+            const float t = dw_time(shapes[s], split[i], n, n_exp, R, K, mats);
+            if (t < least) { least = t; best = { shapes[s], split[i] }; }
+        }
+    }
     return best;
 }
 

@@ -182,6 +182,19 @@ template <class T, bool AC, bool BC, class H, class V, class Copies> struct Sums
             if constexpr (AC) { f.a[i] = lds_col<T, H::BM>(at.a[i % RA] + (uint32_t) (i / RA * 256 + h * 32 * H::BM * 2)); } else { f.a[i] = lds_row<T>(at.a[h] + (uint32_t) (i * 2048)); }
         }
     }
+    // the products of one round that is there, in the first places
+    __device__ __forceinline__ void round(f32x4 (&acc)[FM][FN]) const {
+        At at;
+        at_round(at, 0, 0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            F f;
+#pragma unroll
+            for (int j = 0; j < FM + FN; ++j) { read(f, at, h, j); }
+#pragma unroll
+            for (int j = 0; j < FM * FN; ++j) { acc[j / FN][j % FN] = mfma32(f.b[j % FN], f.a[j / FN], acc[j / FN][j % FN]); }
+        }
+    }
     __device__ __forceinline__ void run(f32x4 (&acc)[FM][FN], int rounds, Copies & c) const {
         constexpr int MF = FM * FN, RD = FM + FN, RG = MF - MF / 4 - 1;   // groups of one product: the first, RG with reads and copies, the rest
         constexpr int LATER = (H::SB - 1) * H::CA + (H::SB - 2) * H::CB < (H::SA - 2) * (H::CA + H::CB) ? (H::SB - 1) * H::CA + (H::SB - 2) * H::CB : (H::SA - 2) * (H::CA + H::CB);
@@ -607,38 +620,117 @@ template <class T, bool PERM, class H> struct DwCopies {
     __device__ __forceinline__ void copy_a(int) const { a.copy(); }
     __device__ __forceinline__ void copy_b(int) const { b.copy(); }
 };
-// one workgroup a tile: [matrix][expert][band of m-tiles][n][m of the band]; an XCD's share is a run of them
-template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm_dw(MatmulGradArgs a, int mt, int nt) {
+// tile i of the launch: [matrix][expert][band of m-tiles][n][m of the band]; a part is a run of the expert's rounds
+struct DwSpot { int e, begin, len, m0, n0, part; bool second; };
+template <class H> __device__ __forceinline__ DwSpot dw_spot(const MatmulGradArgs & a, int i) {
+    constexpr int BAND = 4;
+    const int mt = (a.R + H::BM - 1) / H::BM, nt = (a.K + H::BN - 1) / H::BN, per = mt * nt, all = per * a.n_exp * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0));
+    DwSpot s;
+    s.part = a.dw_parts > 1 ? uni(i / all) : 0;
+    i -= s.part * all;
+    const int which = uni(i / per), in = i - which * per, band = in / (BAND * nt), rows = min(BAND, mt - band * BAND), r = in - band * BAND * nt;
+    s.e = uni(which % a.n_exp);
+    s.second = which >= a.n_exp || !a.dW;
+    const Span sp = span_of(a.offsets, a.n, s.e);
+    s.begin = uni(sp.begin); s.len = uni(sp.end) - s.begin;
+    if (a.dw_parts > 1) {
+        const int rounds = (s.len + BK - 1) / BK, d0 = uni((int) ((int64_t) rounds * s.part / a.dw_parts)), d1 = uni((int) ((int64_t) rounds * (s.part + 1) / a.dw_parts));
+        s.begin += d0 * BK; s.len = min(s.len - d0 * BK, (d1 - d0) * BK);
+    }
+    s.m0 = uni((band * BAND + r % rows) * H::BM); s.n0 = uni(r / rows * H::BN);
+    return s;
+}
+// the results of a tile
+template <class T, bool F32, class V> __device__ __forceinline__ void dw_results(const MatmulGradArgs & a, const DwSpot & s, f32x4 (&acc)[V::FM][V::FN]) {
+    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
+    const size_t w = (size_t) a.R * a.K, t0 = (size_t) s.e * w + (size_t) s.m0 * a.K + s.n0;
+    auto each = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < V::FM; ++m) {
+            const int row = (wm * V::FM + m) * 16 + (lane & 15);
+#pragma unroll
+            for (int j = 0; j < V::FN; j += 2) {
+                const int col = (wn * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
+                float v[8];
+                eight(acc[m][j], acc[m][j + 1], v);
+                if (s.m0 + row < a.R && s.n0 + col < a.K) { f((uint32_t) row * (uint32_t) a.K + (uint32_t) col, v); }
+            }
+        }
+    };
+    typedef typename std::conditional<F32, float, T>::type O;
+    O * d = (O *) (s.second ? a.dW2 : a.dW) + t0;
+    if (a.dw_parts > 1) {
+        float * p = a.dw_part + ((size_t) s.part * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0)) + (a.dW && s.second ? 1 : 0)) * a.n_exp * w + t0;
+        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { put8(p + at, v); });
+    } else if (a.accumulate) {
+        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { add8(d + at, v); put8(d + at, v); });
+    } else {
+        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { put8(d + at, v); });
+    }
+}
+// one workgroup a tile, and an XCD's share a run of them: what a workgroup has written need not have arrived when the next one starts
+__device__ __forceinline__ int dw_tile() {
+    const int all = (int) gridDim.x, x = (int) blockIdx.x % 8;
+    return all / 8 * x + min(x, all % 8) + (int) blockIdx.x / 8;
+}
+template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm_dw(MatmulGradArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef DwCopies<T, PERM, H> C;
-    constexpr int BAND = 4;
     typedef Waves<H, H::BM, 2> V;
-    const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
-    const int all = (int) gridDim.x, x = (int) blockIdx.x % 8, t = all / 8 * x + min(x, all % 8) + (int) blockIdx.x / 8;
-    const int per = mt * nt, which = t / per, e = which % a.n_exp, in = t % per, band = in / (BAND * nt), rows = min(BAND, mt - band * BAND), r = in - band * BAND * nt;
-    const bool second = which >= a.n_exp || !a.dW;
-    const Span sp = span_of(a.offsets, a.n, e);
-    const int begin = uni(sp.begin), len = uni(sp.end) - begin, m0 = (band * BAND + r % rows) * H::BM, n0 = r / rows * H::BN;
     const uint32_t lds = lds_addr(dyn);
+    const DwSpot s = dw_spot<H>(a, dw_tile());
     const Sums<T, true, true, H, V, C> sums(lds);
     C c;
-    c.init(a, second ? a.dz2 : a.dz, begin, len, m0, n0);
-    f32x4 acc[V::FM][V::FN];
+    c.init(a, s.second ? a.dz2 : a.dz, s.begin, s.len, s.m0, s.n0);
     start<H>(c, lds);
-    sums.run(acc, (len + BK - 1) / BK, c);
+    f32x4 acc[V::FM][V::FN];
+    sums.run(acc, (s.len + BK - 1) / BK, c);
+    dw_results<T, F32, V>(a, s, acc);
+}
+// few rows an expert: the results' memory bounds it, and a tile has a round or two. Nothing is kept ahead; four workgroups a CU cover each
+// other's waits (256 experts of 128 rows, 7168 x 2048: @DWFEW@)
+template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm_dw_few(MatmulGradArgs a) {
+    extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
+    typedef DwCopies<T, PERM, H> C;
+    typedef Waves<H, H::BM, 2> V;
+    const uint32_t lds = lds_addr(dyn);
+    const DwSpot s = dw_spot<H>(a, dw_tile());
+    const Sums<T, true, true, H, V, C> sums(lds);
+    f32x4 acc[V::FM][V::FN];
 #pragma unroll
-    for (int m = 0; m < V::FM; ++m) {
-        const int row = m0 + (wm * V::FM + m) * 16 + (lane & 15);
+    for (int i = 0; i < V::FM; ++i) {
 #pragma unroll
-        for (int j = 0; j < V::FN; j += 2) {
-            const int col = n0 + (wn * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
-            float v[8];
-            eight(acc[m][j], acc[m][j + 1], v);
-            if (row >= a.R || col >= a.K) { continue; }
-            const size_t at = ((size_t) e * a.R + row) * a.K + col;
-            if (F32) { float * d = (float *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
-            else { T * d = (T *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
+        for (int j = 0; j < V::FN; ++j) { acc[i][j] = (f32x4) { 0.f, 0.f, 0.f, 0.f }; }
+    }
+    if (s.len > 0) {
+        C c;
+        c.init(a, s.second ? a.dz2 : a.dz, s.begin, s.len, s.m0, s.n0);
+        for (int d = 0; d * BK < s.len; ++d) {
+            c.begin_a(d);
+#pragma unroll
+            for (int j = 0; j < H::CA; ++j) { c.set_a(j, lds); c.copy_a(j); }
+            c.begin_b(d);
+#pragma unroll
+            for (int j = 0; j < H::CB; ++j) { c.set_b(j, lds + H::LB); c.copy_b(j); }
+            wait_copies<0>();
+            meet();
+            sums.round(acc);
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            meet();
         }
+    }
+    dw_results<T, F32, V>(a, s, acc);
+}
+// the parts of dW, in order
+template <class T, bool F32> __global__ void __launch_bounds__(256) k_dw_join(MatmulGradArgs a, int64_t each) {
+    const int mats = (a.dW ? 1 : 0) + (a.dW2 ? 1 : 0);
+    for (int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < each / 8 * mats; i += (int64_t) gridDim.x * 256) {
+        float v[8] = {};
+        for (int p = 0; p < a.dw_parts; ++p) { add8(a.dw_part + p * each * mats + 8 * i, v); }
+        const bool second = i >= each / 8 || !a.dW;
+        const int64_t at = 8 * i - (second && a.dW ? each : 0);
+        if (F32) { float * d = (float *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
+        else { T * d = (T *) (second ? a.dW2 : a.dW) + at; if (a.accumulate) { add8(d, v); } put8(d, v); }
     }
 }
 
@@ -664,6 +756,7 @@ template <class T, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hip
 typedef Shape<256, 256, 3, 2, 1> Large;
 typedef Shape<128, 256, 3, 2, 1> Wide;
 typedef Shape<64, 128, 3, 2, 2> Small;
+typedef Shape<128, 128, 3, 2, 2> Middle;   // (dW)
 template <class T, bool GATED> hipError_t fwd(const MatmulArgs & a, hipStream_t st) {
     switch (a.shape) {
         case MM_LARGE: return fwd<T, GATED, Large>(a, st);
@@ -691,16 +784,27 @@ template <class T> hipError_t dx(const MatmulGradArgs & a, hipStream_t st) {
         default: return dx<T, Small>(a, st);
     }
 }
-template <class T, bool F32, bool PERM, class H> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
+template <class T, bool F32, bool PERM, class H, bool FEW> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
     static LdsLimit limit;
-    if (const hipError_t e = limit((const void *) k_mm_dw<T, F32, PERM, H>, H::LDS)) { return e; }
-    const int mt = (int) ceil_div(a.R, H::BM), nt = (int) ceil_div(a.K, H::BN);
-    k_mm_dw<T, F32, PERM, H><<<(unsigned) (mt * nt * a.n_exp * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0))), H::threads, H::LDS, st>>>(a, mt, nt);
-    return hipGetLastError();
+    const int mats = (a.dW ? 1 : 0) + (a.dW2 ? 1 : 0);
+    const int64_t all = ceil_div(a.R, H::BM) * ceil_div(a.K, H::BN) * a.n_exp * mats * a.dw_parts, each = (int64_t) a.n_exp * a.R * a.K;
+    if constexpr (FEW) {
+        if (const hipError_t e = limit((const void *) k_mm_dw_few<T, F32, PERM, H>, H::LDS)) { return e; }
+        k_mm_dw_few<T, F32, PERM, H><<<(unsigned) all, H::threads, H::LDS, st>>>(a);
+    } else {
+        if (const hipError_t e = limit((const void *) k_mm_dw<T, F32, PERM, H>, H::LDS)) { return e; }
+        k_mm_dw<T, F32, PERM, H><<<(unsigned) all, H::threads, H::LDS, st>>>(a);
+    }
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.dw_parts > 1) {
+        k_dw_join<T, F32><<<(unsigned) std::min<int64_t>(4096, ceil_div(each * mats, 2048)), 256, 0, st>>>(a, each);
+        e = hipGetLastError();
+    }
+    return e;
 }
 template <class T, bool F32, bool PERM> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) {
-    if ((int64_t) a.R * a.K * a.n_exp >= (int64_t) 192 * 256 * 256) { return dw<T, F32, PERM, Large>(a, st); }
-    return dw<T, F32, PERM, Shape<128, 128, 3, 2, 2>>(a, st);
+    if (a.dw_shape == MM_FEW) { return dw<T, F32, PERM, Shape<128, 128, 1, 1, 4>, true>(a, st); }
+    return a.dw_shape == MM_LARGE ? dw<T, F32, PERM, Large, false>(a, st) : dw<T, F32, PERM, Middle, false>(a, st);
 }
 template <class T, bool F32> hipError_t dw(const MatmulGradArgs & a, hipStream_t st) { return a.perm && a.n > 0 ? dw<T, F32, true>(a, st) : dw<T, F32, false>(a, st); }
 

@@ -311,7 +311,9 @@ struct MatmulGradArgs {
     const int * offsets; const int * perm; uint32_t magic; int xrows;
     const void * dz, * dz2, * x, * W, * W2;
     void * dx, * dW, * dW2; int dw_f32, accumulate;
-    int shape, parts; float * part; int * queue;   // (dx's)
+    int shape, parts; float * part;                // dx's, as above
+    int dw_shape, dw_parts; float * dw_part;       // dW's: [parts][matrices][n_exp][R][K]
+    int * queue;
 };
 struct ActGradArgs {
     int type, act, n, R, n_exp; const int * offsets;
