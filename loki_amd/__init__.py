@@ -25,6 +25,7 @@ FL_OK, FL_EINVAL, FL_ENOMEM, FL_EHIP, FL_ERANGE, FL_ESCOPE = 0, -1, -2, -3, -4, 
 
 FL_F32, FL_F16, FL_BF16 = 16, 17, 18
 FL_ACT = {None: 0, "silu": 1, "gelu": 2}
+_TYPES = {"torch.float32": FL_F32, "torch.float16": FL_F16, "torch.bfloat16": FL_BF16}
 
 P_ = ctypes.c_void_p
 
@@ -470,41 +471,61 @@ class Context:
 
     # ---- 16-bit products (bfloat16 or float16), dense and by expert, and their backward pass
     def _type(self, who, t):
-        code = {self.torch.bfloat16: FL_BF16, self.torch.float16: FL_F16, self.torch.float32: FL_F32}.get(t)
+        code = _TYPES.get(str(t)) if t not in _TYPES else _TYPES[t]
         if code is None:
             raise LokiError("%s: bfloat16 or float16 is needed, not %s" % (who, t))
+        _TYPES[t] = code   # (found by the type itself from now on)
         return code
 
-    def _mm(self, who, x, W, up, offsets, perm, topk):
+    def _mm(self, who, x, W, up, offsets, perm):
         """(type code, slots, R, K, experts, rows of x) of a product's operands, checked"""
-        T = x.dtype
+        T, t = x.dtype, self.torch
         code = self._type(who, T)
         if code == FL_F32 or x.dim() != 2 or W.dim() != (2 if offsets is None else 3):
             raise LokiError("%s: x [rows][K] and W %s of bfloat16 or float16 are needed, not %s %s and %s" %
                             (who, "[R][K]" if offsets is None else "[n_exp][R][K]", T, tuple(x.shape), tuple(W.shape)))
         R, K = W.shape[-2:]
-        ne = 1 if offsets is None else W.shape[0]
-        n = x.shape[0] if perm is None else perm.numel()
-        self._need(who, (x, T, (x.shape[0], K)), (W, T, W.shape), (up, T, W.shape))
-        if offsets is not None:
-            self._need(who, (offsets, self.torch.int32, (ne + 1,)), (perm, self.torch.int32, (n,)))
-        elif perm is not None:
-            raise LokiError("%s: perm goes with offsets" % who)
-        return code, n, R, K, ne, x.shape[0]
+        xr = n = x.shape[0]
+        if up is None:
+            self._need(who, (x, T, (n, K)), (W, T, W.shape))
+        else:
+            self._need(who, (x, T, (n, K)), (W, T, W.shape), (up, T, W.shape))
+        if offsets is None:
+            if perm is not None:
+                raise LokiError("%s: perm goes with offsets" % who)
+            return code, n, R, K, 1, xr
+        ne = W.shape[0]
+        if perm is not None:
+            n = perm.numel()
+        self._need(who, (offsets, t.int32, (ne + 1,)), (perm, t.int32, (n,)))
+        return code, n, R, K, ne, xr
 
     def _product(self, who, x, W, offsets, up, bias, act, residual, perm, topk, dtype, keep, y, z, z2):
-        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm, topk)
+        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm)
         T = x.dtype
         if act not in FL_ACT:
             raise LokiError("%s: act is None, 'silu' or 'gelu', not %r" % (who, act))
+        given = []   # the tensors that are not made here
+        if bias is not None:
+            given.append((bias, self.torch.float32, (R,) if offsets is None else (ne, R)))
+        if residual is not None:
+            given.append((residual, T, (n, R)))
         if y is None:
-            y = x.new_empty(n, R, dtype=dtype or T)
-        if keep:
-            z = x.new_empty(n, R) if z is None else z
-            z2 = x.new_empty(n, R) if z2 is None and up is not None else z2
-        self._need(who, (bias, self.torch.float32, (R,) if offsets is None else (ne, R)), (residual, T, (n, R)), (y, dtype or y.dtype, (n, R)), (z, T, (n, R)), (z2, T, (n, R)))
+            y = x.new_empty(n, R) if dtype is None else x.new_empty(n, R, dtype=dtype)
+        else:
+            given.append((y, dtype or y.dtype, (n, R)))
+        if z is not None:
+            given.append((z, T, (n, R)))
+        elif keep:
+            z = x.new_empty(n, R)
+        if z2 is not None:
+            given.append((z2, T, (n, R)))
+        elif keep and up is not None:
+            z2 = x.new_empty(n, R)
+        if given:
+            self._need(who, *given)
         rc = lib().fl_matmul_dev(self.ctx, code, FL_ACT[act], x.data_ptr(), W.data_ptr(), _ptr(up), _ptr(bias), _ptr(residual), n, R, K, ne, _ptr(offsets),
-                                 _ptr(perm), topk, xr, y.data_ptr(), self._type(who, y.dtype), _ptr(z), _ptr(z2))
+                                 _ptr(perm), topk, xr, y.data_ptr(), code if y.dtype is T else self._type(who, y.dtype), _ptr(z), _ptr(z2))
         if rc:
             self.check(rc)
         return y if z is None and z2 is None else (y, z) if up is None else (y, z, z2)
@@ -549,7 +570,7 @@ class Context:
         return dy if out is None else out, dz2, dbias
 
     def _product_grad(self, who, dz, x, W, offsets, dz2, up, perm, topk, dW, dW2, dw_dtype, need_dx, need_dW, dx):
-        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm, topk)
+        code, n, R, K, ne, xr = self._mm(who, x, W, up, offsets, perm)
         T = x.dtype
         if (dz2 is None) != (up is None):
             raise LokiError("%s: dz2 and up go together" % who)
@@ -583,12 +604,15 @@ class Context:
     def combine(self, o, inv, w=None, sel=None, n_exp=N_EXPERT, residual=None, topk=None, dtype=None, y=None):
         """y [n][E] = residual + sum_k w[t][k] o[inv[t][k]] for the slots' rows o [P][E], dispatch()'s inv and route()'s w [n][topk] float32
         (None: ones; topk then from sel, or given). Picks of sel outside 0 .. n_exp - 1 are skipped. dtype: o's (default) or float32."""
-        P, E, n, k, T = self._picks("combine", o, inv, w, sel, topk)
+        P, E, n, k, T, code = self._picks("combine", o, inv, w, sel, topk)
         if y is None:
-            y = o.new_empty(n, E, dtype=dtype or T)
-        self._need("combine", (residual, T, (n, E)), (y, dtype or y.dtype, (n, E)))
-        rc = lib().fl_combine_dev(self.ctx, self._type("combine", T), o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), _ptr(residual), n, k, n_exp, P, E,
-                                  y.data_ptr(), self._type("combine", y.dtype))
+            y = o.new_empty(n, E) if dtype is None else o.new_empty(n, E, dtype=dtype)
+        else:
+            self._need("combine", (y, dtype or y.dtype, (n, E)))
+        if residual is not None:
+            self._need("combine", (residual, T, (n, E)))
+        rc = lib().fl_combine_dev(self.ctx, code, o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), _ptr(residual), n, k, n_exp, P, E,
+                                  y.data_ptr(), code if y.dtype is T else self._type("combine", y.dtype))
         if rc:
             self.check(rc)
         return y
@@ -596,12 +620,14 @@ class Context:
     def combine_grad(self, dy, o, inv, w=None, sel=None, n_exp=N_EXPERT, topk=None, do=None, need_do=True, need_dw=True):
         """(do, dw): the gradients of combine() to the slots' rows (w[t][k] dy[t]; slots of no pick keep what `do` holds) and to the routing
         weights (float32 [n][topk], for route_grad)."""
-        P, E, n, k, T = self._picks("combine_grad", o, inv, w, sel, topk)
-        if do is None and need_do:
-            do = o.new_empty(P, E)
+        P, E, n, k, T, code = self._picks("combine_grad", o, inv, w, sel, topk)
+        if do is not None:
+            self._need("combine_grad", (dy, T, (n, E)), (do, T, (P, E)))
+        else:
+            self._need("combine_grad", (dy, T, (n, E)))
+            do = o.new_empty(P, E) if need_do else None
         dw = o.new_empty(n, k, dtype=self.torch.float32) if need_dw else None
-        self._need("combine_grad", (dy, T, (n, E)), (do, T, (P, E)))
-        rc = lib().fl_combine_grad_dev(self.ctx, self._type("combine_grad", T), dy.data_ptr(), o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), n, k, n_exp, P, E, _ptr(do), _ptr(dw))
+        rc = lib().fl_combine_grad_dev(self.ctx, code, dy.data_ptr(), o.data_ptr(), inv.data_ptr(), _ptr(w), _ptr(sel), n, k, n_exp, P, E, _ptr(do), _ptr(dw))
         if rc:
             self.check(rc)
         return do, dw
@@ -609,11 +635,13 @@ class Context:
     def _picks(self, who, o, inv, w, sel, topk):
         t = self.torch
         k = topk or (w.shape[1] if w is not None else sel.shape[1] if sel is not None else 0)
-        if o.dim() != 2 or o.dtype is t.float32 or k < 1 or inv.numel() % k:
+        T, pairs = o.dtype, inv.numel()
+        code = self._type(who, T)
+        if o.dim() != 2 or code == FL_F32 or k < 1 or pairs % k:
             raise LokiError("%s: o [P][E] of bfloat16 or float16, and w, sel or topk that tells the picks a row, are needed" % who)
-        (P, E), n = o.shape, inv.numel() // k
-        self._need(who, (o, o.dtype, (P, E)), (inv, t.int32, inv.shape), (w, t.float32, (n, k)), (sel, t.int32, (n, k)))
-        return P, E, n, k, o.dtype
+        (P, E), n = o.shape, pairs // k
+        self._need(who, (o, T, (P, E)), (inv, t.int32, inv.shape), (w, t.float32, (n, k)), (sel, t.int32, (n, k)))
+        return P, E, n, k, T, code
 
     def dispatch(self, sel, n_exp=N_EXPERT):
         t = self.torch
