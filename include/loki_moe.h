@@ -189,8 +189,9 @@ int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * l
                       int n_exp, int E, float * dlogits, float * dW, int accumulate, float * dx);
 /* Workspaces of fl_balance_loss_dev, fl_route_grad_dev, Q4_K and 16-bit products are the context's. They grow in the call that needs more
  * (hipMalloc; FL_ENOMEM when that fails, and under graph capture, where nothing is allocated and the capture goes on) and no block is
- * freed before fl_free, so a captured call stays valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured from one context share
- * its workspaces and must not run at the same time. The context's device has to be the current one (FL_EINVAL). */
+ * freed before fl_free, so a captured call stays valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured
+ * from one context share its workspaces (and the counters from which the 16-bit products' workgroups take their tiles) and must not run at
+ * the same time. The context's device has to be the current one (FL_EINVAL). */
 /* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device) */
 int fl_dispatch_dev(FLCtx *, const int * sel, int n, int topk, int n_exp, int * counts, int * offsets, int * perm, int * inv, int * act, int * nact);
 /* Q8_K of nrows x K floats (device): q [nrows][K] int8, d [nrows][K/256] */
@@ -211,8 +212,8 @@ int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_
  * Groups: with offsets [n_exp + 1] (device, ascending, as fl_dispatch_dev leaves them) expert e has the rows ("slots") offsets[e] ..
  * offsets[e + 1] - 1 of the n and a matrix of its own; slots of no expert are not read and their results stay as they were. Offsets
  * are clamped to 0 .. n; ones that are not ascending give unspecified values. Without offsets (NULL) n_exp is 1 and takes all n rows.
- * With perm [n] (fl_dispatch_dev's) slot s reads row perm[s] / topk of the xrows rows of x, at most 2^31 - 2^16 values; a row outside
- * them counts as zeros. Without it slot s reads row s, and topk and xrows are not looked at. */
+ * With perm [n] (fl_dispatch_dev's) slot s reads row perm[s] / topk of the xrows rows of x, at most 2^31 - 2^16 values and 2^28 pairs; a
+ * row outside them counts as zeros. Without it slot s reads row s, and topk and xrows are not looked at. */
 enum { FL_F32 = 16, FL_F16 = 17, FL_BF16 = 18 };
 /* silu(z) = z / (1 + e^-z); gelu in its tanh form, z / (1 + e^(-2 sqrt(2 / pi) (z + 0.044715 z^3))) */
 enum { FL_ACT_NONE = 0, FL_ACT_SILU = 1, FL_ACT_GELU = 2 };
@@ -229,7 +230,7 @@ int fl_act_grad_dev(FLCtx *, int type, int act, const void * dy, const void * z,
                     void * dz, void * dz2, float * dbias, int accumulate);
 /* the products' backward pass: dx [n][K] = dz W (+ dz2 W2), of each slot (with perm too: a row's slots are summed by fl_combine_dev with
  * w NULL), dW [n_exp][R][K] = (accumulate: +=) dz^T x of the expert's slots, dW2 = dz2^T x likewise; each may be NULL: not computed.
- * dW and dW2 are of `type` or FL_F32 (dw_type). An expert without slots gets 0 (accumulate: stays). Deterministic, no atomics. */
+ * dW and dW2 are of `type` or FL_F32 (dw_type); accumulate adds in fp32 and rounds the sum. An expert without slots gets 0 (accumulate: stays). Deterministic, no atomics. */
 int fl_matmul_grad_dev(FLCtx *, int type, const void * dz, const void * dz2, const void * x, const void * W, const void * W2, int n, int R, int K, int n_exp,
                        const int * offsets, const int * perm, int topk, int xrows, void * dx, void * dW, void * dW2, int dw_type, int accumulate);
 /* the picks' sum: y [n][E] = residual + sum over k of w[t][k] o[inv[t][k]], fp32 in k's order; o [P][E] the slots' rows, inv and sel
@@ -238,7 +239,7 @@ int fl_matmul_grad_dev(FLCtx *, int type, const void * dz, const void * dz2, con
 int fl_combine_dev(FLCtx *, int type, const void * o, const int * inv, const float * w, const int * sel, const void * residual, int n, int topk, int n_exp,
                    int P, int E, void * y, int y_type);
 /* its gradients: d_o[inv[t][k]] = w[t][k] dy[t] (slots of no pick stay; may be o's buffer) and dw [n][topk] = <o[inv[t][k]], dy[t]> in fp32
- * (0 for a skipped pick), which fl_route_grad_dev takes; either may be NULL */
+ * (0 for a skipped pick), which fl_route_grad_dev takes; either may be NULL. Two picks with one slot would both write its d_o row */
 int fl_combine_grad_dev(FLCtx *, int type, const void * dy, const void * o, const int * inv, const float * w, const int * sel, int n, int topk, int n_exp,
                         int P, int E, void * d_o, float * dw);
 /* IQ2_XXS ggml layout <-> tiled layout for nmat matrices of R x K at byte strides (device, may not alias) */

@@ -434,6 +434,7 @@ static int mm_shape(FLCtx * c, int type, int n, int R, int K, int n_exp, const i
         if (!offsets) { return fail(c, FL_EINVAL, "perm goes with offsets"); }
         if (topk < 1 || topk > MAXK) { return fail(c, FL_EINVAL, "topk %d outside 1..%d", topk, MAXK); }
         if (xrows < 0 || (int64_t) xrows * K > 2147418112) { return fail(c, FL_ERANGE, "x has %d rows of %d: rows picked through perm are at most 2^31 - 2^16 values", xrows, K); }
+        if ((int64_t) xrows * topk > 1 << 28) { return fail(c, FL_ERANGE, "x has %d rows of %d picks: at most 2^28 pairs", xrows, topk); }
         if (!covers(perm, (size_t) n * 4)) { return fail(c, FL_EINVAL, "perm's allocation is smaller than its shape (n %d)", n); }
         if (topk > 1) { magic = (uint32_t) ((((uint64_t) 1 << 32) + (uint64_t) topk - 1) / (uint64_t) topk); }
     }
@@ -460,7 +461,7 @@ extern "C" int fl_matmul_dev(FLCtx * c, int type, int act, const void * x, const
     const size_t ob[3] = { yb, out * 2, out * 2 };
     for (int i = 0; i < 3; ++i) {
         if (overlap(outs[i], ob[i], x, xb) || overlap(outs[i], ob[i], W, wb) || overlap(outs[i], ob[i], W2, wb) || overlap(outs[i], ob[i], outs[(i + 1) % 3], ob[(i + 1) % 3]) ||
-            (!(i == 0 && y == residual && y_type == type) && overlap(outs[i], ob[i], residual, out * 2))) {
+            overlap(outs[i], ob[i], bias, (size_t) n_exp * R * 4) || (!(i == 0 && y == residual && y_type == type) && overlap(outs[i], ob[i], residual, out * 2))) {
             return fail(c, FL_EINVAL, "results must not overlap the operands or each other (y may be the residual's buffer in the operands' type)");
         }
     }
@@ -501,24 +502,18 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
     a.type = type; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.dz = dz; a.dz2 = dz2; a.x = x; a.W = W; a.W2 = W2; a.dx = dx; a.dW = dW; a.dW2 = dW2; a.dw_f32 = dw_type == FL_F32; a.accumulate = accumulate ? 1 : 0;
     a.queue = c->mm_queue;
-    if (dx && n > 0) {
-        const MmPlan plan = mm_plan(n, n_exp, K, dz2 ? 2 * R : R, false);
-        a.shape = plan.shape; a.parts = plan.parts;
-        if (plan.parts > 1) {
-            if (int rc = grow(c, c->mm, (size_t) plan.parts * n * K * 4)) { return rc; }
-            a.part = (float *) c->mm.p;
-        }
-        TRY(c, launch_matmul_dx(a, c->st));
+    const int mats = (dW ? 1 : 0) + (dW2 ? 1 : 0);
+    const bool has_dx = dx && n > 0;
+    const MmPlan px = mm_plan(n, n_exp, K, dz2 ? 2 * R : R, false), pw = dw_plan(n, n_exp, R, K, mats);
+    a.shape = px.shape; a.parts = px.parts; a.dw_shape = pw.shape; a.dw_parts = pw.parts;
+    const size_t part = has_dx && px.parts > 1 ? (size_t) px.parts * n * K * 4 : 0, dw_part = mats && pw.parts > 1 ? (size_t) pw.parts * mats * wn * 4 : 0;
+    if (part || dw_part) {   // (one after the other; before the first launch, so that a call without memory has done nothing)
+        if (int rc = grow(c, c->mm, std::max(part, dw_part))) { return rc; }
+        a.part = a.dw_part = (float *) c->mm.p;
     }
-    if (dW || dW2) {   // (no rows: 0, or it stays)
-        const int mats = (dW ? 1 : 0) + (dW2 ? 1 : 0);
-        const MmPlan plan = dw_plan(n, n_exp, R, K, mats);
-        a.dw_shape = plan.shape; a.dw_parts = plan.parts;
+    if (has_dx) { TRY(c, launch_matmul_dx(a, c->st)); }
+    if (mats) {   // (no rows: 0, or it stays)
         if (n == 0) { a.perm = nullptr; }
-        if (plan.parts > 1) {
-            if (int rc = grow(c, c->mm, (size_t) plan.parts * mats * wn * 4)) { return rc; }
-            a.dw_part = (float *) c->mm.p;
-        }
         TRY(c, launch_matmul_dw(a, c->st));
     }
     return FL_OK;

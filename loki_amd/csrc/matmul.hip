@@ -688,7 +688,7 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
     dw_results<T, F32, V>(a, s, acc);
 }
 // few rows an expert: the results' memory bounds it, and a tile has a round or two. Nothing is kept ahead; four workgroups a CU cover each
-// other's waits (256 experts of 128 rows, 7168 x 2048: @DWFEW@)
+// other's waits (256 experts of 128 rows, 7168 x 2048: 4 rows 1378 us, Middle 1899, Large 1928; 128 rows 2317, 2629, 2487)
 template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm_dw_few(MatmulGradArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef DwCopies<T, PERM, H> C;
