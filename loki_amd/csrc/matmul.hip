@@ -277,6 +277,21 @@ __device__ __forceinline__ void eight(f32x4 a, f32x4 b, float (&v)[8]) {
     }
 #endif
 }
+// Whole lines: x and y are 16 bytes of row r, lane (r, g), a half line each; after it lane (r, g) has 16 of rows r % 8 (up) and r % 8 + 8
+// (down), x's where r < 8, y's where not
+template <class V> __device__ __forceinline__ void lines(V x, V y, V & up, V & down) {
+    const bool low = (lane_id() & 8) == 0;
+    const u32x4 p = __builtin_bit_cast(u32x4, x), q = __builtin_bit_cast(u32x4, y);
+    u32x4 u, d;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t other = (uint32_t) __builtin_amdgcn_update_dpp(0, (int) (low ? q[i] : p[i]), 0x128, 0xF, 0xF, false);   // (the lane 8 further in its 16)
+        u[i] = low ? p[i] : other;
+        d[i] = low ? other : q[i];
+    }
+    up = __builtin_bit_cast(V, u);
+    down = __builtin_bit_cast(V, d);
+}
 // The workgroups (a multiple of 8) go round the 8 XCDs; an XCD's tiles are a run of the launch's, so that what runs at a time there shares
 // panels in its L2. Tiles differ in cost, so after its first a workgroup takes the XCD's next one (queue[x]); the last to find none
 // sets the two counters back to 0 for the next launch.
@@ -640,32 +655,71 @@ template <class H> __device__ __forceinline__ DwSpot dw_spot(const MatmulGradArg
     s.m0 = uni((band * BAND + r % rows) * H::BM); s.n0 = uni(r / rows * H::BN);
     return s;
 }
-// the results of a tile
+// the results of a tile, past the caches that the operands live in and in whole lines (64 experts of 94 rows, 2 x 1024 x 2048, with dx 355 -> 325 us;
+// half lines 336 us, but 256 of 128, 7168 x 2048, 4.3 -> 4.6 ms)
 template <class T, bool F32, class V> __device__ __forceinline__ void dw_results(const MatmulGradArgs & a, const DwSpot & s, f32x4 (&acc)[V::FM][V::FN]) {
     const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
     const size_t w = (size_t) a.R * a.K, t0 = (size_t) s.e * w + (size_t) s.m0 * a.K + s.n0;
-    auto each = [&](auto f) __attribute__((always_inline)) {
+    // f(offset, columns' 16 bytes) on whole lines: of float, or of T
+    auto floats = [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
         for (int m = 0; m < V::FM; ++m) {
+            const int row = (wm * V::FM + m) * 16 + (lane & 7);
+#pragma unroll
+            for (int j = 0; j < V::FN; j += 2) {
+                const int col = (wn * V::FN + j + ((lane >> 3) & 1)) * 16 + 4 * (lane >> 4);
+                f32x4 up, down;
+                lines(acc[m][j], acc[m][j + 1], up, down);
+                const uint32_t at = (uint32_t) row * (uint32_t) a.K + (uint32_t) col;
+                if (s.n0 + col < a.K) {
+                    if (s.m0 + row < a.R) { f(at, up); }
+                    if (s.m0 + row + 8 < a.R) { f(at + 8 * (uint32_t) a.K, down); }
+                }
+            }
+        }
+    };
+    auto halves = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int m = 0; m < V::FM; ++m) {
+            const int row = (wm * V::FM + m) * 16 + (lane & 7);
+#pragma unroll
+            for (int j = 0; j < V::FN; j += 4) {
+                const int col = (wn * V::FN + j + ((lane >> 4) & 1) + ((lane >> 2) & 2)) * 16 + 8 * (lane >> 5);
+                float v[8], w[8];
+                eight(acc[m][j], acc[m][j + 1], v);
+                eight(acc[m][j + 2], acc[m][j + 3], w);
+                V8<T> up, down;
+                lines(rounded<T>(v), rounded<T>(w), up, down);
+                const uint32_t at = (uint32_t) row * (uint32_t) a.K + (uint32_t) col;
+                if (s.n0 + col < a.K) {
+                    if (s.m0 + row < a.R) { f(at, up); }
+                    if (s.m0 + row + 8 < a.R) { f(at + 8 * (uint32_t) a.K, down); }
+                }
+            }
+        }
+    };
+    if (a.dw_parts > 1) {
+        float * p = a.dw_part + ((size_t) s.part * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0)) + (a.dW && s.second ? 1 : 0)) * a.n_exp * w + t0;
+        floats([&](uint32_t at, f32x4 v) __attribute__((always_inline)) { *(LK_GLOBAL f32x4 *) (p + at) = v; });
+    } else if constexpr (F32) {
+        float * d = (float *) (s.second ? a.dW2 : a.dW) + t0;
+        if (a.accumulate) { floats([&](uint32_t at, f32x4 v) __attribute__((always_inline)) { LK_GLOBAL f32x4 * q = (LK_GLOBAL f32x4 *) (d + at); *q = *q + v; }); }
+        else { floats([&](uint32_t at, f32x4 v) __attribute__((always_inline)) { __builtin_nontemporal_store(v, (LK_GLOBAL f32x4 *) (d + at)); }); }
+    } else {
+        T * d = (T *) (s.second ? a.dW2 : a.dW) + t0;
+        if (!a.accumulate) { halves([&](uint32_t at, V8<T> v) __attribute__((always_inline)) { __builtin_nontemporal_store(v, (LK_GLOBAL V8<T> *) (d + at)); }); return; }
+#pragma unroll
+        for (int m = 0; m < V::FM; ++m) {   // the sum in fp32, rounded once
             const int row = (wm * V::FM + m) * 16 + (lane & 15);
 #pragma unroll
             for (int j = 0; j < V::FN; j += 2) {
                 const int col = (wn * V::FN + j + ((lane >> 4) & 1)) * 16 + 8 * (lane >> 5);
                 float v[8];
                 eight(acc[m][j], acc[m][j + 1], v);
-                if (s.m0 + row < a.R && s.n0 + col < a.K) { f((uint32_t) row * (uint32_t) a.K + (uint32_t) col, v); }
+                T * q = d + ((uint32_t) row * (uint32_t) a.K + (uint32_t) col);
+                if (s.m0 + row < a.R && s.n0 + col < a.K) { add8(q, v); put8(q, v); }
             }
         }
-    };
-    typedef typename std::conditional<F32, float, T>::type O;
-    O * d = (O *) (s.second ? a.dW2 : a.dW) + t0;
-    if (a.dw_parts > 1) {
-        float * p = a.dw_part + ((size_t) s.part * ((a.dW ? 1 : 0) + (a.dW2 ? 1 : 0)) + (a.dW && s.second ? 1 : 0)) * a.n_exp * w + t0;
-        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { put8(p + at, v); });
-    } else if (a.accumulate) {
-        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { add8(d + at, v); put8(d + at, v); });
-    } else {
-        each([&](uint32_t at, float (&v)[8]) __attribute__((always_inline)) { put8(d + at, v); });
     }
 }
 // one workgroup a tile, and an XCD's share a run of them: what a workgroup has written need not have arrived when the next one starts

@@ -118,12 +118,13 @@ struct Tiles {
 };
 
 // ---------------------------------------------------------------- 8 values next to each other
-template <class T> __device__ __forceinline__ void put8(T * p, const float (&v)[8]) {
+template <class T> __device__ __forceinline__ V8<T> rounded(const float (&v)[8]) {
     V8<T> u;
 #pragma unroll
     for (int i = 0; i < 8; ++i) { u[i] = (T) v[i]; }
-    *(LK_GLOBAL V8<T> *) p = u;
+    return u;
 }
+template <class T> __device__ __forceinline__ void put8(T * p, const float (&v)[8]) { *(LK_GLOBAL V8<T> *) p = rounded<T>(v); }
 __device__ __forceinline__ void put8(float * p, const float (&v)[8]) {
     *(LK_GLOBAL f32x4 *) p = (f32x4) { v[0], v[1], v[2], v[3] };
     *(LK_GLOBAL f32x4 *) (p + 4) = (f32x4) { v[4], v[5], v[6], v[7] };
