@@ -305,3 +305,34 @@ def test_entry_refusals(ctx):
     torch.cuda.synchronize()
     assert rc == FL_ENOMEM and bool((dx == 77.0).all()) and bool((dW == 78.0).all())
     c.close()
+
+
+@pytest.mark.parametrize("n,ne,topk", [(1, 8, 2), (70, 16, 4), (900, 200, 6)])
+def test_layer_with_dropped_picks(ctx, n, ne, topk):
+    """the layer forward and backward on dispatch()'s tables where picks were dropped (-1): two linear products, so that everything stays a whole
+    number below 2^11 where it is float16 and below 2^24 where it is float32"""
+    T, E, H = torch.float16, 24, 16
+    g = torch.Generator().manual_seed(n)
+    sel = torch.topk(torch.randn((n, ne), generator=g), topk, dim=1).indices.to(torch.int32)
+    sel[torch.rand(sel.shape, generator=g) < 0.3] = -1
+    sel[-1] = -1
+    sel = sel.cuda()
+    x, Wg, Wd, w, dy, res = whole(1, n, E, dtype=T), whole(2, ne, H, E, dtype=T), whole(3, ne, E, H, dtype=T), whole(4, n, topk, dtype=F4, most=2), whole(5, n, E, dtype=T), whole(6, n, E, dtype=T)
+    _, off, perm, inv, _, _ = ctx.dispatch(sel, n_exp=ne)
+    h = ctx.expert_matmul(x, Wg, off, perm=perm, topk=topk)
+    o = ctx.expert_matmul(h, Wd, off)
+    y = ctx.combine(o, inv, w, sel=sel, n_exp=ne, residual=res, dtype=F4)
+    do, dw = ctx.combine_grad(dy, o, inv, w, sel=sel, n_exp=ne)
+    dh, dWd = ctx.expert_matmul_grad(do, h, Wd, off, dw_dtype=F4)
+    dxs, dWg = ctx.expert_matmul_grad(dh, x, Wg, off, perm=perm, topk=topk, dw_dtype=F4)
+    dx = ctx.combine(dxs, inv, sel=sel, n_exp=ne, topk=topk, dtype=F4)
+    ctx.sync()
+    a = [t.double().cpu().requires_grad_(True) for t in (x, Wg, Wd, w)]
+    want = res.double().cpu()
+    for k in range(topk):
+        e = sel[:, k].cpu().long()
+        z = torch.einsum("te,the->th", a[0], a[1][e.clamp(min=0)])
+        want = want + torch.einsum("th,teh->te", z, a[2][e.clamp(min=0)]) * (a[3][:, k] * (e >= 0))[:, None]
+    (want * dy.double().cpu()).sum().backward()
+    for got, t in ((y, want.detach()), (dx, a[0].grad), (dWg, a[1].grad), (dWd, a[2].grad), (dw, a[3].grad)):
+        assert got.dtype is F4 and torch.equal(got.cpu(), t.float())
