@@ -420,6 +420,11 @@ static bool misaligned(std::initializer_list<const void *> ps) {
 static bool overlap(const void * a, size_t na, const void * b, size_t nb) {
     return a && b && (const char *) a < (const char *) b + nb && (const char *) b < (const char *) a + na;
 }
+// a result shares memory with offsets or perm
+static bool on_groups(std::initializer_list<std::pair<const void *, size_t>> outs, int n, int n_exp, const int * offsets, const int * perm) {
+    for (const auto & o : outs) { if (overlap(o.first, o.second, offsets, (size_t) (n_exp + 1) * 4) || overlap(o.first, o.second, perm, (size_t) n * 4)) { return true; } }
+    return false;
+}
 // sizes, groups and gather of a product; rows: the rows of x
 static int mm_shape(FLCtx * c, int type, int n, int R, int K, int n_exp, const int * offsets, const int * perm, int topk, int xrows, uint32_t & magic) {
     if (type != FL_BF16 && type != FL_F16) { return fail(c, FL_EINVAL, "type %d is not FL_BF16 or FL_F16", type); }
@@ -465,6 +470,7 @@ extern "C" int fl_matmul_dev(FLCtx * c, int type, int act, const void * x, const
             return fail(c, FL_EINVAL, "results must not overlap the operands or each other (y may be the residual's buffer in the operands' type)");
         }
     }
+    if (on_groups({ { y, yb }, { z, out * 2 }, { z2, out * 2 } }, n, n_exp, offsets, perm)) { return fail(c, FL_EINVAL, "results must not overlap offsets or perm"); }
     a.type = type; a.act = act; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.x = x; a.W = W; a.W2 = W2; a.bias = bias; a.residual = residual; a.y = y; a.z = z; a.z2 = z2; a.y_f32 = y_type == FL_F32;
     a.queue = c->mm_queue;
@@ -499,6 +505,7 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
             return fail(c, FL_EINVAL, "results must not overlap the operands or each other");
         }
     }
+    if (on_groups({ { dx, dxb }, { dW, wb }, { dW2, wb } }, n, n_exp, offsets, perm)) { return fail(c, FL_EINVAL, "results must not overlap offsets or perm"); }
     a.type = type; a.n = n; a.R = R; a.K = K; a.n_exp = n_exp; a.offsets = offsets; a.perm = perm; a.xrows = xrows;
     a.dz = dz; a.dz2 = dz2; a.x = x; a.W = W; a.W2 = W2; a.dx = dx; a.dW = dW; a.dW2 = dW2; a.dw_f32 = dw_type == FL_F32; a.accumulate = accumulate ? 1 : 0;
     a.queue = c->mm_queue;
@@ -540,6 +547,7 @@ extern "C" int fl_act_grad_dev(FLCtx * c, int type, int act, const void * dy, co
     }
     if (overlap(dz, b, dz2, b)) { return fail(c, FL_EINVAL, "results must not overlap each other"); }
     for (const void * p : { dy, z, z2 }) { if (overlap(dbias, (size_t) n_exp * R * 4, p, b)) { return fail(c, FL_EINVAL, "dbias must not overlap the operands"); } }
+    if (on_groups({ { dz, b }, { dz2, b }, { dbias, (size_t) n_exp * R * 4 } }, n, n_exp, offsets, nullptr)) { return fail(c, FL_EINVAL, "results must not overlap offsets"); }
     if (n == 0 && !dbias) { return FL_OK; }
     a.type = type; a.act = act; a.n = n; a.R = R; a.n_exp = n_exp; a.offsets = offsets; a.dy = dy; a.z = z; a.z2 = z2; a.dz = dz; a.dz2 = dz2; a.dbias = dbias;
     a.accumulate = accumulate ? 1 : 0; a.chunks = 1;
@@ -566,6 +574,11 @@ static int combine_args(FLCtx * c, const CombineArgs & a) {
     }
     return need_device(c);
 }
+// a result shares memory with the picks' slots, experts or weights
+static bool on_tables(const CombineArgs & a, const void * p, size_t bytes) {
+    const size_t pairs = (size_t) a.n * a.topk * 4;
+    return overlap(p, bytes, a.inv, pairs) || overlap(p, bytes, a.sel, pairs) || overlap(p, bytes, a.w, pairs);
+}
 extern "C" int fl_combine_dev(FLCtx * c, int type, const void * o, const int * inv, const float * w, const int * sel, const void * residual, int n, int topk, int n_exp,
                               int P, int E, void * y, int y_type) {
     if (!c) { return FL_EINVAL; }
@@ -578,7 +591,7 @@ extern "C" int fl_combine_dev(FLCtx * c, int type, const void * o, const int * i
     if (misaligned({ o, residual, y })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
     const size_t yn = (size_t) n * E, yb = yn * (a.y_f32 ? 4 : 2);
     if (!covers(y, yb) || (residual && !covers(residual, yn * 2))) { return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, E %d)", n, E); }
-    if (overlap(y, yb, o, (size_t) P * E * 2) || (!(y == residual && !a.y_f32) && overlap(y, yb, residual, yn * 2))) {
+    if (overlap(y, yb, o, (size_t) P * E * 2) || on_tables(a, y, yb) || (!(y == residual && !a.y_f32) && overlap(y, yb, residual, yn * 2))) {
         return fail(c, FL_EINVAL, "y must not overlap the operands (it may be the residual's buffer in the operands' type)");
     }
     TRY(c, launch_combine16(a, c->st));
@@ -596,7 +609,7 @@ extern "C" int fl_combine_grad_dev(FLCtx * c, int type, const void * dy, const v
     if (misaligned({ dy, o, d_o })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
     const size_t ob = (size_t) P * E * 2, yb = (size_t) n * E * 2, wb = (size_t) n * topk * 4;
     if (!covers(dy, yb) || (d_o && !covers(d_o, ob)) || (dw && !covers(dw, wb))) { return fail(c, FL_EINVAL, "an allocation is smaller than its shape (n %d, topk %d, P %d, E %d)", n, topk, P, E); }
-    if (overlap(d_o, ob, dy, yb) || (d_o != o && overlap(d_o, ob, o, ob)) || overlap(dw, wb, w, wb) || overlap(dw, wb, d_o, ob) || overlap(dw, wb, o, ob) || overlap(dw, wb, dy, yb)) {
+    if (on_tables(a, d_o, ob) || on_tables(a, dw, wb) || overlap(d_o, ob, dy, yb) || (d_o != o && overlap(d_o, ob, o, ob)) || overlap(dw, wb, d_o, ob) || overlap(dw, wb, o, ob) || overlap(dw, wb, dy, yb)) {
         return fail(c, FL_EINVAL, "results must not overlap the operands or each other (d_o may be o's buffer)");
     }
     TRY(c, launch_combine16_grad(a, c->st));

@@ -336,3 +336,37 @@ def test_layer_with_dropped_picks(ctx, n, ne, topk):
     (want * dy.double().cpu()).sum().backward()
     for got, t in ((y, want.detach()), (dx, a[0].grad), (dWg, a[1].grad), (dWd, a[2].grad), (dw, a[3].grad)):
         assert got.dtype is F4 and torch.equal(got.cpu(), t.float())
+
+
+def test_combine_of_more_rows_than_workgroups(ctx):
+    """a launch has 2^22 workgroups at most: rows behind them are taken by the same ones"""
+    n = (1 << 22) + 9
+    for E, P in ((2048, 50), (8, n)):
+        o, w = whole(1, P, E), whole(2, n, 1, dtype=F4, most=3)
+        inv = torch.randint(0, P, (n,), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda", dtype=torch.int32) if P < n else torch.arange(n, dtype=torch.int32, device="cuda").flip(0).contiguous()
+        y = ctx.combine(o, inv, w)
+        for s in (slice(0, 20), slice(n - 30, n)):
+            same(y[s], o[inv[s].long()].float() * w[s])
+        if P == n:   # (each slot once)
+            dy = whole(4, n, E)
+            do, dw = ctx.combine_grad(dy, o, inv, w)
+            same(do, (dy.float() * w).flip(0))
+            same(dw, (o.flip(0).float() * dy.float()).sum(1, keepdim=True))
+        del y
+        torch.cuda.empty_cache()
+
+
+def test_results_on_tables_are_refused(ctx):
+    t = torch.zeros(1 << 16, dtype=torch.uint8, device="cuda")
+    p = t.data_ptr()
+    E = loki_amd.FL_EINVAL
+    mm = lambda y, z=None: lib().fl_matmul_dev(ctx.ctx, FL_BF16, 0, p, p + 4096, None, None, None, 8, 16, 16, 2, p + 8192, p + 12288, 1, 8, y, FL_BF16, z, None)  # noqa: E731
+    gr = lambda dx=None, dW=None: lib().fl_matmul_grad_dev(ctx.ctx, FL_BF16, p, None, p + 2048, p + 4096, None, 8, 16, 16, 2, p + 8192, p + 12288, 1, 8, dx, dW, None, FL_BF16, 0)  # noqa: E731
+    ag = lambda dz=None, db=None: lib().fl_act_grad_dev(ctx.ctx, FL_BF16, 0, p, None, None, 8, 16, 2, p + 8192, dz, None, db, 0)  # noqa: E731
+    cb = lambda y: lib().fl_combine_dev(ctx.ctx, FL_BF16, p, p + 4096, p + 8192, p + 12288, None, 8, 2, 4, 16, 16, y, FL_BF16)  # noqa: E731
+    cg = lambda do=None, dw=None: lib().fl_combine_grad_dev(ctx.ctx, FL_BF16, p, p + 2048, p + 4096, p + 8192, p + 12288, 8, 2, 4, 16, 16, do, dw)  # noqa: E731
+    for y in (p + 8192, p + 12288):
+        assert mm(y) == E and mm(p + 20480, z=y) == E and gr(dx=y) == E and gr(dW=y) == E and cb(y) == E and cg(do=y) == E and cg(dw=y) == E
+    assert ag(dz=p + 8192) == E and ag(db=p + 8192) == E and cb(p + 4096) == E and cg(do=p + 4096) == E and cg(dw=p + 4096) == E
+    assert mm(p + 20480) == 0 and gr(dx=p + 20480) == 0 and ag(dz=p + 20480) == 0 and cb(p + 20480) == 0 and cg(do=p + 20480) == 0
+    ctx.sync()
