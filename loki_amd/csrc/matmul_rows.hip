@@ -206,13 +206,18 @@ constexpr int MOST = 1 << 22;   // workgroups of a launch (a launch has fewer th
 // threads along a row of `nc` pieces of 8: a power of two, at most RT
 constexpr int row_threads(int nc) { int w = 1; while (w < nc && w < RT) { w *= 2; } return w; }
 
+// with a bias's gradient: a line of a row (8 threads) where experts have few rows, so that a workgroup takes them all and nothing is left to join
+// (gelu, us, against whole rows in chunks: 37 rows of 7168 5.9 / 8.5; 64 experts of 94, 1024 12 / 14; 256 of 128, 2048 83 / 92; 64 of 512, 2048 98 / 92; 501 of
+// 7168 16 / 14; 1000 36 / 22)
+constexpr int FEW_ROWS = 128;
+int bias_threads(int n, int R, int n_exp) { return n / n_exp <= FEW_ROWS ? std::min(row_threads(R / 8), 8) : row_threads(R / 8); }
 template <class T, int ACT> hipError_t go_act(const ActGradArgs & a, hipStream_t st) {
     if (!a.dbias) {
         const int64_t all = (int64_t) a.n * (a.R / 8);
         k_act_grad<T, ACT><<<blocks(all, RT) < 16384 ? blocks(all, RT) : 16384, RT, 0, st>>>(a);
         return hipGetLastError();
     }
-    const int cw = row_threads(a.R / 8), cb = (int) blocks(a.R / 8, cw);
+    const int cw = bias_threads(a.n, a.R, a.n_exp), cb = (int) blocks(a.R / 8, cw);
     k_act_grad_bias<T, ACT><<<dim3(cb * a.chunks, a.n_exp), RT, 0, st>>>(a, cw, cb);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.chunks > 1) {
@@ -242,6 +247,7 @@ template <class T> hipError_t go_combine_grad(const CombineArgs & a, hipStream_t
 }  // namespace
 
 int act_grad_chunks(int n, int R, int n_exp) {
+    if (n / n_exp <= FEW_ROWS) { return 1; }
     const int cw = row_threads(R / 8), cb = (int) blocks(R / 8, cw), rows = n / n_exp / (RT / cw);   // rows a thread sums, on average
     int c = 1;
     while (c < 128 && cb * n_exp * c < 1024 && rows > 8 * c) { c *= 2; }
