@@ -370,3 +370,39 @@ def test_results_on_tables_are_refused(ctx):
     assert ag(dz=p + 8192) == E and ag(db=p + 8192) == E and cb(p + 4096) == E and cg(do=p + 4096) == E and cg(dw=p + 4096) == E
     assert mm(p + 20480) == 0 and gr(dx=p + 20480) == 0 and ag(dz=p + 20480) == 0 and cb(p + 20480) == 0 and cg(do=p + 20480) == 0
     ctx.sync()
+
+
+@pytest.mark.parametrize("n", [1, 40, 600])
+def test_fp16_below_its_normal_range(ctx, n):
+    """fp16 operands and results below 2^-14 keep their bits: whole multiples of 2^-24, exact in every form"""
+    R, K = 72, 136
+    x, W = whole(1, n, K, dtype=torch.float16), whole(2, R, K, dtype=torch.float16)
+    tiny = (x.float() * 2.0 ** -24).half()
+    same(ctx.matmul(tiny, W), mm(x, W) * 2.0 ** -24)
+    same(ctx.matmul(x, (W.float() * 2.0 ** -24).half(), dtype=F4), mm(x, W) * 2.0 ** -24)
+    dz = whole(3, n, R, dtype=torch.float16)
+    dx, dW = ctx.matmul_grad((dz.float() * 2.0 ** -24).half(), x, W)
+    same(dx, mm(dz, W.t()) * 2.0 ** -24)
+    same(dW, mm(dz.t(), x.t()) * 2.0 ** -24)
+    same(ctx.combine(tiny, torch.arange(n, dtype=torch.int32, device="cuda"), topk=1), x.float() * 2.0 ** -24)
+
+
+def test_first_call_of_a_context_captured(ctx):
+    """a product without parts needs nothing of the context but its counters: the first call of a context may be the captured one"""
+    n, R, K = 2100, 4104, 72
+    c, s = loki_amd.Context(), torch.cuda.Stream()
+    x, W = whole(1, n, K), whole(2, R, K)
+    y = torch.zeros((n, R), dtype=B, device="cuda")
+    torch.cuda.synchronize()
+    c.check(lib().fl_set_stream(c.ctx, s.cuda_stream))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s), torch.cuda.graph(graph, stream=s):
+        c.matmul(x, W, y=y)
+        c.matmul(x, W, y=y, residual=y)
+    for i in range(3):
+        x.copy_(whole(10 + i, n, K))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(y, 2 * mm(x, W))
+    c.close()
