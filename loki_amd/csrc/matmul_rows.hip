@@ -112,97 +112,93 @@ __device__ __forceinline__ int slot_of(const CombineArgs & a, int64_t i) {
     return (unsigned) s < (unsigned) a.P ? s : -1;
 }
 
-// y = residual + sum over the picks, in their order, 8 columns a thread; a workgroup takes RT / cw rows of cw threads (and, where the launch has
-// fewer workgroups, the rows so many further)
-template <class T> __global__ void __launch_bounds__(RT) k_combine16(CombineArgs a, int cw, int cb) {
+// y = residual + sum over the picks, in their order, 8 columns a thread; a workgroup takes RT / cw rows of cw threads
+template <class T> __global__ void __launch_bounds__(RT) k_combine16(CombineArgs a, int cw, int cb, int t0) {   // (rows from t0 on)
     const int col = (blockIdx.x % cb) * cw + threadIdx.x % cw;
-    if (col >= a.E / 8) { return; }
-    for (int64_t t = (int64_t) (blockIdx.x / cb) * (RT / cw) + threadIdx.x / cw; t < a.n; t += (int64_t) (gridDim.x / cb) * (RT / cw)) {
-        const size_t at = (size_t) t * a.E + 8 * col;
-        V8<T> o[MAXK];
-        float w[MAXK];
+    const int64_t t = t0 + (int64_t) (blockIdx.x / cb) * (RT / cw) + threadIdx.x / cw;
+    if (t >= a.n || col >= a.E / 8) { return; }
+    const size_t at = (size_t) t * a.E + 8 * col;
+    V8<T> o[MAXK];
+    float w[MAXK];
 #pragma unroll
-        for (int k = 0; k < MAXK; ++k) {   // all loads before the sums
-            const int s = k < a.topk ? slot_of(a, t * a.topk + k) : -1;
-            w[k] = s >= 0 ? (a.w ? a.w[t * a.topk + k] : 1.f) : 0.f;
-            o[k] = (V8<T>) {};
-            if (s >= 0) { o[k] = *(const LK_GLOBAL V8<T> *) ((const T *) a.o + (size_t) s * a.E + 8 * col); }
-        }
-        float y[8] = {};
-        if (a.residual) {
-            const Row8<T> r = load8((const T *) a.residual + at);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { y[i] = r.v[i]; }
-        }
-#pragma unroll
-        for (int k = 0; k < MAXK; ++k) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { y[i] = __builtin_fmaf(w[k], (float) o[k][i], y[i]); }
-        }
-        if (a.y_f32) { store8((float *) a.y + at, y); } else { store8((T *) a.y + at, y); }
+    for (int k = 0; k < MAXK; ++k) {   // all loads before the sums
+        const int s = k < a.topk ? slot_of(a, t * a.topk + k) : -1;
+        w[k] = s >= 0 ? (a.w ? a.w[t * a.topk + k] : 1.f) : 0.f;
+        o[k] = (V8<T>) {};
+        if (s >= 0) { o[k] = *(const LK_GLOBAL V8<T> *) ((const T *) a.o + (size_t) s * a.E + 8 * col); }
     }
+    float y[8] = {};
+    if (a.residual) {
+        const Row8<T> r = load8((const T *) a.residual + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { y[i] = r.v[i]; }
+    }
+#pragma unroll
+    for (int k = 0; k < MAXK; ++k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { y[i] = __builtin_fmaf(w[k], (float) o[k][i], y[i]); }
+    }
+    if (a.y_f32) { store8((float *) a.y + at, y); } else { store8((T *) a.y + at, y); }
 }
 
 // d_o and dw of one row: W waves, each its columns, then the waves' sums in order
-template <class T, int W> __global__ void __launch_bounds__(64 * W) k_combine16_grad(CombineArgs a) {
+template <class T, int W> __global__ void __launch_bounds__(64 * W) k_combine16_grad(CombineArgs a, int t0) {
     __shared__ float lds[W][MAXK];
+    const int64_t t = t0 + (int64_t) blockIdx.x;
     const int lane = lane_id(), wave = threadIdx.x >> 6;
-    for (int64_t t = blockIdx.x; t < a.n; t += gridDim.x) {
-        int s[MAXK];
-        float w[MAXK], dot[MAXK];
+    int s[MAXK];
+    float w[MAXK], dot[MAXK];
+#pragma unroll
+    for (int k = 0; k < MAXK; ++k) {
+        s[k] = k < a.topk ? slot_of(a, t * a.topk + k) : -1;
+        w[k] = s[k] >= 0 && a.w ? a.w[t * a.topk + k] : 1.f;
+        dot[k] = 0.f;
+    }
+    for (int col = threadIdx.x; col < a.E / 8; col += 64 * W) {
+        const Row8<T> d = load8((const T *) a.dy + (size_t) t * a.E + 8 * col);
 #pragma unroll
         for (int k = 0; k < MAXK; ++k) {
-            s[k] = k < a.topk ? slot_of(a, t * a.topk + k) : -1;
-            w[k] = s[k] >= 0 && a.w ? a.w[t * a.topk + k] : 1.f;
-            dot[k] = 0.f;
-        }
-        for (int col = threadIdx.x; col < a.E / 8; col += 64 * W) {
-            const Row8<T> d = load8((const T *) a.dy + (size_t) t * a.E + 8 * col);
+            if (s[k] < 0) { continue; }
+            const size_t at = (size_t) s[k] * a.E + 8 * col;
+            if (a.dw) {
+                const Row8<T> o = load8((const T *) a.o + at);
 #pragma unroll
-            for (int k = 0; k < MAXK; ++k) {
-                if (s[k] < 0) { continue; }
-                const size_t at = (size_t) s[k] * a.E + 8 * col;
-                if (a.dw) {
-                    const Row8<T> o = load8((const T *) a.o + at);
+                for (int i = 0; i < 8; ++i) { dot[k] = __builtin_fmaf(o.v[i], d.v[i], dot[k]); }
+            }
+            if (a.d_o) {
+                float v[8];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) { dot[k] = __builtin_fmaf(o.v[i], d.v[i], dot[k]); }
-                }
-                if (a.d_o) {
-                    float v[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { v[i] = w[k] * d.v[i]; }
-                    store8((T *) a.d_o + at, v);
-                }
+                for (int i = 0; i < 8; ++i) { v[i] = w[k] * d.v[i]; }
+                store8((T *) a.d_o + at, v);
             }
         }
-        if (!a.dw) { continue; }
+    }
+    if (!a.dw) { return; }
 #pragma unroll
-        for (int k = 0; k < MAXK; ++k) {
+    for (int k = 0; k < MAXK; ++k) {
 #pragma unroll
-            for (int o = 32; o > 0; o >>= 1) { dot[k] += __shfl_xor(dot[k], o); }
+        for (int o = 32; o > 0; o >>= 1) { dot[k] += __shfl_xor(dot[k], o); }
+    }
+    if (W > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < MAXK; ++k) { lds[wave][k] = dot[k]; }
         }
-        if (W > 1) {
-            if (lane == 0) {
+        __syncthreads();
+    }
+    if ((int) threadIdx.x < a.topk) {
+        float v = 0.f;
+        if (W > 1) { for (int i = 0; i < W; ++i) { v += lds[i][threadIdx.x]; } }
+        else {
 #pragma unroll
-                for (int k = 0; k < MAXK; ++k) { lds[wave][k] = dot[k]; }
-            }
-            __syncthreads();
+            for (int k = 0; k < MAXK; ++k) { v = (int) threadIdx.x == k ? dot[k] : v; }
         }
-        if ((int) threadIdx.x < a.topk) {
-            float v = 0.f;
-            if (W > 1) { for (int i = 0; i < W; ++i) { v += lds[i][threadIdx.x]; } }
-            else {
-#pragma unroll
-                for (int k = 0; k < MAXK; ++k) { v = (int) threadIdx.x == k ? dot[k] : v; }
-            }
-            a.dw[t * a.topk + threadIdx.x] = v;
-        }
-        if (W > 1) { __syncthreads(); }
+        a.dw[t * a.topk + threadIdx.x] = v;
     }
 }
 
 constexpr unsigned blocks(int64_t n, int64_t per) { return (unsigned) ((n + per - 1) / per); }
-constexpr int MOST = 1 << 22;   // workgroups of a launch (a launch has fewer than 2^32 threads)
+constexpr int MOST = 1 << 22;   // workgroups of a launch, which has fewer than 2^32 threads (more rows: more launches)
 // threads along a row of `nc` pieces of 8: a power of two, at most RT
 constexpr int row_threads(int nc) { int w = 1; while (w < nc && w < RT) { w *= 2; } return w; }
 
@@ -232,15 +228,17 @@ template <class T> hipError_t go_act(const ActGradArgs & a, hipStream_t st) {
 }
 template <class T> hipError_t go_combine(const CombineArgs & a, hipStream_t st) {
     const int cw = row_threads(a.E / 8), cb = (int) blocks(a.E / 8, cw);
-    const unsigned rows = std::min<unsigned>(blocks(a.n, RT / cw), (unsigned) (MOST / cb));
-    k_combine16<T><<<rows * cb, RT, 0, st>>>(a, cw, cb);
+    const int most = MOST / cb * (RT / cw);
+    for (int t0 = 0; t0 < a.n; t0 += most) { k_combine16<T><<<blocks(std::min(a.n - t0, most), RT / cw) * cb, RT, 0, st>>>(a, cw, cb, t0); }
     return hipGetLastError();
 }
 template <class T> hipError_t go_combine_grad(const CombineArgs & a, hipStream_t st) {
-    const unsigned rows = (unsigned) std::min(a.n, MOST);
-    if (a.E <= 512) { k_combine16_grad<T, 1><<<rows, 64, 0, st>>>(a); }
-    else if (a.n > 512) { k_combine16_grad<T, 4><<<rows, 256, 0, st>>>(a); }
-    else { k_combine16_grad<T, 16><<<a.n, 1024, 0, st>>>(a); }
+    for (int t0 = 0; t0 < a.n; t0 += MOST) {
+        const unsigned rows = (unsigned) std::min(a.n - t0, MOST);
+        if (a.E <= 512) { k_combine16_grad<T, 1><<<rows, 64, 0, st>>>(a, t0); }
+        else if (a.n > 512) { k_combine16_grad<T, 4><<<rows, 256, 0, st>>>(a, t0); }
+        else { k_combine16_grad<T, 16><<<rows, 1024, 0, st>>>(a, t0); }
+    }
     return hipGetLastError();
 }
 

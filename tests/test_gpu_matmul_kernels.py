@@ -339,7 +339,7 @@ def test_layer_with_dropped_picks(ctx, n, ne, topk):
 
 
 def test_combine_of_more_rows_than_workgroups(ctx):
-    """a launch has 2^22 workgroups at most: rows behind them are taken by the same ones"""
+    """a launch has 2^22 workgroups at most: more rows take more than one"""
     n = (1 << 22) + 9
     for E, P in ((2048, 50), (8, n)):
         o, w = whole(1, P, E), whole(2, n, 1, dtype=F4, most=3)
