@@ -413,7 +413,7 @@ template <class T, bool GATED, class H, class V> __device__ __forceinline__ void
     const int wave = uni((int) threadIdx.x >> 6), lane = lane_id(), wm = wave / V::WN, wn = wave % V::WN;
     const size_t t0 = (size_t) s.slot * a.R + s.n0, all = (size_t) a.n * a.R;
     const int c0 = wn * FC * 16 + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);   // the lane's first column in the tile
-    auto each = [&](auto column, auto f) __attribute__((always_inline)) {   // column(c) and then f(offset, z, z2) on 8 results at a time
+    auto each = [&](auto column, auto ahead, auto f) __attribute__((always_inline)) {   // column(c), ahead(m, c) and f(m, offset, z, z2) on 8 results at a time
 #pragma unroll
         for (int j = 0; j < FC; j += 2) {
             const int g = GATED ? 2 * j : j, c = c0 + 16 * j;   // (W's 2 fragments, W2's 2, and so on)
@@ -422,31 +422,43 @@ template <class T, bool GATED, class H, class V> __device__ __forceinline__ void
             for (int m = 0; m < V::FM; ++m) {
                 const int sr = (wm * V::FM + m) * 16 + (lane & 15);
                 float z[8], z2[8];
+                ahead(m, c);
                 eight(acc[m][g], acc[m][g + 1], z);
                 if (GATED) { eight(acc[m][g + 2], acc[m][g + 3], z2); }
-                if (sr < s.nm && s.n0 + c < a.R) { f((uint32_t) sr * (uint32_t) a.R + (uint32_t) c, z, z2); }
+                if (sr < s.nm && s.n0 + c < a.R) { f(m, (uint32_t) sr * (uint32_t) a.R + (uint32_t) c, z, z2); }
             }
         }
     };
     auto none = [](int) {};
+    auto none2 = [](int, int) {};
     if (a.parts > 1) {   // (k_mm_join does the rest)
         float * p = a.part + (size_t) part * all + t0, * p2 = p + (size_t) a.parts * all;
-        each(none, [&](uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) { put8(p + at, z); if (GATED) { put8(p2 + at, z2); } });
+        each(none, none2, [&](int, uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) { put8(p + at, z); if (GATED) { put8(p2 + at, z2); } });
         return;
     }
     const float * bias = a.bias ? a.bias + (size_t) s.e * a.R + s.n0 : nullptr;
     const T * res = a.residual ? (const T *) a.residual + t0 : nullptr;
     T * y = (T *) a.y + (a.y_f32 ? 2 * t0 : t0), * pz = a.z ? (T *) a.z + t0 : nullptr, * pz2 = GATED && a.z2 ? (T *) a.z2 + t0 : nullptr;
     if (!GATED && !bias && !res && !pz && !a.act && !a.y_f32) {
-        each(none, [&](uint32_t at, float (&z)[8], float (&)[8]) __attribute__((always_inline)) { put8(y + at, z); });
+        each(none, none2, [&](int, uint32_t at, float (&z)[8], float (&)[8]) __attribute__((always_inline)) { put8(y + at, z); });
         return;
     }
     float b8[8];
+    constexpr int RA = V::FM < 4 ? V::FM : 4;
+    V8<T> r8[RA];   // (the residuals of 4 row groups asked for together: 8192 rows, 2048 -> 7168 318 -> 290 us, 512 -> 16384 376 -> 315)
     each([&](int c) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) { b8[u] = 0.f; }
         if (bias && s.n0 + c < a.R) { add8(bias + c, b8); }
-    }, [&](uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) {
+    }, [&](int m0, int c) __attribute__((always_inline)) {
+        if (m0 % RA == 0 && res) {
+#pragma unroll
+            for (int m = 0; m < RA; ++m) {   // (where there is none, the tile's first)
+                const int sr = (wm * V::FM + m0 + m) * 16 + (lane & 15);
+                r8[m] = *(const LK_GLOBAL V8<T> *) (res + (sr < s.nm && s.n0 + c < a.R ? (uint32_t) sr * (uint32_t) a.R + (uint32_t) c : 0u));
+            }
+        }
+    }, [&](int m, uint32_t at, float (&z)[8], float (&z2)[8]) __attribute__((always_inline)) {
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) { z[u] += b8[u]; }
@@ -455,7 +467,10 @@ template <class T, bool GATED, class H, class V> __device__ __forceinline__ void
 #pragma unroll
             for (int u = 0; u < 8; ++u) { v[u] *= z2[u]; }
         }
-        if (res) { add8(res + at, v); }
+        if (res) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) { v[u] += (float) r8[m % RA][u]; }
+        }
         if (a.y_f32) { put8((float *) y + at, v); } else { put8(y + at, v); }
         if (pz) { put8(pz + at, z); }
         if (pz2) { put8(pz2 + at, z2); }
