@@ -230,7 +230,7 @@ int fl_act_grad_dev(FLCtx *, int type, int act, const void * dy, const void * z,
                     void * dz, void * dz2, float * dbias, int accumulate);
 /* the products' backward pass: dx [n][K] = dz W (+ dz2 W2), of each slot (with perm too: a row's slots are summed by fl_combine_dev with
  * w NULL), dW [n_exp][R][K] = (accumulate: +=) dz^T x of the expert's slots, dW2 = dz2^T x likewise; each may be NULL: not computed.
- * dW and dW2 are of `type` or FL_F32 (dw_type); accumulate adds in fp32 and rounds the sum. An expert without slots gets 0 (accumulate: stays). Deterministic, no atomics. */
+ * dW and dW2 are of `type` or FL_F32 (dw_type); accumulate adds in fp32 and rounds the sum. An expert without slots gets 0 (accumulate: stays). Deterministic: no atomics on results. */
 int fl_matmul_grad_dev(FLCtx *, int type, const void * dz, const void * dz2, const void * x, const void * W, const void * W2, int n, int R, int K, int n_exp,
                        const int * offsets, const int * perm, int topk, int xrows, void * dx, void * dW, void * dW2, int dw_type, int accumulate);
 /* the picks' sum: y [n][E] = residual + sum over k of w[t][k] o[inv[t][k]], fp32 in k's order; o [P][E] the slots' rows, inv and sel
