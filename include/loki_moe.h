@@ -208,7 +208,8 @@ int fl_kq_matvec_dev(FLCtx *, int fmt, const void * w, int R, int K, const int8_
 /* ---------------------------------------------------------------- additive: 16-bit products, and what trains with them
  * (no counterpart in the reference, whose matrices are all quantised and which does not train). type: FL_BF16 or FL_F16, of every
  * operand and result that is not named float or int; products are exact and summed in fp32, each result rounded once. R and K are
- * multiples of 8 (R at most 2^20, K 65536), n at most 2^24, pointers 16-byte aligned, tensors contiguous.
+ * multiples of 8 (R at most 2^20, K 65536), n at most 2^24, pointers 16-byte aligned, tensors contiguous. Operands and results of no
+ * elements (n 0, P 0) may be NULL.
  * Groups: with offsets [n_exp + 1] (device, ascending, as fl_dispatch_dev leaves them) expert e has the rows ("slots") offsets[e] ..
  * offsets[e + 1] - 1 of the n and a matrix of its own; slots of no expert are not read and their results stay as they were. Offsets
  * are clamped to 0 .. n; ones that are not ascending give unspecified values. Without offsets (NULL) n_exp is 1 and takes all n rows.

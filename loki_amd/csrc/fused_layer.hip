@@ -489,7 +489,7 @@ extern "C" int fl_matmul_grad_dev(FLCtx * c, int type, const void * dz, const vo
     MatmulGradArgs a{};
     if (int rc = mm_shape(c, type, n, R, K, n_exp, offsets, perm, topk, xrows, a.magic)) { return rc; }
     if (dw_type != type && dw_type != FL_F32) { return fail(c, FL_EINVAL, "dW's type %d is neither the operands' nor FL_F32", dw_type); }
-    if (!dx && !dW && !dW2) { return fail(c, FL_EINVAL, "nothing to compute: dx, dW and dW2 are all null"); }
+    if (!dx && !dW && !dW2) { return n == 0 ? FL_OK : fail(c, FL_EINVAL, "nothing to compute: dx, dW and dW2 are all null"); }   // (a result of no elements may be null)
     if ((n > 0 && (((dx || dW) && !dz) || ((dW || dW2) && !x) || (dx && (!W || (dz2 && !W2))) || (dW2 && !dz2)))) { return fail(c, FL_EINVAL, "null pointer"); }
     if (misaligned({ dz, dz2, x, W, W2, dx, dW, dW2 })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
     const size_t xb = (size_t) (perm ? xrows : n) * K * 2, wn = (size_t) n_exp * R * K, wb = wn * (dw_type == FL_F32 ? 4 : 2), zb = (size_t) n * R * 2, dxb = (size_t) n * K * 2;
@@ -532,7 +532,7 @@ extern "C" int fl_act_grad_dev(FLCtx * c, int type, int act, const void * dy, co
     uint32_t magic;
     if (int rc = mm_shape(c, type, n, R, 8, n_exp, offsets, nullptr, 1, 0, magic)) { return rc; }
     if (act < FL_ACT_NONE || act > FL_ACT_GELU) { return fail(c, FL_EINVAL, "activation %d", act); }
-    if (!dz && !dz2 && !dbias) { return fail(c, FL_EINVAL, "nothing to compute: dz, dz2 and dbias are all null"); }
+    if (!dz && !dz2 && !dbias) { return n == 0 ? FL_OK : fail(c, FL_EINVAL, "nothing to compute: dz, dz2 and dbias are all null"); }
     if ((z2 != nullptr || dz2 != nullptr) && dbias) { return fail(c, FL_EINVAL, "a gated product has no bias"); }
     if (n > 0 && (!dy || ((act != FL_ACT_NONE || z2) && !z) || (dz2 && !z2))) { return fail(c, FL_EINVAL, "null pointer"); }
     if (misaligned({ dy, z, z2, dz, dz2, dbias })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
@@ -603,7 +603,7 @@ extern "C" int fl_combine_grad_dev(FLCtx * c, int type, const void * dy, const v
     CombineArgs a{};
     a.type = type; a.n = n; a.topk = topk; a.n_exp = n_exp; a.P = P; a.E = E; a.inv = inv; a.sel = sel; a.w = w; a.o = o; a.dy = dy; a.d_o = d_o; a.dw = dw;
     if (int rc = combine_args(c, a)) { return rc; }
-    if (!d_o && !dw) { return fail(c, FL_EINVAL, "nothing to compute: d_o and dw are both null"); }
+    if (!d_o && !dw) { return n == 0 || P == 0 ? FL_OK : fail(c, FL_EINVAL, "nothing to compute: d_o and dw are both null"); }
     if (n == 0) { return FL_OK; }
     if (!dy || (dw && P > 0 && !o)) { return fail(c, FL_EINVAL, "null pointer"); }
     if (misaligned({ dy, o, d_o })) { return fail(c, FL_EINVAL, "operands and results must be 16-byte aligned"); }
