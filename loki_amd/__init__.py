@@ -597,13 +597,14 @@ class Context:
         return self._product_grad("matmul_grad", dz, x, W, None, dz2, up, None, 1, dW, dW2, dw_dtype, need_dx, need_dW, dx)
 
     def expert_matmul_grad(self, dz, x, W, offsets, dz2=None, up=None, perm=None, topk=1, dW=None, dW2=None, dw_dtype=None, need_dx=True, need_dW=True, dx=None):
-        """matmul_grad() grouped by expert, as expert_matmul(). dx is each slot's; combine(dx, inv) sums a row's. An expert without slots
-        gets zeros; slots of no expert keep what dx holds."""
+        """matmul_grad() grouped by expert, as expert_matmul(). dx is each slot's; combine(dx, inv, topk=topk) sums a row's. An expert without
+        slots gets zeros; slots of no expert keep what dx holds."""
         return self._product_grad("expert_matmul_grad", dz, x, W, offsets, dz2, up, perm, topk, dW, dW2, dw_dtype, need_dx, need_dW, dx)
 
     def combine(self, o, inv, w=None, sel=None, n_exp=N_EXPERT, residual=None, topk=None, dtype=None, y=None):
         """y [n][E] = residual + sum_k w[t][k] o[inv[t][k]] for the slots' rows o [P][E], dispatch()'s inv and route()'s w [n][topk] float32
-        (None: ones; topk then from sel, or given). Picks of sel outside 0 .. n_exp - 1 are skipped. dtype: o's (default) or float32."""
+        (None: ones; topk then from sel, or given). Picks of sel outside 0 .. n_exp - 1 are skipped, and slots outside 0 .. P - 1 (inv is
+        -1 for a pick that dispatch() dropped, so that sel may be None). dtype: o's (default) or float32."""
         P, E, n, k, T, code = self._picks("combine", o, inv, w, sel, topk)
         if y is None:
             y = o.new_empty(n, E) if dtype is None else o.new_empty(n, E, dtype=dtype)
@@ -644,6 +645,8 @@ class Context:
         return P, E, n, k, T, code
 
     def dispatch(self, sel, n_exp=N_EXPERT):
+        """(counts, offsets, perm, inv, act, nact) of picks sel [n][topk]: slots by expert, perm[slot] the pair (row * topk + pick), inv
+        the other way round. A pick outside 0 .. n_exp - 1 has no slot and its inv is -1; perm behind the last offset is undefined."""
         t = self.torch
         n, topk = sel.shape
         P = n * topk

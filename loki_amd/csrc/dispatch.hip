@@ -3,10 +3,11 @@
 // The order is ggml mul_mat_id's row mapping, which the reference's wide pass builds on the host
 // (byexp at src/server_core_fused.cpp:937; slot tables at :945): for token t ascending and k ascending, pair
 // (t, k) = index t*topk + k is appended to its expert's list. perm lists the pairs expert by expert (ascending id),
-// each expert's pairs in that order; inv is perm's inverse (the slot of each pair); act lists the used experts
-// ascending. One workgroup of 1024 threads: an LDS histogram, a scan, then the pairs in rounds of 1024 where a
-// thread's rank among equal experts comes from wave ballots (8 bit-planes of the expert id) plus the counts of the
-// waves before it, so the result is the stable counting sort whatever the thread timing. Above 4096 pairs, with a
+// each expert's pairs in that order; inv is perm's inverse (the slot of each pair; with `mark`, -1 for a pair that no
+// expert has, so that inv alone tells which slots are a row's); act lists the used experts ascending. One workgroup of
+// 1024 threads: an LDS histogram, a scan, then the pairs in rounds of 1024 where a thread's rank among equal experts
+// comes from wave ballots (8 bit-planes of the expert id) plus the counts of the waves before it, so the result is the
+// stable counting sort whatever the thread timing. Above 4096 pairs, with a
 // scratch buffer, the rounds run as workgroups of their own: k_dispatch_count takes each round's per-expert counts,
 // k_dispatch_scan the totals, offsets, used experts and each round's per-expert base (the counts of the rounds before
 // it), and k_dispatch_place each round's positions by the same ballots -- the same stable order.
@@ -20,7 +21,7 @@ static_assert(NEXP_MAX % 64 == 0 && NEXP_MAX <= 1024, "the scan's waves and the 
 
 __global__ void __launch_bounds__(1024) k_dispatch(const int * __restrict__ sel, int P, int n_exp, int * __restrict__ counts,
                                                    int * __restrict__ offsets, int * __restrict__ perm, int * __restrict__ inv,
-                                                   int * __restrict__ act, int * __restrict__ nact) {
+                                                   int * __restrict__ act, int * __restrict__ nact, int mark) {
     __shared__ int cnt[NEXP_MAX], base[NEXP_MAX];
     __shared__ int wc[DWAVES][NEXP_MAX];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(1024) k_dispatch(const int * __restrict__ sel,
             for (int w = 0; w < wave; ++w) { pre += wc[w][e]; }
             const int pos = base[e] + pre + rank;
             perm[pos] = i; inv[i] = pos;
-        }
+        } else if (mark && i < P) { inv[i] = -1; }
         __syncthreads();
         if (tid < n_exp) {
             int s = 0;
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(NEXP_MAX) k_dispatch_scan(const int * __restri
 }
 // round b's positions: the ballot rank among the wave's equal experts, plus the earlier waves' counts, plus bb[b][e]
 __global__ void __launch_bounds__(1024) k_dispatch_place(const int * __restrict__ sel, int P, int n_exp, const int * __restrict__ bb,
-                                                         int * __restrict__ perm, int * __restrict__ inv) {
+                                                         int * __restrict__ perm, int * __restrict__ inv, int mark) {
     __shared__ int wc[DWAVES][NEXP_MAX];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
     for (int j = tid; j < DWAVES * NEXP_MAX; j += 1024) { (&wc[0][0])[j] = 0; }
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(1024) k_dispatch_place(const int * __restrict_
         for (int w = 0; w < wave; ++w) { pre += wc[w][e]; }
         const int pos = bb[blockIdx.x * NEXP_MAX + e] + pre + rank;
         perm[pos] = i; inv[i] = pos;
-    }
+    } else if (mark && i < P) { inv[i] = -1; }
 }
 
 // from DISP_MULTI pairs the rounds run as workgroups (2048 tokens: 40.5 -> 21.9 us); at 4096 pairs and below the
@@ -160,17 +161,17 @@ constexpr int DISP_MULTI = 4097;
 size_t dispatch_scratch_ints(int P) { return P >= DISP_MULTI ? (size_t) 2 * ((P + 1023) / 1024) * NEXP_MAX : 0; }
 
 hipError_t launch_dispatch(const int * sel, int P, int n_exp, int * counts, int * offsets, int * perm, int * inv,
-                           int * act, int * nact, hipStream_t st, int * scratch) {
+                           int * act, int * nact, hipStream_t st, int * scratch, bool mark) {
     if (n_exp > NEXP_MAX || n_exp <= 0) { return hipErrorInvalidValue; }
     if (P >= DISP_MULTI && scratch) {
         const int R = (P + 1023) / 1024;
         int * bc = scratch, * bb = scratch + (size_t) R * NEXP_MAX;
         k_dispatch_count<<<R, 1024, 0, st>>>(sel, P, n_exp, bc);
         k_dispatch_scan<<<1, NEXP_MAX, 0, st>>>(bc, R, n_exp, counts, offsets, act, nact, bb);
-        k_dispatch_place<<<R, 1024, 0, st>>>(sel, P, n_exp, bb, perm, inv);
+        k_dispatch_place<<<R, 1024, 0, st>>>(sel, P, n_exp, bb, perm, inv, mark);
         return hipGetLastError();
     }
-    k_dispatch<<<1, 1024, 0, st>>>(sel, P, n_exp, counts, offsets, perm, inv, act, nact);
+    k_dispatch<<<1, 1024, 0, st>>>(sel, P, n_exp, counts, offsets, perm, inv, act, nact, mark);
     return hipGetLastError();
 }
 

@@ -270,7 +270,7 @@ extern "C" int fl_dispatch_dev(FLCtx * c, const int * sel, int n, int topk, int 
     if (!sel || !counts || !offsets || !perm || !inv || !act || !nact) { return fail(c, FL_EINVAL, "null pointer"); }
     int * dsc = nullptr;
     if (const size_t nd = dispatch_scratch_ints(n * topk)) { ALLOC(c, c->dscr, nd); dsc = c->dscr.p; }
-    TRY(c, launch_dispatch(sel, n * topk, n_exp, counts, offsets, perm, inv, act, nact, c->st, dsc));
+    TRY(c, launch_dispatch(sel, n * topk, n_exp, counts, offsets, perm, inv, act, nact, c->st, dsc, true));
     return FL_OK;
 }
 
