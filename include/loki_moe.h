@@ -192,8 +192,8 @@ int fl_route_grad_dev(FLCtx *, const float * W, const float * x, const float * l
  * freed before fl_free, so a captured call stays valid after later calls have outgrown it. Calls of one context run on one stream at a time; graphs captured
  * from one context share its workspaces (and the counters from which the 16-bit products' workgroups take their tiles) and must not run at
  * the same time. The context's device has to be the current one (FL_EINVAL). */
-/* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device). A pick outside 0 .. n_exp - 1 has no
- * slot: its inv is -1; perm behind offsets[n_exp] and act behind *nact stay as they were */
+/* dispatch only: counts [n_exp], offsets [n_exp+1], perm/inv [n*topk], act [n_exp], nact [1] (device); sel may be NULL where n is 0. A pick
+ * outside 0 .. n_exp - 1 has no slot: its inv is -1; perm behind offsets[n_exp] and act behind *nact stay as they were */
 int fl_dispatch_dev(FLCtx *, const int * sel, int n, int topk, int n_exp, int * counts, int * offsets, int * perm, int * inv, int * act, int * nact);
 /* Q8_K of nrows x K floats (device): q [nrows][K] int8, d [nrows][K/256] */
 int fl_quant_q8k_dev(FLCtx *, const float * x, int nrows, int K, int8_t * q, float * d);
