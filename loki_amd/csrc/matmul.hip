@@ -364,8 +364,7 @@ template <class H, int COLS, int BYTES, int C> struct ColCopies {
 template <class H, class F> __device__ __forceinline__ void by_rows(int nm, F f) {
     if constexpr (H::BM == 256) { if (nm > 128) { f(Waves<H, 256, 2>()); return; } }
     if constexpr (H::BM >= 128 && H::BN == 256) { if (nm > 64) { f(Waves<H, 128, 1>()); return; } f(Waves<H, 64, 1>()); }
-    else if constexpr (H::BM == 128) { f(Waves<H, 128, 2>()); }
-    else { f(Waves<H, 64, 2>()); }
+    else { static_assert(H::BM == 64, "the waves of another tile"); f(Waves<H, 64, 2>()); }
 }
 
 // ---------------------------------------------------------------- forward
