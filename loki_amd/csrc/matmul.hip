@@ -823,6 +823,7 @@ template <class T, bool GATED, class H> hipError_t fwd(const MatmulArgs & a, hip
 }
 // (B, often weights straight from memory, a round further ahead where LDS holds it: 501 rows, gated, 7168 -> 2 x 7000, weights not in any cache,
 // 124 -> 110 us; A a round less and B one more 138)
+// (Large's sums take half of the registers: k_mm spills 16 of the others, k_mm_dx 25 and k_mm_dw 1 or 2, all outside the loop over the rounds, once a tile)
 typedef Shape<256, 256, 3, 2, 1> Large;
 typedef Shape<128, 256, 3, 3, 1> Wide;
 typedef Shape<64, 128, 3, 3, 2> Small;

@@ -35,10 +35,10 @@ __device__ __forceinline__ f32x4 mfma32(f16x8 a, f16x8 b, f32x4 c) {
 }
 
 // ---------------------------------------------------------------- activations z s(g(z)), s(t) = 1 / (1 + e^-t)
-// silu: g = z; gelu: g = 2 sqrt(2 / pi) (z + 0.044715 z^3), the tanh form. In fp32: e^-t and the reciprocal by their instructions (a division's ten cost 8192
-// x 16384 results 100 us), the former's argument's
-// rounding costs |t| 2^-24 of it; where |t| is large the factor is near 0 or 1 and the error falls away or reaches 100 * 2^-24 of values
-// below e^-100. A factor below 2^-126 is 0.
+// silu: g = z; gelu: g = 2 sqrt(2 / pi) (z + 0.044715 z^3), the tanh form. In fp32: e^-t and the reciprocal by their instructions (a division's ten
+// cost 8192 x 16384 results 100 us). e^-t is 2^(-t log2 e): the constant's and the product's rounding, 1.22 * 2^-24 of the exponent, come to
+// 1.3 |t| 2^-24 of it, and the two instructions and the sum to 5 * 2^-24. What that does to s is (1 - s) of the former: s is within
+// (1.3 |t| (1 - s) + 5) 2^-24 of itself, 5 * 2^-24 where t is large, 120 * 2^-24 at t = -87, where s is 2^-126. A factor below 2^-126 is 0.
 constexpr float GELU_C = 1.5957691216057308f, GELU_A = 0.044715f;
 __device__ __forceinline__ float sigma(float t) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t)); }
 template <int ACT> __device__ __forceinline__ float act_arg(float z) { return ACT == ACT_GELU ? GELU_C * (z + GELU_A * z * z * z) : z; }

@@ -1,5 +1,6 @@
 // matmul_rows.hip -- what goes over rows beside the 16-bit products: the epilogue's gradient with the bias's, the sum of a row's picks
-// under the routing weights and the gradients of both. All of it is bound by memory: every value is read and written once, 16 bytes a lane.
+// under the routing weights and the gradients of both. Many rows are bound by memory: every value is read and written once, 16 bytes a lane.
+// A few rows of picks are bound by loads that wait for each other: 8 picks of 7168, 6 rows, 5.0 and 7.6 us.
 #include "matmul_device.h"
 
 namespace lk {
@@ -121,7 +122,7 @@ template <class T> __global__ void __launch_bounds__(RT) k_combine16(CombineArgs
     V8<T> o[MAXK];
     float w[MAXK];
 #pragma unroll
-    for (int k = 0; k < MAXK; ++k) {   // all loads before the sums
+    for (int k = 0; k < MAXK; ++k) {   // (the rows' loads before the sums; a pick's expert and slot are waited for before the next one's are asked for)
         const int s = k < a.topk ? slot_of(a, t * a.topk + k) : -1;
         w[k] = s >= 0 ? (a.w ? a.w[t * a.topk + k] : 1.f) : 0.f;
         o[k] = (V8<T>) {};
@@ -141,7 +142,8 @@ template <class T> __global__ void __launch_bounds__(RT) k_combine16(CombineArgs
     if (a.y_f32) { store8((float *) a.y + at, y); } else { store8((T *) a.y + at, y); }
 }
 
-// d_o and dw of one row: W waves, each its columns, then the waves' sums in order
+// d_o and dw of one row: W waves, each its columns, then the waves' sums in order. d_o may be o, so a pick's row is read, waited for and its gradient
+// written before the next pick's is asked for
 template <class T, int W> __global__ void __launch_bounds__(64 * W) k_combine16_grad(CombineArgs a, int t0) {
     __shared__ float lds[W][MAXK];
     const int64_t t = t0 + (int64_t) blockIdx.x;
