@@ -104,10 +104,11 @@ constexpr RouteCut route_cut(int n, int E, bool dW, bool dx) {
 // ---------------------------------------------------------------- 16-bit products (matmul.hip)
 // Tiles of bm x bn, `slots` of them at a time on the chip. A tile takes fixed + rounds * (a round of 64 terms) us, a round `one` where
 // few CUs have work and `full` where all have (the clock falls with the power, and Small's two workgroups share a CU). A sum can be split into
-// parts, whose results a second launch adds up. The constants are fitted to 112 sizes (16 .. 2048 rows, 512 .. 16384 columns and
-// terms, weights from memory). Examples, us, Small / Wide / Large, then the best split: 64 rows, 7168 terms -> 2048 columns 54 / 74 / -, 17 (Small, 8
-// parts); 501, 7168 -> 2048 53 / 75 / 141, 33 (Wide, 4); 501, 2048 -> 7168 29 / 29 / 57; 1024, 7168 -> 7168 137 / 93 / 144; 2048, 7168 -> 7168
-// 302 / 203 / 173; 2048, 2048 -> 2048 33 / 31 / 58; 512 rows, columns and terms 7.6 / 13 / 25.
+// parts, whose results a second launch adds up. The constants were fitted to 112 sizes (16 .. 2048 rows, 512 .. 16384 columns and terms, weights from
+// memory) when the kernels copied B two rounds ahead; with the present ones the choice is 2.8 % above the best on average there, 20 % at most.
+// Examples, us, Small / Wide / Large, then the best split: 64 rows, 7168 terms -> 2048 columns 35 / 55 / -, 16 (Small, 6 parts); 501, 7168 -> 2048
+// 36 / 72 / 132, 30 (Small, 2); 501, 2048 -> 7168 25 / 28 / 49; 1024, 7168 -> 7168 133 / 88 / 137; 2048, 7168 -> 7168 288 / 184 / 159; 2048,
+// 2048 -> 2048 28 / 29 / 49; 512 rows, columns and terms 7.5 / 13 / 21.
 enum { MM_SMALL, MM_WIDE, MM_LARGE, MM_FEW };
 struct MmPlan { int shape, parts; };
 struct MmCost { int bm, bn, slots; float fixed, one, full, stream; };
@@ -135,9 +136,9 @@ constexpr float mm_time(int shape, int parts, int n, int n_exp, int cols, int te
     return 2.5f + (sums > memory ? sums + 0.15f * memory : memory + 0.15f * sums) + join;
 }
 // Few rows (matmul_few.hip; up to 16 of an expert with one reading of its matrix): 16 columns a workgroup, whose 8 waves take 64 terms each in turn.
-// Us against the best of the above: 1 row of 2048 terms -> 7168 columns 9.5 / 14, 7168 -> 7168 19 / 24, 7168 -> 131072 358 / 306; 8 rows 10.5 / 14,
-// 24 / 24, 461 / 307; 16 rows 11.5 / 15, 28 / 24; one token's 8 experts of 256, 7168 -> 2 x 2048, 90 / 89, two tokens' 171 / 150; 6 of 64, 2048 ->
-// 2 x 1024, 12 / 21, 48 51 / 60, 192 98 / 97.
+// Us against the best of the above: 1 row of 2048 terms -> 7168 columns 9.7 / 13, 7168 -> 7168 19 / 23, 7168 -> 131072 357 / 309; 8 rows 11 / 14,
+// 24 / 23, 463 / 310; 16 rows 12 / 14, 28 / 23; one token's 8 experts of 256, 7168 -> 2 x 2048, 90 / 84, two tokens' 170 / 151; 6 of 64, 2048 ->
+// 2 x 1024, 12 / 19, 48 51 / 51, 192 98 / 92.
 constexpr float mm_few_time(int n, int n_exp, int cols, int terms) {
     const float used = mm_used(n, n_exp), rows = (float) n / used;
     const float tiles = n_exp == 1 ? (float) ((n + 15) / 16) : rows < 8.f ? used : used * (0.5f + rows / 16.f), groups = tiles * (float) cols / 16.f;
@@ -161,9 +162,10 @@ constexpr MmPlan mm_plan(int n, int n_exp, int cols, int terms, bool forward) {
 }
 
 // dW of `mats` matrices [n_exp][R][K] from n rows: tiles of 256 x 256 (MM_LARGE), of 128 x 128 with two workgroups a CU (MM_SMALL) or four
-// that keep nothing ahead (MM_FEW); the rows can be split into parts. As above, fitted to 25 sizes. Us, MM_SMALL / MM_LARGE / MM_FEW: 16 rows,
-// 7168 x 7168 31 / 35 / 24; 501 68 / 74 / 64; 8192 943 / 673 / 1088; 8192 rows, 2048 x 2048 71 / - / -, 512 x 512 29 and 18 in 8 parts; 256 experts of
-// 4, 128 and 256 rows, 7168 x 2048, 1899 / 1928 / 1378, 2629 / 2487 / 2317, 3720 / 3370 / 3089.
+// that keep nothing ahead (MM_FEW); the rows can be split into parts. Fitted to 25 sizes before the results went past the caches; with the present
+// kernels 2.0 % above the best there, 20 % at most. Us, MM_SMALL / MM_LARGE / MM_FEW: 16 rows, 7168 x 7168 31 / 37 / 23; 501 65 / 69 / 62; 8192
+// 910 / 676 / 1048; 8192 rows, 2048 x 2048 66 / 142 / 129, 512 x 512 57 and 19 in 8 parts; 256 experts of 4, 128 and 256 rows, 7168 x 2048,
+// 1931 / 1777 / 1267, 2455 / 2350 / 2335, 3205 / 2840 / 3009.
 constexpr float dw_time(int shape, int parts, int n, int n_exp, int R, int K, int mats) {
     const int b = shape == MM_LARGE ? 256 : 128, slots = shape == MM_LARGE ? 256 : shape == MM_FEW ? 1024 : 512;
     const float fixed = shape == MM_LARGE ? 10.f : shape == MM_FEW ? 5.4f : 5.f, one = shape == MM_LARGE ? 0.92f : shape == MM_FEW ? 1.05f : 0.5f,

@@ -444,7 +444,7 @@ template <class T, bool GATED, class H, class V> __device__ __forceinline__ void
     }
     float b8[8];
     constexpr int RA = V::FM < 4 ? V::FM : 4;
-    V8<T> r8[RA];   // (the residuals of 4 row groups asked for together: 8192 rows, 2048 -> 7168 318 -> 290 us, 512 -> 16384 376 -> 315)
+    V8<T> r8[RA];   // (the residuals of 4 row groups asked for together: 8192 rows, 2048 -> 7168 318 -> 290 us, 512 -> 16384 376 -> 315; without one, short sums lost 2 to 5 %: 2755 rows, 416 -> 12504 57 -> 60)
     each([&](int c) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) { b8[u] = 0.f; }
@@ -756,7 +756,7 @@ template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds
     dw_results<T, F32, V>(a, s, acc);
 }
 // few rows an expert: the results' memory bounds it, and a tile has a round or two. Nothing is kept ahead; four workgroups a CU cover each
-// other's waits (256 experts of 128 rows, 7168 x 2048: 4 rows 1378 us, Middle 1899, Large 1928; 128 rows 2317, 2629, 2487)
+// other's waits (256 experts, 7168 x 2048: of 4 rows 1267 us, Middle 1931, Large 1777; of 128 rows 2335, 2455, 2350)
 template <class T, bool F32, bool PERM, class H> __global__ void __launch_bounds__(H::threads, H::PER_CU * H::NW / 4) k_mm_dw_few(MatmulGradArgs a) {
     extern __shared__ __attribute__((aligned(1024))) uint8_t dyn[];
     typedef DwCopies<T, PERM, H> C;

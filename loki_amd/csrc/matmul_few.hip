@@ -4,7 +4,7 @@
 // the sum's terms, 64 at a time in turn, straight from memory into registers: lane (r, g) = 16 g + r reads 32 bytes of row r, so that the
 // four lanes of a row ask for a whole line, and the order of the terms in a product instruction is the same for both operands. What lies
 // outside an operand is outside its buffer's range and arrives as 0. The waves' sums meet in LDS, in order. Against the split tiles of matmul.hip,
-// which need a second launch: 1 row, 2048 -> 7168 9.5 us, those 14; 7168 -> 7168 19 and 24 (5.4 TB/s)
+// which need a second launch: 1 row, 2048 -> 7168 9.7 us, those 13; 7168 -> 7168 19 and 23 (5.3 TB/s)
 #include "matmul_device.h"
 
 namespace lk {
