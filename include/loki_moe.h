@@ -225,7 +225,7 @@ enum { FL_ACT_NONE = 0, FL_ACT_SILU = 1, FL_ACT_GELU = 2 };
  * x W2^T, for the backward pass. */
 int fl_matmul_dev(FLCtx *, int type, int act, const void * x, const void * W, const void * W2, const float * bias, const void * residual,
                   int n, int R, int K, int n_exp, const int * offsets, const int * perm, int topk, int xrows, void * y, int y_type, void * z, void * z2);
-/* the epilogue's backward pass: from dy [n][R] and fl_matmul_dev's z and z2 (z2 NULL: not gated; z may be NULL without an activation)
+/* the epilogue's backward pass: from dy [n][R] and fl_matmul_dev's z and z2 (z2 NULL: not gated; z may be NULL with neither z2 nor an activation)
  *   dz = dy act'(z) (* z2),   dz2 = dy act(z),   dbias [n_exp][R] = (accumulate: +=) sum over the expert's rows of dz, before rounding
  * (each may be NULL: not computed). dz and dz2 may be the buffers of dy, z or z2. */
 int fl_act_grad_dev(FLCtx *, int type, int act, const void * dy, const void * z, const void * z2, int n, int R, int n_exp, const int * offsets,
