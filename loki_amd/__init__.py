@@ -648,6 +648,9 @@ class Context:
         """(counts, offsets, perm, inv, act, nact) of picks sel [n][topk]: slots by expert, perm[slot] the pair (row * topk + pick), inv
         the other way round. A pick outside 0 .. n_exp - 1 has no slot and its inv is -1; perm behind the last offset is undefined."""
         t = self.torch
+        if sel.dim() != 2:
+            raise LokiError("dispatch: sel [n][topk] is needed, not %s" % (tuple(sel.shape),))
+        self._need("dispatch", (sel, t.int32, sel.shape))
         n, topk = sel.shape
         P = n * topk
         dev = sel.device
