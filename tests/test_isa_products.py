@@ -64,7 +64,7 @@ def test_no_scratch_in_a_products_loop(tmp_path):
     assert seen == {"k_mm", "k_mm_dx", "k_mm_dw", "k_mm_dw_few", "k_mm_few"}
 
 
-def test_checker_flags_a_planted_spill():
+def test_a_planted_spill_is_found():
     listing = "%016x <k>:\n" % 0x100 + "".join("\t%s // %012X: 00\n" % (i, 0x100 + 4 * n) for n, i in enumerate(
         ["scratch_store_dword off, v1, off", "v_mfma_f32_16x16x32_bf16 a", "%s", "s_cbranch_scc1 9", "scratch_load_dword v1, off, off"]))
     back = listing.replace("s_cbranch_scc1 9 // 00000000010C: 00", "s_cbranch_scc1 9 // 00000000010C: 00 <k+0x4>")
